@@ -1,0 +1,443 @@
+"""The 4-bit K/V cache: writing it, reading it back and attending over it, as measurable cases.
+
+A case is one step of a serving program with a paged cache: a batch of sequences, each with
+`len` tokens of which the last `new` are this step's.  Pages lie in any order in memory.
+
+In a plain form (`own` false) the cache is a pair of tensors, codes and scales, and every
+operator is written with elementary torch operations in 32 bits (the codes' quotients in
+64, so that a value next to the border between two codes falls on the right side).
+Otherwise the calls are those of arf_amd.Context: kv_write, kv_read, kv_attention.
+
+A row's groups of 32 values hold a scale d and codes q in [-8, 7], and stand for d * q:
+s is the group's value of largest magnitude (the positive one of two alike), d = s / -8 rounded
+to 8 significant bits and then to f16, q = x / d rounded to the nearest, ties to even.
+"""
+import math
+
+import numpy as np
+import torch
+
+own = False
+
+GROUP = 32
+DTYPE = {"f32": torch.float32, "f16": torch.float16}
+
+
+def listed():
+    return [
+        # one token of a chat that has just begun: launch and latency
+        dict(name="decode one short", op="attend", batch=1, new=1, len=193, ragged=False, idle=False,
+             q_heads=32, kv_heads=8, dim=128, page=32, window=0, softcap=0.0, causal=True, x="f16"),
+        # one token at the end of a long document, for one user
+        dict(name="decode one long", op="attend", batch=1, new=1, len=131071, ragged=False, idle=False,
+             q_heads=40, kv_heads=8, dim=128, page=64, window=0, softcap=0.0, causal=True, x="f32"),
+        # a serving step: chats of every age, one slot of the batch idle
+        dict(name="decode batch", op="attend", batch=64, new=1, len=8192, ragged=True, idle=True,
+             q_heads=32, kv_heads=4, dim=128, page=64, window=0, softcap=0.0, causal=True, x="f32"),
+        # a sliding-window layer with wide heads and capped scores
+        dict(name="decode window", op="attend", batch=32, new=1, len=6001, ragged=True, idle=False,
+             q_heads=16, kv_heads=8, dim=256, page=16, window=1024, softcap=50.0, causal=True, x="f16"),
+        # a small model without grouped heads
+        dict(name="decode ungrouped", op="attend", batch=16, new=1, len=4097, ragged=True, idle=False,
+             q_heads=32, kv_heads=32, dim=64, page=32, window=0, softcap=0.0, causal=True, x="f16"),
+        # drafted tokens checked in one step
+        dict(name="verify drafts", op="attend", batch=16, new=5, len=4099, ragged=True, idle=False,
+             q_heads=40, kv_heads=8, dim=128, page=64, window=0, softcap=0.0, causal=True, x="f32"),
+        # a prompt in one piece
+        dict(name="prefill", op="attend", batch=1, new=2048, len=2048, ragged=False, idle=False,
+             q_heads=40, kv_heads=8, dim=128, page=64, window=0, softcap=0.0, causal=True, x="f16"),
+        # the next piece of a long document
+        dict(name="prefill chunk", op="attend", batch=1, new=512, len=32868, ragged=False, idle=False,
+             q_heads=40, kv_heads=8, dim=128, page=64, window=0, softcap=0.0, causal=True, x="f32"),
+        # prompts of several users, some after a shared beginning
+        dict(name="prefill ragged", op="attend", batch=7, new=777, len=1500, ragged=True, idle=False,
+             q_heads=24, kv_heads=8, dim=96, page=16, window=0, softcap=0.0, causal=True, x="f16"),
+        # the keys and values of a serving step into the cache, and those rows back
+        dict(name="write decode", op="write", batch=64, new=1, len=8192, ragged=True, idle=True,
+             kv_heads=4, dim=128, page=64, x="f32"),
+        # those of long prompts
+        dict(name="write prefill", op="write", batch=3, new=8192, len=8192, ragged=True, idle=False,
+             kv_heads=8, dim=128, page=64, x="f32"),
+        # whole sequences read back, to move them to another cache
+        dict(name="read back", op="read", batch=8, new=1, len=32768, ragged=True, idle=False,
+             kv_heads=8, dim=128, page=64, x="f16"),
+    ]
+
+
+# bounds of a drawn case: the listed ones' largest key count, matrix work and padded scores
+MAX_CACHE = 1.4e8  # cached values of K
+MAX_FLOPS = 3.4e11
+MAX_SCORES = 6.0e8
+
+
+def _log(rng, lo, hi):
+    return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+
+def draw(rng):
+    """One more case: lengths and batches spread over their logarithm, any head layout."""
+    while True:
+        op = rng.choice(["attend", "attend", "attend", "attend", "write", "read"])
+        kind = rng.choice(["decode", "decode", "verify", "prefill"])
+        c = dict(op=op, kv_heads=rng.choice([1, 2, 4, 8, 16, 32]), dim=rng.choice([64, 96, 128, 128, 256]),
+                 page=rng.choice([16, 32, 48, 64, 128]), ragged=rng.choice([True, False]),
+                 idle=rng.choice([False, False, True]), x=rng.choice(["f32", "f16"]))
+        if op == "attend":
+            c.update(q_heads=c["kv_heads"] * rng.choice([1, 2, 3, 4, 5, 6, 7, 8, 16]), causal=rng.choice([True, True, True, False]),
+                     window=rng.choice([0, 0, 0, _log(rng, 16, 8192)]), softcap=rng.choice([0.0, 0.0, 30.0]))
+            if kind == "decode":
+                c.update(batch=_log(rng, 1, 128), new=1, len=_log(rng, 1, 131072))
+            elif kind == "verify":
+                c.update(batch=_log(rng, 1, 64), new=rng.randint(2, 16), len=_log(rng, 16, 32768))
+            else:
+                n = _log(rng, 17, 4096)
+                c.update(batch=_log(rng, 1, 8), new=n, len=n + rng.choice([0, _log(rng, 1, 32768)]))
+        elif op == "write":
+            n = rng.choice([1, _log(rng, 1, 8192)])
+            c.update(batch=_log(rng, 1, 128), new=n, len=n + _log(rng, 1, 8192))
+        else:
+            c.update(batch=_log(rng, 1, 32), new=1, len=_log(rng, 1, 32768))
+        if c["batch"] == 1:
+            c["idle"] = False
+        cache = c["batch"] * c["len"] * c["kv_heads"] * c["dim"]
+        if cache > MAX_CACHE or c.get("q_heads", 1) > 128:
+            continue
+        if op == "attend" and (work(c)["flops"] > MAX_FLOPS or
+                               c["batch"] * c["q_heads"] * c["new"] * c["len"] > MAX_SCORES or
+                               c["batch"] * c["q_heads"] * c["new"] * c["dim"] > MAX_CACHE):
+            continue
+        return c
+
+
+def _seqs(case):
+    """(new, len) of each sequence; the order they come in is the seed's."""
+    n, length, got = case["new"], case["len"], []
+    for b in range(case["batch"]):
+        if not case["ragged"] or b == 0:
+            got.append((n, length))
+            continue
+        new = 1 + int((n - 1) * ((b * 0.7548776662) % 1.0))
+        got.append((new, new + int((length - n) * ((b * 0.6180339887) % 1.0))))
+    if case["idle"]:
+        got[-1] = (1, 0)  # an idle slot: its token is nobody's
+    return got
+
+
+def _keys(case, new, length):
+    """(token, key) pairs and keys read of one sequence."""
+    pairs, first = 0, length
+    for i in range(new):
+        pos = length - new + i
+        hi = pos + 1 if case["causal"] else length
+        lo = max(0, pos - case["window"] + 1) if case["window"] else 0
+        if pos >= 0 and hi > lo:
+            pairs += hi - lo
+            first = min(first, lo)
+    return pairs, length - first
+
+
+def work(case):
+    """Every cached row, input row and output row once; 4 * dim flops for each (row of q, key)."""
+    size, seqs = (4 if case["x"] == "f32" else 2), _seqs(case)
+    row = case["kv_heads"] * case["dim"]
+    held = 2 * row * 9 / 16  # codes and scales of K and V of one token
+    if case["op"] == "attend":
+        got = [_keys(case, n, ln) for n, ln in seqs]
+        toks = sum(n for n, _ in seqs)
+        io = 2 * toks * case["q_heads"] * case["dim"] * size
+        return {"bytes": sum(k for _, k in got) * held + io,
+                "flops": 4.0 * case["q_heads"] * case["dim"] * sum(p for p, _ in got)}
+    rows = sum(min(n, ln) if case["op"] == "write" else ln for n, ln in seqs)
+    flat = 2 * rows * row * size
+    # written rows are quantised and read back; a value takes a quotient and a product
+    return {"bytes": flat + rows * held if case["op"] == "read" else 2 * flat + 2 * rows * held,
+            "flops": 2.0 * rows * row * (1 if case["op"] == "read" else 2)}
+
+
+# ---- a program's state ----------------------------------------------------------------
+
+
+def _gen(seed, stream):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(int(seed) * 64 + stream)
+    return g
+
+
+def _order(case, seed):
+    """The sequences in the seed's order."""
+    seqs = _seqs(case)
+    g = torch.Generator()
+    g.manual_seed(int(seed) * 64 + 1)
+    return [seqs[i] for i in torch.randperm(len(seqs), generator=g).tolist()]
+
+
+def _cached(case, seed):
+    """K and V of every cached token, sequence after sequence: [rows, kv_heads, dim].  Keys have a few
+    channels eight times larger, as those of language models do."""
+    rows, shape = sum(ln for _, ln in _seqs(case)), (case["kv_heads"], case["dim"])
+    t = DTYPE[case["x"]] if case["op"] == "write" else torch.float16
+    k = torch.randn(rows, *shape, generator=_gen(seed, 2), device="cuda", dtype=t)
+    v = torch.randn(rows, *shape, generator=_gen(seed, 3), device="cuda", dtype=t)
+    k *= torch.where(torch.rand(shape, generator=_gen(seed, 4), device="cuda") < 1 / 32, 8.0, 1.0).to(t)
+    return k, v
+
+
+def _queries(case, seed):
+    toks = sum(n for n, _ in _seqs(case))
+    q = torch.randn(toks, case["q_heads"], case["dim"], generator=_gen(seed, 5), device="cuda")
+    return q.to(DTYPE[case["x"]])
+
+
+def _tables(case, seed, seqs):
+    """start [batch + 1], len [batch] and pages [batch, max_pages] (int32), and the number of pages."""
+    page = case["page"]
+    need = [-(-ln // page) for _, ln in seqs]
+    total, most = max(1, sum(need)), max(1, max(need))
+    g = torch.Generator()
+    g.manual_seed(int(seed) * 64 + 6)
+    ids = torch.randperm(total, generator=g).to(torch.int32)
+    pages = torch.full((len(seqs), most), -1, dtype=torch.int32)
+    at = 0
+    for b, n in enumerate(need):
+        pages[b, :n] = ids[at:at + n]
+        at += n
+    cum = [0]
+    for n, _ in seqs:
+        cum.append(cum[-1] + n)
+    lens = torch.tensor([ln for _, ln in seqs], dtype=torch.int32)
+    return torch.tensor(cum, dtype=torch.int32).cuda(), lens.cuda(), pages.cuda(), total
+
+
+def _whole(lens):
+    """start [batch + 1] of a step whose tokens are all that is cached."""
+    return torch.cat([lens.new_zeros(1), torch.cumsum(lens, 0).to(torch.int32)])
+
+
+class Buffer:
+    """A torch tensor as the binding takes device buffers: address, dtype, shape and size."""
+
+    def __init__(self, t):
+        self.t, self.ptr, self.nbytes, self.shape = t, t.data_ptr(), t.numel() * t.element_size(), tuple(t.shape)
+        self.dtype = np.dtype({torch.float32: np.float32, torch.float16: np.float16, torch.int32: np.int32}[t.dtype])
+
+
+_context = None
+
+
+def context():
+    """One context for the process, as a program keeps one per device."""
+    global _context
+    if _context is None:
+        import arf_amd
+        torch.cuda.init()
+        _context = arf_amd.Context(0)
+    return _context
+
+
+def prepare(case, seed):
+    seqs = _order(case, seed)
+    start, lens, pages, n_pages = _tables(case, seed, seqs)
+    if case["op"] == "read":
+        start = _whole(lens)
+    toks = sum(ln if case["op"] == "read" else n for n, ln in seqs)
+    s = {"case": case, "start": start, "lens": lens, "pages": pages, "tokens": toks}
+    shape = (toks, case["kv_heads"], case["dim"])
+    if case["op"] == "attend":
+        s["q"] = _queries(case, seed)
+    k, v = _cached(case, seed)
+    whole = _whole(lens)
+    if case["op"] == "write":  # this step's rows: each sequence's last, an idle slot's own
+        rows = _new_rows(start, lens, whole, toks)
+        idle = rows < 0
+        s["k"], s["v"] = (torch.where(idle[:, None, None], torch.ones((), device="cuda", dtype=t.dtype), t[rows.clamp(min=0)])
+                          for t in (k, v))
+    if own:
+        import arf_amd
+        ctx = context()
+        s["ctx"], s["kv"] = ctx, ctx.kv_cache(case["kv_heads"], case["dim"], case["page"], n_pages)
+        buf = {n: Buffer(s[n]) for n in ("start", "lens", "pages", "q", "k", "v") if n in s}
+        new_only = case["op"] == "attend" and case["new"] == 1
+        s["buf"], s["seqs"] = buf, arf_amd.KVSeqs(buf["pages"], buf["lens"], None if new_only else buf["start"], toks)
+        t = DTYPE[case["x"]]
+        if case["op"] == "attend":
+            s["out"] = Buffer(torch.empty_like(s["q"]))
+        else:
+            s["out"] = [Buffer(torch.zeros(shape, device="cuda", dtype=t)) for _ in "kv"]
+        if case["op"] != "write":  # the cache as earlier steps left it
+            every = arf_amd.KVSeqs(buf["pages"], buf["lens"], Buffer(whole), k.shape[0])
+            torch.cuda.synchronize()  # the context has a stream of its own
+            ctx.kv_write(s["kv"], every, Buffer(k), Buffer(v))
+    else:
+        d = case["dim"]
+        lead = (n_pages + 1, case["page"], case["kv_heads"])
+        s["kc"], s["vc"] = (torch.zeros(*lead, d // 2, device="cuda", dtype=torch.uint8) for _ in "kv")
+        s["ks"], s["vs"] = (torch.zeros(*lead, d // GROUP, device="cuda", dtype=torch.float16) for _ in "kv")
+        if case["op"] != "write":
+            _write(s, whole, k, v)
+    torch.cuda.synchronize()
+    return s
+
+
+# ---- the plain forms ------------------------------------------------------------------
+
+
+def _new_rows(start, lens, whole, toks):
+    """The row of the cached tokens that each of this step's tokens is; -1 for none."""
+    b, pos = _places(start, lens, toks)
+    return torch.where(pos >= 0, whole[b].long() + pos, -1)
+
+
+def _places(start, lens, toks):
+    """Each token's sequence and its position there."""
+    t = torch.arange(toks, device=start.device, dtype=torch.int32)
+    b = (start[1:, None] <= t).sum(0)
+    return b, (lens[b] - (start[b + 1] - t)).long()
+
+
+def _quantise(x):
+    """Codes (two a byte: value i and i + 16 of a group) and scales of [..., dim]."""
+    g = x.float().reshape(*x.shape[:-1], -1, GROUP)
+    hi, lo = g.amax(-1), g.amin(-1)
+    s = torch.where(hi >= -lo, hi, lo)
+    d = (s / -8).clamp(-8160, 8160).bfloat16().half()
+    wide = d.double()[..., None]
+    q = torch.where(wide == 0, 0.0, torch.round(g.double() / torch.where(wide == 0, 1.0, wide))).clamp(-8, 7)
+    q = (q + 8).to(torch.uint8)
+    return (q[..., :16] | q[..., 16:] << 4).reshape(*x.shape[:-1], -1), d
+
+
+def _values(codes, scales):
+    """[..., dim] in 32 bits."""
+    c = codes.reshape(*scales.shape, 16)
+    q = torch.cat([c & 15, c >> 4], -1).float() - 8
+    return (q * scales.float()[..., None]).reshape(*scales.shape[:-1], -1)
+
+
+def _write(s, start, k, v):
+    b, pos = _places(start, s["lens"], k.shape[0])
+    page = s["case"]["page"]
+    none = pos < 0  # their rows go to a page behind the others
+    at = torch.where(none, s["kc"].shape[0] - 1, s["pages"][b, pos.clamp(min=0) // page].long())
+    off = torch.where(none, 0, pos % page)
+    s["kc"][at, off], s["ks"][at, off] = _quantise(k)
+    s["vc"][at, off], s["vs"][at, off] = _quantise(v)
+
+
+def _read(s, start, toks):
+    """K and V of the step's tokens, zeros where a token has no place."""
+    b, pos = _places(start, s["lens"], toks)
+    page, none = s["case"]["page"], (pos < 0)[:, None, None]
+    pos = pos.clamp(min=0)
+    at, off = s["pages"][b, pos // page].clamp(min=0).long(), pos % page
+    got = (_values(s["kc"][at, off], s["ks"][at, off]), _values(s["vc"][at, off], s["vs"][at, off]))
+    return [t.masked_fill(none, 0.0).to(DTYPE[s["case"]["x"]]) for t in got]
+
+
+def _attend(s):
+    c, q, lens, pages = s["case"], s["q"], s["lens"], s["pages"]
+    toks, heads, dim = q.shape
+    n, kvh = c["batch"], c["kv_heads"]
+    g, new = heads // kvh, c["new"]
+    k, v = (_values(s[x + "c"][pages.clamp(min=0).long()], s[x + "s"][pages.clamp(min=0).long()])
+            .reshape(n, -1, kvh, dim).permute(0, 2, 1, 3) for x in "kv")
+    b, pos = _places(s["start"], lens, toks)
+    row = torch.arange(toks, device=q.device) - s["start"][b]
+    qp = torch.zeros(n, new, heads, dim, device=q.device)
+    qp[b, row] = q.float()
+    at = torch.full((n, new), -1, device=q.device, dtype=torch.long)
+    at[b, row] = pos
+    qp = qp.reshape(n, new, kvh, g, dim).permute(0, 2, 1, 3, 4).reshape(n, kvh, new * g, dim)
+    w = torch.matmul(qp, k.transpose(2, 3).contiguous()) * (1 / math.sqrt(dim))
+    if c["softcap"]:
+        w = c["softcap"] * torch.tanh(w / c["softcap"])
+    j = torch.arange(w.shape[-1], device=q.device)
+    ok = (j < lens[:, None, None]) & (at[:, :, None] >= 0)
+    if c["causal"]:
+        ok = ok & (j <= at[:, :, None])
+    if c["window"]:
+        ok = ok & (j > at[:, :, None] - c["window"])
+    ok = ok[:, None, :, None].expand(n, kvh, new, g, -1).reshape(n, kvh, new * g, -1)
+    w = w.masked_fill_(~ok, -math.inf)
+    top = w.amax(-1, keepdim=True)
+    p = w.sub_(torch.where(torch.isfinite(top), top, 0.0)).exp_()
+    total = p.sum(-1, keepdim=True)
+    o = torch.matmul(p, v.contiguous()) / torch.where(total == 0, 1.0, total)
+    o = o.reshape(n, kvh, new, g, dim).permute(0, 2, 1, 3, 4).reshape(n, new, heads, dim)
+    return o[b, row].to(q.dtype)
+
+
+def run(s):
+    c = s["case"]
+    if own:
+        ctx, kv, seqs, buf = s["ctx"], s["kv"], s["seqs"], s["buf"]
+        if c["op"] == "attend":
+            ctx.kv_attention(kv, seqs, buf["q"], s["out"], c["q_heads"], 1 / math.sqrt(c["dim"]), window=c["window"],
+                             softcap=c["softcap"], causal=c["causal"])
+            return s["out"].t
+        if c["op"] == "write":
+            ctx.kv_write(kv, seqs, buf["k"], buf["v"])
+        ctx.kv_read(kv, seqs, s["out"][0], s["out"][1])
+        return {"k": s["out"][0].t, "v": s["out"][1].t}
+    if c["op"] == "attend":
+        return _attend(s)
+    if c["op"] == "write":
+        _write(s, s["start"], s["k"], s["v"])
+    k, v = _read(s, s["start"], s["tokens"])
+    return {"k": k, "v": v}
+
+
+# ---- the same in 64 bits --------------------------------------------------------------
+
+
+def _stored(x):
+    """What the cache holds for x, from the definition."""
+    g = x.double().unflatten(-1, (-1, GROUP))
+    top, low = g.max(-1).values, g.min(-1).values
+    s = torch.where(top + low >= 0, top, low)
+    m, e = torch.frexp(torch.clamp(-s / 8, -8160, 8160))
+    two = (e.long() - 8 + 1023).bitwise_left_shift(52).view(torch.float64)  # 2^(e - 8), to the bit
+    d = torch.round(m * 256) * two  # 8 significant bits
+    d = torch.where(d.abs() < 2.0 ** -14, torch.round(d * 2.0 ** 24) * 2.0 ** -24, d)[..., None]
+    q = torch.clamp(torch.round(torch.nan_to_num(g / d, nan=0.0, posinf=0.0, neginf=0.0)), -8, 7)
+    return (q * d).flatten(-2)
+
+
+def exact(case, seed):
+    seqs = _order(case, seed)
+    k, v = _cached(case, seed)
+    ends, at = [], 0
+    for _, ln in seqs:
+        at += ln
+        ends.append(at)
+    if case["op"] != "attend":
+        out = []
+        for x in (k, v):
+            rows = []
+            for (n, ln), e in zip(seqs, ends):
+                want = ln if case["op"] == "read" else n
+                have = min(want, ln)
+                rows += [torch.zeros(want - have, *x.shape[1:], device="cuda", dtype=torch.float64), _stored(x[e - have:e])]
+            out.append(torch.cat(rows))
+        return {"k": out[0], "v": out[1]}
+    q = _queries(case, seed).double()
+    kvh, dim = case["kv_heads"], case["dim"]
+    g, out, t = case["q_heads"] // kvh, [], 0
+    for (n, ln), e in zip(seqs, ends):
+        x = q[t:t + n].reshape(n, kvh, g, dim)
+        t += n
+        o = torch.zeros_like(x)
+        if ln:
+            pos = torch.arange(ln - n, ln, device="cuda")[:, None, None]
+            j = torch.arange(ln, device="cuda")
+            no = (j > pos) if case["causal"] else (j < 0) | (pos < -ln)
+            if case["window"]:
+                no = no | (j <= pos - case["window"])
+            for h in range(kvh):
+                ks, vs = _stored(k[e - ln:e, h]), _stored(v[e - ln:e, h])
+                w = (x[:, h].reshape(n * g, dim) @ ks.t()).reshape(n, g, ln) / math.sqrt(dim)
+                if case["softcap"]:
+                    w = case["softcap"] * torch.tanh(w / case["softcap"])
+                p = torch.softmax(w.masked_fill(no, -math.inf), -1).nan_to_num(0.0)
+                o[:, h] = (p.reshape(n * g, ln) @ vs).reshape(n, g, dim)
+        out.append(o.reshape(n, kvh * g, dim))
+    return torch.cat(out)
