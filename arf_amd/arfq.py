@@ -103,6 +103,15 @@ _SIGS = {
     "arfq_matmul_repeat": (_int, [_vp, ctypes.POINTER(_vp), _int, _int, _i64, _vp, _int, _vp]),
     "arfq_ffn": (_int, [_vp, _vp, _vp, _vp, _i64, _vp, _vp]),
     "arfq_ffn_act": (_int, [_vp, _vp, _vp, _vp, _i64, _vp, _vp, _int]),
+    "arfq_kv_create": (_int, [_vp, _int, _int, _int, _i64, ctypes.POINTER(_vp)]),
+    "arfq_kv_free": (_int, [_vp]),
+    "arfq_kv_info": (_int, [_vp, ctypes.POINTER(_int), ctypes.POINTER(_int), ctypes.POINTER(_int),
+                            ctypes.POINTER(_i64), ctypes.POINTER(ctypes.c_size_t)]),
+    "arfq_kv_write": (_int, [_vp, _vp, _vp, _vp, _i64, _vp, _i64, _int]),
+    "arfq_kv_read": (_int, [_vp, _vp, _vp, _vp, _i64, _vp, _i64, _int]),
+    "arfq_kv_attention": (_int, [_vp, _vp, _vp, _int, _vp, _i64, _int, _vp, _i64, _int, ctypes.c_float,
+                                 ctypes.c_float, _i64, _int, _vp, ctypes.c_size_t]),
+    "arfq_kv_attention_workspace": (_int, [_vp, _vp, _i64, _i64, _int, ctypes.POINTER(ctypes.c_size_t)]),
     "arfq_gguf_is_gguf": (_int, [ctypes.c_char_p]),
     "arfq_gguf_open": (_int, [ctypes.c_char_p, ctypes.POINTER(_vp)]),
     "arfq_gguf_close": (_int, [_vp]),
@@ -183,6 +192,11 @@ class DeviceArray:
                load_library().arfq_copy_d2h(self.ctx.handle, out.ctypes.data, self.ptr, self.nbytes))
         return out
 
+    def columns(self, first):
+        """The array from element `first` of its first row on, as rows at this one's stride: the k or v
+        columns of a fused qkv product (pass the stride to the call that takes it)."""
+        return DeviceColumns(self, int(first))
+
     def free(self):
         if self.ptr:
             load_library().arfq_dev_free(self.ctx.handle, self.ptr)
@@ -194,6 +208,16 @@ class DeviceArray:
                 self.free()
         except Exception:
             pass
+
+
+class DeviceColumns:
+    """Part of a DeviceArray, from element `first` on; it keeps the array, and does not own the memory."""
+
+    def __init__(self, base, first):
+        if not 0 <= first * base.dtype.itemsize <= base.nbytes:
+            raise ValueError(f"columns: element {first} is not in the array")
+        self.base, self.dtype = base, base.dtype
+        self.ptr, self.nbytes = base.ptr + first * base.dtype.itemsize, base.nbytes - first * base.dtype.itemsize
 
 
 class Weight:
@@ -224,13 +248,85 @@ class Weight:
             pass
 
 
-class Context:
-    """One HIP device + one stream (GpuContext + CommandPass)."""
+class _KVSeqsStruct(ctypes.Structure):
+    """arfq_kv_seqs"""
+    _fields_ = [("batch", _i64), ("tokens", _i64), ("start", _vp), ("len", _vp), ("pages", _vp), ("max_pages", _i64)]
 
-    def __init__(self, device=0):
+
+class KVSeqs:
+    """A step's batch (arfq_kv_seqs): `pages` [batch, max_pages] and `lens` [batch], int32 device
+    arrays; the step's `tokens` rows `start[b]` .. `start[b + 1] - 1` are sequence b's last tokens
+    (start None: row b is sequence b's last token).  Keeps its arrays; build it once and change
+    their contents from step to step."""
+
+    def __init__(self, pages, lens, start=None, tokens=None):
+        if any(a is not None and a.dtype != np.int32 for a in (pages, lens, start)):
+            raise ValueError("KVSeqs: pages, lens and start are int32")
+        if len(pages.shape) != 2 or tuple(lens.shape) != (pages.shape[0],):
+            raise ValueError("KVSeqs: want pages [batch, max_pages] and lens [batch]")
+        batch = int(pages.shape[0])
+        if start is not None and tuple(start.shape) != (batch + 1,):
+            raise ValueError("KVSeqs: want start [batch + 1]")
+        if tokens is None:
+            if start is not None:
+                raise ValueError("KVSeqs: tokens (the rows of the step) goes with start")
+            tokens = batch
+        self.pages, self.lens, self.start, self.batch, self.tokens = pages, lens, start, batch, int(tokens)
+        self.struct = _KVSeqsStruct(batch, self.tokens, None if start is None else start.ptr, lens.ptr, pages.ptr,
+                                    int(pages.shape[1]))
+        self.ref = ctypes.addressof(self.struct)
+
+
+class KVCache:
+    """A 4-bit K/V cache of one layer: n_pages pages of page_size tokens, `heads` K/V heads."""
+
+    def __init__(self, ctx, handle, heads, head_dim, page_size, n_pages):
+        self.ctx, self.handle = ctx, handle
+        self.heads, self.head_dim, self.page_size, self.n_pages = heads, head_dim, page_size, n_pages
+
+    @property
+    def bytes_num(self):
+        sz = ctypes.c_size_t()
+        _check(self.ctx.handle, load_library().arfq_kv_info(self.handle, None, None, None, None, ctypes.byref(sz)))
+        return sz.value
+
+    def free(self):
+        if self.handle:
+            load_library().arfq_kv_free(self.handle)
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.free()
+        except Exception:
+            pass
+
+
+def _float_type(a, what):
+    """DType of a device array's elements."""
+    if a.dtype == np.float32:
+        return 0
+    if a.dtype == np.float16:
+        return 1
+    raise ValueError(f"{what}: dtype {a.dtype} (want f32 or f16)")
+
+
+def _row_stride(a, tokens, width, stride, what):
+    """Elements from one token of `a` to the next: `stride`, or the packed width; checked against a's size."""
+    stride = width if stride is None else int(stride)
+    if tokens > 0 and (stride < width or a.nbytes < ((tokens - 1) * stride + width) * a.dtype.itemsize):
+        raise ValueError(f"{what}: {a.nbytes} bytes do not hold {tokens} rows of {width} at a stride of {stride}")
+    return stride
+
+
+class Context:
+    """One HIP device + one stream (GpuContext + CommandPass): the context's own, or the hipStream_t
+    `stream` (an address), which the caller keeps until the context is closed."""
+
+    def __init__(self, device=0, stream=None):
         L = load_library()
         h = ctypes.c_void_p()
-        st = L.arfq_ctx_create(int(device), None, ctypes.byref(h))
+        st = L.arfq_ctx_create(int(device), stream, ctypes.byref(h))
         if st != ARFQ_OK:
             raise ArfqError(st, (L.arfq_last_error(None) or b"").decode())
         self.handle = h.value
@@ -333,6 +429,50 @@ class Context:
         fn = load_library().arfq_moe_ids_add if accumulate else load_library().arfq_moe_ids
         _check(self.handle, fn(self.handle, gate.handle, up.handle, down.handle, ids.ptr, weights.ptr,
                                int(tokens), int(top_k), x.ptr, int(xd), y.ptr))
+
+    # -- K/V cache --
+    def kv_cache(self, heads, head_dim, page_size, n_pages):
+        """A 4-bit K/V cache (arfq_kv_create)."""
+        h = ctypes.c_void_p()
+        _check(self.handle, load_library().arfq_kv_create(self.handle, int(heads), int(head_dim), int(page_size),
+                                                          int(n_pages), ctypes.byref(h)))
+        return KVCache(self, h.value, int(heads), int(head_dim), int(page_size), int(n_pages))
+
+    def _kv_pair(self, kv, seqs, k, v, k_stride, v_stride, what):
+        t = _float_type(k, what)
+        if _float_type(v, what) != t:
+            raise ValueError(f"{what}: k and v differ in dtype")
+        w = kv.heads * kv.head_dim
+        return (_row_stride(k, seqs.tokens, w, k_stride, what), _row_stride(v, seqs.tokens, w, v_stride, what), t)
+
+    def kv_write(self, kv, seqs, k, v, k_stride=None, v_stride=None):
+        """Quantise the step's rows k, v [tokens, heads, head_dim] into the cache (arfq_kv_write)."""
+        ks, vs, t = self._kv_pair(kv, seqs, k, v, k_stride, v_stride, "kv_write")
+        _check(self.handle, _lib.arfq_kv_write(self.handle, kv.handle, seqs.ref, k.ptr, ks, v.ptr, vs, t))
+
+    def kv_read(self, kv, seqs, k, v, k_stride=None, v_stride=None):
+        """The step's rows back into k, v (arfq_kv_read)."""
+        ks, vs, t = self._kv_pair(kv, seqs, k, v, k_stride, v_stride, "kv_read")
+        _check(self.handle, _lib.arfq_kv_read(self.handle, kv.handle, seqs.ref, k.ptr, ks, v.ptr, vs, t))
+
+    def kv_attention(self, kv, seqs, q, out, q_heads, scale, window=0, softcap=0.0, causal=True, q_stride=None,
+                     out_stride=None, workspace=None):
+        """out [tokens, q_heads, head_dim] = attention of q over the cache (arfq_kv_attention); `workspace`:
+        a device array of kv_attention_workspace bytes, which a call under stream capture needs."""
+        w = q_heads * kv.head_dim
+        qs = _row_stride(q, seqs.tokens, w, q_stride, "kv_attention: q")
+        os_ = _row_stride(out, seqs.tokens, w, out_stride, "kv_attention: out")
+        ws = (None, 0) if workspace is None else (workspace.ptr, workspace.nbytes)
+        _check(self.handle, _lib.arfq_kv_attention(
+            self.handle, kv.handle, seqs.ref, q_heads, q.ptr, qs, _float_type(q, "kv_attention: q"), out.ptr, os_,
+            _float_type(out, "kv_attention: out"), scale, softcap, window, causal, ws[0], ws[1]))
+
+    def kv_attention_workspace(self, kv, batch, tokens, q_heads):
+        """Bytes of kv_attention's workspace (arfq_kv_attention_workspace)."""
+        sz = ctypes.c_size_t()
+        _check(self.handle, load_library().arfq_kv_attention_workspace(self.handle, kv.handle, int(batch), int(tokens),
+                                                                       int(q_heads), ctypes.byref(sz)))
+        return sz.value
 
     def copy_d2d(self, dst, src, nbytes=None):
         """Enqueue dst <- src (device arrays) on the context's stream."""

@@ -9,6 +9,7 @@
 
 #include "arfq_common.h"
 #include "arfq_internal.h"
+#include "arfq_kv.h"
 
 #include <algorithm>
 #include <cmath>
@@ -443,6 +444,198 @@ int arfq_matmul_repeat(arfq_ctx *ctx, const arfq_weight *const *ws, int n_ws, in
     for (int i = 0; i < iters; i++)
         if (int rc = matmul_enqueue(ctx, ws[i % n_ws], 0, m, x, x_dtype, y)) return rc;
     return ARFQ_OK;
+}
+
+// --------------------------------------------------- 4-bit K/V cache, attention ----
+
+int arfq_kv_create(arfq_ctx *ctx, int heads, int head_dim, int page_size, int64_t n_pages, arfq_kv **out) {
+    if (!ctx) return ARFQ_E_INVALID;
+    if (!out) return fail(ctx, ARFQ_E_INVALID, "kv_create: out is NULL");
+    *out = nullptr;
+    if (heads < 1 || heads > arfq::KV_HEADS_MAX) return fail(ctx, ARFQ_E_SHAPE, "kv_create: heads must be in [1, 1024]");
+    if (head_dim < 1) return fail(ctx, ARFQ_E_SHAPE, "kv_create: head_dim must be positive");
+    if (!arfq::attn_dim_ok(head_dim))
+        return fail(ctx, ARFQ_E_UNSUPPORTED, "kv_create: head_dim must be 64, 96, 128 or 256");
+    if (page_size < arfq::KV_TILE || page_size > arfq::KV_PAGE_MAX || page_size % arfq::KV_TILE)
+        return fail(ctx, ARFQ_E_SHAPE, "kv_create: page_size must be a multiple of 16 up to 256");
+    if (n_pages < 1 || n_pages > INT32_MAX) return fail(ctx, ARFQ_E_SHAPE, "kv_create: n_pages must be in [1, 2^31 - 1]");
+    if (int rc = use_device(ctx)) return rc;
+    arfq_kv *kv = new (std::nothrow) arfq_kv();
+    if (!kv) return fail(ctx, ARFQ_E_NOMEM, "kv_create: host allocation");
+    kv->device = ctx->device;
+    kv->heads = heads;
+    kv->dim = head_dim;
+    kv->page = page_size;
+    kv->pages = n_pages;
+    kv->bytes = (size_t)n_pages * heads * (size_t)arfq::kv_layout(page_size, head_dim).region;
+    hipError_t e = hipMalloc(&kv->data, kv->bytes);
+    if (e != hipSuccess) {
+        (void)hipGetLastError();
+        delete kv;
+        return fail(ctx, ARFQ_E_NOMEM, std::string("kv_create: hipMalloc: ") + hipGetErrorString(e));
+    }
+    // cleared: a tile's keys past a sequence's end are multiplied by p = 0, and stay finite
+    e = hipMemsetAsync(kv->data, 0, kv->bytes, ctx->stream);
+    if (e == hipSuccess) e = hipStreamSynchronize(ctx->stream);
+    if (e != hipSuccess) {
+        arfq_kv_free(kv);
+        return hip_fail(ctx, e, "kv_create: clear");
+    }
+    *out = kv;
+    return ARFQ_OK;
+}
+
+int arfq_kv_free(arfq_kv *kv) {
+    if (!kv) return ARFQ_E_INVALID;
+    (void)hipSetDevice(kv->device);
+    if (kv->data) (void)hipFree(kv->data);
+    delete kv;
+    return ARFQ_OK;
+}
+
+int arfq_kv_info(const arfq_kv *kv, int *heads, int *head_dim, int *page_size, int64_t *n_pages, size_t *device_bytes) {
+    if (!kv) return ARFQ_E_INVALID;
+    if (heads) *heads = kv->heads;
+    if (head_dim) *head_dim = kv->dim;
+    if (page_size) *page_size = kv->page;
+    if (n_pages) *n_pages = kv->pages;
+    if (device_bytes) *device_bytes = kv->bytes;
+    return ARFQ_OK;
+}
+
+// The cache and batch of a call: checks, and the kernels' form of them.
+static int kv_args(arfq_ctx *ctx, const arfq_kv *kv, const arfq_kv_seqs *s, const char *what, arfq::KvArgs *a) {
+    const std::string w = std::string(what) + ": ";
+    if (!kv || !s) return fail(ctx, ARFQ_E_INVALID, w + "null argument");
+    if (kv->device != ctx->device) return fail(ctx, ARFQ_E_INVALID, w + "the cache is on another device than the context");
+    if (s->batch < 0 || s->tokens < 0 || s->max_pages < 0) return fail(ctx, ARFQ_E_SHAPE, w + "negative size");
+    if (s->batch > (int64_t)1 << 24 || s->max_pages > arfq::KV_KEYS_MAX / kv->page)
+        return fail(ctx, ARFQ_E_SHAPE, w + "batch above 2^24, or max_pages * page_size above 2^29");
+    if (s->tokens > arfq::KV_ROWS_MAX / kv->heads) return fail(ctx, ARFQ_E_SHAPE, w + "tokens * heads above 2^30");
+    if (!s->start && s->tokens > s->batch) return fail(ctx, ARFQ_E_SHAPE, w + "more rows than sequences, and no start");
+    if (s->tokens > 0 && s->batch > 0 && (!s->len || (s->max_pages > 0 && !s->pages)))
+        return fail(ctx, ARFQ_E_INVALID, w + "null len or pages");
+    const arfq::KvLayout l = arfq::kv_layout(kv->page, kv->dim);
+    a->data = kv->data;
+    a->region = l.region;
+    a->off_v = l.off_v;
+    a->off_ks = l.off_ks;
+    a->off_vs = l.off_vs;
+    a->heads = kv->heads;
+    a->page = kv->page;
+    a->tiles = kv->page / arfq::KV_TILE;
+    a->tile_magic = a->tiles > 1 ? (uint32_t)((((uint64_t)1 << 32) + a->tiles - 1) / a->tiles) : 0;
+    a->n_pages = (int)kv->pages;
+    a->batch = (int)s->batch;
+    a->tokens = (int)s->tokens;
+    a->start = s->start;
+    a->len = s->len;
+    a->table = s->pages;
+    a->max_pages = s->max_pages;
+    return ARFQ_OK;
+}
+
+// A [tokens, heads, dim] array of a call.
+static int kv_rows(arfq_ctx *ctx, const char *what, const void *p, int64_t stride, int64_t heads, int dim, int dtype) {
+    const std::string w = std::string(what) + ": ";
+    if (dtype != ARFQ_F32 && dtype != ARFQ_F16) return fail(ctx, ARFQ_E_INVALID, w + "unknown dtype");
+    if (!p) return fail(ctx, ARFQ_E_INVALID, w + "null argument");
+    if (stride < heads * dim || stride > (int64_t)1 << 40)
+        return fail(ctx, ARFQ_E_SHAPE, w + "token stride " + std::to_string(stride) + " below heads * head_dim = " +
+                                           std::to_string(heads * dim) + ", or above 2^40");
+    if ((uintptr_t)p % 16 || stride % (dtype == ARFQ_F16 ? 8 : 4))
+        return fail(ctx, ARFQ_E_INVALID, w + "pointers and token strides must be multiples of 16 bytes");
+    return ARFQ_OK;
+}
+
+int arfq_kv_write(arfq_ctx *ctx, arfq_kv *kv, const arfq_kv_seqs *seqs, const void *k, int64_t k_stride,
+                  const void *v, int64_t v_stride, int dtype) {
+    if (!ctx) return ARFQ_E_INVALID;
+    arfq::KvArgs a;
+    if (int rc = kv_args(ctx, kv, seqs, "kv_write", &a)) return rc;
+    if (a.tokens == 0 || a.batch == 0) return ARFQ_OK;
+    if (int rc = kv_rows(ctx, "kv_write: k", k, k_stride, kv->heads, kv->dim, dtype)) return rc;
+    if (int rc = kv_rows(ctx, "kv_write: v", v, v_stride, kv->heads, kv->dim, dtype)) return rc;
+    if (int rc = use_device(ctx)) return rc;
+    const hipError_t e = arfq::launch_kv_write(a, kv->dim, k, k_stride, v, v_stride, dtype, ctx->stream);
+    return e == hipSuccess ? ARFQ_OK : hip_fail(ctx, e, "kv_write launch");
+}
+
+int arfq_kv_read(arfq_ctx *ctx, const arfq_kv *kv, const arfq_kv_seqs *seqs, void *k, int64_t k_stride, void *v,
+                 int64_t v_stride, int dtype) {
+    if (!ctx) return ARFQ_E_INVALID;
+    arfq::KvArgs a;
+    if (int rc = kv_args(ctx, kv, seqs, "kv_read", &a)) return rc;
+    if (a.tokens == 0 || a.batch == 0) return ARFQ_OK;
+    if (int rc = kv_rows(ctx, "kv_read: k", k, k_stride, kv->heads, kv->dim, dtype)) return rc;
+    if (int rc = kv_rows(ctx, "kv_read: v", v, v_stride, kv->heads, kv->dim, dtype)) return rc;
+    if (int rc = use_device(ctx)) return rc;
+    const hipError_t e = arfq::launch_kv_read(a, kv->dim, k, k_stride, v, v_stride, dtype, ctx->stream);
+    return e == hipSuccess ? ARFQ_OK : hip_fail(ctx, e, "kv_read launch");
+}
+
+static int kv_q_heads(arfq_ctx *ctx, const arfq_kv *kv, int64_t batch, int64_t tokens, int q_heads) {
+    if (!kv) return fail(ctx, ARFQ_E_INVALID, "kv_attention: null argument");
+    if (q_heads < 1 || q_heads % kv->heads)
+        return fail(ctx, ARFQ_E_SHAPE, "kv_attention: q_heads must be a multiple of the cache's heads");
+    if (batch < 0 || batch > (int64_t)1 << 24 || tokens < 0 || tokens > arfq::KV_ROWS_MAX / q_heads)
+        return fail(ctx, ARFQ_E_SHAPE, "kv_attention: batch above 2^24, or tokens * q_heads above 2^30");
+    return ARFQ_OK;
+}
+
+int arfq_kv_attention_workspace(arfq_ctx *ctx, const arfq_kv *kv, int64_t batch, int64_t tokens, int q_heads,
+                                size_t *bytes) {
+    if (!ctx) return ARFQ_E_INVALID;
+    if (!bytes) return fail(ctx, ARFQ_E_INVALID, "kv_attention_workspace: null argument");
+    if (int rc = kv_q_heads(ctx, kv, batch, tokens, q_heads)) return rc;
+    *bytes = arfq::attn_plan(ctx->cus, kv->heads, kv->dim, batch, tokens, q_heads).ws_bytes;
+    return ARFQ_OK;
+}
+
+int arfq_kv_attention(arfq_ctx *ctx, const arfq_kv *kv, const arfq_kv_seqs *seqs, int q_heads, const void *q,
+                      int64_t q_stride, int q_dtype, void *out, int64_t out_stride, int out_dtype, float scale,
+                      float softcap, int64_t window, int causal, void *workspace, size_t workspace_bytes) {
+    if (!ctx) return ARFQ_E_INVALID;
+    arfq::AttnArgs a;
+    if (int rc = kv_args(ctx, kv, seqs, "kv_attention", &a.c)) return rc;
+    if (int rc = kv_q_heads(ctx, kv, seqs->batch, seqs->tokens, q_heads)) return rc;
+    if (!std::isfinite(scale) || !std::isfinite(softcap) || softcap < 0.0f)
+        return fail(ctx, ARFQ_E_INVALID, "kv_attention: scale and softcap must be finite, softcap not negative");
+    if (window < 0) return fail(ctx, ARFQ_E_SHAPE, "kv_attention: negative window");
+    if (a.c.tokens == 0 || a.c.batch == 0) return ARFQ_OK;
+    if (int rc = kv_rows(ctx, "kv_attention: q", q, q_stride, q_heads, kv->dim, q_dtype)) return rc;
+    if (int rc = kv_rows(ctx, "kv_attention: out", out, out_stride, q_heads, kv->dim, out_dtype)) return rc;
+    if (int rc = use_device(ctx)) return rc;
+    const arfq::AttnPlan plan = arfq::attn_plan(ctx->cus, kv->heads, kv->dim, seqs->batch, seqs->tokens, q_heads);
+    if (workspace) {
+        if (workspace_bytes < plan.ws_bytes || (uintptr_t)workspace % 16)
+            return fail(ctx, ARFQ_E_SHAPE, "kv_attention: workspace of " + std::to_string(workspace_bytes) + " bytes, " +
+                                               std::to_string(plan.ws_bytes) + " (16-byte aligned) are wanted");
+    } else {
+        hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
+        HIP_TRY(ctx, hipStreamIsCapturing(ctx->stream, &cap));
+        if (cap != hipStreamCaptureStatusNone)
+            return fail(ctx, ARFQ_E_INVALID, "kv_attention: a call under stream capture needs a workspace");
+        if (int rc = ensure_scratch(ctx, plan.ws_bytes)) return rc;
+        workspace = ctx->scratch;
+    }
+    a.q = q;
+    a.out = out;
+    a.q_stride = q_stride;
+    a.out_stride = out_stride;
+    a.q_dtype = q_dtype;
+    a.out_dtype = out_dtype;
+    a.q_heads = q_heads;
+    a.group = q_heads / kv->heads;
+    a.scale = scale;
+    a.softcap = softcap;
+    a.window = (int)std::min<int64_t>(window, INT32_MAX);
+    a.causal = causal != 0;
+    a.target = plan.target;
+    a.slots = plan.slots;
+    a.part = (float *)workspace;
+    const hipError_t e = arfq::launch_attn(a, kv->dim, ctx->stream);
+    return e == hipSuccess ? ARFQ_OK : hip_fail(ctx, e, "kv_attention launch");
 }
 
 // -------------------------------------------------------------------- MoE ----

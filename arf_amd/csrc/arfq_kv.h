@@ -1,0 +1,111 @@
+// arfq_kv.h -- the 4-bit K/V cache: its layout in device memory, the batch description
+// its kernels share and their launchers.
+//
+// A row (one token's K or V of one head, D = 32 NG values) is held as NG groups of a scale
+// and 32 codes: d (f16, at most 8 significant bits) and q in [-8, 7], worth d * q.  8 bits
+// times q's 3 (or a power of two) are at most 11: d * q is an f16 exactly, so MFMA operands
+// made from the cache carry no rounding.
+//
+// Memory: pages of P tokens (P a multiple of 16), in each page one contiguous region per
+// head, [K codes | V codes | K scales | V scales], shaped as the attention kernels' matrix
+// operands, so that those load them into registers with no shuffle:
+//   K codes   [P][4][NG] dwords.  Dword (key, h, g) holds values 32g+8h .. +7 of the row, code
+//             + 8 of value e in nibble (e >> 1) + 4 * (e & 1): nibbles p and p + 4 are
+//             neighbours, which one mask turns into a pair of f16.
+//   V codes   [P / 4][16][4][NG] bytes.  Byte (b, c, key % 4, g) holds values 32g+c (low
+//             nibble) and 32g+16+c: NG dwords have four keys of a matrix row.
+//   K scales  [P][NG] f16;  V scales [P / 4][NG][4] f16 (a dword is a pair of keys).
+#pragma once
+#include "arfq_common.h"
+#include "arfq_internal.h"
+
+struct arfq_kv {
+    int device = 0;
+    int heads = 0, dim = 0, page = 0;
+    int64_t pages = 0;
+    uint8_t *data = nullptr;  // pages * heads regions
+    size_t bytes = 0;
+};
+
+namespace arfq {
+
+constexpr int KV_GROUP = 32;
+constexpr int KV_PAGE_MAX = 256;
+constexpr int KV_TILE = 16;  // keys that share a page: P is a multiple
+constexpr int64_t KV_KEYS_MAX = (int64_t)1 << 29;    // of a sequence (max_pages * P)
+constexpr int64_t KV_ROWS_MAX = (int64_t)1 << 30;    // tokens * heads of a call
+constexpr int KV_HEADS_MAX = 1024;
+
+// byte offsets within a (page, head) region
+struct KvLayout {
+    int64_t region;       // bytes of a (page, head) region
+    int off_v, off_ks, off_vs;
+};
+inline KvLayout kv_layout(int page, int dim) {
+    const int codes = page * dim / 2, scales = page * (dim / KV_GROUP) * 2;
+    return {2 * ((int64_t)codes + scales), codes, 2 * codes, 2 * codes + scales};
+}
+
+// What every kernel of the cache takes: the cache and the batch.
+struct KvArgs {
+    uint8_t *data;
+    int64_t region;
+    int off_v, off_ks, off_vs;
+    int heads, page, tiles;  // tiles = page / KV_TILE
+    uint32_t tile_magic;     // ceil(2^32 / tiles) (tiles > 1)
+    int n_pages;
+    // the batch
+    int batch, tokens;
+    const int32_t *start, *len, *table;
+    int64_t max_pages;
+};
+
+// Page of 16-key tile `t` of a sequence.  t < 2^27 (32-bit positions), tiles <= 16: the product
+// with the rounded-up reciprocal is off by less than t * tiles / 2^32 < 1/2 of a step.
+__device__ __forceinline__ int kv_page_of(const KvArgs &a, int t) {
+    return a.tiles == 1 ? t : (int)__umulhi((uint32_t)t, a.tile_magic);
+}
+
+// First token and token count of sequence b (0 tokens where `start` does not increase or
+// leaves the batch's rows: such entries reach no memory).
+__device__ __forceinline__ void kv_seq(const KvArgs &a, int b, int &t0, int &n) {
+    if (!a.start) {
+        t0 = b;
+        n = b < a.tokens ? 1 : 0;
+        return;
+    }
+    t0 = a.start[b];
+    const int t1 = a.start[b + 1];
+    n = t0 >= 0 && t1 > t0 && t1 <= a.tokens ? t1 - t0 : 0;
+}
+
+hipError_t launch_kv_write(const KvArgs &a, int dim, const void *k, int64_t k_stride, const void *v, int64_t v_stride,
+                           int dtype, hipStream_t s);
+hipError_t launch_kv_read(const KvArgs &a, int dim, void *k, int64_t k_stride, void *v, int64_t v_stride, int dtype,
+                          hipStream_t s);
+
+// ---- attention (arfq_attn.hip) ----
+struct AttnArgs {
+    KvArgs c;
+    const void *q;
+    void *out;
+    int64_t q_stride, out_stride;  // elements between tokens
+    int q_dtype, out_dtype;
+    int q_heads, group;  // group = q_heads / heads
+    float scale, softcap;
+    int window;          // 0: none
+    int causal;
+    // the work list: see attn_plan
+    int target, slots;
+    float *part;         // partials, [slots][heads][16][dim + 2]
+};
+struct AttnPlan {
+    int target = 1;     // pieces per head the keys are cut into, beside one per row tile
+    int slots = 1;      // bound on the work items per head
+    size_t ws_bytes = 0;
+};
+bool attn_dim_ok(int dim);
+AttnPlan attn_plan(int cus, int heads, int dim, int64_t batch, int64_t tokens, int q_heads);
+hipError_t launch_attn(const AttnArgs &a, int dim, hipStream_t s);
+
+}  // namespace arfq

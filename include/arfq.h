@@ -298,6 +298,81 @@ int arfq_ffn_act(arfq_ctx *ctx, const arfq_weight *gate, const arfq_weight *up, 
 int arfq_ffn(arfq_ctx *ctx, const arfq_weight *gate, const arfq_weight *up, const arfq_weight *down,
              int64_t m, const float *x, float *y);
 
+/* ---- 4-bit K/V cache and attention over it ---------------------------------
+ * A paged cache of keys and values, one per layer.  A row (the K or the V of one token and
+ * head, head_dim values) is held in groups of 32: a scale d and 32 codes q in [-8, 7] that
+ * stand for d * q, GGUF's Q4_0 values with a scale of 8 significant bits (4.5 bits a value).
+ * With s the group's value of largest magnitude (the positive one of two alike),
+ *     d = s / -8 rounded to 8 significant bits (ties to even) and to f16,
+ *     q = x / d rounded to the nearest integer (ties to even), at most 7.
+ * Every d * q is an f16, so what attention multiplies is what arfq_kv_read returns, to the bit.
+ * Finite values beyond +-65280 are held as that.  A row of K or V with a NaN or an infinity
+ * makes that token's key of that head NaN (K reads back as NaN, and a query row that attends
+ * to it gives NaN) and each group of V with one zero.
+ * Memory is allocated and cleared by arfq_kv_create, and reached through page tables: page p
+ * has the same `page_size` tokens of every head.
+ * The reference keeps K/V in f32 or 8 bits in a paged cache and attends with split-K
+ * flash-decoding kernels (crates/arf-core/src/cache, shaders/wgsl/attention_splitk*.wgsl). */
+typedef struct arfq_kv arfq_kv;
+
+/* heads: K/V heads (1..1024); head_dim: 64, 96, 128 or 256 (others: ARFQ_E_UNSUPPORTED);
+ * page_size: a multiple of 16 up to 256; n_pages: pages of the cache (1..2^31 - 1). */
+int arfq_kv_create(arfq_ctx *ctx, int heads, int head_dim, int page_size, int64_t n_pages, arfq_kv **out);
+int arfq_kv_free(arfq_kv *kv);
+/* Any out-pointer may be NULL. */
+int arfq_kv_info(const arfq_kv *kv, int *heads, int *head_dim, int *page_size, int64_t *n_pages, size_t *device_bytes);
+
+/* A step's batch, as the three calls below take it (a host struct; its arrays are on the
+ * device, int32, and read when the work runs: a captured graph sees their values at each
+ * replay).  Sequence b has len[b] tokens, its page i is pages[b * max_pages + i] (tokens
+ * i * page_size ..), and the step's rows start[b] .. start[b + 1] - 1 are its LAST tokens: row t
+ * is at position len[b] - (start[b + 1] - t).  start NULL: row b is sequence b's last token.
+ * Rows of no sequence, rows at a negative position (an idle slot: len 0) and keys of a page
+ * id outside [0, n_pages), or past max_pages, name nothing: they are not written or read,
+ * and not attended to.  start must not decrease; a sequence for which it does, or whose rows
+ * leave [0, tokens), has no rows. */
+typedef struct {
+    int64_t batch;        /* sequences */
+    int64_t tokens;       /* rows of k, v, q and out */
+    const int32_t *start; /* [batch + 1], or NULL (tokens <= batch) */
+    const int32_t *len;   /* [batch] */
+    const int32_t *pages; /* [batch, max_pages] */
+    int64_t max_pages;    /* max_pages * page_size <= 2^29 */
+} arfq_kv_seqs;
+
+/* Quantise the rows of k and v [tokens, heads, head_dim] (device, f32 or f16) into the cache.
+ * Rows of a token are contiguous; k_stride and v_stride are the elements from one token to the next
+ * (heads * head_dim when packed; larger for the columns of a fused qkv product).  Pointers
+ * and strides must be multiples of 16 bytes.  Two rows of a call that name the same place leave
+ * it undefined. */
+int arfq_kv_write(arfq_ctx *ctx, arfq_kv *kv, const arfq_kv_seqs *seqs, const void *k, int64_t k_stride,
+                  const void *v, int64_t v_stride, int dtype);
+/* The rows back: k and v [tokens, heads, head_dim] (device, f32 or f16, exact in both).  With
+ * arfq_kv_write's seqs, the rows that it wrote; with start the running sum of len, every
+ * cached token.  Rows that name nothing are left as they were. */
+int arfq_kv_read(arfq_ctx *ctx, const arfq_kv *kv, const arfq_kv_seqs *seqs, void *k, int64_t k_stride, void *v,
+                 int64_t v_stride, int dtype);
+
+/* out[t, h] = sum_j p_j v_j with p = softmax_j(c(scale * q[t, h] . k_j)), K/V head h / (q_heads /
+ * heads), over the cached tokens j of row t's sequence with j <= its position (causal != 0) and,
+ * where window > 0, j > its position - window.  c(s) = softcap * tanh(s / softcap), or s where
+ * softcap is 0.  A row that attends to nothing gives zeros; rows of no sequence are left as
+ * they were.  q and out [tokens, q_heads, head_dim], f32 or f16 each, with token strides as above.
+ * Sums are f32; an f32 q and the weights p enter the matrix products as two f16 parts (22 bits),
+ * one part (q exact, p 11 bits) where q and out are both f16.  Write the step's rows first:
+ * a row's own token is among those that it attends to.
+ * A step of any mix: one token a sequence, several, whole prompts.  Results do not depend on
+ * which run of the same call they come from (no atomics on data).
+ * workspace: arfq_kv_attention_workspace bytes of device memory (16-byte aligned) for the parts of
+ * rows whose keys are spread over the chip, used only while the call's work runs; NULL takes
+ * the context's scratch, except under stream capture, where it is ARFQ_E_INVALID (the
+ * scratch moves when it grows; a captured graph keeps the address). */
+int arfq_kv_attention(arfq_ctx *ctx, const arfq_kv *kv, const arfq_kv_seqs *seqs, int q_heads, const void *q,
+                      int64_t q_stride, int q_dtype, void *out, int64_t out_stride, int out_dtype, float scale,
+                      float softcap, int64_t window, int causal, void *workspace, size_t workspace_bytes);
+int arfq_kv_attention_workspace(arfq_ctx *ctx, const arfq_kv *kv, int64_t batch, int64_t tokens, int q_heads,
+                                size_t *bytes);
+
 /* ---- GGUF reader ---------------------------------------------------------
  * A GGUF v3 file opened read-only and memory-mapped; tensors are read in place
  * (LazyGguf, crates/arf-core/src/model/gguf.rs:365-564).  Errors of
