@@ -111,7 +111,7 @@ _SIGS = {
     "arfq_kv_read": (_int, [_vp, _vp, _vp, _vp, _i64, _vp, _i64, _int]),
     "arfq_kv_attention": (_int, [_vp, _vp, _vp, _int, _vp, _i64, _int, _vp, _i64, _int, ctypes.c_float,
                                  ctypes.c_float, _i64, _int, _vp, ctypes.c_size_t]),
-    "arfq_kv_attention_workspace": (_int, [_vp, _vp, _i64, _i64, _int, ctypes.POINTER(ctypes.c_size_t)]),
+    "arfq_kv_attention_workspace": (_int, [_vp, _vp, _i64, _i64, _i64, _int, ctypes.POINTER(ctypes.c_size_t)]),
     "arfq_gguf_is_gguf": (_int, [ctypes.c_char_p]),
     "arfq_gguf_open": (_int, [ctypes.c_char_p, ctypes.POINTER(_vp)]),
     "arfq_gguf_close": (_int, [_vp]),
@@ -467,11 +467,11 @@ class Context:
             self.handle, kv.handle, seqs.ref, q_heads, q.ptr, qs, _float_type(q, "kv_attention: q"), out.ptr, os_,
             _float_type(out, "kv_attention: out"), scale, softcap, window, causal, ws[0], ws[1]))
 
-    def kv_attention_workspace(self, kv, batch, tokens, q_heads):
-        """Bytes of kv_attention's workspace (arfq_kv_attention_workspace)."""
+    def kv_attention_workspace(self, kv, seqs, q_heads):
+        """Bytes of kv_attention's workspace for such a batch (arfq_kv_attention_workspace)."""
         sz = ctypes.c_size_t()
-        _check(self.handle, load_library().arfq_kv_attention_workspace(self.handle, kv.handle, int(batch), int(tokens),
-                                                                       int(q_heads), ctypes.byref(sz)))
+        _check(self.handle, load_library().arfq_kv_attention_workspace(
+            self.handle, kv.handle, seqs.batch, seqs.tokens, int(seqs.pages.shape[1]), int(q_heads), ctypes.byref(sz)))
         return sz.value
 
     def copy_d2d(self, dst, src, nbytes=None):

@@ -531,7 +531,7 @@ static int kv_args(arfq_ctx *ctx, const arfq_kv *kv, const arfq_kv_seqs *s, cons
     a->start = s->start;
     a->len = s->len;
     a->table = s->pages;
-    a->max_pages = s->max_pages;
+    a->max_pages = (int)s->max_pages;
     return ARFQ_OK;
 }
 
@@ -583,12 +583,14 @@ static int kv_q_heads(arfq_ctx *ctx, const arfq_kv *kv, int64_t batch, int64_t t
     return ARFQ_OK;
 }
 
-int arfq_kv_attention_workspace(arfq_ctx *ctx, const arfq_kv *kv, int64_t batch, int64_t tokens, int q_heads,
-                                size_t *bytes) {
+int arfq_kv_attention_workspace(arfq_ctx *ctx, const arfq_kv *kv, int64_t batch, int64_t tokens, int64_t max_pages,
+                                int q_heads, size_t *bytes) {
     if (!ctx) return ARFQ_E_INVALID;
     if (!bytes) return fail(ctx, ARFQ_E_INVALID, "kv_attention_workspace: null argument");
     if (int rc = kv_q_heads(ctx, kv, batch, tokens, q_heads)) return rc;
-    *bytes = arfq::attn_plan(ctx->cus, kv->heads, kv->dim, batch, tokens, q_heads).ws_bytes;
+    if (max_pages < 0 || max_pages > arfq::KV_KEYS_MAX / kv->page)
+        return fail(ctx, ARFQ_E_SHAPE, "kv_attention_workspace: max_pages * page_size above 2^29");
+    *bytes = arfq::attn_plan(ctx->cus, kv->heads, kv->dim, batch, tokens, q_heads, max_pages * kv->page).ws_bytes;
     return ARFQ_OK;
 }
 
@@ -606,12 +608,13 @@ int arfq_kv_attention(arfq_ctx *ctx, const arfq_kv *kv, const arfq_kv_seqs *seqs
     if (int rc = kv_rows(ctx, "kv_attention: q", q, q_stride, q_heads, kv->dim, q_dtype)) return rc;
     if (int rc = kv_rows(ctx, "kv_attention: out", out, out_stride, q_heads, kv->dim, out_dtype)) return rc;
     if (int rc = use_device(ctx)) return rc;
-    const arfq::AttnPlan plan = arfq::attn_plan(ctx->cus, kv->heads, kv->dim, seqs->batch, seqs->tokens, q_heads);
+    const arfq::AttnPlan plan = arfq::attn_plan(ctx->cus, kv->heads, kv->dim, seqs->batch, seqs->tokens, q_heads,
+                                                    seqs->max_pages * kv->page);
     if (workspace) {
         if (workspace_bytes < plan.ws_bytes || (uintptr_t)workspace % 16)
             return fail(ctx, ARFQ_E_SHAPE, "kv_attention: workspace of " + std::to_string(workspace_bytes) + " bytes, " +
                                                std::to_string(plan.ws_bytes) + " (16-byte aligned) are wanted");
-    } else {
+    } else if (plan.ws_bytes) {
         hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
         HIP_TRY(ctx, hipStreamIsCapturing(ctx->stream, &cap));
         if (cap != hipStreamCaptureStatusNone)
@@ -633,6 +636,7 @@ int arfq_kv_attention(arfq_ctx *ctx, const arfq_kv *kv, const arfq_kv_seqs *seqs
     a.causal = causal != 0;
     a.target = plan.target;
     a.slots = plan.slots;
+    a.joins = plan.joins;
     a.part = (float *)workspace;
     const hipError_t e = arfq::launch_attn(a, kv->dim, ctx->stream);
     return e == hipSuccess ? ARFQ_OK : hip_fail(ctx, e, "kv_attention launch");

@@ -57,7 +57,7 @@ struct KvArgs {
     // the batch
     int batch, tokens;
     const int32_t *start, *len, *table;
-    int64_t max_pages;
+    int max_pages;
 };
 
 // Page of 16-key tile `t` of a sequence.  t < 2^27 (32-bit positions), tiles <= 16: the product
@@ -97,15 +97,17 @@ struct AttnArgs {
     int causal;
     // the work list: see attn_plan
     int target, slots;
-    float *part;         // partials, [slots][heads][16][dim + 2]
+    int joins;           // gridDim.z of the join (0: no tile has two pieces)
+    float *part;         // parts, [slots][heads][16][dim + 4]: maximum, sum, -, -, values
 };
 struct AttnPlan {
     int target = 1;     // pieces per head the keys are cut into, beside one per row tile
     int slots = 1;      // bound on the work items per head
+    int joins = 0;
     size_t ws_bytes = 0;
 };
 bool attn_dim_ok(int dim);
-AttnPlan attn_plan(int cus, int heads, int dim, int64_t batch, int64_t tokens, int q_heads);
+AttnPlan attn_plan(int cus, int heads, int dim, int64_t batch, int64_t tokens, int q_heads, int64_t max_keys);
 hipError_t launch_attn(const AttnArgs &a, int dim, hipStream_t s);
 
 }  // namespace arfq

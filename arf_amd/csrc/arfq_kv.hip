@@ -156,8 +156,9 @@ __global__ __launch_bounds__(256) void kv_write_kernel(KvArgs a, const void *k, 
     for (int j = 0; j < 4; j++) vc[(4 * i + j) * 4 * NG] = (uint8_t)(wv >> (8 * j));
     if (i == 0) {
         // a row with a value that is not finite: its key is NaN, as is what attends to it
+        const int at = ((key >> 2) * NG + g) * 4 + (key & 3);
         ((uint16_t *)(reg + a.off_ks))[key * NG + g] = (uint16_t)(bad ? 0x7e00u : dk);
-        ((uint16_t *)(reg + a.off_vs))[((key >> 2) * NG + g) * 4 + (key & 3)] = (uint16_t)dv;
+        ((uint16_t *)(reg + a.off_vs))[at] = (uint16_t)dv;
     }
 }
 
@@ -172,8 +173,8 @@ __global__ __launch_bounds__(256) void kv_read_kernel(KvArgs a, void *k, int64_t
     const uint8_t *reg = place<RL>(a, row0, rows, token, head, key);
     const int u = lane % RL, g = u >> 2, i = u & 3;
     if (!reg || g >= NG) return;
-    const float dk = h2f(((const uint16_t *)(reg + a.off_ks))[key * NG + g]);
-    const float dv = h2f(((const uint16_t *)(reg + a.off_vs))[((key >> 2) * NG + g) * 4 + (key & 3)]);
+    const int at = ((key >> 2) * NG + g) * 4 + (key & 3);
+    const float dk = h2f(((const uint16_t *)(reg + a.off_ks))[key * NG + g]), dv = h2f(((const uint16_t *)(reg + a.off_vs))[at]);
     const uint32_t wk = *(const uint32_t *)(reg + (int64_t)key * (D / 2) + (i * NG + g) * 4);
     const uint8_t *vc = reg + a.off_v + (key >> 2) * (64 * NG) + (key & 3) * NG + g;
     float xk[8], xv[8];

@@ -370,8 +370,8 @@ int arfq_kv_read(arfq_ctx *ctx, const arfq_kv *kv, const arfq_kv_seqs *seqs, voi
 int arfq_kv_attention(arfq_ctx *ctx, const arfq_kv *kv, const arfq_kv_seqs *seqs, int q_heads, const void *q,
                       int64_t q_stride, int q_dtype, void *out, int64_t out_stride, int out_dtype, float scale,
                       float softcap, int64_t window, int causal, void *workspace, size_t workspace_bytes);
-int arfq_kv_attention_workspace(arfq_ctx *ctx, const arfq_kv *kv, int64_t batch, int64_t tokens, int q_heads,
-                                size_t *bytes);
+int arfq_kv_attention_workspace(arfq_ctx *ctx, const arfq_kv *kv, int64_t batch, int64_t tokens, int64_t max_pages,
+                                int q_heads, size_t *bytes);
 
 /* ---- GGUF reader ---------------------------------------------------------
  * A GGUF v3 file opened read-only and memory-mapped; tensors are read in place

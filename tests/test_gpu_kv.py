@@ -375,7 +375,7 @@ def test_same_bits_again_and_with_a_workspace(gpu_ctx):
     _filled(gpu_ctx, kv, batch, rng)
     q = _rows(rng, batch.tokens, 8, 128, np.float32)
     first = _attend(gpu_ctx, kv, batch, q, np.float32, 0.1)
-    need = gpu_ctx.kv_attention_workspace(kv, 3, batch.tokens, 8)
+    need = gpu_ctx.kv_attention_workspace(kv, batch.seqs, 8)
     ws = gpu_ctx.to_device(np.full(need // 4 + 4, np.nan, np.float32))
     for w in (None, ws, ws):
         assert np.array_equal(_attend(gpu_ctx, kv, batch, q, np.float32, 0.1, workspace=w).view(np.uint32),
@@ -457,9 +457,12 @@ def test_refusals(gpu_ctx):
                      (dict(o=None), E.ARFQ_E_INVALID), (dict(qs=255), E.ARFQ_E_SHAPE), (dict(os=258), E.ARFQ_E_INVALID),
                      (dict(t=5), E.ARFQ_E_INVALID), (dict(ot=-1), E.ARFQ_E_INVALID), (dict(scale=nan), E.ARFQ_E_INVALID),
                      (dict(scale=inf), E.ARFQ_E_INVALID), (dict(cap=-1.0), E.ARFQ_E_INVALID), (dict(cap=inf), E.ARFQ_E_INVALID),
-                     (dict(win=-1), E.ARFQ_E_SHAPE), (dict(ws=x.ptr, wb=16), E.ARFQ_E_SHAPE)]:
+                     (dict(win=-1), E.ARFQ_E_SHAPE)]:
         assert attend(seqs(), **kw) == want, kw
         assert L.arfq_last_error(h).startswith(b"kv_attention")
+    # a workspace for more keys than one piece has
+    assert attend(seqs(most=2 ** 20), ws=x.ptr, wb=16) == E.ARFQ_E_SHAPE and b"workspace" in L.arfq_last_error(h)
+    assert attend(seqs(most=2 ** 20), ws=x.ptr + 4, wb=2 ** 40) == E.ARFQ_E_SHAPE
     with pytest.raises(ValueError):
         gpu_ctx.kv_write(kv, arf_amd.KVSeqs(table, lens), x, gpu_ctx.empty((2, 2, 64), np.float16))
     kv.free()

@@ -19,7 +19,7 @@ def test_null_handles_are_rejected():
     assert L.arfq_kv_write(None, None, None, None, 0, None, 0, 0) == bad
     assert L.arfq_kv_read(None, None, None, None, 0, None, 0, 0) == bad
     assert L.arfq_kv_attention(None, None, None, 8, None, 0, 0, None, 0, 0, 1.0, 0.0, 0, 1, None, 0) == bad
-    assert L.arfq_kv_attention_workspace(None, None, 1, 1, 8, None) == bad
+    assert L.arfq_kv_attention_workspace(None, None, 1, 1, 1, 8, None) == bad
 
 
 class _Array:
