@@ -15,6 +15,8 @@ constexpr int TR = 16;        // rows of a tile: (token, head of the group) pair
 constexpr int STEP = 32;      // keys of a step
 constexpr int WAVES = 4;
 constexpr int MIN_PIECE = 256;  // keys
+// waves of a SIMD (a workgroup has one on each): registers below 512 / that
+constexpr int rows16_waves(int ng) { return ng <= 2 ? 4 : ng <= 4 ? 3 : 2; }
 // p is held as exp2(x - m + P_BIAS), m behind the running maximum by at most M_SLACK: f16 (2^16)
 // is not passed, and a part of p keeps its 11 bits down to 2^-27 of the largest p (below, half
 // a step is 2^-38 of it).  The slack spares most steps the rescaling of the sums.
@@ -48,40 +50,73 @@ __device__ __forceinline__ int pieces_of(const Seq &s, int piece) {
     return max(1, (s.end - s.lo + piece - 1) / piece);
 }
 
-// Keys of a piece (a multiple of STEP), the same in every wave of the launch.  The area is summed
-// in f32 in one fixed order; the 2^-16 added covers its rounding, so that the list has no
-// more than target + tiles items.
-__device__ __forceinline__ int piece_len(const AttnArgs &a) {
-    const int lane = threadIdx.x & 63;
-    float area = 0.0f;
-    for (int b0 = 0; b0 < a.c.batch; b0 += WAVE) {
-        const Seq s = seq_of(a, b0 + lane);
-        area += (float)s.tiles * (float)((s.end - s.lo + STEP - 1) / STEP);
-    }
-    for (int x = 1; x < WAVE && x < a.c.batch; x <<= 1) area += __shfl_xor(area, x);
-    const float steps = ceilf(area / (float)a.target * (1.0f + 1.0f / 65536));
-    const int piece = (int)fminf(steps, (float)(KV_KEYS_MAX / STEP)) * STEP;
-    return __builtin_amdgcn_readfirstlane(max(MIN_PIECE, piece));
+// Running sums over the wave's lanes (six DPP additions: a row of 16 by shifts, then the rows).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp(int v) {
+    return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false);
+}
+__device__ __forceinline__ int wave_scan(int v) {
+    v += dpp<0x111, 0xf>(v);  // row_shr:1, 2, 4, 8
+    v += dpp<0x112, 0xf>(v);
+    v += dpp<0x114, 0xf>(v);
+    v += dpp<0x118, 0xf>(v);
+    v += dpp<0x142, 0xa>(v);  // row_bcast:15 into rows 1 and 3
+    v += dpp<0x143, 0xc>(v);  // row_bcast:31 into rows 2 and 3
+    return v;
+}
+__device__ __forceinline__ float wave_sum(float v) {
+    auto step = [&](int w) { v += __builtin_bit_cast(float, w); };
+    step(dpp<0x111, 0xf>(__builtin_bit_cast(int, v)));
+    step(dpp<0x112, 0xf>(__builtin_bit_cast(int, v)));
+    step(dpp<0x114, 0xf>(__builtin_bit_cast(int, v)));
+    step(dpp<0x118, 0xf>(__builtin_bit_cast(int, v)));
+    step(dpp<0x142, 0xa>(__builtin_bit_cast(int, v)));
+    step(dpp<0x143, 0xc>(__builtin_bit_cast(int, v)));
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
 }
 
 struct Item {
     Seq s;
     int b, tile, piece, pieces;
+    int keys;  // of a piece (a multiple of STEP): the sequence's keys in equal parts
+    int slot;  // place of the (tile, piece) in the list of all
 };
 
 // The `index`-th (tile, piece) of the batch: sequences in order, their tiles one after another,
-// pieces fastest.  False: the list has fewer.
-__device__ __forceinline__ bool find_item(const AttnArgs &a, int piece, int index, Item &it) {
+// pieces fastest; or (PIECES false) the first piece of the index-th tile.  False: the list has
+// fewer.  The keys that make a new piece necessary are the same in every wave of the launch: the
+// fewest that cut the area into at most `target` pieces, or nearly so (a target of workgroups that
+// the chip holds at once: one more round for a few of them would take as long as the first).
+// The area is summed in f32 in one fixed order; the 2^-16 added covers its rounding, so that the
+// list has no more than target + tiles items.
+template <bool PIECES>
+__device__ __forceinline__ bool find_item(const AttnArgs &a, int index, Item &it) {
     const int lane = threadIdx.x & 63;
-    int before = 0;
-    for (int b0 = 0; b0 < a.c.batch; b0 += WAVE) {
-        const Seq s = seq_of(a, b0 + lane);
-        const int np = pieces_of(s, piece), own = (int)min((int64_t)s.tiles * np, (int64_t)1 << 30);
-        int inc = own;
-        for (int x = 1; x < WAVE && x < a.c.batch; x <<= 1) {
-            const int v = __shfl_up(inc, x);
-            if (lane >= x) inc += v;
+    const Seq s0 = seq_of(a, lane);  // (the whole batch, mostly)
+    auto over_batch = [&](auto f) {
+        float v = f(s0);
+        for (int b0 = WAVE; b0 < a.c.batch; b0 += WAVE) v += f(seq_of(a, b0 + lane));
+        return wave_sum(v);
+    };
+    const float area = over_batch([](const Seq &s) { return (float)s.tiles * (float)((s.end - s.lo + STEP - 1) / STEP); });
+    const float target = (float)a.target;
+    auto keys_of = [](float steps) { return (int)fminf(steps, (float)(KV_KEYS_MAX / STEP)) * STEP; };
+    float steps = fmaxf(ceilf(area / target * (1.0f + 1.0f / 65536)), (float)(MIN_PIECE / STEP));
+    if (a.c.batch > 1) {
+        for (int i = 0; i < 3; i++) {
+            const int piece = keys_of(steps);
+            const float items = over_batch([&](const Seq &s) { return (float)s.tiles * (float)pieces_of(s, piece); });
+            if (items <= target) break;
+            // (tiles of one piece stay: the others' pieces shrink in number with their length)
+            steps = ceilf(steps * fminf(items / target, 2.0f));
         }
+    }
+    const int piece = keys_of(steps);
+    int before = 0, items = 0;
+    for (int b0 = 0; b0 < a.c.batch; b0 += WAVE) {
+        const Seq s = b0 ? seq_of(a, b0 + lane) : s0;
+        const int np = pieces_of(s, piece), all = (int)min((int64_t)s.tiles * np, (int64_t)1 << 30);
+        const int own = PIECES ? all : s.tiles, inc = wave_scan(own), sum = PIECES ? inc : wave_scan(all);
         const uint64_t past = __ballot(before + inc > index);
         if (past) {
             const int l = __ffsll((unsigned long long)past) - 1;
@@ -93,12 +128,15 @@ __device__ __forceinline__ bool find_item(const AttnArgs &a, int piece, int inde
             it.s.tiles = __builtin_amdgcn_readlane(s.tiles, l);
             it.pieces = __builtin_amdgcn_readlane(np, l);
             it.b = b0 + l;
+            it.keys = ((it.s.end - it.s.lo + STEP - 1) / STEP + it.pieces - 1) / it.pieces * STEP;
             const int rest = index - before - __builtin_amdgcn_readlane(inc - own, l);
-            it.tile = rest / it.pieces;
-            it.piece = rest - it.tile * it.pieces;
-            return rest >= 0 && it.tile < it.s.tiles;
+            it.tile = PIECES ? rest / it.pieces : rest;
+            it.piece = PIECES ? rest - it.tile * it.pieces : 0;
+            it.slot = PIECES ? index : items + __builtin_amdgcn_readlane(sum - all, l) + it.tile * it.pieces;
+            return rest >= 0 && it.tile < it.s.tiles && it.slot >= 0;
         }
         before += __builtin_amdgcn_readlane(inc, 63);
+        items += __builtin_amdgcn_readlane(sum, 63);
     }
     return false;
 }
@@ -296,22 +334,21 @@ __device__ __forceinline__ void store_out(const AttnArgs &a, int64_t i, f32x4 v)
 // a group (32 values: one MFMA), V's its codes.
 // PARTS: f16 parts of q and p (2: hi + lo, 22 bits, for f32 q or out).
 template <int NG, int PARTS>
-__global__ __launch_bounds__(64 * WAVES, NG <= 2 ? 4 : NG <= 4 ? 3 : 2) void attn_rows16(AttnArgs a) {
+__global__ __launch_bounds__(64 * WAVES, rows16_waves(NG)) void attn_rows16(AttnArgs a) {
     constexpr int D = 32 * NG, NT = 2 * NG;  // NT: 16-row tiles of O^T
     constexpr bool RAW = PARTS == 1;         // K's operands: see k_frag
     constexpr int OS = D + 4;                // LDS floats of a row of O
     extern __shared__ float lds[];           // [WAVES][16][OS], then [WAVES][16][2]
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, h = lane >> 4;
-    const int head = blockIdx.y;
-    const int piece = piece_len(a);
+    const int head = blockIdx.x % a.c.heads;  // (fastest: the list's unused end comes last)
     Item it;
-    if (!find_item(a, piece, blockIdx.x, it)) return;
+    if (!find_item<true>(a, blockIdx.x / a.c.heads, it)) return;
     const Seq &s = it.s;
 
     // keys [lo, hi) of the row of token tok
     auto row_hi = [&](int64_t pos) { return pos < 0 ? 0 : a.causal ? (int)min(pos + 1, (int64_t)s.end) : s.end; };
     auto row_lo = [&](int64_t pos) { return a.window ? (int)max((int64_t)0, min(pos - a.window + 1, (int64_t)s.end)) : 0; };
-    const int rows = s.n * a.group, piece_lo = s.lo + it.piece * piece, piece_hi = min(s.end, piece_lo + piece);
+    const int rows = s.n * a.group, piece_lo = s.lo + it.piece * it.keys, piece_hi = min(s.end, piece_lo + it.keys);
     // the tile's keys in this piece, and those that every row has (both ends rise with the token)
     const int64_t pos0 = (int64_t)s.len - s.n + it.tile * TR / a.group;
     const int64_t pos1 = (int64_t)s.len - s.n + min(it.tile * TR + TR - 1, rows - 1) / a.group;
@@ -528,8 +565,7 @@ __global__ __launch_bounds__(64 * WAVES, NG <= 2 ? 4 : NG <= 4 ? 3 : 2) void att
     if (rr >= s.n * a.group) return;
     const int rt = rr / a.group, rg = rr - rt * a.group;
     const bool whole = it.pieces == 1;
-    const int64_t slot = blockIdx.x;
-    float *part = a.part + ((slot * a.c.heads + head) * TR + er) * (D + 4);
+        float *part = a.part + (((int64_t)it.slot * a.c.heads + head) * TR + er) * (D + 4);
     const int64_t o = ((int64_t)s.t0 + rt) * a.out_stride + (int64_t)(head * a.group + rg) * D;
     const float inv = whole ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f;
 #pragma unroll
@@ -552,45 +588,71 @@ __global__ __launch_bounds__(64 * WAVES, NG <= 2 ? 4 : NG <= 4 ? 3 : 2) void att
     }
 }
 
-// Rows whose keys were cut into pieces: their parts joined, in order.  A workgroup has one row in
-// gridDim.z of the (tile, head) whose first piece is item blockIdx.x: its threads take D / 4
-// columns of four values and 1024 / D pieces at a time.
+// Rows whose keys were cut into pieces: their parts joined, in a fixed order.  A workgroup has one row in
+// gridDim.z of a (tile, head); its threads take D / 4 columns of four values and 1024 / D
+// pieces at a time.
 template <int NG>
 __global__ __launch_bounds__(256) void attn_join(AttnArgs a) {
     constexpr int D = 32 * NG, CT = D / 4, PT = 256 / CT;
     __shared__ f32x4 v_of[PT][CT];
-    __shared__ float l_of[PT];
-    const int head = blockIdx.y;
+    __shared__ float l_of[PT], m_of[PT];
+    const int head = blockIdx.x % a.c.heads;
     Item it;
-    if (!find_item(a, piece_len(a), blockIdx.x, it) || it.pieces == 1 || it.piece) return;
+    if (!find_item<false>(a, blockIdx.x / a.c.heads, it) || it.pieces == 1) return;
     const int pt = threadIdx.x / CT, ct = threadIdx.x - pt * CT;
-    const int rows = min(it.s.n * a.group - it.tile * TR, TR), pieces = min(it.pieces, a.slots - (int)blockIdx.x);
+    const int rows = min(it.s.n * a.group - it.tile * TR, TR), pieces = min(it.pieces, a.slots - it.slot);
     const int64_t next = (int64_t)a.c.heads * TR * (D + 4);
+    // the weight of a part (m, l) below a common maximum; NaN for a NaN part (a NaN key leaves
+    // a wave's maximum at -inf and its sum NaN)
+    auto weight = [](float m, float l, float top) { return l != l ? l : m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - top); };
     for (int r = blockIdx.z; r < rows; r += gridDim.z) {
-        const float *part = a.part + (((int64_t)blockIdx.x * a.c.heads + head) * TR + r) * (D + 4);
+        const float *part = a.part + (((int64_t)it.slot * a.c.heads + head) * TR + r) * (D + 4);
         float mm = -INFINITY, l = 0.0f;
-        for (int p = 0; p < pieces; p++) mm = fmaxf(mm, part[p * next]);
         f32x4 v = {0, 0, 0, 0};
         if (pt < PT) {
-            for (int p = pt; p < pieces; p += PT) {
-                const f32x4 w = *(const f32x4 *)(part + p * next + 4 + 4 * ct);
-                const float mp = part[p * next], lp = part[p * next + 1];
-                float f = mp == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mp - mm);
-                if (lp != lp) f = lp;  // (a NaN key leaves a wave's maximum at -inf and its sum NaN)
-                l += f * lp;
-                v += f * w;
+            constexpr int U = 8;  // loads in flight
+            for (int p0 = pt; p0 < pieces; p0 += U * PT) {
+                float m_p[U], l_p[U];
+                f32x4 w[U];
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    const int p = min(p0 + u * PT, pieces - 1);
+                    const float2 ml = *(const float2 *)(part + p * next);
+                    w[u] = *(const f32x4 *)(part + p * next + 4 + 4 * ct);
+                    m_p[u] = p0 + u * PT < pieces ? ml.x : -INFINITY;
+                    l_p[u] = p0 + u * PT < pieces ? ml.y : 0.0f;
+                }
+                float top = mm;
+#pragma unroll
+                for (int u = 0; u < U; u++) top = fmaxf(top, m_p[u]);
+                const float f0 = weight(mm, l, top);
+                l *= f0;
+                v *= f0;
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    const float f = weight(m_p[u], l_p[u], top);
+                    l += f * l_p[u];
+                    v += f * w[u];
+                }
+                mm = top;
             }
             v_of[pt][ct] = v;
-            if (ct == 0) l_of[pt] = l;
+            if (ct == 0) {
+                m_of[pt] = mm;
+                l_of[pt] = l;
+            }
         }
         __syncthreads();
         if (pt == 0) {
+#pragma unroll
+            for (int p = 0; p < PT; p++) mm = fmaxf(mm, m_of[p]);
             l = 0.0f;
             v = f32x4{0, 0, 0, 0};
 #pragma unroll
             for (int p = 0; p < PT; p++) {
-                l += l_of[p];
-                v += v_of[p][ct];
+                const float f = weight(m_of[p], l_of[p], mm);
+                l += f * l_of[p];
+                v += f * v_of[p][ct];
             }
             const int rr = it.tile * TR + r, rt = rr / a.group, rg = rr - rt * a.group;
             store_out(a, ((int64_t)it.s.t0 + rt) * a.out_stride + (int64_t)(head * a.group + rg) * D + 4 * ct,
@@ -600,19 +662,19 @@ __global__ __launch_bounds__(256) void attn_join(AttnArgs a) {
     }
 }
 
+int64_t tile_bound(int64_t batch, int64_t tokens, int group) {
+    return std::min(tokens * group / TR + batch, tokens * ((group + TR - 1) / TR));
+}
+
 template <int NG, int PARTS>
 hipError_t rows16_launch(const AttnArgs &a, hipStream_t s) {
     static std::atomic<uint64_t> done{0};
     constexpr size_t lds = (size_t)WAVES * TR * (32 * NG + 4 + 2) * sizeof(float);
     const hipError_t e = set_max_lds_once((const void *)attn_rows16<NG, PARTS>, lds, done);
     if (e != hipSuccess) return e;
-    attn_rows16<NG, PARTS><<<dim3((unsigned)a.slots, a.c.heads), 64 * WAVES, lds, s>>>(a);
-    if (a.joins) attn_join<NG><<<dim3((unsigned)a.slots, a.c.heads, a.joins), 256, 0, s>>>(a);
+    attn_rows16<NG, PARTS><<<dim3((unsigned)a.slots * a.c.heads), 64 * WAVES, lds, s>>>(a);
+    if (a.joins) attn_join<NG><<<dim3((unsigned)tile_bound(a.c.batch, a.c.tokens, a.group) * a.c.heads, 1, a.joins), 256, 0, s>>>(a);
     return hipGetLastError();
-}
-
-int64_t tile_bound(int64_t batch, int64_t tokens, int group) {
-    return std::min(tokens * group / TR + batch, tokens * ((group + TR - 1) / TR));
 }
 
 template <int NG>
@@ -627,13 +689,14 @@ bool attn_dim_ok(int dim) { return dim == 64 || dim == 96 || dim == 128 || dim =
 AttnPlan attn_plan(int cus, int heads, int dim, int64_t batch, int64_t tokens, int q_heads, int64_t max_keys) {
     AttnPlan p;
     const int64_t tiles = tile_bound(batch, tokens, q_heads / heads), most = (max_keys + MIN_PIECE - 1) / MIN_PIECE;
-    p.target = std::max(1, 3 * cus / heads);
+    p.target = std::max(1, rows16_waves(dim / KV_GROUP) * cus / heads);
     // the area cut into `target` pieces, and at most one more for each tile; none shorter than MIN_PIECE
     p.slots = (int)std::min(p.target + tiles, tiles * std::max<int64_t>(most, 1));
     if (most > 1) {
         p.ws_bytes = (size_t)p.slots * heads * TR * (dim + 4) * sizeof(float);
-        // few workgroups: one for each row
-        p.joins = (int64_t)p.slots * heads <= 8 * cus ? TR : 1;
+        // workgroups of a (tile, head): one for each row of it, while they are about the chip's
+        const int64_t rows = std::min<int64_t>(TR, tokens > batch ? TR : q_heads / heads);
+        p.joins = (int)std::max<int64_t>(1, std::min<int64_t>(rows, 4 * cus / (tiles * heads)));
     }
     return p;
 }
