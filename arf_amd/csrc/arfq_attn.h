@@ -1,0 +1,395 @@
+// arfq_attn.h -- what the attention kernels share: the work list, the matrix operands made from
+// the cache, and the rows' scaling.
+#pragma once
+#include <math.h>
+
+#include "arfq_kv.h"
+
+namespace arfq {
+namespace {
+
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int STEP = 32;      // keys of a step
+// p is held as exp2(x - m + P_BIAS), m behind the running maximum by at most M_SLACK: f16 (2^16)
+// is not passed, and a part of p keeps its 11 bits down to 2^-27 of the largest p (below, half
+// a step is 2^-38 of it).  The slack spares most steps the rescaling of the sums.
+constexpr float P_BIAS = 13.0f, M_SLACK = 2.0f;
+
+// ---- the work list -----------------------------------------------------------------------
+// A row is a (token, head of the group) pair, head fastest.  Sequences with at most few_rows rows
+// are in the list of 16-row tiles (a decode step), others in that of 128-row tiles (prompts); a
+// kernel works through each.  A sequence's keys [lo, end) are cut into pieces; a work item is a
+// (tile, piece).  The piece length is what cuts the whole batch's
+// (tile, key) area into about `target` pieces, so that a long sequence is spread over the chip
+// whatever its neighbours are: decided here, from the lengths, which are on the device.
+
+// keys of the shortest piece: below, its set-up and the joining of its rows take longer than its keys
+constexpr int min_piece(int tr) { return tr == 16 ? 256 : 512; }
+
+struct Seq {
+    int t0, n, len;
+    int lo, end;  // keys that some row may attend to; lo is a multiple of STEP
+    int tiles;
+};
+
+template <int TR>
+__device__ __forceinline__ const AttnList &list_of(const AttnArgs &a) { return TR == 16 ? a.few : a.many; }
+
+template <int TR>
+__device__ __forceinline__ Seq seq_of(const AttnArgs &a, int b) {
+    Seq s = {0, 0, 0, 0, 0, 0};
+    if (b >= a.c.batch) return s;
+    kv_seq(a.c, b, s.t0, s.n);
+    s.len = a.c.len[b];
+    s.end = (int)min((int64_t)max(s.len, 0), (int64_t)a.c.max_pages * a.c.page);
+    if (a.window) s.lo = (int)max((int64_t)0, min((int64_t)s.len - s.n - a.window + 1, (int64_t)s.end)) & ~(STEP - 1);
+    const int64_t rows = (int64_t)s.n * a.group;
+    if ((TR == 16) == (rows <= a.few_rows)) s.tiles = (int)((rows + TR - 1) / TR);
+    return s;
+}
+
+__device__ __forceinline__ int pieces_of(const Seq &s, int piece) {
+    return max(1, (s.end - s.lo + piece - 1) / piece);
+}
+
+// Running sums over the wave's lanes (six DPP additions: a row of 16 by shifts, then the rows).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp(int v) {
+    return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false);
+}
+__device__ __forceinline__ int wave_scan(int v) {
+    v += dpp<0x111, 0xf>(v);  // row_shr:1, 2, 4, 8
+    v += dpp<0x112, 0xf>(v);
+    v += dpp<0x114, 0xf>(v);
+    v += dpp<0x118, 0xf>(v);
+    v += dpp<0x142, 0xa>(v);  // row_bcast:15 into rows 1 and 3
+    v += dpp<0x143, 0xc>(v);  // row_bcast:31 into rows 2 and 3
+    return v;
+}
+__device__ __forceinline__ float wave_sum(float v) {
+    auto step = [&](int w) { v += __builtin_bit_cast(float, w); };
+    step(dpp<0x111, 0xf>(__builtin_bit_cast(int, v)));
+    step(dpp<0x112, 0xf>(__builtin_bit_cast(int, v)));
+    step(dpp<0x114, 0xf>(__builtin_bit_cast(int, v)));
+    step(dpp<0x118, 0xf>(__builtin_bit_cast(int, v)));
+    step(dpp<0x142, 0xa>(__builtin_bit_cast(int, v)));
+    step(dpp<0x143, 0xc>(__builtin_bit_cast(int, v)));
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
+}
+
+struct Item {
+    Seq s;
+    int b, tile, piece, pieces;
+    int keys;  // of a piece (a multiple of STEP): the sequence's keys in equal parts
+    int slot;  // place of the (tile, piece) in the list of all
+};
+
+// The `index`-th (tile, piece) of the batch: sequences in order, their tiles one after another,
+// pieces fastest; or (PIECES false) the first piece of the index-th tile.  False: the list has
+// fewer.  The keys that make a new piece necessary are the same in every wave of the launch: the
+// fewest that cut the area into at most `target` pieces, or nearly so (a target of workgroups that
+// the chip holds at once: one more round for a few of them would take as long as the first).
+// The area is summed in f32 in one fixed order; the 2^-16 added covers its rounding, so that the
+// list has no more than target + tiles items.
+template <int TR, bool PIECES>
+__device__ __forceinline__ bool find_item(const AttnArgs &a, int index, Item &it) {
+    const int lane = threadIdx.x & 63;
+    const Seq s0 = seq_of<TR>(a, lane);  // (the whole batch, mostly)
+    auto over_batch = [&](auto f) {
+        float v = f(s0);
+        for (int b0 = WAVE; b0 < a.c.batch; b0 += WAVE) v += f(seq_of<TR>(a, b0 + lane));
+        return wave_sum(v);
+    };
+    const float area = over_batch([](const Seq &s) { return (float)s.tiles * (float)((s.end - s.lo + STEP - 1) / STEP); });
+    const float target = (float)list_of<TR>(a).target;
+    auto keys_of = [](float steps) { return (int)fminf(steps, (float)(KV_KEYS_MAX / STEP)) * STEP; };
+    float steps = fmaxf(ceilf(area / target * (1.0f + 1.0f / 65536)), (float)(min_piece(TR) / STEP));
+    for (int i = 0; i < 3; i++) {
+        const int piece = keys_of(steps);
+        const float items = over_batch([&](const Seq &s) { return (float)s.tiles * (float)pieces_of(s, piece); });
+        if (items <= target) break;
+        // (tiles of one piece stay: the others' pieces shrink in number with their length)
+        steps = ceilf(steps * fminf(items / target, 2.0f));
+    }
+    const int piece = keys_of(steps);
+    int before = 0, items = 0;
+    for (int b0 = 0; b0 < a.c.batch; b0 += WAVE) {
+        const Seq s = b0 ? seq_of<TR>(a, b0 + lane) : s0;
+        const int np = pieces_of(s, piece), all = (int)min((int64_t)s.tiles * np, (int64_t)1 << 30);
+        const int own = PIECES ? all : s.tiles, inc = wave_scan(own), sum = PIECES ? inc : wave_scan(all);
+        const uint64_t past = __ballot(before + inc > index);
+        if (past) {
+            const int l = __ffsll((unsigned long long)past) - 1;
+            it.s.t0 = __builtin_amdgcn_readlane(s.t0, l);
+            it.s.n = __builtin_amdgcn_readlane(s.n, l);
+            it.s.len = __builtin_amdgcn_readlane(s.len, l);
+            it.s.lo = __builtin_amdgcn_readlane(s.lo, l);
+            it.s.end = __builtin_amdgcn_readlane(s.end, l);
+            it.s.tiles = __builtin_amdgcn_readlane(s.tiles, l);
+            it.pieces = __builtin_amdgcn_readlane(np, l);
+            it.b = b0 + l;
+            it.keys = ((it.s.end - it.s.lo + STEP - 1) / STEP + it.pieces - 1) / it.pieces * STEP;
+            const int rest = index - before - __builtin_amdgcn_readlane(inc - own, l);
+            it.tile = PIECES ? rest / it.pieces : rest;
+            it.piece = PIECES ? rest - it.tile * it.pieces : 0;
+            it.slot = PIECES ? index : items + __builtin_amdgcn_readlane(sum - all, l) + it.tile * it.pieces;
+            return rest >= 0 && it.tile < it.s.tiles && it.slot >= 0;
+        }
+        before += __builtin_amdgcn_readlane(inc, 63);
+        items += __builtin_amdgcn_readlane(sum, 63);
+    }
+    return false;
+}
+
+// Where a step's two 16-key tiles are: the (page, head) regions (page 0's for a page that is not the cache's:
+// loads stay in it, its keys are masked) and the tiles' places in them.
+struct Places {
+    const uint8_t *reg[2];
+    uint32_t sub[2];
+    bool in[2];  // whether the tile's page is the cache's
+};
+// The page ids of a sequence, 64 pages at a time in a register across the wave.  (Not a scalar load each
+// step: the wait for LDS data is for scalar loads too, and these miss the scalar cache.)
+struct Pages {
+    const int32_t *table;
+    const uint8_t *base;  // the head's region of page 0
+    int first, ids;
+    __device__ __forceinline__ Pages(const KvArgs &a, int b, int head)
+        : table(a.table + (int64_t)b * a.max_pages), base(a.data + head * a.region), first(INT32_MIN), ids(0) {}
+    // the step of keys k0 .. +31 (past the table's end: of its last page); max_pages > 0
+    __device__ __forceinline__ Places at(const KvArgs &a, int k0) {
+        Places p;
+        const int t0 = k0 / KV_TILE, pg0 = kv_page_of(a, t0), pg1 = kv_page_of(a, t0 + 1);
+        const int most = a.max_pages - 1, l0 = min(pg0, most), l1 = min(pg1, most);
+        if (l0 < first || l1 - first >= WAVE) {
+            first = l0;
+            ids = table[min(l0 + (int)(threadIdx.x & 63), most)];
+            __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0) here, and not at each use
+        }
+        const int id[2] = {__builtin_amdgcn_readlane(ids, l0 - first), __builtin_amdgcn_readlane(ids, l1 - first)};
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            p.in[i] = (uint32_t)id[i] < (uint32_t)a.n_pages;
+            p.reg[i] = base + (uint64_t)(uint32_t)(p.in[i] ? id[i] : 0) * a.page_bytes;
+            p.sub[i] = (uint32_t)(t0 + i - (i ? pg1 : pg0) * a.tiles);
+        }
+        return p;
+    }
+};
+
+// ---- operands ----------------------------------------------------------------------------
+
+// Two codes + 8 in bits 0..3 (LO) or 4..7 of the halves -> the codes as f16: or-ed into 1024
+// (2^10: a unit in the last place is 1) they read 1024 + c, or 1024 + 16 c; the steps that
+// follow are exact.  `magic` is that 1024 twice in a vector register, which the compiler does
+// not see through: with a literal there it splits v_and_or_b32 into two instructions.
+__device__ __forceinline__ uint32_t magic_1024() {
+    uint32_t m;
+    asm("v_mov_b32 %0, 0x64006400" : "=v"(m));
+    return m;
+}
+template <bool LO>
+__device__ __forceinline__ f16x2 codes_f16(uint32_t w, uint32_t magic) {
+    const f16x2 h = __builtin_bit_cast(f16x2, (w & (LO ? 0x000f000fu : 0x00f000f0u)) | magic);
+    if constexpr (LO) return h - f16x2{(_Float16)1032, (_Float16)1032};
+    return h * f16x2{(_Float16)0.0625f, (_Float16)0.0625f} - f16x2{(_Float16)72, (_Float16)72};
+}
+
+union Frag {
+    f16x2 w[4];
+    f16x8 v;
+};
+
+// What a lane of the step's 32 keys loads: K of two 16-key tiles (key lane % 16, chunk lane / 16)
+// and V of the keys 4 * (lane / 16) .. +3 of both (matrix rows lane % 16).
+template <int NG>
+struct Raw {
+    uint32_t k[2][NG], v[2][NG];
+    uint32_t ks[2][2 * NG];              // of keys 4 * (lane / 16) .. +3: [4][NG] f16
+    uint32_t vs[2][2 * NG];              // of the same, in pairs: [NG][2]
+    uint32_t ka[2][(NG + 1) / 2];        // of key lane % 16 (RAW)
+};
+
+// N dwords at an address that is a multiple of A bytes.
+template <int N, int A>
+__device__ __forceinline__ void load_aligned(const void *p, uint32_t (&o)[N]) {
+    static_assert(A == 4 || A == 8 || A == 16, "");
+    if constexpr (A == 16 && N % 4 == 0) {
+#pragma unroll
+        for (int i = 0; i < N / 4; i++) {
+            const u32x4 v = ((const u32x4 *)p)[i];
+            o[4 * i] = v.x; o[4 * i + 1] = v.y; o[4 * i + 2] = v.z; o[4 * i + 3] = v.w;
+        }
+    } else if constexpr (A >= 8 && N % 2 == 0) {
+#pragma unroll
+        for (int i = 0; i < N / 2; i++) {
+            const u32x2 v = ((const u32x2 *)p)[i];
+            o[2 * i] = v.x; o[2 * i + 1] = v.y;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i++) o[i] = ((const uint32_t *)p)[i];
+    }
+}
+
+// Byte offsets of a lane's operands in a 16-key tile (from the region, its V codes, scales and V scales).
+template <int NG>
+struct Offs {
+    uint32_t k, v, s, a;
+};
+template <int NG>
+__device__ __forceinline__ Offs<NG> lane_offs() {
+    const uint32_t lane = threadIdx.x & 63, c = lane & 15, h = lane >> 4;
+    return {c * (16 * NG) + h * (4 * NG), h * (64 * NG) + c * (4 * NG), h * (8 * NG), c * (2 * NG)};
+}
+// p + o with p uniform: hidden from the compiler, which would widen o once and keep it in two registers
+// instead of the loads' scalar base and 32-bit offset.
+__device__ __forceinline__ const uint8_t *at(const uint8_t *p, uint32_t o) {
+    asm("" : "+v"(o));
+    return p + o;
+}
+// reg (uniform): the tile's (page, head) region; sub: the 16-key tile within the page
+template <bool RAW, int NG>
+__device__ __forceinline__ void load_k(const uint8_t *reg, const KvArgs &a, uint32_t sub, int half, const Offs<NG> &o, Raw<NG> &r) {
+    constexpr int AL = NG % 4 == 0 ? 16 : NG % 2 == 0 ? 8 : 4;
+    load_aligned<NG, AL>(at(reg + sub * (256u * NG), o.k), r.k[half]);
+    const uint8_t *ks = reg + (a.off_ks + sub * (32u * NG));
+    load_aligned<2 * NG, 8>(at(ks, o.s), r.ks[half]);
+    if constexpr (!RAW) {
+    } else if constexpr (NG % 2 == 0) {
+        load_aligned<NG / 2, NG % 8 == 0 ? 16 : NG % 4 == 0 ? 8 : 4>(at(ks, o.a), r.ka[half]);
+    } else {
+        const uint16_t *k1 = (const uint16_t *)at(ks, o.a);
+#pragma unroll
+        for (int i = 0; i < NG / 2; i++) r.ka[half][i] = k1[2 * i] | (uint32_t)k1[2 * i + 1] << 16;
+        r.ka[half][NG / 2] = k1[NG - 1];
+    }
+}
+template <int NG>
+__device__ __forceinline__ void load_v(const uint8_t *reg, const KvArgs &a, uint32_t sub, int half, const Offs<NG> &o, Raw<NG> &r) {
+    constexpr int AL = NG % 4 == 0 ? 16 : NG % 2 == 0 ? 8 : 4;
+    load_aligned<NG, AL>(at(reg + (a.off_v + sub * (256u * NG)), o.v), r.v[half]);
+    load_aligned<2 * NG, 8>(at(reg + (a.off_vs + sub * (32u * NG)), o.s), r.vs[half]);
+}
+
+// The f16 in half i of w.
+__device__ __forceinline__ _Float16 half_of(uint32_t w, int i) {
+    return __builtin_bit_cast(_Float16, (unsigned short)(i ? w >> 16 : w));
+}
+
+// MFMA operand of group g of the K tile, eight codes of one key.
+// RAW: as they lie, plus 8, as subnormal f16 numbers of c * 2^-24 (nibbles in bits 0..3) and 16 c * 2^-24
+// (bits 4..7); q's values for the latter slots (2, 3, 6, 7) come divided by 16.  The matrix core
+// multiplies subnormals, but aligns its sums by the exponent field: 2^-14 of the sum is lost,
+// an eighth of an f16 q's own rounding and far above an f32 one's.
+// Otherwise the codes themselves.
+template <bool RAW, int NG>
+__device__ __forceinline__ f16x8 k_frag(const Raw<NG> &r, int half, int g, uint32_t magic) {
+    const uint32_t w = r.k[half][g], w8 = w >> 8;
+    Frag f;
+    if constexpr (RAW) {
+        f.w[0] = __builtin_bit_cast(f16x2, w & 0x000f000fu);
+        f.w[1] = __builtin_bit_cast(f16x2, w & 0x00f000f0u);
+        f.w[2] = __builtin_bit_cast(f16x2, w8 & 0x000f000fu);
+        f.w[3] = __builtin_bit_cast(f16x2, w8 & 0x00f000f0u);
+    } else {
+        f.w[0] = codes_f16<true>(w, magic);
+        f.w[1] = codes_f16<false>(w, magic);
+        f.w[2] = codes_f16<true>(w8, magic);
+        f.w[3] = codes_f16<false>(w8, magic);
+    }
+    return f.v;
+}
+
+// V's bytes of group g of keys 2 pr and 2 pr + 1 of a four-key block (NG dwords: [4][NG] bytes), one in each half.
+template <int NG>
+__device__ __forceinline__ uint32_t pair_bytes(const uint32_t (&v)[NG], int pr, int g) {
+    const int b0 = 2 * pr * NG + g, b1 = b0 + NG;
+    const uint32_t sel = 0x0c000c00u | (uint32_t)((b1 & 3) + 4) << 16 | (uint32_t)(b0 & 3);
+    return __builtin_amdgcn_perm(v[b1 >> 2], v[b0 >> 2], sel);
+}
+// The same of group 2i + odd, odd (0 or 1) uniform and not known to the compiler.
+template <int NG>
+__device__ __forceinline__ uint32_t pair_bytes(const uint32_t (&v)[NG], int pr, int i, int odd) {
+    if constexpr (NG % 2) {
+        const uint32_t even = pair_bytes<NG>(v, pr, 2 * i), other = pair_bytes<NG>(v, pr, min(2 * i + 1, NG - 1));
+        return odd ? other : even;
+    }
+    const int b0 = 2 * pr * NG + 2 * i, b1 = b0 + NG;  // even: both groups' bytes are in one dword
+    const uint32_t sel = 0x0c000c00u | (uint32_t)((b1 & 3) + 4) << 16 | (uint32_t)(b0 & 3);
+    return __builtin_amdgcn_perm(v[b1 >> 2], v[b0 >> 2], sel + (odd ? 0x00010001u : 0u));
+}
+
+// MFMA operands of group g of the V tile: eight keys of the values 32g + lane % 16 (lo) and
+// 32g + 16 + lane % 16 (hi).
+template <int NG>
+__device__ __forceinline__ void v_frags(const Raw<NG> &r, int g, uint32_t magic, f16x8 &lo, f16x8 &hi) {
+    Frag l, h;
+#pragma unroll
+    for (int half = 0; half < 2; half++)
+#pragma unroll
+        for (int pr = 0; pr < 2; pr++) {
+            const uint32_t t = pair_bytes<NG>(r.v[half], pr, g);
+            const f16x2 d = __builtin_bit_cast(f16x2, r.vs[half][2 * g + pr]);
+            l.w[2 * half + pr] = codes_f16<true>(t, magic) * d;
+            h.w[2 * half + pr] = codes_f16<false>(t, magic) * d;
+        }
+    lo = l.v;
+    hi = h.v;
+}
+
+// tanh to 2^-22 of its range: (1 - t) / (1 + t) with t = exp(-2 |v|), and its series below 1/4
+// (the next term is 2^-27 of the value there), where 1 - t loses bits.
+__device__ __forceinline__ float tanh_of(float v) {
+    const float t = __builtin_amdgcn_exp2f(fabsf(v) * -2.8853900817779268f);
+    const float w = v * v;
+    const float s = v + v * w * (-1.0f / 3 + w * (2.0f / 15 + w * (-17.0f / 315 + w * (62.0f / 2835))));
+    return fabsf(v) < 0.25f ? s : copysignf((1.0f - t) * __builtin_amdgcn_rcpf(1.0f + t), v);
+}
+
+// A power of two that puts a row's largest |q| into [2^14, 2^15), where two f16 parts hold 22 bits of it,
+// with the sign of `scale` (the scores' sign goes into q: larger products, larger scores), and its inverse.
+struct RowScale {
+    float up, down;
+};
+__device__ __forceinline__ RowScale row_scale(float top, float scale) {
+    const int ex = min(max(top > 0.0f ? 141 - (int)(__builtin_bit_cast(uint32_t, top) >> 23) : 0, -126), 126);
+    return {__builtin_bit_cast(float, (uint32_t)(ex + 127) << 23) * (scale < 0.0f ? -1.0f : 1.0f),
+            __builtin_bit_cast(float, (uint32_t)(127 - ex) << 23)};
+}
+
+__device__ __forceinline__ float row_max(float v) {  // over the lanes of one matrix column
+    v = fmaxf(v, __shfl_xor(v, 16));
+    return fmaxf(v, __shfl_xor(v, 32));
+}
+
+// Eight values of q from element i on (zeros where !on).
+__device__ __forceinline__ void load8_q(const AttnArgs &a, int64_t i, bool on, float (&o)[8]) {
+#pragma unroll
+    for (int e = 0; e < 8; e++) o[e] = 0.0f;
+    if (!on) return;
+    if (a.q_dtype == ARFQ_F16) {
+        const f16x8 v = *(const f16x8 *)((const _Float16 *)a.q + i);
+#pragma unroll
+        for (int e = 0; e < 8; e++) o[e] = (float)v[e];
+    } else {
+        const f32x4 v = *(const f32x4 *)((const float *)a.q + i), w = *(const f32x4 *)((const float *)a.q + i + 4);
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            o[e] = v[e];
+            o[4 + e] = w[e];
+        }
+    }
+}
+
+__device__ __forceinline__ void store_out(const AttnArgs &a, int64_t i, f32x4 v) {
+    if (a.out_dtype == ARFQ_F16)
+        *(u32x2 *)((_Float16 *)a.out + i) = u32x2{pack_f16x2(v[0], v[1]), pack_f16x2(v[2], v[3])};
+    else
+        *(f32x4 *)((float *)a.out + i) = v;
+}
+
+}  // namespace
+}  // namespace arfq

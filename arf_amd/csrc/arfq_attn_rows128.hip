@@ -1,0 +1,331 @@
+// arfq_attn_rows128.hip -- attention over the 4-bit K/V cache for prompts: tiles of 128 rows.
+//
+// A workgroup's four waves take 32 rows each and step through the keys together, 32 at a time: they
+// turn K and V of a step into f16 once, in LDS, and every wave multiplies all of it.  As in the
+// kernel of few rows, S^T = K Q^T and O^T = V^T P^T (v_mfma_f32_32x32x16_f16): a row is a lane's
+// column throughout, so its maximum and sum are registers, and the scores' registers 8b .. 8b + 7 are, as
+// they lie, the second product's operand for keys
+//     16b + 4h + {0, 1, 2, 3} and 16b + 8 + 4h + {0, 1, 2, 3}      (h = lane / 32),
+// the order in which V goes to LDS.
+#include "arfq_attn.h"
+
+namespace arfq {
+namespace {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+constexpr int TR = 128, WR = 32;  // rows of a tile, of a wave
+constexpr int WAVES = TR / WR, THREADS = 64 * WAVES;
+
+// LDS of a step: K [32][D + 8] f16 (rows 16 bytes apart in the banks), V [4][D][8] f16: lane
+// half and key block, value, keys.
+template <int NG>
+struct Step {
+    static constexpr int D = 32 * NG, KS = D + 8;
+    static constexpr int K_BYTES = STEP * KS * 2, BYTES = K_BYTES + STEP * D * 2;
+};
+
+// What a thread turns into f16: dwords t, t + 256, .. of the two K tiles (64 NG dwords each), and of V
+// the four keys (t / 16) % 8 of row t % 16, groups t / 128, t / 128 + 2, ..
+template <int NG>
+struct Part {
+    static constexpr int NK = (128 * NG + THREADS - 1) / THREADS, NV = (NG + 1) / 2;
+    uint32_t k[NK], ks[NK], v[NG], vs[NV][2];
+};
+
+template <int NG, int PARTS>
+__global__ __launch_bounds__(THREADS, NG <= 4 && PARTS == 1 ? 3 : rows128_waves(NG)) void attn_rows128(AttnArgs a) {
+    constexpr int D = 32 * NG, KS = Step<NG>::KS;
+    extern __shared__ uint8_t lds[];
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), c = lane & 31, h = lane >> 5;
+    const int head = blockIdx.x % a.c.heads;
+    Item it;
+    if (!find_item<TR, true>(a, blockIdx.x / a.c.heads, it)) return;
+    const Seq &s = it.s;
+    if (a.causal) it.tile = s.tiles - 1 - it.tile;  // (the longest first; a tile's pieces stay together)
+    const int slot = a.causal ? it.slot + (2 * it.tile - s.tiles + 1) * it.pieces : it.slot;
+
+    auto row_hi = [&](int64_t pos) { return pos < 0 ? 0 : a.causal ? (int)min(pos + 1, (int64_t)s.end) : s.end; };
+    auto row_lo = [&](int64_t pos) { return a.window ? (int)max((int64_t)0, min(pos - a.window + 1, (int64_t)s.end)) : 0; };
+    const int rows = s.n * a.group, piece_lo = s.lo + it.piece * it.keys, piece_hi = min(s.end, piece_lo + it.keys);
+    auto pos_of = [&](int row) { return (int64_t)s.len - s.n + min(row, rows - 1) / a.group; };
+    // keys of the tile in this piece; of the wave's rows; and those that every row of the wave has
+    const int first = max(row_lo(pos_of(it.tile * TR)) & ~(STEP - 1), piece_lo);
+    const int last = min(row_hi(pos_of(it.tile * TR + TR - 1)), piece_hi);
+    const int row0 = it.tile * TR + wave * WR;
+    const int64_t pos0 = pos_of(row0), pos1 = pos_of(row0 + WR - 1);
+    const int wave_lo = row_lo(pos0), wave_hi = row0 < rows ? min(row_hi(pos1), piece_hi) : 0;
+    const int inner_lo = row_lo(pos1), inner_hi = min(row_hi(pos0), piece_hi);
+    const int row = row0 + c;
+    const bool valid = row < rows;
+    const int tok = valid ? row / a.group : 0, gh = valid ? row - tok * a.group : 0;
+    const int64_t pos = (int64_t)s.len - s.n + tok;
+    const int lo = row_lo(pos), hi = min(valid ? row_hi(pos) : 0, piece_hi);
+
+    // ---- a step's K and V: from the cache to registers, and to LDS as f16 ----
+    Pages pages(a.c, it.b, head);
+    constexpr int NK = Part<NG>::NK, NV = Part<NG>::NV;
+    int k_half[NK];
+    uint32_t k_off[NK], ks_off[NK];
+#pragma unroll
+    for (int i = 0; i < NK; i++) {
+        const int w = t + i * THREADS;  // dword of the tiles (the same tile for a whole wave)
+        k_half[i] = __builtin_amdgcn_readfirstlane(w / (64 * NG));
+        const int o = w - k_half[i] * 64 * NG;
+        k_off[i] = 4 * o;
+        ks_off[i] = (o / (4 * NG) * NG + o % NG) * 2;
+    }
+    const uint32_t v_off = ((t >> 4) & 3) * (64 * NG) + (t & 15) * (4 * NG), vs_off = ((t >> 4) & 3) * (8 * NG);
+    auto load = [&](const Places &at_p, Part<NG> &p) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < NK; i++) {
+            if ((128 * NG) % THREADS && t + i * THREADS >= 128 * NG) break;
+            const uint8_t *reg = k_half[i] ? at_p.reg[1] : at_p.reg[0];
+            const uint32_t sub = k_half[i] ? at_p.sub[1] : at_p.sub[0];
+            p.k[i] = *(const uint32_t *)at(reg + sub * (256u * NG), k_off[i]);
+            p.ks[i] = *(const uint16_t *)at(reg + (a.c.off_ks + sub * (32u * NG)), ks_off[i]);
+        }
+        const uint8_t *reg = wave & 1 ? at_p.reg[1] : at_p.reg[0];
+        const uint32_t sub = wave & 1 ? at_p.sub[1] : at_p.sub[0];
+        constexpr int AL = NG % 4 == 0 ? 16 : NG % 2 == 0 ? 8 : 4;
+        load_aligned<NG, AL>(at(reg + (a.c.off_v + sub * (256u * NG)), v_off), p.v);
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            const int g = min((wave >> 1) + 2 * i, NG - 1);
+            load_aligned<2, 8>(at(reg + (a.c.off_vs + sub * (32u * NG) + g * 8), vs_off), p.vs[i]);
+        }
+    };
+    const uint32_t magic = magic_1024();
+    auto store = [&](uint8_t *kb, const Part<NG> &p) __attribute__((always_inline)) {
+        uint8_t *vb = kb + Step<NG>::K_BYTES;
+#pragma unroll
+        for (int i = 0; i < NK; i++) {
+            const int w = t + i * THREADS;
+            if ((128 * NG) % THREADS && w >= 128 * NG) break;
+            const int key = w / (4 * NG), chunk = w % NG * 4 + w / NG % 4;  // (dword (key, quarter, group))
+            const uint32_t w8 = p.k[i] >> 8;
+            uint32_t d1 = p.ks[i];
+            asm volatile("" : "+v"(d1));  // (or two scales are packed into one register as soon as they are loaded: a wait)
+            const f16x2 d = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(d1, d1, 0x01000100u));
+            Frag f;
+            f.w[0] = codes_f16<true>(p.k[i], magic) * d;
+            f.w[1] = codes_f16<false>(p.k[i], magic) * d;
+            f.w[2] = codes_f16<true>(w8, magic) * d;
+            f.w[3] = codes_f16<false>(w8, magic) * d;
+            *(f16x8 *)(kb + key * (KS * 2) + chunk * 16) = f.v;
+        }
+        const int half = wave & 1, q = (t >> 4) & 3;
+        uint8_t *to = vb + ((half * 2 + (q & 1)) * D + (t & 15)) * 16 + (q >> 1) * 8;
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            // (the group is the wave's: a byte of each key's dwords by a selector in a register)
+            const int g = (wave >> 1) + 2 * i;
+            if (NG % 2 && g >= NG) break;
+            f16x2 l[2], u[2];
+#pragma unroll
+            for (int pr = 0; pr < 2; pr++) {
+                const uint32_t w = pair_bytes<NG>(p.v, pr, i, wave >> 1);
+                const f16x2 d = __builtin_bit_cast(f16x2, p.vs[i][pr]);
+                l[pr] = codes_f16<true>(w, magic) * d;
+                u[pr] = codes_f16<false>(w, magic) * d;
+            }
+            *(u32x2 *)(to + g * 512) = u32x2{__builtin_bit_cast(uint32_t, l[0]), __builtin_bit_cast(uint32_t, l[1])};
+            *(u32x2 *)(to + g * 512 + 256) = u32x2{__builtin_bit_cast(uint32_t, u[0]), __builtin_bit_cast(uint32_t, u[1])};
+        }
+    };
+
+    Part<NG> part;
+    bool in[2] = {false, false}, nin[2] = {false, false};  // the tiles that are multiplied, and those in registers
+    if (first < last) {
+        const Places p = pages.at(a.c, first);
+        in[0] = p.in[0];
+        in[1] = p.in[1];
+        load(p, part);
+    }
+
+    // ---- q as operands, values 16i + 8h .. +7 of the row, scaled as in the kernel of few rows ----
+    f16x8 q[PARTS][2 * NG];
+    float sc = fabsf(a.scale);
+    {
+        float top = 0.0f;
+        const int64_t qo = ((int64_t)s.t0 + tok) * a.q_stride + (int64_t)(head * a.group + gh) * D + 8 * h;
+        float x[8];
+        if constexpr (PARTS == 2) {
+#pragma unroll
+            for (int i = 0; i < 2 * NG; i++) {
+                load8_q(a, qo + 16 * i, valid, x);
+#pragma unroll
+                for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(x[e]));
+            }
+            top = fmaxf(top, __shfl_xor(top, 32));
+        }
+        const RowScale rs = row_scale(PARTS == 2 ? top : 0.0f, a.scale);
+        sc *= rs.down;
+#pragma unroll
+        for (int i = 0; i < 2 * NG; i++) {
+            load8_q(a, qo + 16 * i, valid, x);
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const float v = x[e] * rs.up;
+                const _Float16 f = (_Float16)v;
+                q[0][i][e] = f;
+                if constexpr (PARTS == 2) q[1][i][e] = (_Float16)(v - (float)f);
+            }
+        }
+    }
+    constexpr float LOG2E = 1.4426950408889634f;
+    const float cap = a.softcap, x_of_s = fmaxf(cap > 0.0f ? sc / cap : sc * LOG2E, 1.1754944e-38f), x_of_t = cap * LOG2E;
+
+    f32x16 acc[NG];
+    const f32x16 zero = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < NG; i++) acc[i] = zero;
+    float m = -INFINITY, sum = 0.0f;
+
+    // one step: multiplies K and V of keys k0 .. in `cur`, puts those of the next step, in registers, into
+    // `other` and loads the ones after
+    auto step = [&](int k0, const uint8_t *kb, uint8_t *other) __attribute__((always_inline)) {
+        const uint8_t *vb = kb + Step<NG>::K_BYTES;
+        const bool in0 = in[0], in1 = in[1];
+        if (k0 + STEP < last) {
+            store(other, part);
+            in[0] = nin[0];
+            in[1] = nin[1];
+            if (k0 + 2 * STEP < last) {
+                const Places p = pages.at(a.c, k0 + 2 * STEP);
+                nin[0] = p.in[0];
+                nin[1] = p.in[1];
+                load(p, part);
+            }
+        }
+        if (k0 < wave_hi && k0 + STEP > wave_lo) {
+            f32x16 x = zero;
+#pragma unroll
+            for (int i = 0; i < 2 * NG; i++) {
+                const f16x8 kf = *(const f16x8 *)(kb + c * (KS * 2) + (2 * i + h) * 16);
+#pragma unroll
+                for (int p = 0; p < PARTS; p++) x = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, q[p][i], x, 0, 0, 0);
+            }
+            float unit = x_of_s;
+            if (cap > 0.0f) {
+#pragma unroll
+                for (int i = 0; i < 16; i++) x[i] = tanh_of(x[i] * x_of_s) * x_of_t;
+                unit = 1.0f;
+            }
+            if (k0 < inner_lo || k0 + STEP > inner_hi || !in0 || !in1) {
+#pragma unroll
+                for (int half = 0; half < 2; half++) {
+                    const uint32_t from = (uint32_t)(k0 + half * 16 + 4 * h - lo), width = (half ? in1 : in0) ? (uint32_t)max(hi - lo, 0) : 0u;
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const int at = (i >> 2) * 8 + (i & 3);
+                        x[8 * half + i] = from + at < width ? x[8 * half + i] : -INFINITY;
+                    }
+                }
+            }
+            float top = x[0];
+#pragma unroll
+            for (int i = 1; i < 16; i++) top = fmaxf(top, x[i]);
+            top *= unit;
+            if (__ballot(top > m + M_SLACK)) {
+                const float mn = fmaxf(m, fmaxf(top, __shfl_xor(top, 32)));
+                const float f = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+                m = mn;
+                sum *= f;
+#pragma unroll
+                for (int i = 0; i < NG; i++) acc[i] *= f;
+            }
+            const float mb = P_BIAS - (m == -INFINITY ? 0.0f : m);
+#pragma unroll
+            for (int b = 0; b < 2; b++) {
+                Frag p[PARTS];
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const float v0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[8 * b + 2 * i], unit, mb));
+                    const float v1 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[8 * b + 2 * i + 1], unit, mb));
+                    const f16x2 f = {(_Float16)v0, (_Float16)v1};
+                    p[0].w[i] = f;
+                    if constexpr (PARTS == 2) {
+                        p[1].w[i] = f16x2{(_Float16)(v0 - (float)f[0]), (_Float16)(v1 - (float)f[1])};
+                        sum += v0 + v1;
+                    } else {
+                        // (what the values are multiplied with: a rounding of p then moves both alike)
+                        sum = __builtin_amdgcn_fdot2(f, f16x2{(_Float16)1, (_Float16)1}, sum, false);
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < NG; i++) {
+                    const f16x8 vf = *(const f16x8 *)(vb + ((b * 2 + h) * D + 32 * i + c) * 16);
+#pragma unroll
+                    for (int pp = 0; pp < PARTS; pp++)
+                        acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, p[pp].v, acc[i], 0, 0, 0);
+                }
+            }
+        }
+        lds_barrier();
+    };
+    uint8_t *buf0 = lds, *buf1 = lds + Step<NG>::BYTES;
+    if (first < last) {
+        store(buf0, part);
+        if (first + STEP < last) {
+            const Places p = pages.at(a.c, first + STEP);
+            nin[0] = p.in[0];
+            nin[1] = p.in[1];
+            load(p, part);
+        }
+    }
+    lds_barrier();
+    for (int k0 = first; k0 < last; k0 += 2 * STEP) {
+        step(k0, buf0, buf1);
+        if (k0 + STEP < last) step(k0 + STEP, buf1, buf0);
+    }
+
+    sum += __shfl_xor(sum, 32);
+    if (!valid) return;
+    const int64_t o = ((int64_t)s.t0 + tok) * a.out_stride + (int64_t)(head * a.group + gh) * D;
+    const bool whole = it.pieces == 1;
+    if (!whole && (slot < 0 || slot >= a.many.slots)) return;
+    float *to = a.many.part + (((int64_t)slot * a.c.heads + head) * TR + wave * WR + c) * (D + 4);
+    const float inv = whole ? (sum == 0.0f ? 0.0f : 1.0f / sum) : 1.0f;
+#pragma unroll
+    for (int i = 0; i < NG; i++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            f32x4 v = {acc[i][4 * j], acc[i][4 * j + 1], acc[i][4 * j + 2], acc[i][4 * j + 3]};
+            const int e = 32 * i + 8 * j + 4 * h;
+            if (whole)
+                store_out(a, o + e, v * inv);
+            else
+                *(f32x4 *)(to + 4 + e) = v;
+        }
+    if (!whole && h == 0) *(float2 *)to = make_float2(m, sum);
+}
+
+template <int NG, int PARTS>
+hipError_t rows128_launch(const AttnArgs &a, hipStream_t s) {
+    static std::atomic<uint64_t> done{0};
+    constexpr size_t bytes = 2 * Step<NG>::BYTES;
+    const hipError_t e = set_max_lds_once((const void *)attn_rows128<NG, PARTS>, bytes, done);
+    if (e != hipSuccess) return e;
+    attn_rows128<NG, PARTS><<<dim3((unsigned)a.many.slots * a.c.heads), THREADS, bytes, s>>>(a);
+    return hipGetLastError();
+}
+
+template <int NG>
+hipError_t rows128_launch(const AttnArgs &a, hipStream_t s) {
+    return a.q_dtype == ARFQ_F16 && a.out_dtype == ARFQ_F16 ? rows128_launch<NG, 1>(a, s) : rows128_launch<NG, 2>(a, s);
+}
+
+}  // namespace
+
+hipError_t launch_attn_rows128(const AttnArgs &a, int dim, hipStream_t s) {
+    switch (dim) {
+    case 64: return rows128_launch<2>(a, s);
+    case 96: return rows128_launch<3>(a, s);
+    case 128: return rows128_launch<4>(a, s);
+    case 256: return rows128_launch<8>(a, s);
+    }
+    return hipErrorInvalidValue;
+}
+
+}  // namespace arfq

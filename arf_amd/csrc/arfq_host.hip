@@ -525,6 +525,8 @@ static int kv_args(arfq_ctx *ctx, const arfq_kv *kv, const arfq_kv_seqs *s, cons
     a->page = kv->page;
     a->tiles = kv->page / arfq::KV_TILE;
     a->tile_magic = a->tiles > 1 ? (uint32_t)((((uint64_t)1 << 32) + a->tiles - 1) / a->tiles) : 0;
+    a->tile_mask = a->tiles > 1 ? 0 : ~0u;
+    a->page_bytes = (uint32_t)(l.region * kv->heads);
     a->n_pages = (int)kv->pages;
     a->batch = (int)s->batch;
     a->tokens = (int)s->tokens;
@@ -590,7 +592,8 @@ int arfq_kv_attention_workspace(arfq_ctx *ctx, const arfq_kv *kv, int64_t batch,
     if (int rc = kv_q_heads(ctx, kv, batch, tokens, q_heads)) return rc;
     if (max_pages < 0 || max_pages > arfq::KV_KEYS_MAX / kv->page)
         return fail(ctx, ARFQ_E_SHAPE, "kv_attention_workspace: max_pages * page_size above 2^29");
-    *bytes = arfq::attn_plan(ctx->cus, kv->heads, kv->dim, batch, tokens, q_heads, max_pages * kv->page).ws_bytes;
+    // (with a start: the larger)
+    *bytes = arfq::attn_plan(ctx->cus, kv->heads, kv->dim, batch, tokens, q_heads, max_pages * kv->page, false).ws_bytes;
     return ARFQ_OK;
 }
 
@@ -609,7 +612,7 @@ int arfq_kv_attention(arfq_ctx *ctx, const arfq_kv *kv, const arfq_kv_seqs *seqs
     if (int rc = kv_rows(ctx, "kv_attention: out", out, out_stride, q_heads, kv->dim, out_dtype)) return rc;
     if (int rc = use_device(ctx)) return rc;
     const arfq::AttnPlan plan = arfq::attn_plan(ctx->cus, kv->heads, kv->dim, seqs->batch, seqs->tokens, q_heads,
-                                                    seqs->max_pages * kv->page);
+                                                    seqs->max_pages * kv->page, !seqs->start);
     if (workspace) {
         if (workspace_bytes < plan.ws_bytes || (uintptr_t)workspace % 16)
             return fail(ctx, ARFQ_E_SHAPE, "kv_attention: workspace of " + std::to_string(workspace_bytes) + " bytes, " +
@@ -628,16 +631,15 @@ int arfq_kv_attention(arfq_ctx *ctx, const arfq_kv *kv, const arfq_kv_seqs *seqs
     a.out_stride = out_stride;
     a.q_dtype = q_dtype;
     a.out_dtype = out_dtype;
-    a.q_heads = q_heads;
     a.group = q_heads / kv->heads;
     a.scale = scale;
     a.softcap = softcap;
     a.window = (int)std::min<int64_t>(window, INT32_MAX);
     a.causal = causal != 0;
-    a.target = plan.target;
-    a.slots = plan.slots;
+    a.few_rows = plan.few_rows;
+    a.few = {plan.few.tiles, plan.few.target, plan.few.slots, (float *)workspace};
+    a.many = {plan.many.tiles, plan.many.target, plan.many.slots, (float *)((char *)workspace + plan.few.ws_bytes)};
     a.joins = plan.joins;
-    a.part = (float *)workspace;
     const hipError_t e = arfq::launch_attn(a, kv->dim, ctx->stream);
     return e == hipSuccess ? ARFQ_OK : hip_fail(ctx, e, "kv_attention launch");
 }

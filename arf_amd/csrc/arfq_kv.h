@@ -52,7 +52,9 @@ struct KvArgs {
     int64_t region;
     int off_v, off_ks, off_vs;
     int heads, page, tiles;  // tiles = page / KV_TILE
-    uint32_t tile_magic;     // ceil(2^32 / tiles) (tiles > 1)
+    uint32_t page_bytes;     // of all heads: at most 1024 * 72 KB
+    uint32_t tile_magic;     // ceil(2^32 / tiles); 0 for one tile a page
+    uint32_t tile_mask;      // all bits for one tile a page; 0
     int n_pages;
     // the batch
     int batch, tokens;
@@ -63,7 +65,7 @@ struct KvArgs {
 // Page of 16-key tile `t` of a sequence.  t < 2^27 (32-bit positions), tiles <= 16: the product
 // with the rounded-up reciprocal is off by less than t * tiles / 2^32 < 1/2 of a step.
 __device__ __forceinline__ int kv_page_of(const KvArgs &a, int t) {
-    return a.tiles == 1 ? t : (int)__umulhi((uint32_t)t, a.tile_magic);
+    return (int)(__umulhi((uint32_t)t, a.tile_magic) + ((uint32_t)t & a.tile_mask));
 }
 
 // First token and token count of sequence b (0 tokens where `start` does not increase or
@@ -84,30 +86,45 @@ hipError_t launch_kv_write(const KvArgs &a, int dim, const void *k, int64_t k_st
 hipError_t launch_kv_read(const KvArgs &a, int dim, void *k, int64_t k_stride, void *v, int64_t v_stride, int dtype,
                           hipStream_t s);
 
-// ---- attention (arfq_attn.hip) ----
+// ---- attention (arfq_attn.hip, arfq_attn_rows128.hip) ----
+// A work list (arfq_attn.h): its tiles at most, the pieces it aims at, its items at most, and
+// the parts of rows of more than one piece, [slots][heads][rows of a tile][dim + 4]: maximum,
+// sum, -, -, values.
+struct AttnListPlan {
+    int tiles = 0, target = 1, slots = 0;
+    size_t ws_bytes = 0;
+};
+struct AttnList {
+    int tiles, target, slots;
+    float *part;
+};
 struct AttnArgs {
     KvArgs c;
     const void *q;
     void *out;
     int64_t q_stride, out_stride;  // elements between tokens
     int q_dtype, out_dtype;
-    int q_heads, group;  // group = q_heads / heads
+    int group;  // q heads of a K/V head
     float scale, softcap;
-    int window;          // 0: none
+    int window;  // 0: none
     int causal;
-    // the work list: see attn_plan
-    int target, slots;
-    int joins;           // gridDim.z of the join (0: no tile has two pieces)
-    float *part;         // parts, [slots][heads][16][dim + 4]: maximum, sum, -, -, values
+    int few_rows;         // sequences with at most so many rows are in `few` (16-row tiles), others in `many` (128)
+    AttnList few, many;
+    int joins;  // gridDim.z of the join (0: no row has two pieces)
 };
 struct AttnPlan {
-    int target = 1;     // pieces per head the keys are cut into, beside one per row tile
-    int slots = 1;      // bound on the work items per head
+    int few_rows = 0;
+    AttnListPlan few, many;
     int joins = 0;
-    size_t ws_bytes = 0;
+    size_t ws_bytes = 0;  // few's parts, then many's
 };
 bool attn_dim_ok(int dim);
-AttnPlan attn_plan(int cus, int heads, int dim, int64_t batch, int64_t tokens, int q_heads, int64_t max_keys);
+// max_keys: of a sequence; one_each: a token of every sequence (no start)
+AttnPlan attn_plan(int cus, int heads, int dim, int64_t batch, int64_t tokens, int q_heads, int64_t max_keys, bool one_each);
 hipError_t launch_attn(const AttnArgs &a, int dim, hipStream_t s);
+// `many`'s tiles
+hipError_t launch_attn_rows128(const AttnArgs &a, int dim, hipStream_t s);
+// workgroups of it that a compute unit holds (a wave each on every SIMD), at ng groups of 32 values
+constexpr int rows128_waves(int ng) { return ng <= 4 ? 2 : 1; }
 
 }  // namespace arfq
