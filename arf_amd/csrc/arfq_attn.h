@@ -83,17 +83,16 @@ struct Item {
     Seq s;
     int b, tile, piece, pieces;
     int keys;  // of a piece (a multiple of STEP): the sequence's keys in equal parts
-    int slot;  // place of the (tile, piece) in the list of all
+    int slot;  // place in the list
 };
 
 // The `index`-th (tile, piece) of the batch: sequences in order, their tiles one after another,
-// pieces fastest; or (PIECES false) the first piece of the index-th tile.  False: the list has
-// fewer.  The keys that make a new piece necessary are the same in every wave of the launch: the
-// fewest that cut the area into at most `target` pieces, or nearly so (a target of workgroups that
-// the chip holds at once: one more round for a few of them would take as long as the first).
-// The area is summed in f32 in one fixed order; the 2^-16 added covers its rounding, so that the
-// list has no more than target + tiles items.
-template <int TR, bool PIECES>
+// pieces fastest.  False: the list has fewer.  The keys that make a new piece necessary are the same
+// in every wave of the launch: the fewest that cut the area into at most `target` pieces, or
+// nearly so (a target of workgroups that the chip holds at once: one more round for a few of
+// them would take as long as the first).  The area is summed in f32 in one fixed order; the 2^-16
+// added covers its rounding, so that the list has no more than target + tiles items.
+template <int TR>
 __device__ __forceinline__ bool find_item(const AttnArgs &a, int index, Item &it) {
     const int lane = threadIdx.x & 63;
     const Seq s0 = seq_of<TR>(a, lane);  // (the whole batch, mostly)
@@ -114,11 +113,10 @@ __device__ __forceinline__ bool find_item(const AttnArgs &a, int index, Item &it
         steps = ceilf(steps * fminf(items / target, 2.0f));
     }
     const int piece = keys_of(steps);
-    int before = 0, items = 0;
+    int before = 0;
     for (int b0 = 0; b0 < a.c.batch; b0 += WAVE) {
         const Seq s = b0 ? seq_of<TR>(a, b0 + lane) : s0;
-        const int np = pieces_of(s, piece), all = (int)min((int64_t)s.tiles * np, (int64_t)1 << 30);
-        const int own = PIECES ? all : s.tiles, inc = wave_scan(own), sum = PIECES ? inc : wave_scan(all);
+        const int np = pieces_of(s, piece), own = (int)min((int64_t)s.tiles * np, (int64_t)1 << 30), inc = wave_scan(own);
         const uint64_t past = __ballot(before + inc > index);
         if (past) {
             const int l = __ffsll((unsigned long long)past) - 1;
@@ -130,17 +128,39 @@ __device__ __forceinline__ bool find_item(const AttnArgs &a, int index, Item &it
             it.s.tiles = __builtin_amdgcn_readlane(s.tiles, l);
             it.pieces = __builtin_amdgcn_readlane(np, l);
             it.b = b0 + l;
+            it.slot = index;
             it.keys = ((it.s.end - it.s.lo + STEP - 1) / STEP + it.pieces - 1) / it.pieces * STEP;
             const int rest = index - before - __builtin_amdgcn_readlane(inc - own, l);
-            it.tile = PIECES ? rest / it.pieces : rest;
-            it.piece = PIECES ? rest - it.tile * it.pieces : 0;
-            it.slot = PIECES ? index : items + __builtin_amdgcn_readlane(sum - all, l) + it.tile * it.pieces;
-            return rest >= 0 && it.tile < it.s.tiles && it.slot >= 0;
+            it.tile = rest / it.pieces;
+            it.piece = rest - it.tile * it.pieces;
+            // Prompts: the longest tile first, and every other round of workgroups (one a compute unit)
+            // backwards, so that a unit's first and second tile are long and short.
+            if (TR == 128 && a.causal) {
+                const int round = list_of<TR>(a).round, tiles = it.s.tiles;
+                if (it.pieces == 1 && a.c.batch == 1 && (it.tile / round & 1)) {
+                    const int lo = it.tile / round * round, hi = min(lo + round, tiles);
+                    it.tile = hi - 1 - (it.tile - lo);
+                }
+                it.tile = tiles - 1 - it.tile;
+            }
+            return rest >= 0 && it.tile >= 0 && it.tile < it.s.tiles;
         }
         before += __builtin_amdgcn_readlane(inc, 63);
-        items += __builtin_amdgcn_readlane(sum, 63);
     }
     return false;
+}
+
+// The workgroup's item, and what the join has to know of it (the list's every place is written).
+template <int TR>
+__device__ __forceinline__ bool take_item(const AttnArgs &a, int block, Item &it) {
+    const AttnList &list = list_of<TR>(a);
+    const int slot = block / a.c.heads;
+    const bool got = find_item<TR>(a, slot, it);
+    if (list.join && block % a.c.heads == 0 && threadIdx.x == 0) {
+        const bool first = got && it.piece == 0 && it.pieces > 1;
+        list.join[slot] = make_int4(first ? it.pieces : 0, it.tile * TR, it.s.n * a.group, it.s.t0);
+    }
+    return got;
 }
 
 // Where a step's two 16-key tiles are: the (page, head) regions (page 0's for a page that is not the cache's:

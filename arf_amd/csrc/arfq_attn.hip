@@ -1,273 +1,18 @@
 // arfq_attn.hip -- attention over the 4-bit K/V cache: few rows a sequence (decode), and the joining
 // of rows whose keys were cut into pieces.
-#include "arfq_attn.h"
+#include "arfq_attn_rows16.h"
 
 #include <algorithm>
 
 namespace arfq {
 namespace {
 
-constexpr int TR = 16;    // rows of a tile
-constexpr int WAVES = 4;  // of a workgroup
 // rows of a sequence that the 16-row tiles take
 constexpr int64_t FEW_ROWS = 64;
-// waves of a SIMD (a workgroup has one on each): registers below 512 / that
-constexpr int rows16_waves(int ng) { return ng <= 2 ? 4 : ng <= 4 ? 3 : 2; }
-constexpr float BIAS_UNIT = 32768.0f;
 
-// ---- rows of 16, keys spread over the waves ------------------------------------------------
-// S^T = K Q^T, O^T = V^T P^T with v_mfma_f32_16x16x32_f16: the 16 rows are matrix columns, so a
-// lane's four results of a tile belong to one row, its statistics are a register, and P^T in
-// the layout of a result is the layout of the next product's operand (which keys a lane's
-// eight slots stand for is free, as V is loaded to match).  K's scales multiply the products of
-// a group (32 values: one MFMA), V's its codes.
-// PARTS: f16 parts of q and p (2: hi + lo, 22 bits, for f32 q or out).
-template <int NG, int PARTS>
-__global__ __launch_bounds__(64 * WAVES, rows16_waves(NG)) void attn_rows16(AttnArgs a) {
-    constexpr int D = 32 * NG, NT = 2 * NG;  // NT: 16-row tiles of O^T
-    constexpr bool RAW = PARTS == 1;         // K's operands: see k_frag
-    constexpr int OS = D + 4;                // LDS floats of a row of O
-    extern __shared__ float lds[];           // [WAVES][16][OS], then [WAVES][16][2]
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, h = lane >> 4;
-    const int head = blockIdx.x % a.c.heads;  // (fastest: the list's unused end comes last)
-    Item it;
-    if (!find_item<TR, true>(a, blockIdx.x / a.c.heads, it)) return;
-    const Seq &s = it.s;
-
-    // keys [lo, hi) of the row of token tok
-    auto row_hi = [&](int64_t pos) { return pos < 0 ? 0 : a.causal ? (int)min(pos + 1, (int64_t)s.end) : s.end; };
-    auto row_lo = [&](int64_t pos) { return a.window ? (int)max((int64_t)0, min(pos - a.window + 1, (int64_t)s.end)) : 0; };
-    const int rows = s.n * a.group, piece_lo = s.lo + it.piece * it.keys, piece_hi = min(s.end, piece_lo + it.keys);
-    // the tile's keys in this piece, and those that every row has (both ends rise with the token)
-    const int64_t pos0 = (int64_t)s.len - s.n + it.tile * TR / a.group;
-    const int64_t pos1 = (int64_t)s.len - s.n + min(it.tile * TR + TR - 1, rows - 1) / a.group;
-    const int first = max(row_lo(pos0) & ~(STEP - 1), piece_lo), last = min(row_hi(pos1), piece_hi);
-    const int inner_lo = row_lo(pos1), inner_hi = min(row_hi(pos0), piece_hi);
-    // this lane's row
-    const int row = it.tile * TR + c;
-    const bool valid = row < rows;
-    const int tok = valid ? row / a.group : 0, gh = valid ? row - tok * a.group : 0;
-    const int64_t pos = (int64_t)s.len - s.n + tok;
-    const int lo = row_lo(pos), hi = min(valid ? row_hi(pos) : 0, piece_hi);
-
-    Pages pages(a.c, it.b, head);
-    constexpr int NEXT = WAVES * STEP;
-    const Offs<NG> offs = lane_offs<NG>();
-    Raw<NG> r;
-    int k0 = first + wave * STEP;
-    bool in[2] = {false, false};  // this step's tiles
-    Places next = {{nullptr, nullptr}, {0, 0}, {false, false}};
-    auto load_ks = [&](const Places &p) {
-#pragma unroll
-        for (int half = 0; half < 2; half++) load_k<RAW>(p.reg[half], a.c, p.sub[half], half, offs, r);
-    };
-    auto load_vs = [&](const Places &p) {
-#pragma unroll
-        for (int half = 0; half < 2; half++) load_v<NG>(p.reg[half], a.c, p.sub[half], half, offs, r);
-    };
-    if (k0 < last) {  // (keys: the table has a page)
-        next = pages.at(a.c, k0);
-        in[0] = next.in[0];
-        in[1] = next.in[1];
-        load_ks(next);
-        load_vs(next);
-        next = pages.at(a.c, k0 + NEXT);
-    }
-
-    // q as operands: values 32g + 8h .. +7 of the row, times a power of two that puts the row's
-    // largest into [2^14, 2^15): hi + lo hold 22 bits (an f16 q its 11)
-    f16x8 q[PARTS][NG];
-    // RAW codes come with 8 added: -8 times the sum of a group's q, in three f16 parts (lanes 0..15, 16..31,
-    // 32..47 of a row's), times K's scales is one more product
-    Frag bias;
-    const int64_t qo = ((int64_t)s.t0 + tok) * a.q_stride + (int64_t)(head * a.group + gh) * D + 8 * h;
-    float sc = fabsf(a.scale);
-    {
-        float x[NG][8], top = 0.0f;
-#pragma unroll
-        for (int g = 0; g < NG; g++) load8_q(a, qo + 32 * g, valid, x[g]);
-#pragma unroll
-        for (int g = 0; g < NG; g++)
-#pragma unroll
-            for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(x[g][e]));
-        top = row_max(top);
-        const RowScale rs = row_scale(top, a.scale);
-        sc *= rs.down;
-#pragma unroll
-        for (int i = 0; i < 4; i++) bias.w[i] = f16x2{(_Float16)0, (_Float16)0};
-#pragma unroll
-        for (int g = 0; g < NG; g++) {
-            float all = 0.0f;
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const float v = x[g][e] * rs.up * (RAW && (e & 2) ? 0.0625f : 1.0f);
-                const _Float16 t = (_Float16)v, l = (_Float16)(v - (float)t);
-                q[0][g][e] = t;
-                if constexpr (PARTS == 2) q[1][g][e] = l;
-                all += (float)t * (e & 2 ? 16.0f : 1.0f);
-            }
-            if constexpr (!RAW) continue;
-            all += __shfl_xor(all, 16);
-            all += __shfl_xor(all, 32);
-            all *= -8.0f / 16777216 * BIAS_UNIT;  // at most 8 * 32 * 2^15 / 2^24 * 2^15 = 2^14
-            const float b0 = (float)(_Float16)all, b1 = (float)(_Float16)(all - b0), b2 = all - b0 - b1;
-            bias.w[g / 2][g % 2] = (_Float16)(h == 0 ? b0 : h == 1 ? b1 : h == 2 ? b2 : 0.0f);
-        }
-    }
-    constexpr float LOG2E = 1.4426950408889634f;
-    constexpr float UNIT = RAW ? 16777216.0f : 1.0f;  // of the products (RAW: of codes * 2^-24)
-    // a product in the scores' log2, or in the cap (not below the smallest normal
-    // number, where products of it are 0 beside p's 24 bits: a masked score is -inf, and -inf * 0 would be NaN)
-    const float cap = a.softcap, x_of_s = fmaxf((cap > 0.0f ? sc / cap : sc * LOG2E) * UNIT, 1.1754944e-38f);
-    const float x_of_t = cap * LOG2E;
-
-    f32x4 acc[NT], sum = {0, 0, 0, 0};
-#pragma unroll
-    for (int t = 0; t < NT; t++) acc[t] = f32x4{0, 0, 0, 0};
-    float m = -INFINITY;
-    Frag ones;
-#pragma unroll
-    for (int i = 0; i < 4; i++) ones.w[i] = f16x2{(_Float16)1, (_Float16)1};
-    const uint32_t magic = magic_1024();
-
-    while (k0 < last) {
-        const int k1 = k0 + NEXT;
-        float x[8], unit = x_of_s;  // scores; a unit of them in log2
-#pragma unroll
-        for (int half = 0; half < 2; half++) {
-            const f32x4 z = {0, 0, 0, 0};
-            if constexpr (RAW) {
-                Frag ka;
-#pragma unroll
-                for (int i = 0; i < 4; i++) ka.w[i] = __builtin_bit_cast(f16x2, i < (NG + 1) / 2 ? r.ka[half][i] : 0u);
-                const f32x4 o = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka.v, bias.v, z, 0, 0, 0);
-#pragma unroll
-                for (int i = 0; i < 4; i++) x[4 * half + i] = o[i] * (1.0f / BIAS_UNIT);
-            }
-#pragma unroll
-            for (int g = 0; g < NG; g++) {
-                const f16x8 kf = k_frag<RAW>(r, half, g, magic);
-                f32x4 t = z;
-#pragma unroll
-                for (int p = 0; p < PARTS; p++) t = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, q[p][g], t, 0, 0, 0);
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const float d = (float)half_of(r.ks[half][(i * NG + g) / 2], (i * NG + g) & 1);
-                    x[4 * half + i] = !RAW && g == 0 ? t[i] * d : __builtin_fmaf(t[i], d, x[4 * half + i]);
-                }
-            }
-            // the scores are formed here: K's registers are free for the next step's loads
-            asm volatile("" : "+v"(x[4 * half]), "+v"(x[4 * half + 1]), "+v"(x[4 * half + 2]), "+v"(x[4 * half + 3]));
-        }
-        if (k1 < last) load_ks(next);
-        if (cap > 0.0f) {
-#pragma unroll
-            for (int i = 0; i < 8; i++) x[i] = tanh_of(x[i] * x_of_s) * x_of_t;
-            unit = 1.0f;
-        }
-        if (k0 < inner_lo || k0 + STEP > inner_hi || !in[0] || !in[1]) {
-#pragma unroll
-            for (int half = 0; half < 2; half++) {
-                const uint32_t from = (uint32_t)(k0 + half * 16 + 4 * h - lo), width = in[half] ? (uint32_t)max(hi - lo, 0) : 0u;
-#pragma unroll
-                for (int i = 0; i < 4; i++) x[4 * half + i] = from + i < width ? x[4 * half + i] : -INFINITY;
-            }
-        }
-        float top = x[0];
-#pragma unroll
-        for (int i = 1; i < 8; i++) top = fmaxf(top, x[i]);
-        top *= unit;
-        if (__ballot(top > m + M_SLACK)) {
-            const float mn = fmaxf(m, row_max(top));
-            const float f = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
-            m = mn;
-            sum *= f;
-#pragma unroll
-            for (int t = 0; t < NT; t++) acc[t] *= f;
-        }
-        const float mb = P_BIAS - (m == -INFINITY ? 0.0f : m);
-        f16x8 p[PARTS];
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const float v = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], unit, mb));
-            const _Float16 t = (_Float16)v;
-            p[0][i] = t;
-            if constexpr (PARTS == 2) p[1][i] = (_Float16)__builtin_fmaf((float)t, -1.0f, v);
-        }
-#pragma unroll
-        for (int pp = 0; pp < PARTS; pp++) sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones.v, p[pp], sum, 0, 0, 0);
-#pragma unroll
-        for (int g = 0; g < NG; g++) {
-            f16x8 vl, vh;
-            v_frags<NG>(r, g, magic, vl, vh);
-#pragma unroll
-            for (int pp = 0; pp < PARTS; pp++) {
-                acc[2 * g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl, p[pp], acc[2 * g], 0, 0, 0);
-                acc[2 * g + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, p[pp], acc[2 * g + 1], 0, 0, 0);
-            }
-        }
-        if (k1 < last) {
-            load_vs(next);
-            in[0] = next.in[0];
-            in[1] = next.in[1];
-            next = pages.at(a.c, k1 + NEXT);
-        }
-        k0 = k1;
-    }
-
-    // the waves' parts of the tile
-    float *ml = lds + WAVES * TR * OS;
-    if (h == 0) {
-        ml[(wave * TR + c) * 2] = m;
-        ml[(wave * TR + c) * 2 + 1] = sum[0];
-    }
-#pragma unroll
-    for (int t = 0; t < NT; t++) *(f32x4 *)(lds + (wave * TR + c) * OS + 16 * t + 4 * h) = acc[t];
-    __syncthreads();
-    // row er of the tile: 16 threads, 4 values at a time
-    const int er = threadIdx.x >> 4, u = threadIdx.x & 15;
-    float f[WAVES], mm = -INFINITY, l = 0.0f;
-#pragma unroll
-    for (int w = 0; w < WAVES; w++) mm = fmaxf(mm, ml[(w * TR + er) * 2]);
-#pragma unroll
-    for (int w = 0; w < WAVES; w++) {
-        const float mw = ml[(w * TR + er) * 2];
-        f[w] = mw == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mw - mm);
-        // (a NaN key leaves a wave's maximum at -inf and its sum NaN)
-        const float lw = ml[(w * TR + er) * 2 + 1];
-        if (lw != lw) f[w] = lw;
-        l += f[w] * lw;
-    }
-    const int rr = it.tile * TR + er;
-    if (rr >= s.n * a.group) return;
-    const int rt = rr / a.group, rg = rr - rt * a.group;
-    const bool whole = it.pieces == 1;
-    float *part = a.few.part + (((int64_t)it.slot * a.c.heads + head) * TR + er) * (D + 4);
-    const int64_t o = ((int64_t)s.t0 + rt) * a.out_stride + (int64_t)(head * a.group + rg) * D;
-    const float inv = whole ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f;
-#pragma unroll
-    for (int d = 0; d < D; d += 64) {
-        const int e = d + 4 * u;
-        if (D % 64 && e >= D) break;
-        f32x4 v = {0, 0, 0, 0};
-#pragma unroll
-        for (int w = 0; w < WAVES; w++) v += f[w] * *(const f32x4 *)(lds + (w * TR + er) * OS + e);
-        v *= inv;
-        if (whole) {
-            store_out(a, o + e, v);
-        } else {
-            *(f32x4 *)(part + 4 + e) = v;
-        }
-    }
-    if (!whole && u == 0) {
-        part[0] = mm;
-        part[1] = l;
-    }
-}
-
-// Rows whose keys were cut into pieces: their parts joined, in a fixed order.  A workgroup has one row in
-// gridDim.z of a (tile, head); its threads take D / 4 columns of four values and 1024 / D
-// pieces at a time.
+// Rows whose keys were cut into pieces: their parts joined, in a fixed order.  A thread has four
+// columns of a row; with few pieces it takes them all, 1024 / D rows a workgroup, with many the
+// workgroup's threads share a row's.
 template <int NG>
 struct JoinLds {
     static constexpr int D = 32 * NG, CT = D / 4, PT = 256 / CT;
@@ -275,48 +20,64 @@ struct JoinLds {
     float l[PT], m[PT];
 };
 template <int NG, int TR>
-__device__ __forceinline__ void join_tile(const AttnArgs &a, int index, int head, JoinLds<NG> &sh) {
+__device__ __forceinline__ void join_rows(const AttnArgs &a, int slot, int head, JoinLds<NG> &sh) {
     constexpr int D = 32 * NG, CT = JoinLds<NG>::CT, PT = JoinLds<NG>::PT;
     const AttnList &list = list_of<TR>(a);
-    Item it;
-    if (!find_item<TR, false>(a, index, it) || it.pieces == 1) return;
+    const int4 j = list.join[slot];
+    if (j.x <= 1) return;
     const int pt = threadIdx.x / CT, ct = threadIdx.x - pt * CT;
-    const int rows = min(it.s.n * a.group - it.tile * TR, TR), pieces = min(it.pieces, list.slots - it.slot);
+    const int rows = min(j.z - j.y, TR), pieces = min(j.x, list.slots - slot);
     const int64_t next = (int64_t)a.c.heads * TR * (D + 4);
     // the weight of a part (m, l) below a common maximum; NaN for a NaN part (a NaN key leaves
     // a wave's maximum at -inf and its sum NaN)
     auto weight = [](float m, float l, float top) { return l != l ? l : m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - top); };
-    for (int r = blockIdx.z; r < rows; r += gridDim.z) {
-        const float *part = list.part + (((int64_t)it.slot * a.c.heads + head) * TR + r) * (D + 4);
+    constexpr int U = 8;  // pieces loaded at a time
+    // pieces p0, p0 + by, .. (U of them at most) of a row, onto its (mm, l, v) so far
+    auto add = [&](const float *part, int p0, int by, float &mm, float &l, f32x4 &v) {
+        float m_p[U], l_p[U];
+        f32x4 w[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int p = min(p0 + u * by, pieces - 1);
+            const float2 ml = *(const float2 *)(part + p * next);
+            w[u] = *(const f32x4 *)(part + p * next + 4 + 4 * ct);
+            m_p[u] = p0 + u * by < pieces ? ml.x : -INFINITY;
+            l_p[u] = p0 + u * by < pieces ? ml.y : 0.0f;
+        }
+        float top = mm;
+#pragma unroll
+        for (int u = 0; u < U; u++) top = fmaxf(top, m_p[u]);
+        const float f0 = weight(mm, l, top);
+        l *= f0;
+        v *= f0;
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const float f = weight(m_p[u], l_p[u], top);
+            l += f * l_p[u];
+            v += f * w[u];
+        }
+        mm = top;
+    };
+    auto part_of = [&](int r) { return list.part + (((int64_t)slot * a.c.heads + head) * TR + r) * (D + 4); };
+    auto put = [&](int r, float l, f32x4 v) {
+        const int rr = j.y + r, rt = rr / a.group, rg = rr - rt * a.group;
+        store_out(a, ((int64_t)j.w + rt) * a.out_stride + (int64_t)(head * a.group + rg) * D + 4 * ct, v * (l == 0.0f ? 0.0f : 1.0f / l));
+    };
+    if (pieces <= U) {  // a row for each CT threads
+        if (pt >= PT) return;
+        for (int r = blockIdx.z * PT + pt; r < rows; r += gridDim.z * PT) {
+            float mm = -INFINITY, l = 0.0f;
+            f32x4 v = {0, 0, 0, 0};
+            add(part_of(r), 0, 1, mm, l, v);
+            put(r, l, v);
+        }
+        return;
+    }
+    for (int r = blockIdx.z; r < rows; r += gridDim.z) {  // all threads on a row
         float mm = -INFINITY, l = 0.0f;
         f32x4 v = {0, 0, 0, 0};
         if (pt < PT) {
-            constexpr int U = 8;  // loads in flight
-            for (int p0 = pt; p0 < pieces; p0 += U * PT) {
-                float m_p[U], l_p[U];
-                f32x4 w[U];
-#pragma unroll
-                for (int u = 0; u < U; u++) {
-                    const int p = min(p0 + u * PT, pieces - 1);
-                    const float2 ml = *(const float2 *)(part + p * next);
-                    w[u] = *(const f32x4 *)(part + p * next + 4 + 4 * ct);
-                    m_p[u] = p0 + u * PT < pieces ? ml.x : -INFINITY;
-                    l_p[u] = p0 + u * PT < pieces ? ml.y : 0.0f;
-                }
-                float top = mm;
-#pragma unroll
-                for (int u = 0; u < U; u++) top = fmaxf(top, m_p[u]);
-                const float f0 = weight(mm, l, top);
-                l *= f0;
-                v *= f0;
-#pragma unroll
-                for (int u = 0; u < U; u++) {
-                    const float f = weight(m_p[u], l_p[u], top);
-                    l += f * l_p[u];
-                    v += f * w[u];
-                }
-                mm = top;
-            }
+            for (int p0 = pt; p0 < pieces; p0 += U * PT) add(part_of(r), p0, PT, mm, l, v);
             sh.v[pt][ct] = v;
             if (ct == 0) {
                 sh.m[pt] = mm;
@@ -335,9 +96,7 @@ __device__ __forceinline__ void join_tile(const AttnArgs &a, int index, int head
                 l += f * sh.l[p];
                 v += f * sh.v[p][ct];
             }
-            const int rr = it.tile * TR + r, rt = rr / a.group, rg = rr - rt * a.group;
-            store_out(a, ((int64_t)it.s.t0 + rt) * a.out_stride + (int64_t)(head * a.group + rg) * D + 4 * ct,
-                      v * (l == 0.0f ? 0.0f : 1.0f / l));
+            put(r, l, v);
         }
         __syncthreads();
     }
@@ -346,31 +105,37 @@ __device__ __forceinline__ void join_tile(const AttnArgs &a, int index, int head
 template <int NG>
 __global__ __launch_bounds__(256) void attn_join(AttnArgs a) {
     __shared__ JoinLds<NG> sh;
-    const int head = blockIdx.x % a.c.heads, tile = blockIdx.x / a.c.heads;
-    if (tile < a.few.tiles)
-        join_tile<NG, 16>(a, tile, head, sh);
+    const int head = blockIdx.x % a.c.heads, slot = blockIdx.x / a.c.heads;
+    const int few = a.few.join ? a.few.slots : 0;
+    if (slot < few)
+        join_rows<NG, 16>(a, slot, head, sh);
     else
-        join_tile<NG, 128>(a, tile - a.few.tiles, head, sh);
+        join_rows<NG, 128>(a, slot - few, head, sh);
+}
+
+template <int NG, int PARTS>
+__global__ __launch_bounds__(256, rows16_k::rows16_waves(NG)) void attn_rows16(AttnArgs a) {
+    extern __shared__ float lds[];
+    rows16_k::rows16<NG, PARTS>(a, blockIdx.x, lds);
 }
 
 template <int NG, int PARTS>
 hipError_t rows16_launch(const AttnArgs &a, hipStream_t s) {
     static std::atomic<uint64_t> done{0};
-    constexpr size_t lds = (size_t)WAVES * TR * (32 * NG + 4 + 2) * sizeof(float);
+    constexpr size_t lds = rows16_k::lds_bytes(NG);
     const hipError_t e = set_max_lds_once((const void *)attn_rows16<NG, PARTS>, lds, done);
     if (e != hipSuccess) return e;
-    attn_rows16<NG, PARTS><<<dim3((unsigned)a.few.slots * a.c.heads), 64 * WAVES, lds, s>>>(a);
+    attn_rows16<NG, PARTS><<<dim3((unsigned)a.few.slots * a.c.heads), 256, lds, s>>>(a);
     return hipGetLastError();
 }
 
 template <int NG>
 hipError_t dim_launch(const AttnArgs &a, hipStream_t s) {
     const bool f16 = a.q_dtype == ARFQ_F16 && a.out_dtype == ARFQ_F16;
-    hipError_t e = hipSuccess;
-    if (a.few.slots) e = f16 ? rows16_launch<NG, 1>(a, s) : rows16_launch<NG, 2>(a, s);
-    if (e == hipSuccess && a.many.slots) e = launch_attn_rows128(a, 32 * NG, s);
+    hipError_t e = a.many.slots ? launch_attn_mixed(a, 32 * NG, s) : f16 ? rows16_launch<NG, 1>(a, s) : rows16_launch<NG, 2>(a, s);
     if (e == hipSuccess && a.joins) {
-        attn_join<NG><<<dim3((unsigned)(a.few.tiles + a.many.tiles) * a.c.heads, 1, a.joins), 256, 0, s>>>(a);
+        const int64_t slots = (a.few.join ? a.few.slots : 0) + (a.many.join ? a.many.slots : 0);
+        attn_join<NG><<<dim3((unsigned)(slots * a.c.heads), 1, a.joins), 256, 0, s>>>(a);
         e = hipGetLastError();
     }
     return e;
@@ -389,22 +154,26 @@ AttnPlan attn_plan(int cus, int heads, int dim, int64_t batch, int64_t tokens, i
     // pieces shorter than min_piece
     auto plan = [&](AttnListPlan &l, int tr, int waves, int64_t tiles) {
         const int64_t most = std::max<int64_t>(1, (max_keys + min_piece(tr) - 1) / min_piece(tr));
-        l.tiles = (int)tiles;
         l.target = std::max(1, waves * cus / heads);
+        l.round = std::max(1, cus / heads);
         l.slots = (int)std::min(l.target + tiles, tiles * most);
-        l.ws_bytes = most > 1 ? (size_t)l.slots * heads * tr * (dim + 4) * sizeof(float) : 0;
+        if (most > 1) {
+            l.part_bytes = (size_t)l.slots * heads * tr * (dim + 4) * sizeof(float);
+            l.join_bytes = (size_t)l.slots * sizeof(int4);
+            p.ws_bytes += l.part_bytes + l.join_bytes;
+        }
     };
     // sequences of at most FEW_ROWS rows, and the longer ones
+    const bool many = (one_each ? group : rows) > FEW_ROWS;
     if (group <= FEW_ROWS)
-        plan(p.few, TR, rows16_waves(ng),
-             std::min({rows / TR + batch, batch * ((FEW_ROWS + TR - 1) / TR), tokens * ((group + TR - 1) / TR)}));
-    if ((one_each ? group : rows) > FEW_ROWS)
-        plan(p.many, 128, rows128_waves(ng), rows / 128 + std::min(batch, rows / (FEW_ROWS + 1)));
-    p.ws_bytes = p.few.ws_bytes + p.many.ws_bytes;
+        plan(p.few, 16, many ? std::min(mixed_waves(ng), rows16_k::rows16_waves(ng)) : rows16_k::rows16_waves(ng),
+             std::min({rows / 16 + batch, batch * ((FEW_ROWS + 15) / 16), tokens * ((group + 15) / 16)}));
+    if (many) plan(p.many, 128, mixed_waves(ng), rows / 128 + std::min(batch, rows / (FEW_ROWS + 1)));
     if (p.ws_bytes) {
-        // workgroups of a (tile, head): one for each row of it, while they are not many times the chip's
-        const int64_t most = p.many.ws_bytes ? 16 : std::min<int64_t>(TR, one_each ? group : TR);
-        p.joins = (int)std::max<int64_t>(1, std::min<int64_t>(most, 16 * cus / ((p.few.tiles + p.many.tiles) * (int64_t)heads)));
+        // workgroups of a (tile, head): one for each of a few rows, or for 1024 / D of 128, while those of all the
+        // list's places, most of which have nothing to join, are not many times the chip's
+        const int64_t most = p.many.part_bytes ? 16 : std::min<int64_t>(16, one_each ? group : 16);
+        p.joins = (int)std::max<int64_t>(1, std::min<int64_t>(most, 16 * cus / ((p.few.slots + p.many.slots) * (int64_t)heads)));
     }
     return p;
 }

@@ -1,0 +1,48 @@
+// arfq_attn_mixed.hip -- attention for batches with prompts in them: the 128-row tiles of those and the
+// 16-row tiles of the other sequences in one launch, side by side.
+#include "arfq_attn_rows128.h"
+#include "arfq_attn_rows16.h"
+
+#include <algorithm>
+
+namespace arfq {
+namespace {
+
+template <int NG, int PARTS>
+__global__ __launch_bounds__(256, mixed_waves(NG)) void attn_mixed(AttnArgs a) {
+    extern __shared__ float lds[];
+    const int many = a.many.slots * a.c.heads, block = blockIdx.x;  // (first: they take longer)
+    if (block < many)
+        rows128_k::rows128<NG, PARTS>(a, block, (uint8_t *)lds);
+    else
+        rows16_k::rows16<NG, PARTS>(a, block - many, lds);
+}
+
+template <int NG, int PARTS>
+hipError_t mixed_launch(const AttnArgs &a, hipStream_t s) {
+    static std::atomic<uint64_t> done{0};
+    constexpr size_t lds = std::max(rows16_k::lds_bytes(NG), rows128_k::lds_bytes(NG));
+    const hipError_t e = set_max_lds_once((const void *)attn_mixed<NG, PARTS>, lds, done);
+    if (e != hipSuccess) return e;
+    attn_mixed<NG, PARTS><<<dim3((unsigned)(a.many.slots + a.few.slots) * a.c.heads), 256, lds, s>>>(a);
+    return hipGetLastError();
+}
+
+template <int NG>
+hipError_t mixed_launch(const AttnArgs &a, hipStream_t s) {
+    return a.q_dtype == ARFQ_F16 && a.out_dtype == ARFQ_F16 ? mixed_launch<NG, 1>(a, s) : mixed_launch<NG, 2>(a, s);
+}
+
+}  // namespace
+
+hipError_t launch_attn_mixed(const AttnArgs &a, int dim, hipStream_t s) {
+    switch (dim) {
+    case 64: return mixed_launch<2>(a, s);
+    case 96: return mixed_launch<3>(a, s);
+    case 128: return mixed_launch<4>(a, s);
+    case 256: return mixed_launch<8>(a, s);
+    }
+    return hipErrorInvalidValue;
+}
+
+}  // namespace arfq

@@ -1,4 +1,4 @@
-// arfq_attn_rows128.hip -- attention over the 4-bit K/V cache for prompts: tiles of 128 rows.
+// arfq_attn_rows128.h -- attention for prompts: tiles of 128 rows.
 //
 // A workgroup's four waves take 32 rows each and step through the keys together, 32 at a time: they
 // turn K and V of a step into f16 once, in LDS, and every wave multiplies all of it.  As in the
@@ -7,10 +7,12 @@
 // they lie, the second product's operand for keys
 //     16b + 4h + {0, 1, 2, 3} and 16b + 8 + 4h + {0, 1, 2, 3}      (h = lane / 32),
 // the order in which V goes to LDS.
+#pragma once
 #include "arfq_attn.h"
 
 namespace arfq {
 namespace {
+namespace rows128_k {
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
@@ -33,28 +35,26 @@ struct Part {
     uint32_t k[NK], ks[NK], v[NG], vs[NV][2];
 };
 
+// block: (item, head), head fastest.
 template <int NG, int PARTS>
-__global__ __launch_bounds__(THREADS, NG <= 4 && PARTS == 1 ? 3 : rows128_waves(NG)) void attn_rows128(AttnArgs a) {
+__device__ __forceinline__ void rows128(const AttnArgs &a, int block, uint8_t *lds) {
     constexpr int D = 32 * NG, KS = Step<NG>::KS;
-    extern __shared__ uint8_t lds[];
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), c = lane & 31, h = lane >> 5;
-    const int head = blockIdx.x % a.c.heads;
+    const int head = block % a.c.heads;
     Item it;
-    if (!find_item<TR, true>(a, blockIdx.x / a.c.heads, it)) return;
+    if (!take_item<TR>(a, block, it)) return;
     const Seq &s = it.s;
-    if (a.causal) it.tile = s.tiles - 1 - it.tile;  // (the longest first; a tile's pieces stay together)
-    const int slot = a.causal ? it.slot + (2 * it.tile - s.tiles + 1) * it.pieces : it.slot;
+    const int slot = it.slot;
 
     auto row_hi = [&](int64_t pos) { return pos < 0 ? 0 : a.causal ? (int)min(pos + 1, (int64_t)s.end) : s.end; };
     auto row_lo = [&](int64_t pos) { return a.window ? (int)max((int64_t)0, min(pos - a.window + 1, (int64_t)s.end)) : 0; };
     const int rows = s.n * a.group, piece_lo = s.lo + it.piece * it.keys, piece_hi = min(s.end, piece_lo + it.keys);
     auto pos_of = [&](int row) { return (int64_t)s.len - s.n + min(row, rows - 1) / a.group; };
-    // keys of the tile in this piece; of the wave's rows; and those that every row of the wave has
+    // keys of the tile in this piece, and those that every row of the wave has
     const int first = max(row_lo(pos_of(it.tile * TR)) & ~(STEP - 1), piece_lo);
     const int last = min(row_hi(pos_of(it.tile * TR + TR - 1)), piece_hi);
     const int row0 = it.tile * TR + wave * WR;
     const int64_t pos0 = pos_of(row0), pos1 = pos_of(row0 + WR - 1);
-    const int wave_lo = row_lo(pos0), wave_hi = row0 < rows ? min(row_hi(pos1), piece_hi) : 0;
     const int inner_lo = row_lo(pos1), inner_hi = min(row_hi(pos0), piece_hi);
     const int row = row0 + c;
     const bool valid = row < rows;
@@ -187,6 +187,11 @@ __global__ __launch_bounds__(THREADS, NG <= 4 && PARTS == 1 ? 3 : rows128_waves(
     auto step = [&](int k0, const uint8_t *kb, uint8_t *other) __attribute__((always_inline)) {
         const uint8_t *vb = kb + Step<NG>::K_BYTES;
         const bool in0 = in[0], in1 = in[1];
+        // K's operands are on their way from LDS while the next step's are made, V's while p is
+        f16x8 kf[2 * NG];
+#pragma unroll
+        for (int i = 0; i < 2 * NG; i++) kf[i] = *(const f16x8 *)(kb + c * (KS * 2) + (2 * i + h) * 16);
+        __builtin_amdgcn_sched_barrier(0);
         if (k0 + STEP < last) {
             store(other, part);
             in[0] = nin[0];
@@ -198,14 +203,18 @@ __global__ __launch_bounds__(THREADS, NG <= 4 && PARTS == 1 ? 3 : rows128_waves(
                 load(p, part);
             }
         }
-        if (k0 < wave_hi && k0 + STEP > wave_lo) {
+        {
             f32x16 x = zero;
 #pragma unroll
-            for (int i = 0; i < 2 * NG; i++) {
-                const f16x8 kf = *(const f16x8 *)(kb + c * (KS * 2) + (2 * i + h) * 16);
+            for (int i = 0; i < 2 * NG; i++)
 #pragma unroll
-                for (int p = 0; p < PARTS; p++) x = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, q[p][i], x, 0, 0, 0);
-            }
+                for (int p = 0; p < PARTS; p++) x = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[i], q[p][i], x, 0, 0, 0);
+            f16x8 vf[2][NG];
+#pragma unroll
+            for (int b = 0; b < 2; b++)
+#pragma unroll
+                for (int i = 0; i < NG; i++) vf[b][i] = *(const f16x8 *)(vb + ((b * 2 + h) * D + 32 * i + c) * 16);
+            __builtin_amdgcn_sched_barrier(0);
             float unit = x_of_s;
             if (cap > 0.0f) {
 #pragma unroll
@@ -254,12 +263,10 @@ __global__ __launch_bounds__(THREADS, NG <= 4 && PARTS == 1 ? 3 : rows128_waves(
                     }
                 }
 #pragma unroll
-                for (int i = 0; i < NG; i++) {
-                    const f16x8 vf = *(const f16x8 *)(vb + ((b * 2 + h) * D + 32 * i + c) * 16);
+                for (int i = 0; i < NG; i++)
 #pragma unroll
                     for (int pp = 0; pp < PARTS; pp++)
-                        acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, p[pp].v, acc[i], 0, 0, 0);
-                }
+                        acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[b][i], p[pp].v, acc[i], 0, 0, 0);
             }
         }
         lds_barrier();
@@ -301,31 +308,8 @@ __global__ __launch_bounds__(THREADS, NG <= 4 && PARTS == 1 ? 3 : rows128_waves(
     if (!whole && h == 0) *(float2 *)to = make_float2(m, sum);
 }
 
-template <int NG, int PARTS>
-hipError_t rows128_launch(const AttnArgs &a, hipStream_t s) {
-    static std::atomic<uint64_t> done{0};
-    constexpr size_t bytes = 2 * Step<NG>::BYTES;
-    const hipError_t e = set_max_lds_once((const void *)attn_rows128<NG, PARTS>, bytes, done);
-    if (e != hipSuccess) return e;
-    attn_rows128<NG, PARTS><<<dim3((unsigned)a.many.slots * a.c.heads), THREADS, bytes, s>>>(a);
-    return hipGetLastError();
-}
+constexpr size_t lds_bytes(int ng) { return 2 * (size_t)STEP * ((32 * ng + 8) + 32 * ng) * 2; }
 
-template <int NG>
-hipError_t rows128_launch(const AttnArgs &a, hipStream_t s) {
-    return a.q_dtype == ARFQ_F16 && a.out_dtype == ARFQ_F16 ? rows128_launch<NG, 1>(a, s) : rows128_launch<NG, 2>(a, s);
-}
-
+}  // namespace rows128_k
 }  // namespace
-
-hipError_t launch_attn_rows128(const AttnArgs &a, int dim, hipStream_t s) {
-    switch (dim) {
-    case 64: return rows128_launch<2>(a, s);
-    case 96: return rows128_launch<3>(a, s);
-    case 128: return rows128_launch<4>(a, s);
-    case 256: return rows128_launch<8>(a, s);
-    }
-    return hipErrorInvalidValue;
-}
-
 }  // namespace arfq

@@ -637,8 +637,13 @@ int arfq_kv_attention(arfq_ctx *ctx, const arfq_kv *kv, const arfq_kv_seqs *seqs
     a.window = (int)std::min<int64_t>(window, INT32_MAX);
     a.causal = causal != 0;
     a.few_rows = plan.few_rows;
-    a.few = {plan.few.tiles, plan.few.target, plan.few.slots, (float *)workspace};
-    a.many = {plan.many.tiles, plan.many.target, plan.many.slots, (float *)((char *)workspace + plan.few.ws_bytes)};
+    char *ws = (char *)workspace;
+    auto list = [&](const arfq::AttnListPlan &l, size_t part, size_t join) {
+        return arfq::AttnList{l.target, l.slots, l.round, (float *)(ws + part), l.join_bytes ? (int4 *)(ws + join) : nullptr};
+    };
+    const size_t parts = plan.few.part_bytes + plan.many.part_bytes;
+    a.few = list(plan.few, 0, parts);
+    a.many = list(plan.many, plan.few.part_bytes, parts + plan.few.join_bytes);
     a.joins = plan.joins;
     const hipError_t e = arfq::launch_attn(a, kv->dim, ctx->stream);
     return e == hipSuccess ? ARFQ_OK : hip_fail(ctx, e, "kv_attention launch");

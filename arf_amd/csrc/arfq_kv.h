@@ -86,17 +86,18 @@ hipError_t launch_kv_write(const KvArgs &a, int dim, const void *k, int64_t k_st
 hipError_t launch_kv_read(const KvArgs &a, int dim, void *k, int64_t k_stride, void *v, int64_t v_stride, int dtype,
                           hipStream_t s);
 
-// ---- attention (arfq_attn.hip, arfq_attn_rows128.hip) ----
-// A work list (arfq_attn.h): its tiles at most, the pieces it aims at, its items at most, and
-// the parts of rows of more than one piece, [slots][heads][rows of a tile][dim + 4]: maximum,
-// sum, -, -, values.
+// ---- attention (arfq_attn.hip, arfq_attn_mixed.hip) ----
+// A work list (arfq_attn.h): the pieces it aims at, its items at most, the parts of rows of more than one
+// piece, [slots][heads][rows of a tile][dim + 4] (maximum, sum, -, -, values), and for each item
+// what the join takes: pieces (0: not a first one of several), first row, rows, first token.
 struct AttnListPlan {
-    int tiles = 0, target = 1, slots = 0;
-    size_t ws_bytes = 0;
+    int target = 1, slots = 0, round = 1;
+    size_t part_bytes = 0, join_bytes = 0;
 };
 struct AttnList {
-    int tiles, target, slots;
+    int target, slots, round;  // round: items that give every compute unit a workgroup
     float *part;
+    int4 *join;                // null: no row has two pieces
 };
 struct AttnArgs {
     KvArgs c;
@@ -116,15 +117,15 @@ struct AttnPlan {
     int few_rows = 0;
     AttnListPlan few, many;
     int joins = 0;
-    size_t ws_bytes = 0;  // few's parts, then many's
+    size_t ws_bytes = 0;  // few's parts, many's, few's join, many's
 };
 bool attn_dim_ok(int dim);
 // max_keys: of a sequence; one_each: a token of every sequence (no start)
 AttnPlan attn_plan(int cus, int heads, int dim, int64_t batch, int64_t tokens, int q_heads, int64_t max_keys, bool one_each);
 hipError_t launch_attn(const AttnArgs &a, int dim, hipStream_t s);
-// `many`'s tiles
-hipError_t launch_attn_rows128(const AttnArgs &a, int dim, hipStream_t s);
-// workgroups of it that a compute unit holds (a wave each on every SIMD), at ng groups of 32 values
-constexpr int rows128_waves(int ng) { return ng <= 4 ? 2 : 1; }
+// both lists
+hipError_t launch_attn_mixed(const AttnArgs &a, int dim, hipStream_t s);
+// its workgroups that a compute unit holds (a wave each on every SIMD), at ng groups of 32 values
+constexpr int mixed_waves(int ng) { return ng <= 4 ? 2 : 1; }
 
 }  // namespace arfq
