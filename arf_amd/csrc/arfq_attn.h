@@ -170,30 +170,42 @@ struct Places {
     uint32_t sub[2];
     bool in[2];  // whether the tile's page is the cache's
 };
-// The page ids of a sequence, 64 pages at a time in a register across the wave.  (Not a scalar load each
-// step: the wait for LDS data is for scalar loads too, and these miss the scalar cache.)
-struct Pages {
+// A wave's steps through a sequence, SS tiles apart: lane 2j + i has the place of tile i of step j, for 32 steps at
+// a time.  A step takes its two from there: no scalar load (the wait for LDS data is for scalar
+// loads too, and these miss the scalar cache), and few scalar instructions.
+template <int SS>
+struct Steps {
     const int32_t *table;
-    const uint8_t *base;  // the head's region of page 0
-    int first, ids;
-    __device__ __forceinline__ Pages(const KvArgs &a, int b, int head)
-        : table(a.table + (int64_t)b * a.max_pages), base(a.data + head * a.region), first(INT32_MIN), ids(0) {}
-    // the step of keys k0 .. +31 (past the table's end: of its last page); max_pages > 0
-    __device__ __forceinline__ Places at(const KvArgs &a, int k0) {
-        Places p;
-        const int t0 = k0 / KV_TILE, pg0 = kv_page_of(a, t0), pg1 = kv_page_of(a, t0 + 1);
-        const int most = a.max_pages - 1, l0 = min(pg0, most), l1 = min(pg1, most);
-        if (l0 < first || l1 - first >= WAVE) {
-            first = l0;
-            ids = table[min(l0 + (int)(threadIdx.x & 63), most)];
+    int first;  // the tile of lane 0
+    uint32_t lo, hi, sub;  // sub: bit 31 where the page is not the cache's
+    // the wave's steps from key k0 on (k0 a multiple of 16; max_pages > 0)
+    __device__ __forceinline__ Steps(const KvArgs &a, int b) : table(a.table + (int64_t)b * a.max_pages), first(INT32_MIN / 2) {
+        lo = hi = sub = 0;
+    }
+    // (past the table's end: of its last page)
+    __device__ __forceinline__ Places at(const KvArgs &a, int head, int k0) {
+        const int t0 = k0 / KV_TILE;
+        int j = (t0 - first) / SS;
+        if (j >= WAVE / 2) {
+            const int lane = threadIdx.x & 63, t = t0 + (lane >> 1) * SS + (lane & 1), pg = kv_page_of(a, t);
+            const int id = table[min(pg, a.max_pages - 1)];
+            const bool in = (uint32_t)id < (uint32_t)a.n_pages;
+            const uint64_t p = (uint64_t)(uint32_t)(in ? id : 0) * a.page_bytes + (uint64_t)head * a.region;
+            lo = (uint32_t)p;
+            hi = (uint32_t)(p >> 32);
+            sub = (uint32_t)(t - pg * a.tiles) | (in ? 0u : 0x80000000u);
             __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0) here, and not at each use
+            first = t0;
+            j = 0;
         }
-        const int id[2] = {__builtin_amdgcn_readlane(ids, l0 - first), __builtin_amdgcn_readlane(ids, l1 - first)};
+        Places p;
 #pragma unroll
         for (int i = 0; i < 2; i++) {
-            p.in[i] = (uint32_t)id[i] < (uint32_t)a.n_pages;
-            p.reg[i] = base + (uint64_t)(uint32_t)(p.in[i] ? id[i] : 0) * a.page_bytes;
-            p.sub[i] = (uint32_t)(t0 + i - (i ? pg1 : pg0) * a.tiles);
+            const uint32_t l = __builtin_amdgcn_readlane(lo, 2 * j + i), h = __builtin_amdgcn_readlane(hi, 2 * j + i);
+            const uint32_t s = __builtin_amdgcn_readlane(sub, 2 * j + i);
+            p.reg[i] = a.data + ((uint64_t)h << 32 | l);  // (an offset, not an address: the loads stay global ones)
+            p.sub[i] = s & 0x7fffffffu;
+            p.in[i] = (int32_t)s >= 0;
         }
         return p;
     }

@@ -63,7 +63,7 @@ __device__ __forceinline__ void rows128(const AttnArgs &a, int block, uint8_t *l
     const int lo = row_lo(pos), hi = min(valid ? row_hi(pos) : 0, piece_hi);
 
     // ---- a step's K and V: from the cache to registers, and to LDS as f16 ----
-    Pages pages(a.c, it.b, head);
+    Steps<STEP / KV_TILE> steps(a.c, it.b);
     constexpr int NK = Part<NG>::NK, NV = Part<NG>::NV;
     int k_half[NK];
     uint32_t k_off[NK], ks_off[NK];
@@ -137,7 +137,7 @@ __device__ __forceinline__ void rows128(const AttnArgs &a, int block, uint8_t *l
     Part<NG> part;
     bool in[2] = {false, false}, nin[2] = {false, false};  // the tiles that are multiplied, and those in registers
     if (first < last) {
-        const Places p = pages.at(a.c, first);
+        const Places p = steps.at(a.c, head, first);
         in[0] = p.in[0];
         in[1] = p.in[1];
         load(p, part);
@@ -197,7 +197,7 @@ __device__ __forceinline__ void rows128(const AttnArgs &a, int block, uint8_t *l
             in[0] = nin[0];
             in[1] = nin[1];
             if (k0 + 2 * STEP < last) {
-                const Places p = pages.at(a.c, k0 + 2 * STEP);
+                const Places p = steps.at(a.c, head, k0 + 2 * STEP);
                 nin[0] = p.in[0];
                 nin[1] = p.in[1];
                 load(p, part);
@@ -275,7 +275,7 @@ __device__ __forceinline__ void rows128(const AttnArgs &a, int block, uint8_t *l
     if (first < last) {
         store(buf0, part);
         if (first + STEP < last) {
-            const Places p = pages.at(a.c, first + STEP);
+            const Places p = steps.at(a.c, head, first + STEP);
             nin[0] = p.in[0];
             nin[1] = p.in[1];
             load(p, part);

@@ -47,8 +47,8 @@ __device__ __forceinline__ void rows16(const AttnArgs &a, int block, float *lds)
     const int64_t pos = (int64_t)s.len - s.n + tok;
     const int lo = row_lo(pos), hi = min(valid ? row_hi(pos) : 0, piece_hi);
 
-    Pages pages(a.c, it.b, head);
     constexpr int NEXT = WAVES * STEP;
+    Steps<NEXT / KV_TILE> steps(a.c, it.b);
     const Offs<NG> offs = lane_offs<NG>();
     Raw<NG> r;
     int k0 = first + wave * STEP;
@@ -63,12 +63,12 @@ __device__ __forceinline__ void rows16(const AttnArgs &a, int block, float *lds)
         for (int half = 0; half < 2; half++) load_v<NG>(p.reg[half], a.c, p.sub[half], half, offs, r);
     };
     if (k0 < last) {  // (keys: the table has a page)
-        next = pages.at(a.c, k0);
+        next = steps.at(a.c, head, k0);
         in[0] = next.in[0];
         in[1] = next.in[1];
         load_ks(next);
         load_vs(next);
-        next = pages.at(a.c, k0 + NEXT);
+        next = steps.at(a.c, head, k0 + NEXT);
     }
 
     // q as operands: values 32g + 8h .. +7 of the row, times a power of two that puts the row's
@@ -207,7 +207,7 @@ __device__ __forceinline__ void rows16(const AttnArgs &a, int block, float *lds)
             load_vs(next);
             in[0] = next.in[0];
             in[1] = next.in[1];
-            next = pages.at(a.c, k1 + NEXT);
+            next = steps.at(a.c, head, k1 + NEXT);
         }
         k0 = k1;
     }
