@@ -163,12 +163,12 @@ __device__ __forceinline__ bool take_item(const AttnArgs &a, int block, Item &it
     return got;
 }
 
-// Where a step's two 16-key tiles are: the (page, head) regions (page 0's for a page that is not the cache's:
-// loads stay in it, its keys are masked) and the tiles' places in them.
-struct Places {
-    const uint8_t *reg[2];
-    uint32_t sub[2];
-    bool in[2];  // whether the tile's page is the cache's
+// Where a 16-key tile is: the (page, head) region (page 0's for a page that is not the cache's: loads stay in
+// it, its keys are masked), its place there, and whether its page is the cache's.
+struct Place {
+    const uint8_t *reg;
+    uint32_t sub;
+    bool in;
 };
 // A wave's steps through a sequence, SS tiles apart: lane 2j + i has the place of tile i of step j, for 32 steps at
 // a time.  A step takes its two from there: no scalar load (the wait for LDS data is for scalar
@@ -182,33 +182,29 @@ struct Steps {
     __device__ __forceinline__ Steps(const KvArgs &a, int b) : table(a.table + (int64_t)b * a.max_pages), first(INT32_MIN / 2) {
         lo = hi = sub = 0;
     }
-    // (past the table's end: of its last page)
-    __device__ __forceinline__ Places at(const KvArgs &a, int head, int k0) {
-        const int t0 = k0 / KV_TILE;
-        int j = (t0 - first) / SS;
-        if (j >= WAVE / 2) {
-            const int lane = threadIdx.x & 63, t = t0 + (lane >> 1) * SS + (lane & 1), pg = kv_page_of(a, t);
-            const int id = table[min(pg, a.max_pages - 1)];
-            const bool in = (uint32_t)id < (uint32_t)a.n_pages;
-            const uint64_t p = (uint64_t)(uint32_t)(in ? id : 0) * a.page_bytes + (uint64_t)head * a.region;
-            lo = (uint32_t)p;
-            hi = (uint32_t)(p >> 32);
-            sub = (uint32_t)(t - pg * a.tiles) | (in ? 0u : 0x80000000u);
-            __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0) here, and not at each use
-            first = t0;
-            j = 0;
-        }
-        Places p;
-#pragma unroll
-        for (int i = 0; i < 2; i++) {
-            const uint32_t l = __builtin_amdgcn_readlane(lo, 2 * j + i), h = __builtin_amdgcn_readlane(hi, 2 * j + i);
-            const uint32_t s = __builtin_amdgcn_readlane(sub, 2 * j + i);
-            p.reg[i] = a.data + ((uint64_t)h << 32 | l);  // (an offset, not an address: the loads stay global ones)
-            p.sub[i] = s & 0x7fffffffu;
-            p.in[i] = (int32_t)s >= 0;
-        }
-        return p;
+    // The lane of the step's first tile.
+    __device__ __forceinline__ int step(const KvArgs &a, int head, int k0) {
+        const int t0 = k0 / KV_TILE, j = (t0 - first) / SS;
+        if (j < WAVE / 2) return 2 * j;
+        // (past the table's end: of its last page)
+        const int lane = threadIdx.x & 63, t = t0 + (lane >> 1) * SS + (lane & 1), pg = kv_page_of(a, t);
+        const int id = table[min(pg, a.max_pages - 1)];
+        const bool in = (uint32_t)id < (uint32_t)a.n_pages;
+        const uint64_t p = (uint64_t)(uint32_t)(in ? id : 0) * a.page_bytes + (uint64_t)head * a.region;
+        lo = (uint32_t)p;
+        hi = (uint32_t)(p >> 32);
+        sub = (uint32_t)(t - pg * a.tiles) | (in ? 0u : 0x80000000u);
+        __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0) here, and not at each use
+        first = t0;
+        return 0;
     }
+    // The tile of lane l.  (An offset, not an address, in the lanes: the loads stay global ones.)
+    __device__ __forceinline__ Place at(const KvArgs &a, int l) const {
+        const uint32_t s = __builtin_amdgcn_readlane(sub, l);
+        return {a.data + ((uint64_t)(uint32_t)__builtin_amdgcn_readlane(hi, l) << 32 | (uint32_t)__builtin_amdgcn_readlane(lo, l)),
+                s & 0x7fffffffu, (int32_t)s >= 0};
+    }
+    __device__ __forceinline__ bool in(int l) const { return __builtin_amdgcn_readlane((int)sub, l) >= 0; }
 };
 
 // ---- operands ----------------------------------------------------------------------------
@@ -342,18 +338,6 @@ __device__ __forceinline__ uint32_t pair_bytes(const uint32_t (&v)[NG], int pr, 
     const uint32_t sel = 0x0c000c00u | (uint32_t)((b1 & 3) + 4) << 16 | (uint32_t)(b0 & 3);
     return __builtin_amdgcn_perm(v[b1 >> 2], v[b0 >> 2], sel);
 }
-// The same of group 2i + odd, odd (0 or 1) uniform and not known to the compiler.
-template <int NG>
-__device__ __forceinline__ uint32_t pair_bytes(const uint32_t (&v)[NG], int pr, int i, int odd) {
-    if constexpr (NG % 2) {
-        const uint32_t even = pair_bytes<NG>(v, pr, 2 * i), other = pair_bytes<NG>(v, pr, min(2 * i + 1, NG - 1));
-        return odd ? other : even;
-    }
-    const int b0 = 2 * pr * NG + 2 * i, b1 = b0 + NG;  // even: both groups' bytes are in one dword
-    const uint32_t sel = 0x0c000c00u | (uint32_t)((b1 & 3) + 4) << 16 | (uint32_t)(b0 & 3);
-    return __builtin_amdgcn_perm(v[b1 >> 2], v[b0 >> 2], sel + (odd ? 0x00010001u : 0u));
-}
-
 // MFMA operands of group g of the V tile: eight keys of the values 32g + lane % 16 (lo) and
 // 32g + 16 + lane % 16 (hi).
 template <int NG>

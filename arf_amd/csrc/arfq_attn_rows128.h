@@ -27,12 +27,12 @@ struct Step {
     static constexpr int K_BYTES = STEP * KS * 2, BYTES = K_BYTES + STEP * D * 2;
 };
 
-// What a thread turns into f16: dwords t, t + 256, .. of the two K tiles (64 NG dwords each), and of V
-// the four keys (t / 16) % 8 of row t % 16, groups t / 128, t / 128 + 2, ..
+// What a lane turns into f16: a wave has K or V of one of the step's two 16-key tiles, 64 units of NG
+// dwords.  K: chunk lane % 4 of key lane / 4, and the key's scales; V: matrix row lane % 16 of the four
+// keys lane / 16, and their scales in pairs.
 template <int NG>
 struct Part {
-    static constexpr int NK = (128 * NG + THREADS - 1) / THREADS, NV = (NG + 1) / 2;
-    uint32_t k[NK], ks[NK], v[NG], vs[NV][2];
+    uint32_t x[NG], s[2 * NG];
 };
 
 // block: (item, head), head fastest.
@@ -64,84 +64,71 @@ __device__ __forceinline__ void rows128(const AttnArgs &a, int block, uint8_t *l
 
     // ---- a step's K and V: from the cache to registers, and to LDS as f16 ----
     Steps<STEP / KV_TILE> steps(a.c, it.b);
-    constexpr int NK = Part<NG>::NK, NV = Part<NG>::NV;
-    int k_half[NK];
-    uint32_t k_off[NK], ks_off[NK];
+    const int half = wave >> 1;  // the wave's tile
+    const bool is_v = wave & 1;
+    const uint32_t x_off = lane * (4 * NG), s_off = is_v ? (lane >> 4) * (8 * NG) : (lane >> 2) * (2 * NG);
+    constexpr int AL = NG % 4 == 0 ? 16 : NG % 2 == 0 ? 8 : 4;
+    const uint32_t x_at = is_v ? a.c.off_v : 0, s_at = is_v ? a.c.off_vs : a.c.off_ks;
+    // (in0, in1: whether the step's tiles are the cache's)
+    auto load = [&](int k0, Part<NG> &p, bool &in0, bool &in1) __attribute__((always_inline)) {
+        const int l = steps.step(a.c, head, k0);
+        in0 = steps.in(l);
+        in1 = steps.in(l + 1);
+        const Place pl = steps.at(a.c, l + half);
+        const uint8_t *x = at(pl.reg + (x_at + pl.sub * (256u * NG)), x_off);
+        const uint8_t *sc = at(pl.reg + (s_at + pl.sub * (32u * NG)), s_off);
+        load_aligned<NG, AL>(x, p.x);
+        if (is_v) {
+            load_aligned<2 * NG, 8>(sc, p.s);
+            asm volatile("");  // (or the branches' stores are made one, to memory)
+        } else if constexpr (NG % 2) {
 #pragma unroll
-    for (int i = 0; i < NK; i++) {
-        const int w = t + i * THREADS;  // dword of the tiles (the same tile for a whole wave)
-        k_half[i] = __builtin_amdgcn_readfirstlane(w / (64 * NG));
-        const int o = w - k_half[i] * 64 * NG;
-        k_off[i] = 4 * o;
-        ks_off[i] = (o / (4 * NG) * NG + o % NG) * 2;
-    }
-    const uint32_t v_off = ((t >> 4) & 3) * (64 * NG) + (t & 15) * (4 * NG), vs_off = ((t >> 4) & 3) * (8 * NG);
-    auto load = [&](const Places &at_p, Part<NG> &p) __attribute__((always_inline)) {
+            for (int g = 0; g < NG; g++) p.s[g] = ((const uint16_t *)sc)[g];
+        } else {
+            uint32_t w[NG / 2];
+            load_aligned<NG / 2, NG % 8 == 0 ? 16 : NG % 4 == 0 ? 8 : 4>(sc, w);
 #pragma unroll
-        for (int i = 0; i < NK; i++) {
-            if ((128 * NG) % THREADS && t + i * THREADS >= 128 * NG) break;
-            const uint8_t *reg = k_half[i] ? at_p.reg[1] : at_p.reg[0];
-            const uint32_t sub = k_half[i] ? at_p.sub[1] : at_p.sub[0];
-            p.k[i] = *(const uint32_t *)at(reg + sub * (256u * NG), k_off[i]);
-            p.ks[i] = *(const uint16_t *)at(reg + (a.c.off_ks + sub * (32u * NG)), ks_off[i]);
-        }
-        const uint8_t *reg = wave & 1 ? at_p.reg[1] : at_p.reg[0];
-        const uint32_t sub = wave & 1 ? at_p.sub[1] : at_p.sub[0];
-        constexpr int AL = NG % 4 == 0 ? 16 : NG % 2 == 0 ? 8 : 4;
-        load_aligned<NG, AL>(at(reg + (a.c.off_v + sub * (256u * NG)), v_off), p.v);
-#pragma unroll
-        for (int i = 0; i < NV; i++) {
-            const int g = min((wave >> 1) + 2 * i, NG - 1);
-            load_aligned<2, 8>(at(reg + (a.c.off_vs + sub * (32u * NG) + g * 8), vs_off), p.vs[i]);
+            for (int g = 0; g < NG / 2; g++) p.s[g] = w[g];
         }
     };
     const uint32_t magic = magic_1024();
-    auto store = [&](uint8_t *kb, const Part<NG> &p) __attribute__((always_inline)) {
-        uint8_t *vb = kb + Step<NG>::K_BYTES;
+    // (K's rows; V's (key block, half of a lane's eight keys) and matrix row)
+    const uint32_t to = is_v ? Step<NG>::K_BYTES + ((half * 2 + ((lane >> 4) & 1)) * D + (lane & 15)) * 16 + (lane >> 5) * 8
+                             : (half * 16 + (lane >> 2)) * (KS * 2) + (lane & 3) * 16;
+    auto store = [&](uint8_t *buf, const Part<NG> &p) __attribute__((always_inline)) {
+        uint8_t *o = buf + to;
+        if (is_v) {
 #pragma unroll
-        for (int i = 0; i < NK; i++) {
-            const int w = t + i * THREADS;
-            if ((128 * NG) % THREADS && w >= 128 * NG) break;
-            const int key = w / (4 * NG), chunk = w % NG * 4 + w / NG % 4;  // (dword (key, quarter, group))
-            const uint32_t w8 = p.k[i] >> 8;
-            uint32_t d1 = p.ks[i];
-            asm volatile("" : "+v"(d1));  // (or two scales are packed into one register as soon as they are loaded: a wait)
-            const f16x2 d = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(d1, d1, 0x01000100u));
-            Frag f;
-            f.w[0] = codes_f16<true>(p.k[i], magic) * d;
-            f.w[1] = codes_f16<false>(p.k[i], magic) * d;
-            f.w[2] = codes_f16<true>(w8, magic) * d;
-            f.w[3] = codes_f16<false>(w8, magic) * d;
-            *(f16x8 *)(kb + key * (KS * 2) + chunk * 16) = f.v;
-        }
-        const int half = wave & 1, q = (t >> 4) & 3;
-        uint8_t *to = vb + ((half * 2 + (q & 1)) * D + (t & 15)) * 16 + (q >> 1) * 8;
+            for (int g = 0; g < NG; g++) {
+                f16x2 l[2], u[2];
 #pragma unroll
-        for (int i = 0; i < NV; i++) {
-            // (the group is the wave's: a byte of each key's dwords by a selector in a register)
-            const int g = (wave >> 1) + 2 * i;
-            if (NG % 2 && g >= NG) break;
-            f16x2 l[2], u[2];
-#pragma unroll
-            for (int pr = 0; pr < 2; pr++) {
-                const uint32_t w = pair_bytes<NG>(p.v, pr, i, wave >> 1);
-                const f16x2 d = __builtin_bit_cast(f16x2, p.vs[i][pr]);
-                l[pr] = codes_f16<true>(w, magic) * d;
-                u[pr] = codes_f16<false>(w, magic) * d;
+                for (int pr = 0; pr < 2; pr++) {
+                    const uint32_t w = pair_bytes<NG>(p.x, pr, g);
+                    const f16x2 d = __builtin_bit_cast(f16x2, p.s[2 * g + pr]);
+                    l[pr] = codes_f16<true>(w, magic) * d;
+                    u[pr] = codes_f16<false>(w, magic) * d;
+                }
+                *(u32x2 *)(o + g * 512) = u32x2{__builtin_bit_cast(uint32_t, l[0]), __builtin_bit_cast(uint32_t, l[1])};
+                *(u32x2 *)(o + g * 512 + 256) = u32x2{__builtin_bit_cast(uint32_t, u[0]), __builtin_bit_cast(uint32_t, u[1])};
             }
-            *(u32x2 *)(to + g * 512) = u32x2{__builtin_bit_cast(uint32_t, l[0]), __builtin_bit_cast(uint32_t, l[1])};
-            *(u32x2 *)(to + g * 512 + 256) = u32x2{__builtin_bit_cast(uint32_t, u[0]), __builtin_bit_cast(uint32_t, u[1])};
+        } else {
+#pragma unroll
+            for (int g = 0; g < NG; g++) {
+                const uint32_t w = p.x[g], w8 = w >> 8, d2 = p.s[NG % 2 ? g : g / 2];
+                const f16x2 d = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(d2, d2, NG % 2 || g % 2 == 0 ? 0x01000100u : 0x03020302u));
+                Frag f;
+                f.w[0] = codes_f16<true>(w, magic) * d;
+                f.w[1] = codes_f16<false>(w, magic) * d;
+                f.w[2] = codes_f16<true>(w8, magic) * d;
+                f.w[3] = codes_f16<false>(w8, magic) * d;
+                *(f16x8 *)(o + g * 64) = f.v;
+            }
         }
     };
 
     Part<NG> part;
-    bool in[2] = {false, false}, nin[2] = {false, false};  // the tiles that are multiplied, and those in registers
-    if (first < last) {
-        const Places p = steps.at(a.c, head, first);
-        in[0] = p.in[0];
-        in[1] = p.in[1];
-        load(p, part);
-    }
+    bool in0 = false, in1 = false, nin0 = false, nin1 = false;  // of the tiles that are multiplied, and those in registers
+    if (first < last) load(first, part, in0, in1);
 
     // ---- q as operands, values 16i + 8h .. +7 of the row, scaled as in the kernel of few rows ----
     f16x8 q[PARTS][2 * NG];
@@ -186,7 +173,7 @@ __device__ __forceinline__ void rows128(const AttnArgs &a, int block, uint8_t *l
     // `other` and loads the ones after
     auto step = [&](int k0, const uint8_t *kb, uint8_t *other) __attribute__((always_inline)) {
         const uint8_t *vb = kb + Step<NG>::K_BYTES;
-        const bool in0 = in[0], in1 = in[1];
+        const bool was0 = in0, was1 = in1;
         // K's operands are on their way from LDS while the next step's are made, V's while p is
         f16x8 kf[2 * NG];
 #pragma unroll
@@ -194,14 +181,9 @@ __device__ __forceinline__ void rows128(const AttnArgs &a, int block, uint8_t *l
         __builtin_amdgcn_sched_barrier(0);
         if (k0 + STEP < last) {
             store(other, part);
-            in[0] = nin[0];
-            in[1] = nin[1];
-            if (k0 + 2 * STEP < last) {
-                const Places p = steps.at(a.c, head, k0 + 2 * STEP);
-                nin[0] = p.in[0];
-                nin[1] = p.in[1];
-                load(p, part);
-            }
+            in0 = nin0;
+            in1 = nin1;
+            if (k0 + 2 * STEP < last) load(k0 + 2 * STEP, part, nin0, nin1);
         }
         {
             f32x16 x = zero;
@@ -221,14 +203,14 @@ __device__ __forceinline__ void rows128(const AttnArgs &a, int block, uint8_t *l
                 for (int i = 0; i < 16; i++) x[i] = tanh_of(x[i] * x_of_s) * x_of_t;
                 unit = 1.0f;
             }
-            if (k0 < inner_lo || k0 + STEP > inner_hi || !in0 || !in1) {
+            if (k0 < inner_lo || k0 + STEP > inner_hi || !was0 || !was1) {
 #pragma unroll
-                for (int half = 0; half < 2; half++) {
-                    const uint32_t from = (uint32_t)(k0 + half * 16 + 4 * h - lo), width = (half ? in1 : in0) ? (uint32_t)max(hi - lo, 0) : 0u;
+                for (int u = 0; u < 2; u++) {
+                    const uint32_t from = (uint32_t)(k0 + u * 16 + 4 * h - lo), width = (u ? was1 : was0) ? (uint32_t)max(hi - lo, 0) : 0u;
 #pragma unroll
                     for (int i = 0; i < 8; i++) {
                         const int at = (i >> 2) * 8 + (i & 3);
-                        x[8 * half + i] = from + at < width ? x[8 * half + i] : -INFINITY;
+                        x[8 * u + i] = from + at < width ? x[8 * u + i] : -INFINITY;
                     }
                 }
             }
@@ -274,12 +256,7 @@ __device__ __forceinline__ void rows128(const AttnArgs &a, int block, uint8_t *l
     uint8_t *buf0 = lds, *buf1 = lds + Step<NG>::BYTES;
     if (first < last) {
         store(buf0, part);
-        if (first + STEP < last) {
-            const Places p = steps.at(a.c, head, first + STEP);
-            nin[0] = p.in[0];
-            nin[1] = p.in[1];
-            load(p, part);
-        }
+        if (first + STEP < last) load(first + STEP, part, nin0, nin1);
     }
     lds_barrier();
     for (int k0 = first; k0 < last; k0 += 2 * STEP) {
@@ -292,7 +269,7 @@ __device__ __forceinline__ void rows128(const AttnArgs &a, int block, uint8_t *l
     const int64_t o = ((int64_t)s.t0 + tok) * a.out_stride + (int64_t)(head * a.group + gh) * D;
     const bool whole = it.pieces == 1;
     if (!whole && (slot < 0 || slot >= a.many.slots)) return;
-    float *to = a.many.part + (((int64_t)slot * a.c.heads + head) * TR + wave * WR + c) * (D + 4);
+    float *dst = a.many.part + (((int64_t)slot * a.c.heads + head) * TR + wave * WR + c) * (D + 4);
     const float inv = whole ? (sum == 0.0f ? 0.0f : 1.0f / sum) : 1.0f;
 #pragma unroll
     for (int i = 0; i < NG; i++)
@@ -303,9 +280,9 @@ __device__ __forceinline__ void rows128(const AttnArgs &a, int block, uint8_t *l
             if (whole)
                 store_out(a, o + e, v * inv);
             else
-                *(f32x4 *)(to + 4 + e) = v;
+                *(f32x4 *)(dst + 4 + e) = v;
         }
-    if (!whole && h == 0) *(float2 *)to = make_float2(m, sum);
+    if (!whole && h == 0) *(float2 *)dst = make_float2(m, sum);
 }
 
 constexpr size_t lds_bytes(int ng) { return 2 * (size_t)STEP * ((32 * ng + 8) + 32 * ng) * 2; }

@@ -52,23 +52,28 @@ __device__ __forceinline__ void rows16(const AttnArgs &a, int block, float *lds)
     const Offs<NG> offs = lane_offs<NG>();
     Raw<NG> r;
     int k0 = first + wave * STEP;
-    bool in[2] = {false, false};  // this step's tiles
-    Places next = {{nullptr, nullptr}, {0, 0}, {false, false}};
-    auto load_ks = [&](const Places &p) {
-#pragma unroll
-        for (int half = 0; half < 2; half++) load_k<RAW>(p.reg[half], a.c, p.sub[half], half, offs, r);
+    bool in0 = false, in1 = false;  // whether this step's tiles are the cache's
+    Place p0 = {a.c.data, 0, false}, p1 = p0;
+    auto load_ks = [&]() {
+        load_k<RAW>(p0.reg, a.c, p0.sub, 0, offs, r);
+        load_k<RAW>(p1.reg, a.c, p1.sub, 1, offs, r);
     };
-    auto load_vs = [&](const Places &p) {
-#pragma unroll
-        for (int half = 0; half < 2; half++) load_v<NG>(p.reg[half], a.c, p.sub[half], half, offs, r);
+    auto load_vs = [&]() {
+        load_v<NG>(p0.reg, a.c, p0.sub, 0, offs, r);
+        load_v<NG>(p1.reg, a.c, p1.sub, 1, offs, r);
+    };
+    auto places = [&](int k) {
+        const int l = steps.step(a.c, head, k);
+        p0 = steps.at(a.c, l);
+        p1 = steps.at(a.c, l + 1);
     };
     if (k0 < last) {  // (keys: the table has a page)
-        next = steps.at(a.c, head, k0);
-        in[0] = next.in[0];
-        in[1] = next.in[1];
-        load_ks(next);
-        load_vs(next);
-        next = steps.at(a.c, head, k0 + NEXT);
+        places(k0);
+        in0 = p0.in;
+        in1 = p1.in;
+        load_ks();
+        load_vs();
+        places(k0 + NEXT);
     }
 
     // q as operands: values 32g + 8h .. +7 of the row, times a power of two that puts the row's
@@ -156,16 +161,16 @@ __device__ __forceinline__ void rows16(const AttnArgs &a, int block, float *lds)
             // the scores are formed here: K's registers are free for the next step's loads
             asm volatile("" : "+v"(x[4 * half]), "+v"(x[4 * half + 1]), "+v"(x[4 * half + 2]), "+v"(x[4 * half + 3]));
         }
-        if (k1 < last) load_ks(next);
+        if (k1 < last) load_ks();
         if (cap > 0.0f) {
 #pragma unroll
             for (int i = 0; i < 8; i++) x[i] = tanh_of(x[i] * x_of_s) * x_of_t;
             unit = 1.0f;
         }
-        if (k0 < inner_lo || k0 + STEP > inner_hi || !in[0] || !in[1]) {
+        if (k0 < inner_lo || k0 + STEP > inner_hi || !in0 || !in1) {
 #pragma unroll
             for (int half = 0; half < 2; half++) {
-                const uint32_t from = (uint32_t)(k0 + half * 16 + 4 * h - lo), width = in[half] ? (uint32_t)max(hi - lo, 0) : 0u;
+                const uint32_t from = (uint32_t)(k0 + half * 16 + 4 * h - lo), width = (half ? in1 : in0) ? (uint32_t)max(hi - lo, 0) : 0u;
 #pragma unroll
                 for (int i = 0; i < 4; i++) x[4 * half + i] = from + i < width ? x[4 * half + i] : -INFINITY;
             }
@@ -204,10 +209,10 @@ __device__ __forceinline__ void rows16(const AttnArgs &a, int block, float *lds)
             }
         }
         if (k1 < last) {
-            load_vs(next);
-            in[0] = next.in[0];
-            in[1] = next.in[1];
-            next = steps.at(a.c, head, k1 + NEXT);
+            load_vs();
+            in0 = p0.in;
+            in1 = p1.in;
+            places(k1 + NEXT);
         }
         k0 = k1;
     }
