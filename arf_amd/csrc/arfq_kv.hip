@@ -26,6 +26,59 @@ __device__ __forceinline__ void store4(void *p, int64_t i, bool f16, const float
         *(float4 *)((float *)p + i) = make_float4(o[0], o[1], o[2], o[3]);
 }
 
+__device__ __forceinline__ void store8(void *p, int64_t i, bool f16, const float *o) {
+    if (f16) {
+        *(u32x4 *)((_Float16 *)p + i) =
+            u32x4{pack_f16x2(o[0], o[1]), pack_f16x2(o[2], o[3]), pack_f16x2(o[4], o[5]), pack_f16x2(o[6], o[7])};
+    } else {
+        store4(p, i, false, o);
+        store4(p, i + 4, false, o + 4);
+    }
+}
+
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, false);
+}
+template <int CTRL>
+__device__ __forceinline__ float dpp(float v) {
+    return __builtin_bit_cast(float, dpp<CTRL>(__builtin_bit_cast(uint32_t, v)));
+}
+
+// Byte b of lane a of a quad <-> byte a of lane b: pairs of lanes, then pairs of those.
+__device__ __forceinline__ uint32_t quad_transpose(uint32_t w) {
+    const uint32_t lane = threadIdx.x, y = dpp<0xb1>(w);  // quad_perm:[1,0,3,2]
+    w = __builtin_amdgcn_perm(y, w, lane & 1 ? 0x03070105u : 0x06020400u);
+    const uint32_t z = dpp<0x4e>(w);  // quad_perm:[2,3,0,1]
+    return __builtin_amdgcn_perm(z, w, lane & 2 ? 0x03020706u : 0x05040100u);
+}
+
+// Where a row's lane u has its V: values 4i .. +3 and 16 + 4i .. +3 of group g.  NG a multiple of 4: a dword of the
+// cache has a matrix row's bytes of four groups, and a quad of lanes turns the dwords of four such
+// rows into one group's bytes each; so g runs fastest over the lanes.  Otherwise byte by byte.
+template <int NG>
+struct VLane {
+    static constexpr bool DWORDS = NG % 4 == 0;
+    int g, i;
+    __device__ __forceinline__ VLane(int u) : g(DWORDS ? (u & 3) + (u >> 4) * 4 : u >> 2), i(DWORDS ? (u >> 2) & 3 : u & 3) {}
+    // what the lane of i ^ 1 has
+    static __device__ __forceinline__ uint32_t pair(uint32_t v) {
+        if constexpr (DWORDS) return (uint32_t)__builtin_amdgcn_ds_swizzle((int)v, 0x101f);  // lane ^ 4
+        return dpp<0xb1>(v);
+    }
+    // over the lanes of a group (i)
+    template <class F>
+    static __device__ __forceinline__ float all(float v, F f) {
+        if constexpr (DWORDS) {
+            v = f(v, dpp<0x124>(v));  // row_ror:4, 8
+            return f(v, dpp<0x128>(v));
+        } else {
+            v = f(v, dpp<0xb1>(v));
+            return f(v, dpp<0x4e>(v));
+        }
+    }
+};
+
 // Scale of a group from its extremes: s is the value of largest magnitude, the positive one of
 // two alike; d = s / -8 (a power of two: exact), at most 8160 so that 8 d is an f16, to 8
 // significant bits (ties to even) and to f16, whose subnormals hold multiples of 2^-24.
@@ -50,76 +103,72 @@ __device__ __forceinline__ uint32_t code_of(float x, float d, float rd) {
     return (uint32_t)((int)fminf(fmaxf(k, -8.0f), 7.0f) + 8);
 }
 
-// Sequence of the wave's tokens t[0 .. R): sequences b with start[b + 1] <= t come before it,
-// 64 compared at once.
-template <int R>
-__device__ __forceinline__ void find_seqs(const KvArgs &a, const int (&t)[R], int (&b)[R]) {
-    const int lane = threadIdx.x & 63;
+// The places in the cache of the rows that a lane works on, S of them, a wave's rows (row0 + set * R + lane / RL)
+// apart: regions (null: none), keys within the pages, tokens and heads.  Rows are (token, head) pairs,
+// head fastest.  The searches of all sets go side by side, and so do their loads of lengths
+// and page ids: one after another they take longer than the rows themselves.
+template <int RL, int S>
+struct Rows {
+    static constexpr int R = WAVE / RL;  // rows of a wave in a set
+    uint8_t *reg[S];
+    int key[S], token[S], head[S];
+    __device__ __forceinline__ Rows(const KvArgs &a, int row0, int rows) {
+        const int lane = threadIdx.x & 63;
+        int b[S];
 #pragma unroll
-    for (int r = 0; r < R; r++) b[r] = 0;
-    for (int b0 = 0; b0 < a.batch; b0 += WAVE) {
-        const int v = b0 + lane < a.batch ? a.start[b0 + lane + 1] : INT32_MAX;
+        for (int s = 0; s < S; s++) {
+            const int row = min(row0 + s * R + lane / RL, rows - 1);
+            token[s] = row / a.heads;
+            head[s] = row - token[s] * a.heads;
+            b[s] = a.start ? 0 : token[s];
+        }
+        if (a.start) {
+            // sequences b with start[b + 1] <= t come before t's, 64 compared at once
+            const int t0 = row0 / a.heads, t1 = min(row0 + S * R, rows) - 1;
+            for (int b0 = 0; b0 < a.batch; b0 += WAVE) {
+                const int v = b0 + lane < a.batch ? a.start[b0 + lane + 1] : INT32_MAX;
+                for (int t = t0; t <= t1 / a.heads; t++) {
+                    const int n = __popcll(__ballot(v <= t));
 #pragma unroll
-        for (int r = 0; r < R; r++) b[r] += __popcll(__ballot(v <= t[r]));
+                    for (int s = 0; s < S; s++) b[s] += token[s] == t ? n : 0;
+                }
+            }
+        }
+        int64_t pos[S];
+        int pg[S], id[S];
+#pragma unroll
+        for (int s = 0; s < S; s++) {
+            pos[s] = -1;
+            if (row0 + s * R + lane / RL < rows && b[s] < a.batch) {
+                int t0, n;
+                kv_seq(a, b[s], t0, n);
+                if (token[s] >= t0 && token[s] < t0 + n) pos[s] = (int64_t)a.len[b[s]] - ((int64_t)t0 + n - token[s]);
+            }
+        }
+#pragma unroll
+        for (int s = 0; s < S; s++) {
+            pg[s] = kv_page_of(a, (int)(pos[s] >> 4));
+            const bool in = pos[s] >= 0 && pos[s] <= INT32_MAX && pg[s] < a.max_pages;
+            id[s] = in ? a.table[(int64_t)b[s] * a.max_pages + pg[s]] : -1;
+        }
+#pragma unroll
+        for (int s = 0; s < S; s++) {
+            key[s] = (int)(pos[s] - (int64_t)pg[s] * a.page);
+            reg[s] = (uint32_t)id[s] < (uint32_t)a.n_pages ? a.data + ((int64_t)id[s] * a.heads + head[s]) * a.region : nullptr;
+        }
     }
-}
+};
 
-// The place in the cache of the row that this lane works on: its region (null: none) and its
-// key within the page.  Rows are (token, head) pairs, head fastest.
-template <int RL>
-__device__ __forceinline__ uint8_t *place(const KvArgs &a, int64_t row0, int64_t rows, int &token, int &head, int &key) {
-    constexpr int R = WAVE / RL;  // rows of a wave
-    const int lane = threadIdx.x & 63;
-    int ts[R], bs[R];
-#pragma unroll
-    for (int r = 0; r < R; r++) ts[r] = (int)(min(row0 + r, rows - 1) / a.heads);
-    const int mine = lane / RL;
-    const int64_t row = row0 + mine;
-    token = (int)(min(row, rows - 1) / a.heads);
-    head = (int)(min(row, rows - 1) - (int64_t)token * a.heads);
-    int b = token;
-    if (a.start) {
-        find_seqs<R>(a, ts, bs);
-        b = bs[0];
-#pragma unroll
-        for (int r = 1; r < R; r++) b = mine == r ? bs[r] : b;
-    }
-    if (row >= rows || b >= a.batch) return nullptr;
-    int t0, n;
-    kv_seq(a, b, t0, n);
-    const int64_t pos = (int64_t)a.len[b] - ((int64_t)t0 + n - token);
-    if (token < t0 || token >= t0 + n || pos < 0 || pos > INT32_MAX) return nullptr;
-    const int tile = (int)(pos >> 4), pg = kv_page_of(a, tile);
-    if (pg >= a.max_pages) return nullptr;
-    const int id = a.table[(int64_t)b * a.max_pages + pg];
-    if (id < 0 || id >= a.n_pages) return nullptr;
-    key = (int)(pos - (int64_t)pg * a.page);
-    return a.data + ((int64_t)id * a.heads + head) * a.region;
-}
-
+// A row: quantised and written.  (All lanes of the wave call it.)
 template <int NG>
-__global__ __launch_bounds__(256) void kv_write_kernel(KvArgs a, const void *k, int64_t k_stride, const void *v,
-                                                       int64_t v_stride, int f16, int64_t rows) {
+__device__ __forceinline__ void write_row(const KvArgs &a, const float (&xk)[8], const float (&xv)[8], uint8_t *reg, int key) {
     constexpr int RL = row_lanes<NG>(), D = 32 * NG;
     const int lane = threadIdx.x & 63;
-    const int64_t row0 = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * (WAVE / RL);
-    if (row0 >= rows) return;
-    int token, head, key = 0;
-    uint8_t *reg = place<RL>(a, row0, rows, token, head, key);
     const int u = lane % RL, g = u >> 2, i = u & 3;
+    const VLane<NG> vl(u);
     const bool on = reg && g < NG;
-    float xk[8], xv[8];
-#pragma unroll
-    for (int e = 0; e < 8; e++) xk[e] = xv[e] = 0.0f;
-    if (on) {
-        const int64_t ok = token * k_stride + head * D + 32 * g, ov = token * v_stride + head * D + 32 * g;
-        load4(k, ok + 8 * i, f16, xk);
-        load4(k, ok + 8 * i + 4, f16, xk + 4);
-        load4(v, ov + 4 * i, f16, xv);
-        load4(v, ov + 4 * i + 16, f16, xv + 4);
-    }
     // not finite: 0 * x is NaN
-    float nk = 0.0f, nv = 0.0f, kh = xk[0], kl = xk[0], vh = xv[0], vl = xv[0];
+    float nk = 0.0f, nv = 0.0f, kh = xk[0], kl = xk[0], vh = xv[0], vlow = xv[0];
 #pragma unroll
     for (int e = 0; e < 8; e++) {
         nk += 0.0f * xk[e];
@@ -127,20 +176,22 @@ __global__ __launch_bounds__(256) void kv_write_kernel(KvArgs a, const void *k, 
         kh = fmaxf(kh, xk[e]);
         kl = fminf(kl, xk[e]);
         vh = fmaxf(vh, xv[e]);
-        vl = fminf(vl, xv[e]);
+        vlow = fminf(vlow, xv[e]);
     }
-#pragma unroll
-    for (int x = 1; x <= 2; x <<= 1) {
-        kh = fmaxf(kh, __shfl_xor(kh, x));
-        kl = fminf(kl, __shfl_xor(kl, x));
-        vh = fmaxf(vh, __shfl_xor(vh, x));
-        vl = fminf(vl, __shfl_xor(vl, x));
-    }
-    const uint64_t quad = 0xfull << (lane & ~3);
-    const uint64_t mine = (RL == 64 ? ~0ull : ((1ull << RL) - 1)) << (lane / RL * RL);
-    const uint64_t bad_v = __ballot(nv != 0.0f || nv != nv), bad = (__ballot(nk != 0.0f || nk != nk) | bad_v) & mine;
+    auto hi = [](float a, float b) { return fmaxf(a, b); };
+    auto lo = [](float a, float b) { return fminf(a, b); };
+    auto sum = [](float a, float b) { return a + b; };  // (NaN if one is)
+    kh = hi(kh, dpp<0xb1>(kh));
+    kh = hi(kh, dpp<0x4e>(kh));
+    kl = lo(kl, dpp<0xb1>(kl));
+    kl = lo(kl, dpp<0x4e>(kl));
+    vh = VLane<NG>::all(vh, hi);
+    vlow = VLane<NG>::all(vlow, lo);
+    const uint64_t mine = ((1ull << RL) - 1) << (lane / RL * RL);
+    const uint64_t bad = __ballot(nk != nk || nv != nv) & mine;
+    nv = VLane<NG>::all(nv, sum);
     if (!on) return;
-    uint32_t dk = group_scale(kh, kl), dv = bad_v & quad ? 0u : group_scale(vh, vl);
+    const uint32_t dk = group_scale(kh, kl), dv = nv != nv ? 0u : group_scale(vh, vlow);
     const float fk = h2f(dk), fv = h2f(dv), rk = 1.0f / fk, rv = 1.0f / fv;
     uint32_t wk = 0, wv = 0;
 #pragma unroll
@@ -151,53 +202,109 @@ __global__ __launch_bounds__(256) void kv_write_kernel(KvArgs a, const void *k, 
         wv |= cv << (e < 4 ? 8 * e : 8 * (e - 4) + 4);
     }
     *(uint32_t *)(reg + (int64_t)key * (D / 2) + (i * NG + g) * 4) = wk;
-    uint8_t *vc = reg + a.off_v + (key >> 2) * (64 * NG) + (key & 3) * NG + g;
+    uint8_t *vc = reg + a.off_v + (key >> 2) * (64 * NG) + (key & 3) * NG;
+    if constexpr (VLane<NG>::DWORDS) {
+        *(uint32_t *)(vc + (u & 15) * (4 * NG) + (u >> 4) * 4) = quad_transpose(wv);
+    } else {
 #pragma unroll
-    for (int j = 0; j < 4; j++) vc[(4 * i + j) * 4 * NG] = (uint8_t)(wv >> (8 * j));
-    if (i == 0) {
-        // a row with a value that is not finite: its key is NaN, as is what attends to it
-        const int at = ((key >> 2) * NG + g) * 4 + (key & 3);
-        ((uint16_t *)(reg + a.off_ks))[key * NG + g] = (uint16_t)(bad ? 0x7e00u : dk);
-        ((uint16_t *)(reg + a.off_vs))[at] = (uint16_t)dv;
+        for (int j = 0; j < 4; j++) vc[(4 * i + j) * 4 * NG + g] = (uint8_t)(wv >> (8 * j));
     }
+    // a row with a value that is not finite: its key is NaN, as is what attends to it
+    if (i == 0) ((uint16_t *)(reg + a.off_ks))[key * NG + g] = (uint16_t)(bad ? 0x7e00u : dk);
+    if (vl.i == 0) ((uint16_t *)(reg + a.off_vs))[((key >> 2) * NG + vl.g) * 4 + (key & 3)] = (uint16_t)dv;
 }
 
 template <int NG>
-__global__ __launch_bounds__(256) void kv_read_kernel(KvArgs a, void *k, int64_t k_stride, void *v, int64_t v_stride,
-                                                      int f16, int64_t rows) {
+__global__ __launch_bounds__(256) void kv_write_kernel(KvArgs a, const void *k, int64_t k_stride, const void *v,
+                                                       int64_t v_stride, int f16, int rows) {
     constexpr int RL = row_lanes<NG>(), D = 32 * NG;
-    const int lane = threadIdx.x & 63;
-    const int64_t row0 = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * (WAVE / RL);
+    const int row0 = __builtin_amdgcn_readfirstlane((blockIdx.x * 4 + (threadIdx.x >> 6)) * (WAVE / RL));
     if (row0 >= rows) return;
-    int token, head, key = 0;
-    const uint8_t *reg = place<RL>(a, row0, rows, token, head, key);
-    const int u = lane % RL, g = u >> 2, i = u & 3;
-    if (!reg || g >= NG) return;
-    const int at = ((key >> 2) * NG + g) * 4 + (key & 3);
-    const float dk = h2f(((const uint16_t *)(reg + a.off_ks))[key * NG + g]), dv = h2f(((const uint16_t *)(reg + a.off_vs))[at]);
-    const uint32_t wk = *(const uint32_t *)(reg + (int64_t)key * (D / 2) + (i * NG + g) * 4);
-    const uint8_t *vc = reg + a.off_v + (key >> 2) * (64 * NG) + (key & 3) * NG + g;
+    const Rows<RL, 1> r(a, row0, rows);
+    const int u = threadIdx.x % RL, g = u >> 2, i = u & 3;
+    const VLane<NG> vl(u);
     float xk[8], xv[8];
 #pragma unroll
-    for (int e = 0; e < 8; e++) xk[e] = dk * (float)((int)(wk >> (4 * ((e >> 1) + 4 * (e & 1))) & 15u) - 8);
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-        const uint32_t b = vc[(4 * i + j) * 4 * NG];
-        xv[j] = dv * (float)((int)(b & 15u) - 8);
-        xv[4 + j] = dv * (float)((int)(b >> 4) - 8);
+    for (int e = 0; e < 8; e++) xk[e] = xv[e] = 0.0f;
+    if (r.reg[0] && g < NG) {
+        const int64_t ok = r.token[0] * k_stride + r.head[0] * D + 32 * g, ov = r.token[0] * v_stride + r.head[0] * D + 32 * vl.g;
+        load4(k, ok + 8 * i, f16, xk);
+        load4(k, ok + 8 * i + 4, f16, xk + 4);
+        load4(v, ov + 4 * vl.i, f16, xv);
+        load4(v, ov + 4 * vl.i + 16, f16, xv + 4);
     }
-    const int64_t ok = token * k_stride + head * D + 32 * g, ov = token * v_stride + head * D + 32 * g;
-    store4(k, ok + 8 * i, f16, xk);
-    store4(k, ok + 8 * i + 4, f16, xk + 4);
-    store4(v, ov + 4 * i, f16, xv);
-    store4(v, ov + 4 * i + 16, f16, xv + 4);
+    write_row<NG>(a, xk, xv, r.reg[0], r.key[0]);
 }
 
-template <int NG, class K, class... A>
+template <int NG, int S>
+__global__ __launch_bounds__(256) void kv_read_kernel(KvArgs a, void *k, int64_t k_stride, void *v, int64_t v_stride,
+                                                      int f16, int rows) {
+    constexpr int RL = row_lanes<NG>(), D = 32 * NG;
+    const int row0 = __builtin_amdgcn_readfirstlane((blockIdx.x * 4 + (threadIdx.x >> 6)) * (WAVE / RL * S));
+    if (row0 >= rows) return;
+    const Rows<RL, S> r(a, row0, rows);
+    const int u = threadIdx.x % RL, g = u >> 2, i = u & 3;
+    const VLane<NG> vl(u);
+    uint32_t wk[S], wv[S];
+    uint16_t sk[S], sv[S];
+#pragma unroll
+    for (int s = 0; s < S; s++) {
+        wk[s] = wv[s] = sk[s] = sv[s] = 0;
+        if (!r.reg[s] || g >= NG) continue;
+        const uint8_t *reg = r.reg[s];
+        const int key = r.key[s];
+        sk[s] = ((const uint16_t *)(reg + a.off_ks))[key * NG + g];
+        sv[s] = ((const uint16_t *)(reg + a.off_vs))[((key >> 2) * NG + vl.g) * 4 + (key & 3)];
+        wk[s] = *(const uint32_t *)(reg + (int64_t)key * (D / 2) + (i * NG + g) * 4);
+        const uint8_t *vc = reg + a.off_v + (key >> 2) * (64 * NG) + (key & 3) * NG;
+        if constexpr (VLane<NG>::DWORDS) {
+            wv[s] = *(const uint32_t *)(vc + (u & 15) * (4 * NG) + (u >> 4) * 4);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; j++) wv[s] |= (uint32_t)vc[(4 * i + j) * 4 * NG + g] << (8 * j);
+        }
+    }
+#pragma unroll
+    for (int s = 0; s < S; s++) {
+        if (!r.reg[s] || g >= NG) continue;
+        const float dk = h2f(sk[s]), dv = h2f(sv[s]);
+        const uint32_t w = VLane<NG>::DWORDS ? quad_transpose(wv[s]) : wv[s];
+        // eight neighbours a lane: of i and i ^ 1, the even one takes values 4i .. +7, the odd one 4i + 12 .. +7
+        const uint32_t other = VLane<NG>::pair(w), odd = vl.i & 1;
+        const uint32_t first = (odd ? other >> 4 : w) & 0x0f0f0f0fu, second = (odd ? w >> 4 : other) & 0x0f0f0f0fu;
+        float xk[8], xv[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) xk[e] = dk * (float)((int)(wk[s] >> (4 * ((e >> 1) + 4 * (e & 1))) & 15u) - 8);
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            xv[e] = dv * (float)((int)byte_of(first, e) - 8);
+            xv[4 + e] = dv * (float)((int)byte_of(second, e) - 8);
+        }
+        const int64_t ok = r.token[s] * k_stride + r.head[s] * D + 32 * g, ov = r.token[s] * v_stride + r.head[s] * D + 32 * vl.g;
+        store8(k, ok + 8 * i, f16, xk);
+        store8(v, ov + 4 * vl.i + (odd ? 12 : 0), f16, xv);
+    }
+}
+
+// Sets of rows a wave reads: four where that still fills the chip (32 waves a compute unit), one otherwise
+// (540 MB of f16 from eight sequences: one 253 us, four 194, eight 208).  Writing keeps to one: its
+// rows are wider in registers (345 MB in and out, f32: one 84 us, two 87, four 95).
+constexpr int SETS = 4;
+template <int NG, int S, class K, class... A>
 hipError_t rows_launch(K kernel, const KvArgs &a, hipStream_t s, A... args) {
-    const int64_t rows = (int64_t)a.tokens * a.heads, per = 4 * (WAVE / row_lanes<NG>());
-    kernel<<<dim3((unsigned)((rows + per - 1) / per)), 256, 0, s>>>(a, args..., rows);
+    const int64_t rows = (int64_t)a.tokens * a.heads, per = 4 * S * (WAVE / row_lanes<NG>());
+    kernel<<<dim3((unsigned)((rows + per - 1) / per)), 256, 0, s>>>(a, args..., (int)rows);
     return hipGetLastError();
+}
+template <int NG, class... A>
+hipError_t write_launch(const KvArgs &a, hipStream_t s, A... args) {
+    return rows_launch<NG, 1>(kv_write_kernel<NG>, a, s, args...);
+}
+template <int NG, class... A>
+hipError_t read_launch(const KvArgs &a, hipStream_t s, A... args) {
+    const bool many = (int64_t)a.tokens * a.heads >= (int64_t)256 * 32 * SETS * (WAVE / row_lanes<NG>());
+    return many ? rows_launch<NG, SETS>(kv_read_kernel<NG, SETS>, a, s, args...)
+                : rows_launch<NG, 1>(kv_read_kernel<NG, 1>, a, s, args...);
 }
 
 }  // namespace
@@ -206,10 +313,10 @@ hipError_t launch_kv_write(const KvArgs &a, int dim, const void *k, int64_t k_st
                            int dtype, hipStream_t s) {
     const int f16 = dtype == ARFQ_F16;
     switch (dim) {
-    case 64: return rows_launch<2>(kv_write_kernel<2>, a, s, k, k_stride, v, v_stride, f16);
-    case 96: return rows_launch<3>(kv_write_kernel<3>, a, s, k, k_stride, v, v_stride, f16);
-    case 128: return rows_launch<4>(kv_write_kernel<4>, a, s, k, k_stride, v, v_stride, f16);
-    case 256: return rows_launch<8>(kv_write_kernel<8>, a, s, k, k_stride, v, v_stride, f16);
+    case 64: return write_launch<2>(a, s, k, k_stride, v, v_stride, f16);
+    case 96: return write_launch<3>(a, s, k, k_stride, v, v_stride, f16);
+    case 128: return write_launch<4>(a, s, k, k_stride, v, v_stride, f16);
+    case 256: return write_launch<8>(a, s, k, k_stride, v, v_stride, f16);
     }
     return hipErrorInvalidValue;
 }
@@ -218,10 +325,10 @@ hipError_t launch_kv_read(const KvArgs &a, int dim, void *k, int64_t k_stride, v
                           hipStream_t s) {
     const int f16 = dtype == ARFQ_F16;
     switch (dim) {
-    case 64: return rows_launch<2>(kv_read_kernel<2>, a, s, k, k_stride, v, v_stride, f16);
-    case 96: return rows_launch<3>(kv_read_kernel<3>, a, s, k, k_stride, v, v_stride, f16);
-    case 128: return rows_launch<4>(kv_read_kernel<4>, a, s, k, k_stride, v, v_stride, f16);
-    case 256: return rows_launch<8>(kv_read_kernel<8>, a, s, k, k_stride, v, v_stride, f16);
+    case 64: return read_launch<2>(a, s, k, k_stride, v, v_stride, f16);
+    case 96: return read_launch<3>(a, s, k, k_stride, v, v_stride, f16);
+    case 128: return read_launch<4>(a, s, k, k_stride, v, v_stride, f16);
+    case 256: return read_launch<8>(a, s, k, k_stride, v, v_stride, f16);
     }
     return hipErrorInvalidValue;
 }
