@@ -230,6 +230,14 @@ union Frag {
     f16x8 v;
 };
 
+// v0 and v1 as two f16 parts each: hi rounded, lo what is left (one rounding each: v - hi is formed in f32
+// on the way into lo's half).
+__device__ __forceinline__ void split2(float v0, float v1, f16x2 &hi, f16x2 &lo) {
+    hi = f16x2{(_Float16)v0, (_Float16)v1};
+    asm("v_fma_mixlo_f16 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(lo) : "v"(hi), "v"(v0));
+    asm("v_fma_mixhi_f16 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "+v"(lo) : "v"(hi), "v"(v1));
+}
+
 // What a lane of the step's 32 keys loads: K of two 16-key tiles (key lane % 16, chunk lane / 16)
 // and V of the keys 4 * (lane / 16) .. +3 of both (matrix rows lane % 16).
 template <int NG>

@@ -234,13 +234,13 @@ __device__ __forceinline__ void rows128(const AttnArgs &a, int block, uint8_t *l
                 for (int i = 0; i < 4; i++) {
                     const float v0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[8 * b + 2 * i], unit, mb));
                     const float v1 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[8 * b + 2 * i + 1], unit, mb));
-                    const f16x2 f = {(_Float16)v0, (_Float16)v1};
-                    p[0].w[i] = f;
                     if constexpr (PARTS == 2) {
-                        p[1].w[i] = f16x2{(_Float16)(v0 - (float)f[0]), (_Float16)(v1 - (float)f[1])};
+                        split2(v0, v1, p[0].w[i], p[1].w[i]);
                         sum += v0 + v1;
                     } else {
                         // (what the values are multiplied with: a rounding of p then moves both alike)
+                        const f16x2 f = {(_Float16)v0, (_Float16)v1};
+                        p[0].w[i] = f;
                         sum = __builtin_amdgcn_fdot2(f, f16x2{(_Float16)1, (_Float16)1}, sum, false);
                     }
                 }

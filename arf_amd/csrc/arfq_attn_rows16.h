@@ -188,24 +188,26 @@ __device__ __forceinline__ void rows16(const AttnArgs &a, int block, float *lds)
             for (int t = 0; t < NT; t++) acc[t] *= f;
         }
         const float mb = P_BIAS - (m == -INFINITY ? 0.0f : m);
-        f16x8 p[PARTS];
+        Frag p[PARTS];
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const float v = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], unit, mb));
-            const _Float16 t = (_Float16)v;
-            p[0][i] = t;
-            if constexpr (PARTS == 2) p[1][i] = (_Float16)__builtin_fmaf((float)t, -1.0f, v);
+        for (int i = 0; i < 4; i++) {
+            const float v0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[2 * i], unit, mb));
+            const float v1 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[2 * i + 1], unit, mb));
+            if constexpr (PARTS == 2)
+                split2(v0, v1, p[0].w[i], p[1].w[i]);
+            else
+                p[0].w[i] = f16x2{(_Float16)v0, (_Float16)v1};
         }
 #pragma unroll
-        for (int pp = 0; pp < PARTS; pp++) sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones.v, p[pp], sum, 0, 0, 0);
+        for (int pp = 0; pp < PARTS; pp++) sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones.v, p[pp].v, sum, 0, 0, 0);
 #pragma unroll
         for (int g = 0; g < NG; g++) {
             f16x8 vl, vh;
             v_frags<NG>(r, g, magic, vl, vh);
 #pragma unroll
             for (int pp = 0; pp < PARTS; pp++) {
-                acc[2 * g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl, p[pp], acc[2 * g], 0, 0, 0);
-                acc[2 * g + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, p[pp], acc[2 * g + 1], 0, 0, 0);
+                acc[2 * g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl, p[pp].v, acc[2 * g], 0, 0, 0);
+                acc[2 * g + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, p[pp].v, acc[2 * g + 1], 0, 0, 0);
             }
         }
         if (k1 < last) {
