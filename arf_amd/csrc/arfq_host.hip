@@ -460,6 +460,9 @@ int arfq_kv_create(arfq_ctx *ctx, int heads, int head_dim, int page_size, int64_
         return fail(ctx, ARFQ_E_SHAPE, "kv_create: page_size must be a multiple of 16 up to 256");
     if (n_pages < 1 || n_pages > INT32_MAX) return fail(ctx, ARFQ_E_SHAPE, "kv_create: n_pages must be in [1, 2^31 - 1]");
     if (int rc = use_device(ctx)) return rc;
+    hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
+    HIP_TRY(ctx, hipStreamIsCapturing(ctx->stream, &cap));
+    if (cap != hipStreamCaptureStatusNone) return fail(ctx, ARFQ_E_INVALID, "kv_create: the stream is being captured");
     arfq_kv *kv = new (std::nothrow) arfq_kv();
     if (!kv) return fail(ctx, ARFQ_E_NOMEM, "kv_create: host allocation");
     kv->device = ctx->device;
@@ -592,8 +595,11 @@ int arfq_kv_attention_workspace(arfq_ctx *ctx, const arfq_kv *kv, int64_t batch,
     if (int rc = kv_q_heads(ctx, kv, batch, tokens, q_heads)) return rc;
     if (max_pages < 0 || max_pages > arfq::KV_KEYS_MAX / kv->page)
         return fail(ctx, ARFQ_E_SHAPE, "kv_attention_workspace: max_pages * page_size above 2^29");
-    // (with a start: the larger)
-    *bytes = arfq::attn_plan(ctx->cus, kv->heads, kv->dim, batch, tokens, q_heads, max_pages * kv->page, false).ws_bytes;
+    // (the call has a start, or none: the larger of the two)
+    *bytes = 0;
+    for (const bool one_each : {false, true})
+        *bytes = std::max(*bytes, arfq::attn_plan(ctx->cus, kv->heads, kv->dim, batch, tokens, q_heads, max_pages * kv->page,
+                                                  one_each).ws_bytes);
     return ARFQ_OK;
 }
 

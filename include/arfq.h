@@ -316,7 +316,9 @@ int arfq_ffn(arfq_ctx *ctx, const arfq_weight *gate, const arfq_weight *up, cons
 typedef struct arfq_kv arfq_kv;
 
 /* heads: K/V heads (1..1024); head_dim: 64, 96, 128 or 256 (others: ARFQ_E_UNSUPPORTED);
- * page_size: a multiple of 16 up to 256; n_pages: pages of the cache (1..2^31 - 1). */
+ * page_size: a multiple of 16 up to 256; n_pages: pages of the cache (1..2^31 - 1).
+ * Synchronous; ARFQ_E_INVALID while the context's stream is captured.  arfq_kv_free: as for
+ * a weight, after the work that uses it. */
 int arfq_kv_create(arfq_ctx *ctx, int heads, int head_dim, int page_size, int64_t n_pages, arfq_kv **out);
 int arfq_kv_free(arfq_kv *kv);
 /* Any out-pointer may be NULL. */
@@ -364,9 +366,10 @@ int arfq_kv_read(arfq_ctx *ctx, const arfq_kv *kv, const arfq_kv_seqs *seqs, voi
  * A step of any mix: one token a sequence, several, whole prompts.  Results do not depend on
  * which run of the same call they come from (no atomics on data).
  * workspace: arfq_kv_attention_workspace bytes of device memory (16-byte aligned) for the parts of
- * rows whose keys are spread over the chip, used only while the call's work runs; NULL takes
- * the context's scratch, except under stream capture, where it is ARFQ_E_INVALID (the
- * scratch moves when it grows; a captured graph keeps the address). */
+ * rows whose keys are spread over the chip, used only while the call's work runs (calls and graphs
+ * that run one after another may share it); NULL takes the context's scratch, except under
+ * stream capture, where it is ARFQ_E_INVALID unless 0 bytes are wanted (the scratch moves
+ * when it grows; a captured graph keeps the address). */
 int arfq_kv_attention(arfq_ctx *ctx, const arfq_kv *kv, const arfq_kv_seqs *seqs, int q_heads, const void *q,
                       int64_t q_stride, int q_dtype, void *out, int64_t out_stride, int out_dtype, float scale,
                       float softcap, int64_t window, int causal, void *workspace, size_t workspace_bytes);
