@@ -8,6 +8,8 @@
 //     16b + 4h + {0, 1, 2, 3} and 16b + 8 + 4h + {0, 1, 2, 3}      (h = lane / 32),
 // the order in which V goes to LDS.
 #pragma once
+#include <type_traits>
+
 #include "arfq_attn.h"
 
 namespace arfq {
@@ -24,7 +26,7 @@ constexpr int WAVES = TR / WR, THREADS = 64 * WAVES;
 template <int NG>
 struct Step {
     static constexpr int D = 32 * NG, KS = D + 8;
-    static constexpr int K_BYTES = STEP * KS * 2, BYTES = K_BYTES + STEP * D * 2;
+    static constexpr int K_BYTES = STEP * KS * 2, V_BYTES = STEP * D * 2;
 };
 
 // What a lane turns into f16: a wave has K or V of one of the step's two 16-key tiles, 64 units of NG
@@ -69,42 +71,46 @@ __device__ __forceinline__ void rows128(const AttnArgs &a, int block, uint8_t *l
     const uint32_t x_off = lane * (4 * NG), s_off = is_v ? (lane >> 4) * (8 * NG) : (lane >> 2) * (2 * NG);
     constexpr int AL = NG % 4 == 0 ? 16 : NG % 2 == 0 ? 8 : 4;
     const uint32_t x_at = is_v ? a.c.off_v : 0, s_at = is_v ? a.c.off_vs : a.c.off_ks;
-    // (in0, in1: whether the step's tiles are the cache's)
-    auto load = [&](int k0, Part<NG> &p, bool &in0, bool &in1) __attribute__((always_inline)) {
+    // keys k0 .. of the wave's tile into registers (past the last: some of the cache's, unused; no branch, so that
+    // a wait for one part leaves the next one's loads in flight); whether the step's tiles are the cache's, in
+    // the lowest bits of `in`
+    constexpr int AHEAD = PARTS == 1 ? 2 : 1;  // parts in flight
+    Part<NG> parts[AHEAD];
+    uint32_t in = 0;
+    auto load = [&](auto v, Part<NG> &part, int k0) __attribute__((always_inline)) {
         const int l = steps.step(a.c, head, k0);
-        in0 = steps.in(l);
-        in1 = steps.in(l + 1);
+        in = in << 2 | (steps.in(l) ? 1u : 0u) | (steps.in(l + 1) ? 2u : 0u);
         const Place pl = steps.at(a.c, l + half);
         const uint8_t *x = at(pl.reg + (x_at + pl.sub * (256u * NG)), x_off);
         const uint8_t *sc = at(pl.reg + (s_at + pl.sub * (32u * NG)), s_off);
-        load_aligned<NG, AL>(x, p.x);
-        if (is_v) {
-            load_aligned<2 * NG, 8>(sc, p.s);
-            asm volatile("");  // (or the branches' stores are made one, to memory)
+        load_aligned<NG, AL>(x, part.x);
+        if constexpr (v) {
+            load_aligned<2 * NG, 8>(sc, part.s);
         } else if constexpr (NG % 2) {
 #pragma unroll
-            for (int g = 0; g < NG; g++) p.s[g] = ((const uint16_t *)sc)[g];
+            for (int g = 0; g < NG; g++) part.s[g] = ((const uint16_t *)sc)[g];
         } else {
             uint32_t w[NG / 2];
             load_aligned<NG / 2, NG % 8 == 0 ? 16 : NG % 4 == 0 ? 8 : 4>(sc, w);
 #pragma unroll
-            for (int g = 0; g < NG / 2; g++) p.s[g] = w[g];
+            for (int g = 0; g < NG / 2; g++) part.s[g] = w[g];
         }
+        asm volatile("");  // (or the stores of K's and V's branch are made one, to memory)
     };
     const uint32_t magic = magic_1024();
     // (K's rows; V's (key block, half of a lane's eight keys) and matrix row)
-    const uint32_t to = is_v ? Step<NG>::K_BYTES + ((half * 2 + ((lane >> 4) & 1)) * D + (lane & 15)) * 16 + (lane >> 5) * 8
+    const uint32_t to = is_v ? ((half * 2 + ((lane >> 4) & 1)) * D + (lane & 15)) * 16 + (lane >> 5) * 8
                              : (half * 16 + (lane >> 2)) * (KS * 2) + (lane & 3) * 16;
-    auto store = [&](uint8_t *buf, const Part<NG> &p) __attribute__((always_inline)) {
+    auto store = [&](auto v, const Part<NG> &part, uint8_t *buf) __attribute__((always_inline)) {
         uint8_t *o = buf + to;
-        if (is_v) {
+        if constexpr (v) {
 #pragma unroll
             for (int g = 0; g < NG; g++) {
                 f16x2 l[2], u[2];
 #pragma unroll
                 for (int pr = 0; pr < 2; pr++) {
-                    const uint32_t w = pair_bytes<NG>(p.x, pr, g);
-                    const f16x2 d = __builtin_bit_cast(f16x2, p.s[2 * g + pr]);
+                    const uint32_t w = pair_bytes<NG>(part.x, pr, g);
+                    const f16x2 d = __builtin_bit_cast(f16x2, part.s[2 * g + pr]);
                     l[pr] = codes_f16<true>(w, magic) * d;
                     u[pr] = codes_f16<false>(w, magic) * d;
                 }
@@ -114,7 +120,7 @@ __device__ __forceinline__ void rows128(const AttnArgs &a, int block, uint8_t *l
         } else {
 #pragma unroll
             for (int g = 0; g < NG; g++) {
-                const uint32_t w = p.x[g], w8 = w >> 8, d2 = p.s[NG % 2 ? g : g / 2];
+                const uint32_t w = part.x[g], w8 = w >> 8, d2 = part.s[NG % 2 ? g : g / 2];
                 const f16x2 d = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(d2, d2, NG % 2 || g % 2 == 0 ? 0x01000100u : 0x03020302u));
                 Frag f;
                 f.w[0] = codes_f16<true>(w, magic) * d;
@@ -125,10 +131,15 @@ __device__ __forceinline__ void rows128(const AttnArgs &a, int block, uint8_t *l
             }
         }
     };
-
-    Part<NG> part;
-    bool in0 = false, in1 = false, nin0 = false, nin1 = false;  // of the tiles that are multiplied, and those in registers
-    if (first < last) load(first, part, in0, in1);
+    constexpr std::true_type V{};
+    constexpr std::false_type K{};
+    Part<NG> &part0 = parts[0];
+    if (first < last) {
+        if (is_v)
+            load(V, part0, first);
+        else
+            load(K, part0, first);
+    }
 
     // ---- q as operands, values 16i + 8h .. +7 of the row, scaled as in the kernel of few rows ----
     f16x8 q[PARTS][2 * NG];
@@ -169,99 +180,116 @@ __device__ __forceinline__ void rows128(const AttnArgs &a, int block, uint8_t *l
     for (int i = 0; i < NG; i++) acc[i] = zero;
     float m = -INFINITY, sum = 0.0f;
 
-    // one step: multiplies K and V of keys k0 .. in `cur`, puts those of the next step, in registers, into
-    // `other` and loads the ones after
-    auto step = [&](int k0, const uint8_t *kb, uint8_t *other) __attribute__((always_inline)) {
-        const uint8_t *vb = kb + Step<NG>::K_BYTES;
-        const bool was0 = in0, was1 = in1;
-        // K's operands are on their way from LDS while the next step's are made, V's while p is
+    // K's step is one ahead of V's: while the softmax of step i is computed, its p entering V's products, the
+    // matrix cores multiply K of step i + 1, and in the shadow of V's products the wave turns its
+    // part of the step after into operands.  LDS: K of two steps, V of two.
+    uint8_t *const kb = lds, *const vb = lds + 2 * Step<NG>::K_BYTES;
+    auto scores = [&](const uint8_t *b, f32x16 &x) __attribute__((always_inline)) {
         f16x8 kf[2 * NG];
 #pragma unroll
-        for (int i = 0; i < 2 * NG; i++) kf[i] = *(const f16x8 *)(kb + c * (KS * 2) + (2 * i + h) * 16);
-        __builtin_amdgcn_sched_barrier(0);
-        if (k0 + STEP < last) {
-            store(other, part);
-            in0 = nin0;
-            in1 = nin1;
-            if (k0 + 2 * STEP < last) load(k0 + 2 * STEP, part, nin0, nin1);
+        for (int i = 0; i < 2 * NG; i++) kf[i] = *(const f16x8 *)(b + c * (KS * 2) + (2 * i + h) * 16);
+        x = zero;
+#pragma unroll
+        for (int i = 0; i < 2 * NG; i++)
+#pragma unroll
+            for (int p = 0; p < PARTS; p++) x = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[i], q[p][i], x, 0, 0, 0);
+    };
+    f32x16 x = zero;
+    auto step = [&](auto v, int k0, int odd) __attribute__((always_inline)) {
+        const uint32_t was = in >> 2 * (AHEAD + (v ? 0 : 1));  // (of this step: as many loads ago)
+        float unit = x_of_s;
+        if (cap > 0.0f) {
+#pragma unroll
+            for (int i = 0; i < 16; i++) x[i] = tanh_of(x[i] * x_of_s) * x_of_t;
+            unit = 1.0f;
         }
-        {
-            f32x16 x = zero;
+        if (k0 < inner_lo || k0 + STEP > inner_hi || (was & 3) != 3) {
 #pragma unroll
-            for (int i = 0; i < 2 * NG; i++)
+            for (int u = 0; u < 2; u++) {
+                const uint32_t from = (uint32_t)(k0 + u * 16 + 4 * h - lo), width = (was >> u & 1) ? (uint32_t)max(hi - lo, 0) : 0u;
 #pragma unroll
-                for (int p = 0; p < PARTS; p++) x = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[i], q[p][i], x, 0, 0, 0);
-            f16x8 vf[2][NG];
+                for (int i = 0; i < 8; i++) {
+                    const int at = (i >> 2) * 8 + (i & 3);
+                    x[8 * u + i] = from + at < width ? x[8 * u + i] : -INFINITY;
+                }
+            }
+        }
+        float top = x[0];
 #pragma unroll
-            for (int b = 0; b < 2; b++)
+        for (int i = 1; i < 16; i++) top = fmaxf(top, x[i]);
+        top *= unit;
+        if (__ballot(top > m + M_SLACK)) {
+            const float mn = fmaxf(m, fmaxf(top, __shfl_xor(top, 32)));
+            const float f = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+            m = mn;
+            sum *= f;
 #pragma unroll
-                for (int i = 0; i < NG; i++) vf[b][i] = *(const f16x8 *)(vb + ((b * 2 + h) * D + 32 * i + c) * 16);
+            for (int i = 0; i < NG; i++) acc[i] *= f;
+        }
+        const float mb = P_BIAS - (m == -INFINITY ? 0.0f : m);
+        f32x16 y;
+        // (past the last step: of what lies there, unused)
+        if constexpr (PARTS == 1) scores(kb + (odd ^ 1) * Step<NG>::K_BYTES, y);
+        f16x8 vf[2][NG];
+#pragma unroll
+        for (int b = 0; b < 2; b++)
+#pragma unroll
+            for (int i = 0; i < NG; i++) vf[b][i] = *(const f16x8 *)(vb + odd * Step<NG>::V_BYTES + ((b * 2 + h) * D + 32 * i + c) * 16);
+        Frag p[2][PARTS];
+#pragma unroll
+        for (int b = 0; b < 2; b++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float v0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[8 * b + 2 * i], unit, mb));
+                const float v1 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[8 * b + 2 * i + 1], unit, mb));
+                if constexpr (PARTS == 2) {
+                    split2(v0, v1, p[b][0].w[i], p[b][1].w[i]);
+                    sum += v0 + v1;
+                } else {
+                    // (what the values are multiplied with: a rounding of p then moves both alike)
+                    const f16x2 f = {(_Float16)v0, (_Float16)v1};
+                    p[b][0].w[i] = f;
+                    sum = __builtin_amdgcn_fdot2(f, f16x2{(_Float16)1, (_Float16)1}, sum, false);
+                }
+            }
+#pragma unroll
+        for (int b = 0; b < 2; b++)
+#pragma unroll
+            for (int i = 0; i < NG; i++)
+#pragma unroll
+                for (int pp = 0; pp < PARTS; pp++)
+                    acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[b][i], p[b][pp].v, acc[i], 0, 0, 0);
+        if constexpr (PARTS == 2) {  // (no registers for both steps' scores)
             __builtin_amdgcn_sched_barrier(0);
-            float unit = x_of_s;
-            if (cap > 0.0f) {
-#pragma unroll
-                for (int i = 0; i < 16; i++) x[i] = tanh_of(x[i] * x_of_s) * x_of_t;
-                unit = 1.0f;
-            }
-            if (k0 < inner_lo || k0 + STEP > inner_hi || !was0 || !was1) {
-#pragma unroll
-                for (int u = 0; u < 2; u++) {
-                    const uint32_t from = (uint32_t)(k0 + u * 16 + 4 * h - lo), width = (u ? was1 : was0) ? (uint32_t)max(hi - lo, 0) : 0u;
-#pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        const int at = (i >> 2) * 8 + (i & 3);
-                        x[8 * u + i] = from + at < width ? x[8 * u + i] : -INFINITY;
-                    }
-                }
-            }
-            float top = x[0];
-#pragma unroll
-            for (int i = 1; i < 16; i++) top = fmaxf(top, x[i]);
-            top *= unit;
-            if (__ballot(top > m + M_SLACK)) {
-                const float mn = fmaxf(m, fmaxf(top, __shfl_xor(top, 32)));
-                const float f = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
-                m = mn;
-                sum *= f;
-#pragma unroll
-                for (int i = 0; i < NG; i++) acc[i] *= f;
-            }
-            const float mb = P_BIAS - (m == -INFINITY ? 0.0f : m);
-#pragma unroll
-            for (int b = 0; b < 2; b++) {
-                Frag p[PARTS];
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const float v0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[8 * b + 2 * i], unit, mb));
-                    const float v1 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[8 * b + 2 * i + 1], unit, mb));
-                    if constexpr (PARTS == 2) {
-                        split2(v0, v1, p[0].w[i], p[1].w[i]);
-                        sum += v0 + v1;
-                    } else {
-                        // (what the values are multiplied with: a rounding of p then moves both alike)
-                        const f16x2 f = {(_Float16)v0, (_Float16)v1};
-                        p[0].w[i] = f;
-                        sum = __builtin_amdgcn_fdot2(f, f16x2{(_Float16)1, (_Float16)1}, sum, false);
-                    }
-                }
-#pragma unroll
-                for (int i = 0; i < NG; i++)
-#pragma unroll
-                    for (int pp = 0; pp < PARTS; pp++)
-                        acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[b][i], p[pp].v, acc[i], 0, 0, 0);
-            }
+            scores(kb + (odd ^ 1) * Step<NG>::K_BYTES, y);
         }
+        Part<NG> &part = parts[odd % AHEAD];
+        store(v, part, v ? vb + (odd ^ 1) * Step<NG>::V_BYTES : kb + odd * Step<NG>::K_BYTES);  // (past the last step: to where nothing is read)
+        x = y;
+        load(v, part, k0 + ((v ? 1 : 2) + AHEAD) * STEP);
         lds_barrier();
     };
-    uint8_t *buf0 = lds, *buf1 = lds + Step<NG>::BYTES;
+    auto loop = [&](auto v) __attribute__((always_inline)) {
+        store(v, part0, v ? vb : kb);
+        load(v, part0, first + STEP);
+        if constexpr (!v) {
+            store(v, part0, kb + Step<NG>::K_BYTES);
+            load(v, part0, first + 2 * STEP);
+        }
+        if constexpr (AHEAD == 2) load(v, parts[1], first + (v ? 2 : 3) * STEP);
+        lds_barrier();
+        scores(kb, x);
+        lds_barrier();
+        for (int k0 = first; k0 < last; k0 += 2 * STEP) {
+            step(v, k0, 0);
+            step(v, k0 + STEP, 1);  // (without a branch, as the loads are; past the last: every key masked)
+        }
+    };
     if (first < last) {
-        store(buf0, part);
-        if (first + STEP < last) load(first + STEP, part, nin0, nin1);
-    }
-    lds_barrier();
-    for (int k0 = first; k0 < last; k0 += 2 * STEP) {
-        step(k0, buf0, buf1);
-        if (k0 + STEP < last) step(k0 + STEP, buf1, buf0);
+        if (is_v)
+            loop(V);
+        else
+            loop(K);
     }
 
     sum += __shfl_xor(sum, 32);
