@@ -7,12 +7,15 @@
 namespace arfq {
 namespace {
 
-// rows of a sequence that the 16-row tiles take
+// Rows of a sequence that the 16-row tiles take.  Each tile turns K and V into operands for itself; a 128-row tile
+// does so once, but takes its time for few rows too (sequences x rows x keys, us with the 16-row tiles and with
+// the 128-row ones: f16 16 x 36 x 4096 56 and 53, 1 x 56 x 8192 19 and 25, f32 16 x 56 x 4096 65 and 71;
+// above, 16 x 80 x 4096 86 and 58, f32 16 x 128 x 4096 122 and 92, 1 x 128 x 8192 24 and 27).
 constexpr int64_t FEW_ROWS = 64;
 
-// Rows whose keys were cut into pieces: their parts joined, in a fixed order.  A thread has four
-// columns of a row; with few pieces it takes them all, 1024 / D rows a workgroup, with many the
-// workgroup's threads share a row's.
+// Rows whose keys were cut into pieces: their parts joined, in a fixed order.  As many workgroups share a
+// tile's rows as it has pieces.  A thread has four columns of a row: of the parts it takes them all, 1024 / D rows
+// a workgroup side by side, or (few rows, many pieces) the workgroup's threads share a row's.
 template <int NG>
 struct JoinLds {
     static constexpr int D = 32 * NG, CT = D / 4, PT = 256 / CT;
@@ -24,9 +27,10 @@ __device__ __forceinline__ void join_rows(const AttnArgs &a, int slot, int head,
     constexpr int D = 32 * NG, CT = JoinLds<NG>::CT, PT = JoinLds<NG>::PT;
     const AttnList &list = list_of<TR>(a);
     const int4 j = list.join[slot];
-    if (j.x <= 1) return;
+    if (j.x == 0) return;
     const int pt = threadIdx.x / CT, ct = threadIdx.x - pt * CT;
-    const int rows = min(j.z - j.y, TR), pieces = min(j.x, list.slots - slot);
+    const int rows = min(j.z - j.y, TR), pieces = j.x & 0xffff, piece = j.x >> 16, slot0 = slot - piece;
+    if (slot0 < 0 || slot0 + pieces > list.slots) return;
     const int64_t next = (int64_t)a.c.heads * TR * (D + 4);
     // the weight of a part (m, l) below a common maximum; NaN for a NaN part (a NaN key leaves
     // a wave's maximum at -inf and its sum NaN)
@@ -58,22 +62,26 @@ __device__ __forceinline__ void join_rows(const AttnArgs &a, int slot, int head,
         }
         mm = top;
     };
-    auto part_of = [&](int r) { return list.part + (((int64_t)slot * a.c.heads + head) * TR + r) * (D + 4); };
+    auto part_of = [&](int r) { return list.part + (((int64_t)slot0 * a.c.heads + head) * TR + r) * (D + 4); };
     auto put = [&](int r, float l, f32x4 v) {
         const int rr = j.y + r, rt = rr / a.group, rg = rr - rt * a.group;
         store_out(a, ((int64_t)j.w + rt) * a.out_stride + (int64_t)(head * a.group + rg) * D + 4 * ct, v * (l == 0.0f ? 0.0f : 1.0f / l));
     };
-    if (pieces <= U) {  // a row for each CT threads
+    // the loads that follow one another: rows side by side, or one by one (with the LDS sum as one more).  (8 rows in
+    // 512 pieces: 63 us with the attention side by side, 21 one by one; 512 rows in 16: 44 and 111.)
+    const int beside = (rows + pieces * PT - 1) / (pieces * PT) * ((pieces + U - 1) / U);
+    const int each = (rows + pieces - 1) / pieces * ((pieces + U * PT - 1) / (U * PT) + 1);
+    if (beside <= each) {  // a row for each CT threads
         if (pt >= PT) return;
-        for (int r = blockIdx.z * PT + pt; r < rows; r += gridDim.z * PT) {
+        for (int r = piece * PT + pt; r < rows; r += pieces * PT) {
             float mm = -INFINITY, l = 0.0f;
             f32x4 v = {0, 0, 0, 0};
-            add(part_of(r), 0, 1, mm, l, v);
+            for (int p0 = 0; p0 < pieces; p0 += U) add(part_of(r), p0, 1, mm, l, v);
             put(r, l, v);
         }
         return;
     }
-    for (int r = blockIdx.z; r < rows; r += gridDim.z) {  // all threads on a row
+    for (int r = piece; r < rows; r += pieces) {  // all threads on a row
         float mm = -INFINITY, l = 0.0f;
         f32x4 v = {0, 0, 0, 0};
         if (pt < PT) {
@@ -133,9 +141,9 @@ template <int NG>
 hipError_t dim_launch(const AttnArgs &a, hipStream_t s) {
     const bool f16 = a.q_dtype == ARFQ_F16 && a.out_dtype == ARFQ_F16;
     hipError_t e = a.many.slots ? launch_attn_mixed(a, 32 * NG, s) : f16 ? rows16_launch<NG, 1>(a, s) : rows16_launch<NG, 2>(a, s);
-    if (e == hipSuccess && a.joins) {
+    if (e == hipSuccess && (a.few.join || a.many.join)) {
         const int64_t slots = (a.few.join ? a.few.slots : 0) + (a.many.join ? a.many.slots : 0);
-        attn_join<NG><<<dim3((unsigned)(slots * a.c.heads), 1, a.joins), 256, 0, s>>>(a);
+        attn_join<NG><<<dim3((unsigned)(slots * a.c.heads)), 256, 0, s>>>(a);
         e = hipGetLastError();
     }
     return e;
@@ -151,9 +159,9 @@ AttnPlan attn_plan(int cus, int heads, int dim, int64_t batch, int64_t tokens, i
     const int ng = dim / KV_GROUP;
     p.few_rows = FEW_ROWS;
     // a list's items: the area cut into `target` pieces, and at most one more for each tile; none of its
-    // pieces shorter than min_piece
+    // pieces shorter than MIN_PIECE
     auto plan = [&](AttnListPlan &l, int tr, int waves, int64_t tiles) {
-        const int64_t most = std::max<int64_t>(1, (max_keys + min_piece(tr) - 1) / min_piece(tr));
+        const int64_t most = std::max<int64_t>(1, (max_keys + MIN_PIECE - 1) / MIN_PIECE);
         l.target = std::max(1, waves * cus / heads);
         l.round = std::max(1, cus / heads);
         l.slots = (int)std::min(l.target + tiles, tiles * most);
@@ -169,12 +177,6 @@ AttnPlan attn_plan(int cus, int heads, int dim, int64_t batch, int64_t tokens, i
         plan(p.few, 16, many ? std::min(mixed_waves(ng), rows16_k::rows16_waves(ng)) : rows16_k::rows16_waves(ng),
              std::min({rows / 16 + batch, batch * ((FEW_ROWS + 15) / 16), tokens * ((group + 15) / 16)}));
     if (many) plan(p.many, 128, mixed_waves(ng), rows / 128 + std::min(batch, rows / (FEW_ROWS + 1)));
-    if (p.ws_bytes) {
-        // workgroups of a (tile, head): one for each of a few rows, or for 1024 / D of 128, while those of all the
-        // list's places, most of which have nothing to join, are not many times the chip's
-        const int64_t most = p.many.part_bytes ? 16 : std::min<int64_t>(16, one_each ? group : 16);
-        p.joins = (int)std::max<int64_t>(1, std::min<int64_t>(most, 16 * cus / ((p.few.slots + p.many.slots) * (int64_t)heads)));
-    }
     return p;
 }
 

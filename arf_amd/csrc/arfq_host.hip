@@ -650,7 +650,6 @@ int arfq_kv_attention(arfq_ctx *ctx, const arfq_kv *kv, const arfq_kv_seqs *seqs
     const size_t parts = plan.few.part_bytes + plan.many.part_bytes;
     a.few = list(plan.few, 0, parts);
     a.many = list(plan.many, plan.few.part_bytes, parts + plan.few.join_bytes);
-    a.joins = plan.joins;
     const hipError_t e = arfq::launch_attn(a, kv->dim, ctx->stream);
     return e == hipSuccess ? ARFQ_OK : hip_fail(ctx, e, "kv_attention launch");
 }

@@ -89,7 +89,7 @@ hipError_t launch_kv_read(const KvArgs &a, int dim, void *k, int64_t k_stride, v
 // ---- attention (arfq_attn.hip, arfq_attn_mixed.hip) ----
 // A work list (arfq_attn.h): the pieces it aims at, its items at most, the parts of rows of more than one
 // piece, [slots][heads][rows of a tile][dim + 4] (maximum, sum, -, -, values), and for each item
-// what the join takes: pieces (0: not a first one of several), first row, rows, first token.
+// what the join takes: pieces (0: one, or no item) and which of them, first row, rows, first token.
 struct AttnListPlan {
     int target = 1, slots = 0, round = 1;
     size_t part_bytes = 0, join_bytes = 0;
@@ -111,12 +111,10 @@ struct AttnArgs {
     int causal;
     int few_rows;         // sequences with at most so many rows are in `few` (16-row tiles), others in `many` (128)
     AttnList few, many;
-    int joins;  // gridDim.z of the join (0: no row has two pieces)
 };
 struct AttnPlan {
     int few_rows = 0;
     AttnListPlan few, many;
-    int joins = 0;
     size_t ws_bytes = 0;  // few's parts, many's, few's join, many's
 };
 bool attn_dim_ok(int dim);
