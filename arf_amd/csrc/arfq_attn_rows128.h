@@ -1,12 +1,19 @@
 // arfq_attn_rows128.h -- attention for prompts: tiles of 128 rows.
 //
 // A workgroup's four waves take 32 rows each and step through the keys together, 32 at a time: they
-// turn K and V of a step into f16 once, in LDS, and every wave multiplies all of it.  As in the
-// kernel of few rows, S^T = K Q^T and O^T = V^T P^T (v_mfma_f32_32x32x16_f16): a row is a lane's
-// column throughout, so its maximum and sum are registers, and the scores' registers 8b .. 8b + 7 are, as
-// they lie, the second product's operand for keys
+// turn K and V of a step into f16 once, in LDS (two waves K's, two V's tiles), and every wave multiplies
+// all of it.  As in the kernel of few rows, S^T = K Q^T and O^T = V^T P^T (v_mfma_f32_32x32x16_f16): a
+// row is a lane's column throughout, so its maximum and sum are registers, and the scores' registers
+// 8b .. 8b + 7 are, as they lie, the second product's operand for keys
 //     16b + 4h + {0, 1, 2, 3} and 16b + 8 + 4h + {0, 1, 2, 3}      (h = lane / 32),
 // the order in which V goes to LDS.
+//
+// Bound by the matrix cores and the softmax beside them, two waves a SIMD (the accumulators and q take 128 registers
+// of 256 at D = 128 and one part, 192 at two).  Measured at 40 x 128 q heads on 8: 8192 tokens of f16 781 us
+// (880 TFLOP/s of the 1131 that a plain f16 product reaches), 2048 tokens 72 (597; its longest tile's
+// 64 steps one after another take 60); 512 f32 tokens after 32356 others 623 (549, that is 1098 of
+// f16 products, as f32's two parts double them; matrix cores and vector unit busy half the time each).
+// f16 24 x 96 on 8, seven prompts of up to 777 tokens: 51 (382).
 #pragma once
 #include <type_traits>
 
@@ -252,6 +259,9 @@ __device__ __forceinline__ void rows128(const AttnArgs &a, int block, uint8_t *l
                     sum = __builtin_amdgcn_fdot2(f, f16x2{(_Float16)1, (_Float16)1}, sum, false);
                 }
             }
+        // (the products of a wave that has them ahead go first, the other wave's softmax falls beside them: 634 us
+        // down to 623 at 512 tokens of 32868, f32; with one part, where a wave overlaps its own, no gain)
+        if constexpr (PARTS == 2) __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int b = 0; b < 2; b++)
 #pragma unroll
@@ -265,6 +275,7 @@ __device__ __forceinline__ void rows128(const AttnArgs &a, int block, uint8_t *l
         }
         Part<NG> &part = parts[odd % AHEAD];
         store(v, part, v ? vb + (odd ^ 1) * Step<NG>::V_BYTES : kb + odd * Step<NG>::K_BYTES);  // (past the last step: to where nothing is read)
+        if constexpr (PARTS == 2) __builtin_amdgcn_s_setprio(0);
         x = y;
         load(v, part, k0 + ((v ? 1 : 2) + AHEAD) * STEP);
         lds_barrier();
