@@ -248,7 +248,6 @@ struct Raw {
     uint32_t k[2][NG], v[2][NG];
     uint32_t ks[2][2 * NG];              // of keys 4 * (lane / 16) .. +3: [4][NG] f16
     uint32_t vs[2][2 * NG];              // of the same, in pairs: [NG][2]
-    uint32_t ka[2][(NG + 1) / 2];        // of key lane % 16 (RAW)
 };
 
 // N dwords at an address that is a multiple of A bytes.
@@ -276,12 +275,12 @@ __device__ __forceinline__ void load_aligned(const void *p, uint32_t (&o)[N]) {
 // Byte offsets of a lane's operands in a 16-key tile (from the region, its V codes, scales and V scales).
 template <int NG>
 struct Offs {
-    uint32_t k, v, s, a;
+    uint32_t k, v, s;
 };
 template <int NG>
 __device__ __forceinline__ Offs<NG> lane_offs() {
     const uint32_t lane = threadIdx.x & 63, c = lane & 15, h = lane >> 4;
-    return {c * (16 * NG) + h * (4 * NG), h * (64 * NG) + c * (4 * NG), h * (8 * NG), c * (2 * NG)};
+    return {c * (16 * NG) + h * (4 * NG), h * (64 * NG) + c * (4 * NG), h * (8 * NG)};
 }
 // p + o with p uniform: hidden from the compiler, which would widen o once and keep it in two registers
 // instead of the loads' scalar base and 32-bit offset.
@@ -290,21 +289,11 @@ __device__ __forceinline__ const uint8_t *at(const uint8_t *p, uint32_t o) {
     return p + o;
 }
 // reg (uniform): the tile's (page, head) region; sub: the 16-key tile within the page
-template <bool RAW, int NG>
+template <int NG>
 __device__ __forceinline__ void load_k(const uint8_t *reg, const KvArgs &a, uint32_t sub, int half, const Offs<NG> &o, Raw<NG> &r) {
     constexpr int AL = NG % 4 == 0 ? 16 : NG % 2 == 0 ? 8 : 4;
     load_aligned<NG, AL>(at(reg + sub * (256u * NG), o.k), r.k[half]);
-    const uint8_t *ks = reg + (a.off_ks + sub * (32u * NG));
-    load_aligned<2 * NG, 8>(at(ks, o.s), r.ks[half]);
-    if constexpr (!RAW) {
-    } else if constexpr (NG % 2 == 0) {
-        load_aligned<NG / 2, NG % 8 == 0 ? 16 : NG % 4 == 0 ? 8 : 4>(at(ks, o.a), r.ka[half]);
-    } else {
-        const uint16_t *k1 = (const uint16_t *)at(ks, o.a);
-#pragma unroll
-        for (int i = 0; i < NG / 2; i++) r.ka[half][i] = k1[2 * i] | (uint32_t)k1[2 * i + 1] << 16;
-        r.ka[half][NG / 2] = k1[NG - 1];
-    }
+    load_aligned<2 * NG, 8>(at(reg + (a.off_ks + sub * (32u * NG)), o.s), r.ks[half]);
 }
 template <int NG>
 __device__ __forceinline__ void load_v(const uint8_t *reg, const KvArgs &a, uint32_t sub, int half, const Offs<NG> &o, Raw<NG> &r) {
@@ -318,27 +307,15 @@ __device__ __forceinline__ _Float16 half_of(uint32_t w, int i) {
     return __builtin_bit_cast(_Float16, (unsigned short)(i ? w >> 16 : w));
 }
 
-// MFMA operand of group g of the K tile, eight codes of one key.
-// RAW: as they lie, plus 8, as subnormal f16 numbers of c * 2^-24 (nibbles in bits 0..3) and 16 c * 2^-24
-// (bits 4..7); q's values for the latter slots (2, 3, 6, 7) come divided by 16.  The matrix core
-// multiplies subnormals, but aligns its sums by the exponent field: 2^-14 of the sum is lost,
-// an eighth of an f16 q's own rounding and far above an f32 one's.
-// Otherwise the codes themselves.
-template <bool RAW, int NG>
+// MFMA operand of group g of the K tile: eight codes of one key.
+template <int NG>
 __device__ __forceinline__ f16x8 k_frag(const Raw<NG> &r, int half, int g, uint32_t magic) {
     const uint32_t w = r.k[half][g], w8 = w >> 8;
     Frag f;
-    if constexpr (RAW) {
-        f.w[0] = __builtin_bit_cast(f16x2, w & 0x000f000fu);
-        f.w[1] = __builtin_bit_cast(f16x2, w & 0x00f000f0u);
-        f.w[2] = __builtin_bit_cast(f16x2, w8 & 0x000f000fu);
-        f.w[3] = __builtin_bit_cast(f16x2, w8 & 0x00f000f0u);
-    } else {
-        f.w[0] = codes_f16<true>(w, magic);
-        f.w[1] = codes_f16<false>(w, magic);
-        f.w[2] = codes_f16<true>(w8, magic);
-        f.w[3] = codes_f16<false>(w8, magic);
-    }
+    f.w[0] = codes_f16<true>(w, magic);
+    f.w[1] = codes_f16<false>(w, magic);
+    f.w[2] = codes_f16<true>(w8, magic);
+    f.w[3] = codes_f16<false>(w8, magic);
     return f.v;
 }
 

@@ -10,7 +10,6 @@ constexpr int TR = 16;    // rows of a tile
 constexpr int WAVES = 4;  // of a workgroup
 // waves of a SIMD (a workgroup has one on each): registers below 512 / that
 constexpr int rows16_waves(int ng) { return ng <= 2 ? 4 : ng <= 4 ? 3 : 2; }
-constexpr float BIAS_UNIT = 32768.0f;
 
 // ---- rows of 16, keys spread over the waves ------------------------------------------------
 // S^T = K Q^T, O^T = V^T P^T with v_mfma_f32_16x16x32_f16: the 16 rows are matrix columns, so a
@@ -23,7 +22,6 @@ constexpr float BIAS_UNIT = 32768.0f;
 template <int NG, int PARTS>
 __device__ __forceinline__ void rows16(const AttnArgs &a, int block, float *lds) {
     constexpr int D = 32 * NG, NT = 2 * NG;  // NT: 16-row tiles of O^T
-    constexpr bool RAW = PARTS == 1;         // K's operands: see k_frag
     constexpr int OS = D + 4;                // LDS floats of a row of O: [WAVES][16][OS], then [WAVES][16][2]
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, h = lane >> 4;
     const int head = block % a.c.heads;  // (fastest: the list's unused end comes last)
@@ -55,8 +53,8 @@ __device__ __forceinline__ void rows16(const AttnArgs &a, int block, float *lds)
     bool in0 = false, in1 = false;  // whether this step's tiles are the cache's
     Place p0 = {a.c.data, 0, false}, p1 = p0;
     auto load_ks = [&]() {
-        load_k<RAW>(p0.reg, a.c, p0.sub, 0, offs, r);
-        load_k<RAW>(p1.reg, a.c, p1.sub, 1, offs, r);
+        load_k(p0.reg, a.c, p0.sub, 0, offs, r);
+        load_k(p1.reg, a.c, p1.sub, 1, offs, r);
     };
     auto load_vs = [&]() {
         load_v<NG>(p0.reg, a.c, p0.sub, 0, offs, r);
@@ -79,9 +77,6 @@ __device__ __forceinline__ void rows16(const AttnArgs &a, int block, float *lds)
     // q as operands: values 32g + 8h .. +7 of the row, times a power of two that puts the row's
     // largest into [2^14, 2^15): hi + lo hold 22 bits (an f16 q its 11)
     f16x8 q[PARTS][NG];
-    // RAW codes come with 8 added: -8 times the sum of a group's q, in three f16 parts (lanes 0..15, 16..31,
-    // 32..47 of a row's), times K's scales is one more product
-    Frag bias;
     const int64_t qo = ((int64_t)s.t0 + tok) * a.q_stride + (int64_t)(head * a.group + gh) * D + 8 * h;
     float sc = fabsf(a.scale);
     {
@@ -96,31 +91,19 @@ __device__ __forceinline__ void rows16(const AttnArgs &a, int block, float *lds)
         const RowScale rs = row_scale(top, a.scale);
         sc *= rs.down;
 #pragma unroll
-        for (int i = 0; i < 4; i++) bias.w[i] = f16x2{(_Float16)0, (_Float16)0};
-#pragma unroll
-        for (int g = 0; g < NG; g++) {
-            float all = 0.0f;
+        for (int g = 0; g < NG; g++)
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                const float v = x[g][e] * rs.up * (RAW && (e & 2) ? 0.0625f : 1.0f);
-                const _Float16 t = (_Float16)v, l = (_Float16)(v - (float)t);
+                const float v = x[g][e] * rs.up;
+                const _Float16 t = (_Float16)v;
                 q[0][g][e] = t;
-                if constexpr (PARTS == 2) q[1][g][e] = l;
-                all += (float)t * (e & 2 ? 16.0f : 1.0f);
+                if constexpr (PARTS == 2) q[1][g][e] = (_Float16)(v - (float)t);
             }
-            if constexpr (!RAW) continue;
-            all += __shfl_xor(all, 16);
-            all += __shfl_xor(all, 32);
-            all *= -8.0f / 16777216 * BIAS_UNIT;  // at most 8 * 32 * 2^15 / 2^24 * 2^15 = 2^14
-            const float b0 = (float)(_Float16)all, b1 = (float)(_Float16)(all - b0), b2 = all - b0 - b1;
-            bias.w[g / 2][g % 2] = (_Float16)(h == 0 ? b0 : h == 1 ? b1 : h == 2 ? b2 : 0.0f);
-        }
     }
     constexpr float LOG2E = 1.4426950408889634f;
-    constexpr float UNIT = RAW ? 16777216.0f : 1.0f;  // of the products (RAW: of codes * 2^-24)
     // a product in the scores' log2, or in the cap (not below the smallest normal
     // number, where products of it are 0 beside p's 24 bits: a masked score is -inf, and -inf * 0 would be NaN)
-    const float cap = a.softcap, x_of_s = fmaxf((cap > 0.0f ? sc / cap : sc * LOG2E) * UNIT, 1.1754944e-38f);
+    const float cap = a.softcap, x_of_s = fmaxf(cap > 0.0f ? sc / cap : sc * LOG2E, 1.1754944e-38f);
     const float x_of_t = cap * LOG2E;
 
     f32x4 acc[NT], sum = {0, 0, 0, 0};
@@ -138,24 +121,16 @@ __device__ __forceinline__ void rows16(const AttnArgs &a, int block, float *lds)
 #pragma unroll
         for (int half = 0; half < 2; half++) {
             const f32x4 z = {0, 0, 0, 0};
-            if constexpr (RAW) {
-                Frag ka;
-#pragma unroll
-                for (int i = 0; i < 4; i++) ka.w[i] = __builtin_bit_cast(f16x2, i < (NG + 1) / 2 ? r.ka[half][i] : 0u);
-                const f32x4 o = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka.v, bias.v, z, 0, 0, 0);
-#pragma unroll
-                for (int i = 0; i < 4; i++) x[4 * half + i] = o[i] * (1.0f / BIAS_UNIT);
-            }
 #pragma unroll
             for (int g = 0; g < NG; g++) {
-                const f16x8 kf = k_frag<RAW>(r, half, g, magic);
+                const f16x8 kf = k_frag(r, half, g, magic);
                 f32x4 t = z;
 #pragma unroll
                 for (int p = 0; p < PARTS; p++) t = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, q[p][g], t, 0, 0, 0);
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     const float d = (float)half_of(r.ks[half][(i * NG + g) / 2], (i * NG + g) & 1);
-                    x[4 * half + i] = !RAW && g == 0 ? t[i] * d : __builtin_fmaf(t[i], d, x[4 * half + i]);
+                    x[4 * half + i] = g == 0 ? t[i] * d : __builtin_fmaf(t[i], d, x[4 * half + i]);
                 }
             }
             // the scores are formed here: K's registers are free for the next step's loads
