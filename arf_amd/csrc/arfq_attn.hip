@@ -15,7 +15,8 @@ constexpr int64_t FEW_ROWS = 64;
 
 // Rows whose keys were cut into pieces: their parts joined, in a fixed order.  As many workgroups share a
 // tile's rows as it has pieces.  A thread has four columns of a row: of the parts it takes them all, 1024 / D rows
-// a workgroup side by side, or (few rows, many pieces) the workgroup's threads share a row's.
+// a workgroup side by side, or (few rows, many pieces) the workgroup's threads share a row's.  Bound by
+// latency: 4 to 5 us, two loads that follow one another after the launch.
 template <int NG>
 struct JoinLds {
     static constexpr int D = 32 * NG, CT = D / 4, PT = 256 / CT;

@@ -1,5 +1,7 @@
 // arfq_attn_mixed.hip -- attention for batches with prompts in them: the 128-row tiles of those and the
-// 16-row tiles of the other sequences in one launch, side by side.
+// 16-row tiles of the other sequences in one launch, side by side.  (The step's lengths are on the
+// device: this is launched whenever a sequence may have more rows than the 16-row tiles take.  One launch:
+// neither list waits for the other's last tiles.)
 #include "arfq_attn_rows128.h"
 #include "arfq_attn_rows16.h"
 

@@ -9,11 +9,11 @@
 // the order in which V goes to LDS.
 //
 // Bound by the matrix cores and the softmax beside them, two waves a SIMD (the accumulators and q take 128 registers
-// of 256 at D = 128 and one part, 192 at two).  Measured at 40 x 128 q heads on 8: 8192 tokens of f16 781 us
-// (880 TFLOP/s of the 1131 that a plain f16 product reaches), 2048 tokens 72 (597; its longest tile's
-// 64 steps one after another take 60); 512 f32 tokens after 32356 others 623 (549, that is 1098 of
+// of 256 at D = 128 and one part, 192 at two).  Measured at 40 x 128 q heads on 8: 8192 tokens of f16 789 us
+// (871 TFLOP/s of the 1131 that a plain f16 product reaches), 2048 tokens 74 (580; its longest tile's
+// 64 steps one after another take 60); 512 f32 tokens after 32356 others 630 (543, that is 1086 of
 // f16 products, as f32's two parts double them; matrix cores and vector unit busy half the time each).
-// f16 24 x 96 on 8, seven prompts of up to 777 tokens: 51 (382).
+// f16 24 x 96 on 8, seven prompts of up to 777 tokens: 53 (367).
 #pragma once
 #include <type_traits>
 
@@ -260,7 +260,7 @@ __device__ __forceinline__ void rows128(const AttnArgs &a, int block, uint8_t *l
                 }
             }
         // (the products of a wave that has them ahead go first, the other wave's softmax falls beside them: 634 us
-        // down to 623 at 512 tokens of 32868, f32; with one part, where a wave overlaps its own, no gain)
+        // down to 624 at 512 tokens of 32868, f32; with one part, where a wave overlaps its own, no gain)
         if constexpr (PARTS == 2) __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int b = 0; b < 2; b++)

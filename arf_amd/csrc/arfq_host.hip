@@ -512,8 +512,8 @@ static int kv_args(arfq_ctx *ctx, const arfq_kv *kv, const arfq_kv_seqs *s, cons
     if (!kv || !s) return fail(ctx, ARFQ_E_INVALID, w + "null argument");
     if (kv->device != ctx->device) return fail(ctx, ARFQ_E_INVALID, w + "the cache is on another device than the context");
     if (s->batch < 0 || s->tokens < 0 || s->max_pages < 0) return fail(ctx, ARFQ_E_SHAPE, w + "negative size");
-    if (s->batch > (int64_t)1 << 24 || s->max_pages > arfq::KV_KEYS_MAX / kv->page)
-        return fail(ctx, ARFQ_E_SHAPE, w + "batch above 2^24, or max_pages * page_size above 2^29");
+    if (s->batch > arfq::KV_BATCH_MAX || s->max_pages > arfq::KV_KEYS_MAX / kv->page)
+        return fail(ctx, ARFQ_E_SHAPE, w + "batch above 16384, or max_pages * page_size above 2^29");
     if (s->tokens > arfq::KV_ROWS_MAX / kv->heads) return fail(ctx, ARFQ_E_SHAPE, w + "tokens * heads above 2^30");
     if (!s->start && s->tokens > s->batch) return fail(ctx, ARFQ_E_SHAPE, w + "more rows than sequences, and no start");
     if (s->tokens > 0 && s->batch > 0 && (!s->len || (s->max_pages > 0 && !s->pages)))
@@ -583,8 +583,8 @@ static int kv_q_heads(arfq_ctx *ctx, const arfq_kv *kv, int64_t batch, int64_t t
     if (!kv) return fail(ctx, ARFQ_E_INVALID, "kv_attention: null argument");
     if (q_heads < 1 || q_heads % kv->heads)
         return fail(ctx, ARFQ_E_SHAPE, "kv_attention: q_heads must be a multiple of the cache's heads");
-    if (batch < 0 || batch > (int64_t)1 << 24 || tokens < 0 || tokens > arfq::KV_ROWS_MAX / q_heads)
-        return fail(ctx, ARFQ_E_SHAPE, "kv_attention: batch above 2^24, or tokens * q_heads above 2^30");
+    if (batch < 0 || batch > arfq::KV_BATCH_MAX || tokens < 0 || tokens > arfq::KV_ROWS_MAX / q_heads)
+        return fail(ctx, ARFQ_E_SHAPE, "kv_attention: batch above 16384, or tokens * q_heads above 2^30");
     return ARFQ_OK;
 }
 

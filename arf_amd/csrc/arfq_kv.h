@@ -33,6 +33,8 @@ constexpr int KV_GROUP = 32;
 constexpr int KV_PAGE_MAX = 256;
 constexpr int KV_TILE = 16;  // keys that share a page: P is a multiple
 constexpr int64_t KV_KEYS_MAX = (int64_t)1 << 29;    // of a sequence (max_pages * P)
+// sequences of a call: each row of a write, and each item of the attention, looks through them, 64 at a time
+constexpr int64_t KV_BATCH_MAX = 16384;
 constexpr int64_t KV_ROWS_MAX = (int64_t)1 << 30;    // tokens * heads of a call
 constexpr int KV_HEADS_MAX = 1024;
 

@@ -1,4 +1,11 @@
 // arfq_kv.hip -- writing K and V rows into the 4-bit cache and reading them back.
+//
+// Four lanes have a group of 32 values, its K and its V, eight of each a lane: a group's extremes are two
+// exchanges within a quad, and what a lane has is a dword of the cache.  Bound by memory, and by the chain of
+// dependent loads in front of it (the row's sequence, its length, its page): f32 rows of three prompts,
+// 18552 tokens of 8 x 128, written in 54 us (173 MB, 3.2 TB/s; the codes' exact quotients are a third of
+// that time's vector work), read back in 35 (5.0 TB/s); 540 MB of f16 from eight sequences, 740 MB in
+// all, in 194 (3.8 TB/s; a plain copy reaches 4.8).
 #include "arfq_kv.h"
 
 namespace arfq {

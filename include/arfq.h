@@ -334,8 +334,8 @@ int arfq_kv_info(const arfq_kv *kv, int *heads, int *head_dim, int *page_size, i
  * and not attended to.  start must not decrease; a sequence for which it does, or whose rows
  * leave [0, tokens), has no rows. */
 typedef struct {
-    int64_t batch;        /* sequences */
-    int64_t tokens;       /* rows of k, v, q and out */
+    int64_t batch;        /* sequences, at most 16384 */
+    int64_t tokens;       /* rows of k, v, q and out; tokens * heads (q's for the attention) at most 2^30 */
     const int32_t *start; /* [batch + 1], or NULL (tokens <= batch) */
     const int32_t *len;   /* [batch] */
     const int32_t *pages; /* [batch, max_pages] */

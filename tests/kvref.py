@@ -58,12 +58,10 @@ def attention(q, k, v, scale, window=0, softcap=0.0, causal=True, absent=None):
         for h in range(hq):
             kk, vv, qq = k[ok, h // g], v[ok, h // g], q[t, h].astype(np.float64)
             s = kk @ qq * scale
-            # q in parts of 22 bits of the row's largest.  The products' f32 sums are of codes + 8, less 8 times the sum
-            # of q: terms of |q| (|k| + 8 |d|), 8 |d| being a group's largest |k|; a group's 32 products
-            # and 10 additions of its q, dim / 32 groups
+            # q in parts of 22 bits of the row's largest.  The products' f32 sums: a group's 32 products of codes and
+            # q (exact each), and a multiplication and addition for each of dim / 32 groups
             part = np.abs(kk).sum(1) * np.abs(qq).max() * 2.0 ** -22
-            top = np.abs(kk).reshape(len(kk), -1, GROUP).max(-1).repeat(GROUP, -1)
-            add = ((np.abs(kk) + top) @ np.abs(qq)) * (dim / 32 + 16) * 2.0 ** -24
+            add = (np.abs(kk) @ np.abs(qq)) * (dim / 32 + 16) * 2.0 ** -24
             err = (part + add) * abs(scale) + np.abs(s) * 2.0 ** -22
             if softcap:
                 s = softcap * np.tanh(s / softcap)

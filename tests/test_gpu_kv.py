@@ -442,7 +442,8 @@ def test_refusals(gpu_ctx):
     for s, want in [(None, E.ARFQ_E_INVALID), (seqs(ln=None), E.ARFQ_E_INVALID), (seqs(pages=None), E.ARFQ_E_INVALID),
                     (seqs(batch=-1), E.ARFQ_E_SHAPE), (seqs(tokens=-1), E.ARFQ_E_SHAPE), (seqs(most=-1), E.ARFQ_E_SHAPE),
                     (seqs(tokens=3), E.ARFQ_E_SHAPE), (seqs(most=2 ** 25 + 1), E.ARFQ_E_SHAPE),
-                    (seqs(batch=2 ** 25), E.ARFQ_E_SHAPE), (seqs(tokens=2 ** 30, start=lens.ptr), E.ARFQ_E_SHAPE)]:
+                    (seqs(batch=2 ** 25), E.ARFQ_E_SHAPE), (seqs(batch=16385), E.ARFQ_E_SHAPE),
+                    (seqs(tokens=2 ** 30, start=lens.ptr), E.ARFQ_E_SHAPE)]:
         assert write(s) == want and attend(s) == want
         assert L.arfq_kv_read(h, kv.handle, ctypes.byref(s) if s else None, x.ptr, 128, x.ptr, 128, 0) == want
     # nothing to do: nothing is looked at
