@@ -86,7 +86,8 @@ struct Item {
     Seq s;
     int b, tile, piece, pieces;
     int keys;  // of a piece (a multiple of STEP): the sequence's keys in equal parts
-    int slot;  // place in the list
+    int cut;   // items of the list that are pieces of several
+    int part;  // this one's place among them
 };
 
 // The `index`-th (tile, piece) of the batch: sequences in order, their tiles one after another,
@@ -94,7 +95,8 @@ struct Item {
 // in every wave of the launch: the fewest that cut the area into at most `target` pieces, or
 // nearly so (a target of workgroups that the chip holds at once: one more round for a few of
 // them would take as long as the first).  The area is summed in f32 in one fixed order; the 2^-16
-// added covers its rounding, so that the list has no more than target + tiles items.
+// added covers its rounding, so that the list has no more than target + tiles items, and no more than
+// 2 target of them are pieces of several (ceil(x) < 2 x for x > 1).
 template <int TR>
 __device__ __forceinline__ bool find_item(const AttnArgs &a, int index, Item &it) {
     const int lane = threadIdx.x & 63;
@@ -116,10 +118,15 @@ __device__ __forceinline__ bool find_item(const AttnArgs &a, int index, Item &it
         steps = ceilf(steps * fminf(items / target, 2.0f));
     }
     const int piece = keys_of(steps);
-    int before = 0;
+    it.cut = (int)over_batch([&](const Seq &s) {
+        const int np = pieces_of(s, piece);
+        return np > 1 ? (float)s.tiles * (float)np : 0.0f;
+    });
+    int before = 0, cut_before = 0;
     for (int b0 = 0; b0 < a.c.batch; b0 += WAVE) {
         const Seq s = b0 ? seq_of<TR>(a, b0 + lane) : s0;
         const int np = pieces_of(s, piece), own = (int)min((int64_t)s.tiles * np, (int64_t)1 << 30), inc = wave_scan(own);
+        const int cut = np > 1 ? own : 0, cut_inc = wave_scan(cut);
         const uint64_t past = __ballot(before + inc > index);
         if (past) {
             const int l = __ffsll((unsigned long long)past) - 1;
@@ -131,9 +138,9 @@ __device__ __forceinline__ bool find_item(const AttnArgs &a, int index, Item &it
             it.s.tiles = __builtin_amdgcn_readlane(s.tiles, l);
             it.pieces = __builtin_amdgcn_readlane(np, l);
             it.b = b0 + l;
-            it.slot = index;
             it.keys = ((it.s.end - it.s.lo + STEP - 1) / STEP + it.pieces - 1) / it.pieces * STEP;
             const int rest = index - before - __builtin_amdgcn_readlane(inc - own, l);
+            it.part = cut_before + __builtin_amdgcn_readlane(cut_inc - cut, l) + rest;
             it.tile = rest / it.pieces;
             it.piece = rest - it.tile * it.pieces;
             // Prompts: the longest tile first, and every other round of workgroups (one a compute unit)
@@ -150,19 +157,23 @@ __device__ __forceinline__ bool find_item(const AttnArgs &a, int index, Item &it
             return rest >= 0 && it.tile >= 0 && it.tile < it.s.tiles;
         }
         before += __builtin_amdgcn_readlane(inc, 63);
+        cut_before += __builtin_amdgcn_readlane(cut_inc, 63);
     }
     return false;
 }
 
-// The workgroup's item, and what the join has to know of it (the list's every place is written): the
+// The workgroup's item, and what the join has to know of it (every place is written): the
 // tile's pieces (bits 0..15) and which of them it is, its rows, the sequence's first token.
 template <int TR>
 __device__ __forceinline__ bool take_item(const AttnArgs &a, int block, Item &it) {
     const AttnList &list = list_of<TR>(a);
     const int slot = block / a.c.heads;
     const bool got = find_item<TR>(a, slot, it);
-    if (list.join && block % a.c.heads == 0 && threadIdx.x == 0)
-        list.join[slot] = make_int4(got && it.pieces > 1 ? it.pieces | it.piece << 16 : 0, it.tile * TR, it.s.n * a.group, it.s.t0);
+    if (list.join && block % a.c.heads == 0 && threadIdx.x == 0) {
+        if (slot >= it.cut && slot < list.cut) list.join[slot] = make_int4(0, 0, 0, 0);
+        if (got && it.pieces > 1 && (uint32_t)it.part < (uint32_t)list.cut)
+            list.join[it.part] = make_int4(it.pieces | it.piece << 16, it.tile * TR, it.s.n * a.group, it.s.t0);
+    }
     return got;
 }
 

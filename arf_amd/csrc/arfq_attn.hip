@@ -31,7 +31,7 @@ __device__ __forceinline__ void join_rows(const AttnArgs &a, int slot, int head,
     if (j.x == 0) return;
     const int pt = threadIdx.x / CT, ct = threadIdx.x - pt * CT;
     const int rows = min(j.z - j.y, TR), pieces = j.x & 0xffff, piece = j.x >> 16, slot0 = slot - piece;
-    if (slot0 < 0 || slot0 + pieces > list.slots) return;
+    if (slot0 < 0 || slot0 + pieces > list.cut) return;
     const int64_t next = (int64_t)a.c.heads * TR * (D + 4);
     // the weight of a part (m, l) below a common maximum; NaN for a NaN part (a NaN key leaves
     // a wave's maximum at -inf and its sum NaN)
@@ -115,7 +115,7 @@ template <int NG>
 __global__ __launch_bounds__(256) void attn_join(AttnArgs a) {
     __shared__ JoinLds<NG> sh;
     const int head = blockIdx.x % a.c.heads, slot = blockIdx.x / a.c.heads;
-    const int few = a.few.join ? a.few.slots : 0;
+    const int few = a.few.join ? a.few.cut : 0;
     if (slot < few)
         join_rows<NG, 16>(a, slot, head, sh);
     else
@@ -143,7 +143,7 @@ hipError_t dim_launch(const AttnArgs &a, hipStream_t s) {
     const bool f16 = a.q_dtype == ARFQ_F16 && a.out_dtype == ARFQ_F16;
     hipError_t e = a.many.slots ? launch_attn_mixed(a, 32 * NG, s) : f16 ? rows16_launch<NG, 1>(a, s) : rows16_launch<NG, 2>(a, s);
     if (e == hipSuccess && (a.few.join || a.many.join)) {
-        const int64_t slots = (a.few.join ? a.few.slots : 0) + (a.many.join ? a.many.slots : 0);
+        const int64_t slots = (a.few.join ? a.few.cut : 0) + (a.many.join ? a.many.cut : 0);
         attn_join<NG><<<dim3((unsigned)(slots * a.c.heads)), 256, 0, s>>>(a);
         e = hipGetLastError();
     }
@@ -167,8 +167,9 @@ AttnPlan attn_plan(int cus, int heads, int dim, int64_t batch, int64_t tokens, i
         l.round = std::max(1, cus / heads);
         l.slots = (int)std::min(l.target + tiles, tiles * most);
         if (most > 1) {
-            l.part_bytes = (size_t)l.slots * heads * tr * (dim + 4) * sizeof(float);
-            l.join_bytes = (size_t)l.slots * sizeof(int4);
+            l.cut = std::min(l.slots, 2 * l.target);
+            l.part_bytes = (size_t)l.cut * heads * tr * (dim + 4) * sizeof(float);
+            l.join_bytes = (size_t)l.cut * sizeof(int4);
             p.ws_bytes += l.part_bytes + l.join_bytes;
         }
     };

@@ -53,7 +53,6 @@ __device__ __forceinline__ void rows128(const AttnArgs &a, int block, uint8_t *l
     Item it;
     if (!take_item<TR>(a, block, it)) return;
     const Seq &s = it.s;
-    const int slot = it.slot;
 
     auto row_hi = [&](int64_t pos) { return pos < 0 ? 0 : a.causal ? (int)min(pos + 1, (int64_t)s.end) : s.end; };
     auto row_lo = [&](int64_t pos) { return a.window ? (int)max((int64_t)0, min(pos - a.window + 1, (int64_t)s.end)) : 0; };
@@ -307,8 +306,8 @@ __device__ __forceinline__ void rows128(const AttnArgs &a, int block, uint8_t *l
     if (!valid) return;
     const int64_t o = ((int64_t)s.t0 + tok) * a.out_stride + (int64_t)(head * a.group + gh) * D;
     const bool whole = it.pieces == 1;
-    if (!whole && (slot < 0 || slot >= a.many.slots)) return;
-    float *dst = a.many.part + (((int64_t)slot * a.c.heads + head) * TR + wave * WR + c) * (D + 4);
+    if (!whole && (uint32_t)it.part >= (uint32_t)a.many.cut) return;
+    float *dst = a.many.part + (((int64_t)it.part * a.c.heads + head) * TR + wave * WR + c) * (D + 4);
     const float inv = whole ? (sum == 0.0f ? 0.0f : 1.0f / sum) : 1.0f;
 #pragma unroll
     for (int i = 0; i < NG; i++)

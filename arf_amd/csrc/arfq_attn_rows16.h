@@ -229,7 +229,8 @@ __device__ __forceinline__ void rows16(const AttnArgs &a, int block, float *lds)
     if (rr >= s.n * a.group) return;
     const int rt = rr / a.group, rg = rr - rt * a.group;
     const bool whole = it.pieces == 1;
-    float *part = a.few.part + (((int64_t)it.slot * a.c.heads + head) * TR + er) * (D + 4);
+    if (!whole && (uint32_t)it.part >= (uint32_t)a.few.cut) return;
+    float *part = a.few.part + (((int64_t)it.part * a.c.heads + head) * TR + er) * (D + 4);
     const int64_t o = ((int64_t)s.t0 + rt) * a.out_stride + (int64_t)(head * a.group + rg) * D;
     const float inv = whole ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f;
 #pragma unroll

@@ -645,7 +645,7 @@ int arfq_kv_attention(arfq_ctx *ctx, const arfq_kv *kv, const arfq_kv_seqs *seqs
     a.few_rows = plan.few_rows;
     char *ws = (char *)workspace;
     auto list = [&](const arfq::AttnListPlan &l, size_t part, size_t join) {
-        return arfq::AttnList{l.target, l.slots, l.round, (float *)(ws + part), l.join_bytes ? (int4 *)(ws + join) : nullptr};
+        return arfq::AttnList{l.target, l.slots, l.cut, l.round, (float *)(ws + part), l.join_bytes ? (int4 *)(ws + join) : nullptr};
     };
     const size_t parts = plan.few.part_bytes + plan.many.part_bytes;
     a.few = list(plan.few, 0, parts);

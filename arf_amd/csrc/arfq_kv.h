@@ -89,17 +89,17 @@ hipError_t launch_kv_read(const KvArgs &a, int dim, void *k, int64_t k_stride, v
                           hipStream_t s);
 
 // ---- attention (arfq_attn.hip, arfq_attn_mixed.hip) ----
-// A work list (arfq_attn.h): the pieces it aims at, its items at most, the parts of rows of more than one
-// piece, [slots][heads][rows of a tile][dim + 4] (maximum, sum, -, -, values), and for each item
-// what the join takes: pieces (0: one, or no item) and which of them, first row, rows, first token.
+// A work list (arfq_attn.h): the pieces it aims at, its items at most, those of tiles in more than one piece
+// (`cut`), their rows' parts, [cut][heads][rows of a tile][dim + 4] (maximum, sum, -, -, values), and
+// for each what the join takes: pieces (0: no item) and which of them, first row, rows, first token.
 struct AttnListPlan {
-    int target = 1, slots = 0, round = 1;
+    int target = 1, slots = 0, cut = 0, round = 1;
     size_t part_bytes = 0, join_bytes = 0;
 };
 struct AttnList {
-    int target, slots, round;  // round: items that give every compute unit a workgroup
+    int target, slots, cut, round;  // round: items that give every compute unit a workgroup
     float *part;
-    int4 *join;                // null: no row has two pieces
+    int4 *join;                     // null: no row has two pieces
 };
 struct AttnArgs {
     KvArgs c;

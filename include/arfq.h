@@ -311,8 +311,7 @@ int arfq_ffn(arfq_ctx *ctx, const arfq_weight *gate, const arfq_weight *up, cons
  * to it gives NaN) and each group of V with one zero.
  * Memory is allocated and cleared by arfq_kv_create, and reached through page tables: page p
  * has the same `page_size` tokens of every head.
- * The reference keeps K/V in f32 or 8 bits in a paged cache and attends with split-K
- * flash-decoding kernels (crates/arf-core/src/cache, shaders/wgsl/attention_splitk*.wgsl). */
+ * The reference attends with split-K kernels (shaders/wgsl/attention_splitk*.wgsl). */
 typedef struct arfq_kv arfq_kv;
 
 /* heads: K/V heads (1..1024); head_dim: 64, 96, 128 or 256 (others: ARFQ_E_UNSUPPORTED);

@@ -264,3 +264,12 @@ def test_sequences_that_share_pages(gpu_ctx):
     q = _rows(rng, 3, 4, 128, np.float32)
     got = _attend(gpu_ctx, kv, batch, q, np.float32, 0.09)
     _check(batch, got, q, hk, hv, 0.09)
+
+
+def test_workspace_does_not_grow_with_a_prompt(gpu_ctx):
+    # parts are kept only of rows whose keys are cut, and a step with many tiles cuts none
+    kv = gpu_ctx.kv_cache(8, 128, 64, 4)
+    table, lens, start = (gpu_ctx.to_device(np.zeros(n, np.int32)) for n in ((1, 1000), 1, 2))
+    sizes = [gpu_ctx.kv_attention_workspace(kv, arf_amd.KVSeqs(table, lens, start, t), 32) for t in (1, 8192, 32768, 2 ** 20)]
+    assert 0 < sizes[0] < sizes[1] == sizes[2] == sizes[3] < 2 ** 27
+    kv.free()
