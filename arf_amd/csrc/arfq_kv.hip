@@ -3,43 +3,41 @@
 // Four lanes have a group of 32 values, its K and its V, eight of each a lane: a group's extremes are two
 // exchanges within a quad, and what a lane has is a dword of the cache.  Bound by memory, and by the chain of
 // dependent loads in front of it (the row's sequence, its length, its page): f32 rows of three prompts,
-// 18552 tokens of 8 x 128, written in 54 us (173 MB, 3.2 TB/s; the codes' exact quotients are a third of
-// that time's vector work), read back in 35 (5.0 TB/s); 540 MB of f16 from eight sequences, 740 MB in
-// all, in 194 (3.8 TB/s; a plain copy reaches 4.8).
+// 18552 tokens of 8 x 128, written in 52 us (173 MB, 3.3 TB/s; the codes' exact quotients are a third of
+// that time's vector work), read back in 35 (5.0 TB/s); 141000 tokens read as f16, 740 MB in
+// all, in 186 (4.0 TB/s; a plain copy reaches 4.8).
 #include "arfq_kv.h"
 
 namespace arfq {
 namespace {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 // Lanes of a (token, head) row: four for each group of 32 values, up to a power of two
 // (a row's lanes lie in one wave; D = 96 leaves four of its sixteen idle).
 template <int NG>
 constexpr int row_lanes() { return NG <= 2 ? 8 : NG <= 4 ? 16 : 32; }
 
+// (non-temporal: each value is read once; 83 us for 85 at 18552 f32 rows written and read)
 __device__ __forceinline__ void load4(const void *p, int64_t i, bool f16, float *o) {
     if (f16) {
-        const u32x2 w = *(const u32x2 *)((const _Float16 *)p + i);
+        const u32x2 w = __builtin_nontemporal_load((const u32x2 *)((const _Float16 *)p + i));
         o[0] = h2f(w.x); o[1] = h2f(w.x >> 16); o[2] = h2f(w.y); o[3] = h2f(w.y >> 16);
     } else {
-        const float4 w = *(const float4 *)((const float *)p + i);
+        const f32x4 w = __builtin_nontemporal_load((const f32x4 *)((const float *)p + i));
         o[0] = w.x; o[1] = w.y; o[2] = w.z; o[3] = w.w;
     }
 }
 
-__device__ __forceinline__ void store4(void *p, int64_t i, bool f16, const float *o) {
-    if (f16)
-        *(u32x2 *)((_Float16 *)p + i) = u32x2{pack_f16x2(o[0], o[1]), pack_f16x2(o[2], o[3])};
-    else
-        *(float4 *)((float *)p + i) = make_float4(o[0], o[1], o[2], o[3]);
-}
-
+// (non-temporal where a lane's one store has whole pieces of a line: f16 186 us for 194 at 141000 tokens; f32's
+// two halves of each 32 bytes 110 for 85 at 18552)
 __device__ __forceinline__ void store8(void *p, int64_t i, bool f16, const float *o) {
     if (f16) {
-        *(u32x4 *)((_Float16 *)p + i) =
-            u32x4{pack_f16x2(o[0], o[1]), pack_f16x2(o[2], o[3]), pack_f16x2(o[4], o[5]), pack_f16x2(o[6], o[7])};
+        const u32x4 w = {pack_f16x2(o[0], o[1]), pack_f16x2(o[2], o[3]), pack_f16x2(o[4], o[5]), pack_f16x2(o[6], o[7])};
+        __builtin_nontemporal_store(w, (u32x4 *)((_Float16 *)p + i));
     } else {
-        store4(p, i, false, o);
-        store4(p, i + 4, false, o + 4);
+        *(f32x4 *)((float *)p + i) = f32x4{o[0], o[1], o[2], o[3]};
+        *(f32x4 *)((float *)p + i + 4) = f32x4{o[4], o[5], o[6], o[7]};
     }
 }
 
@@ -294,7 +292,7 @@ __global__ __launch_bounds__(256) void kv_read_kernel(KvArgs a, void *k, int64_t
 }
 
 // Sets of rows a wave reads: four where that still fills the chip (32 waves a compute unit), one otherwise
-// (540 MB of f16 from eight sequences: one 253 us, four 194, eight 208).  Writing keeps to one: its
+// (141000 tokens of f16 from eight sequences: one 253 us, four 194, eight 208, before the stores were non-temporal).  Writing keeps to one: its
 // rows are wider in registers (345 MB in and out, f32: one 84 us, two 87, four 95).
 constexpr int SETS = 4;
 template <int NG, int S, class K, class... A>
