@@ -29,16 +29,16 @@ __device__ __forceinline__ void load4(const void *p, int64_t i, bool f16, float 
     }
 }
 
-// (non-temporal where a lane's one store has whole pieces of a line: f16 186 us for 194 at 141000 tokens; f32's
-// two halves of each 32 bytes 110 for 85 at 18552)
-__device__ __forceinline__ void store8(void *p, int64_t i, bool f16, const float *o) {
-    if (f16) {
-        const u32x4 w = {pack_f16x2(o[0], o[1]), pack_f16x2(o[2], o[3]), pack_f16x2(o[4], o[5]), pack_f16x2(o[6], o[7])};
-        __builtin_nontemporal_store(w, (u32x4 *)((_Float16 *)p + i));
-    } else {
-        *(f32x4 *)((float *)p + i) = f32x4{o[0], o[1], o[2], o[3]};
-        *(f32x4 *)((float *)p + i + 4) = f32x4{o[4], o[5], o[6], o[7]};
-    }
+// 16 bytes; PAST: not kept in the caches (see read_launch).
+template <bool PAST, class T>
+__device__ __forceinline__ void store16(void *p, T v) {
+    if constexpr (PAST)
+        __builtin_nontemporal_store(v, (T *)p);
+    else
+        *(T *)p = v;
+}
+__device__ __forceinline__ u32x4 pack8(const float *o) {
+    return u32x4{pack_f16x2(o[0], o[1]), pack_f16x2(o[2], o[3]), pack_f16x2(o[4], o[5]), pack_f16x2(o[6], o[7])};
 }
 
 template <int CTRL>
@@ -241,9 +241,9 @@ __global__ __launch_bounds__(256) void kv_write_kernel(KvArgs a, const void *k, 
     write_row<NG>(a, xk, xv, r.reg[0], r.key[0]);
 }
 
-template <int NG, int S>
+template <int NG, int S, bool F16, bool PAST>
 __global__ __launch_bounds__(256) void kv_read_kernel(KvArgs a, void *k, int64_t k_stride, void *v, int64_t v_stride,
-                                                      int f16, int rows) {
+                                                      int rows) {
     constexpr int RL = row_lanes<NG>(), D = 32 * NG;
     const int row0 = __builtin_amdgcn_readfirstlane((blockIdx.x * 4 + (threadIdx.x >> 6)) * (WAVE / RL * S));
     if (row0 >= rows) return;
@@ -274,20 +274,39 @@ __global__ __launch_bounds__(256) void kv_read_kernel(KvArgs a, void *k, int64_t
         if (!r.reg[s] || g >= NG) continue;
         const float dk = h2f(sk[s]), dv = h2f(sv[s]);
         const uint32_t w = VLane<NG>::DWORDS ? quad_transpose(wv[s]) : wv[s];
-        // eight neighbours a lane: of i and i ^ 1, the even one takes values 4i .. +7, the odd one 4i + 12 .. +7
-        const uint32_t other = VLane<NG>::pair(w), odd = vl.i & 1;
-        const uint32_t first = (odd ? other >> 4 : w) & 0x0f0f0f0fu, second = (odd ? w >> 4 : other) & 0x0f0f0f0fu;
-        float xk[8], xv[8];
-#pragma unroll
-        for (int e = 0; e < 8; e++) xk[e] = dk * (float)((int)(wk[s] >> (4 * ((e >> 1) + 4 * (e & 1))) & 15u) - 8);
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-            xv[e] = dv * (float)((int)byte_of(first, e) - 8);
-            xv[4 + e] = dv * (float)((int)byte_of(second, e) - 8);
-        }
         const int64_t ok = r.token[s] * k_stride + r.head[s] * D + 32 * g, ov = r.token[s] * v_stride + r.head[s] * D + 32 * vl.g;
-        store8(k, ok + 8 * i, f16, xk);
-        store8(v, ov + 4 * vl.i + (odd ? 12 : 0), f16, xv);
+        float xk[8], xv[8];
+        // a quad stores 64 bytes of a group at a time: f16 as eight neighbours a lane, f32 as four, twice
+        if constexpr (F16) {
+            // V: of i and i ^ 1, the even one takes values 4i .. +7, the odd one 4i + 12 .. +7
+            const uint32_t other = VLane<NG>::pair(w), odd = vl.i & 1;
+            const uint32_t first = (odd ? other >> 4 : w) & 0x0f0f0f0fu, second = (odd ? w >> 4 : other) & 0x0f0f0f0fu;
+#pragma unroll
+            for (int e = 0; e < 8; e++) xk[e] = dk * (float)((int)(wk[s] >> (4 * ((e >> 1) + 4 * (e & 1))) & 15u) - 8);
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                xv[e] = dv * (float)((int)byte_of(first, e) - 8);
+                xv[4 + e] = dv * (float)((int)byte_of(second, e) - 8);
+            }
+            store16<PAST>((_Float16 *)k + ok + 8 * i, pack8(xk));
+            store16<PAST>((_Float16 *)v + ov + 4 * vl.i + (odd ? 12 : 0), pack8(xv));
+        } else {
+            // K: values 4i .. +3 are half i % 2 of lane i / 2's, 16 + 4i .. +3 of lane 2 + i / 2's
+            const uint32_t sh = (i & 1) * 8, wa = dpp<0x50>(wk[s]) >> sh, wb = dpp<0xfa>(wk[s]) >> sh;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int at = 4 * ((e >> 1) + 4 * (e & 1));
+                xk[e] = dk * (float)((int)(wa >> at & 15u) - 8);
+                xk[4 + e] = dk * (float)((int)(wb >> at & 15u) - 8);
+                xv[e] = dv * (float)((int)byte_of(w & 0x0f0f0f0fu, e) - 8);
+                xv[4 + e] = dv * (float)((int)byte_of(w >> 4 & 0x0f0f0f0fu, e) - 8);
+            }
+#pragma unroll
+            for (int e = 0; e < 8; e += 4) {
+                store16<PAST>((float *)k + ok + 4 * i + 4 * e, f32x4{xk[e], xk[e + 1], xk[e + 2], xk[e + 3]});
+                store16<PAST>((float *)v + ov + 4 * vl.i + 4 * e, f32x4{xv[e], xv[e + 1], xv[e + 2], xv[e + 3]});
+            }
+        }
     }
 }
 
@@ -305,11 +324,21 @@ template <int NG, class... A>
 hipError_t write_launch(const KvArgs &a, hipStream_t s, A... args) {
     return rows_launch<NG, 1>(kv_write_kernel<NG>, a, s, args...);
 }
-template <int NG, class... A>
+// f16 goes past the caches, f32 from PAST_BYTES on (the last cache has 256 MB; below, what follows finds it
+// there).  us past them and not: f16 43 MB 12.6 and 15.2, 107 MB 30.5 and 40.9, 578 MB 186 and 194; f32
+// 80 MB 18.5 and 18.9, 152 MB after their writing 92 and 82 with it, 214 MB 56 and 77, 428 MB 127 and 144.
+constexpr int64_t PAST_BYTES = (int64_t)192 << 20;
+template <int NG, bool F16, bool PAST, class... A>
 hipError_t read_launch(const KvArgs &a, hipStream_t s, A... args) {
     const bool many = (int64_t)a.tokens * a.heads >= (int64_t)256 * 32 * SETS * (WAVE / row_lanes<NG>());
-    return many ? rows_launch<NG, SETS>(kv_read_kernel<NG, SETS>, a, s, args...)
-                : rows_launch<NG, 1>(kv_read_kernel<NG, 1>, a, s, args...);
+    return many ? rows_launch<NG, SETS>(kv_read_kernel<NG, SETS, F16, PAST>, a, s, args...)
+                : rows_launch<NG, 1>(kv_read_kernel<NG, 1, F16, PAST>, a, s, args...);
+}
+template <int NG, class... A>
+hipError_t read_launch(const KvArgs &a, hipStream_t s, bool f16, A... args) {
+    if (f16) return read_launch<NG, true, true>(a, s, args...);
+    return (int64_t)a.tokens * a.heads * (2 * 32 * NG * 4) >= PAST_BYTES ? read_launch<NG, false, true>(a, s, args...)
+                                                                         : read_launch<NG, false, false>(a, s, args...);
 }
 
 }  // namespace
@@ -328,12 +357,12 @@ hipError_t launch_kv_write(const KvArgs &a, int dim, const void *k, int64_t k_st
 
 hipError_t launch_kv_read(const KvArgs &a, int dim, void *k, int64_t k_stride, void *v, int64_t v_stride, int dtype,
                           hipStream_t s) {
-    const int f16 = dtype == ARFQ_F16;
+    const bool f16 = dtype == ARFQ_F16;
     switch (dim) {
-    case 64: return read_launch<2>(a, s, k, k_stride, v, v_stride, f16);
-    case 96: return read_launch<3>(a, s, k, k_stride, v, v_stride, f16);
-    case 128: return read_launch<4>(a, s, k, k_stride, v, v_stride, f16);
-    case 256: return read_launch<8>(a, s, k, k_stride, v, v_stride, f16);
+    case 64: return read_launch<2>(a, s, f16, k, k_stride, v, v_stride);
+    case 96: return read_launch<3>(a, s, f16, k, k_stride, v, v_stride);
+    case 128: return read_launch<4>(a, s, f16, k, k_stride, v, v_stride);
+    case 256: return read_launch<8>(a, s, f16, k, k_stride, v, v_stride);
     }
     return hipErrorInvalidValue;
 }
