@@ -4,8 +4,8 @@
 // exchanges within a quad, and what a lane has is a dword of the cache.  Bound by memory, and by the chain of
 // dependent loads in front of it (the row's sequence, its length, its page): f32 rows of three prompts,
 // 18552 tokens of 8 x 128, written in 52 us (173 MB, 3.3 TB/s; the codes' exact quotients are a third of
-// that time's vector work), read back in 35 (5.0 TB/s); 141000 tokens read as f16, 740 MB in
-// all, in 186 (4.0 TB/s; a plain copy reaches 4.8).
+// that time's vector work), read back in 32 (5.4 TB/s); 141000 tokens read as f16, 740 MB in
+// all, in 187 (4.0 TB/s; a plain copy reaches 4.8).
 #include "arfq_kv.h"
 
 namespace arfq {
