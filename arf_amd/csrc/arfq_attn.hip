@@ -2,16 +2,8 @@
 // of rows whose keys were cut into pieces.
 #include "arfq_attn_rows16.h"
 
-#include <algorithm>
-
 namespace arfq {
 namespace {
-
-// Rows of a sequence that the 16-row tiles take.  Each tile turns K and V into operands for itself; a 128-row tile
-// does so once, but takes its time for few rows too (sequences x rows x keys, us with the 16-row tiles and with
-// the 128-row ones: f16 16 x 36 x 4096 56 and 53, 1 x 56 x 8192 19 and 25, f32 16 x 56 x 4096 65 and 71;
-// above, 16 x 80 x 4096 86 and 58, f32 16 x 128 x 4096 122 and 92, 1 x 128 x 8192 24 and 27).
-constexpr int64_t FEW_ROWS = 64;
 
 // Rows whose keys were cut into pieces: their parts joined, in a fixed order.  As many workgroups share a
 // tile's rows as it has pieces.  A thread has four columns of a row: of the parts it takes them all, 1024 / D rows
@@ -123,7 +115,7 @@ __global__ __launch_bounds__(256) void attn_join(AttnArgs a) {
 }
 
 template <int NG, int PARTS>
-__global__ __launch_bounds__(256, rows16_k::rows16_waves(NG)) void attn_rows16(AttnArgs a) {
+__global__ __launch_bounds__(256, rows16_waves(NG)) void attn_rows16(AttnArgs a) {
     extern __shared__ float lds[];
     rows16_k::rows16<NG, PARTS>(a, blockIdx.x, lds);
 }
@@ -153,34 +145,6 @@ hipError_t dim_launch(const AttnArgs &a, hipStream_t s) {
 }  // namespace
 
 bool attn_dim_ok(int dim) { return dim == 64 || dim == 96 || dim == 128 || dim == 256; }
-
-AttnPlan attn_plan(int cus, int heads, int dim, int64_t batch, int64_t tokens, int q_heads, int64_t max_keys, bool one_each) {
-    AttnPlan p;
-    const int64_t group = q_heads / heads, rows = tokens * group;
-    const int ng = dim / KV_GROUP;
-    p.few_rows = FEW_ROWS;
-    // a list's items: the area cut into `target` pieces, and at most one more for each tile; none of its
-    // pieces shorter than MIN_PIECE
-    auto plan = [&](AttnListPlan &l, int tr, int waves, int64_t tiles) {
-        const int64_t most = std::max<int64_t>(1, (max_keys + MIN_PIECE - 1) / MIN_PIECE);
-        l.target = std::max(1, waves * cus / heads);
-        l.round = std::max(1, cus / heads);
-        l.slots = (int)std::min(l.target + tiles, tiles * most);
-        if (most > 1) {
-            l.cut = std::min(l.slots, 2 * l.target);
-            l.part_bytes = (size_t)l.cut * heads * tr * (dim + 4) * sizeof(float);
-            l.join_bytes = (size_t)l.cut * sizeof(int4);
-            p.ws_bytes += l.part_bytes + l.join_bytes;
-        }
-    };
-    // sequences of at most FEW_ROWS rows, and the longer ones
-    const bool many = (one_each ? group : rows) > FEW_ROWS;
-    if (group <= FEW_ROWS)
-        plan(p.few, 16, many ? std::min(mixed_waves(ng), rows16_k::rows16_waves(ng)) : rows16_k::rows16_waves(ng),
-             std::min({rows / 16 + batch, batch * ((FEW_ROWS + 15) / 16), tokens * ((group + 15) / 16)}));
-    if (many) plan(p.many, 128, mixed_waves(ng), rows / 128 + std::min(batch, rows / (FEW_ROWS + 1)));
-    return p;
-}
 
 hipError_t launch_attn(const AttnArgs &a, int dim, hipStream_t s) {
     switch (dim) {

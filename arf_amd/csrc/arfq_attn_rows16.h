@@ -8,10 +8,6 @@ namespace rows16_k {
 
 constexpr int TR = 16;    // rows of a tile
 constexpr int WAVES = 4;  // of a workgroup
-// waves of a SIMD (a workgroup has one on each): registers below 512 / that.  (One fewer, us: the 64 sequences below
-// 52 for 45, the window 33 for 27, the ungrouped heads 29 for 25.)
-constexpr int rows16_waves(int ng) { return ng <= 2 ? 4 : ng <= 4 ? 3 : 2; }
-
 // ---- rows of 16, keys spread over the waves ------------------------------------------------
 // S^T = K Q^T, O^T = V^T P^T with v_mfma_f32_16x16x32_f16: the 16 rows are matrix columns, so a
 // lane's four results of a tile belong to one row, its statistics are a register, and P^T in

@@ -9,7 +9,7 @@
 
 #include "arfq_common.h"
 #include "arfq_internal.h"
-#include "arfq_kv.h"
+#include "arfq_attn_list.h"
 
 #include <algorithm>
 #include <cmath>

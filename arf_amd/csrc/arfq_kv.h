@@ -70,8 +70,12 @@ __device__ __forceinline__ int kv_page_of(const KvArgs &a, int t) {
     return (int)(__umulhi((uint32_t)t, a.tile_magic) + ((uint32_t)t & a.tile_mask));
 }
 
-// First token and token count of sequence b (0 tokens where `start` does not increase or
-// leaves the batch's rows: such entries reach no memory).
+// Rows of sequences: start[b] .. start[b + 1] - 1.  `start` does not decrease; where it does, no sequence from
+// there on has rows, nor has one whose rows leave the batch's: no two sequences share a row, and all rows lie in
+// [0, tokens), whatever the array holds (the bounds on the attention's work list rest on that).
+
+// First token and token count of sequence b, the first with start[b + 1] above some token (none before it
+// decreases).
 __device__ __forceinline__ void kv_seq(const KvArgs &a, int b, int &t0, int &n) {
     if (!a.start) {
         t0 = b;
@@ -83,13 +87,29 @@ __device__ __forceinline__ void kv_seq(const KvArgs &a, int b, int &t0, int &n) 
     n = t0 >= 0 && t1 > t0 && t1 <= a.tokens ? t1 - t0 : 0;
 }
 
+// The same for 64 sequences, b in each lane of a wave (0 tokens from a.batch on).  ended: start has decreased before
+// them; on return, among them too.
+__device__ __forceinline__ void kv_seq64(const KvArgs &a, int b, bool &ended, int &t0, int &n) {
+    t0 = b;
+    n = b < min(a.batch, a.tokens) ? 1 : 0;
+    if (!a.start) return;
+    int t1 = t0 = 0;
+    if (b < a.batch) {
+        t0 = a.start[b];
+        t1 = a.start[b + 1];
+    }
+    const uint64_t falls = __ballot(t1 < t0), before = ((uint64_t)2 << (threadIdx.x & 63)) - 1;  // (and itself)
+    n = !ended && !(falls & before) && t0 >= 0 && t1 > t0 && t1 <= a.tokens ? t1 - t0 : 0;
+    ended = ended || falls;
+}
+
 hipError_t launch_kv_write(const KvArgs &a, int dim, const void *k, int64_t k_stride, const void *v, int64_t v_stride,
                            int dtype, hipStream_t s);
 hipError_t launch_kv_read(const KvArgs &a, int dim, void *k, int64_t k_stride, void *v, int64_t v_stride, int dtype,
                           hipStream_t s);
 
 // ---- attention (arfq_attn.hip, arfq_attn_mixed.hip) ----
-// A work list (arfq_attn.h): the pieces it aims at, its items at most, those of tiles in more than one piece
+// A work list (arfq_attn_list.h): the pieces it aims at, its items at most, those of tiles in more than one piece
 // (`cut`), their rows' parts, [cut][heads][rows of a tile][dim + 4] (maximum, sum, -, -, values), and
 // for each what the join takes: pieces (0: no item) and which of them, first row, rows, first token.
 struct AttnListPlan {
@@ -120,12 +140,8 @@ struct AttnPlan {
     size_t ws_bytes = 0;  // few's parts, many's, few's join, many's
 };
 bool attn_dim_ok(int dim);
-// max_keys: of a sequence; one_each: a token of every sequence (no start)
-AttnPlan attn_plan(int cus, int heads, int dim, int64_t batch, int64_t tokens, int q_heads, int64_t max_keys, bool one_each);
 hipError_t launch_attn(const AttnArgs &a, int dim, hipStream_t s);
 // both lists
 hipError_t launch_attn_mixed(const AttnArgs &a, int dim, hipStream_t s);
-// its workgroups that a compute unit holds (a wave each on every SIMD), at ng groups of 32 values
-constexpr int mixed_waves(int ng) { return ng <= 4 ? 2 : 1; }
 
 }  // namespace arfq

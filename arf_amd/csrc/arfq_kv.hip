@@ -128,15 +128,20 @@ struct Rows {
             b[s] = a.start ? 0 : token[s];
         }
         if (a.start) {
-            // sequences b with start[b + 1] <= t come before t's, 64 compared at once
+            // sequences b with start[b + 1] <= t come before t's, 64 compared at once; none from where start
+            // decreases on (kv_seq then finds that one without rows)
             const int t0 = row0 / a.heads, t1 = min(row0 + S * R, rows) - 1;
             for (int b0 = 0; b0 < a.batch; b0 += WAVE) {
-                const int v = b0 + lane < a.batch ? a.start[b0 + lane + 1] : INT32_MAX;
+                const bool mine = b0 + lane < a.batch;
+                const int u = mine ? a.start[b0 + lane] : 0, v = mine ? a.start[b0 + lane + 1] : INT32_MAX;
+                const uint64_t falls = __ballot(v < u), before = ((uint64_t)2 << lane) - 1;
+                const int end = falls & before ? INT32_MAX : v;
                 for (int t = t0; t <= t1 / a.heads; t++) {
-                    const int n = __popcll(__ballot(v <= t));
+                    const int n = __popcll(__ballot(end <= t));
 #pragma unroll
                     for (int s = 0; s < S; s++) b[s] += token[s] == t ? n : 0;
                 }
+                if (falls) break;
             }
         }
         int64_t pos[S];

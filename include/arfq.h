@@ -330,8 +330,8 @@ int arfq_kv_info(const arfq_kv *kv, int *heads, int *head_dim, int *page_size, i
  * is at position len[b] - (start[b + 1] - t).  start NULL: row b is sequence b's last token.
  * Rows of no sequence, rows at a negative position (an idle slot: len 0) and keys of a page
  * id outside [0, n_pages), or past max_pages, name nothing: they are not written or read,
- * and not attended to.  start must not decrease; a sequence for which it does, or whose rows
- * leave [0, tokens), has no rows. */
+ * and not attended to.  start must not decrease: where it does, no sequence from there on has
+ * rows (so no two share one); nor has a sequence whose rows leave [0, tokens). */
 typedef struct {
     int64_t batch;        /* sequences, at most 16384 */
     int64_t tokens;       /* rows of k, v, q and out; tokens * heads (q's for the attention) at most 2^30 */
