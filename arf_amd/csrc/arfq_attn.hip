@@ -117,7 +117,7 @@ __global__ __launch_bounds__(256) void attn_join(AttnArgs a) {
 template <int NG, int PARTS>
 __global__ __launch_bounds__(256, rows16_waves(NG)) void attn_rows16(AttnArgs a) {
     extern __shared__ float lds[];
-    rows16_k::rows16<NG, PARTS>(a, blockIdx.x, lds);
+    rows16_k::rows16<NG, PARTS>(a, block_of(), lds);
 }
 
 template <int NG, int PARTS>
@@ -126,7 +126,7 @@ hipError_t rows16_launch(const AttnArgs &a, hipStream_t s) {
     constexpr size_t lds = rows16_k::lds_bytes(NG);
     const hipError_t e = set_max_lds_once((const void *)attn_rows16<NG, PARTS>, lds, done);
     if (e != hipSuccess) return e;
-    attn_rows16<NG, PARTS><<<dim3((unsigned)a.few.slots * a.c.heads), 256, lds, s>>>(a);
+    attn_rows16<NG, PARTS><<<grid_of((int64_t)a.few.slots * a.c.heads), 256, lds, s>>>(a);
     return hipGetLastError();
 }
 

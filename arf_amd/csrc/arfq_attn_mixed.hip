@@ -13,7 +13,7 @@ namespace {
 template <int NG, int PARTS>
 __global__ __launch_bounds__(256, mixed_waves(NG)) void attn_mixed(AttnArgs a) {
     extern __shared__ float lds[];
-    const int many = a.many.slots * a.c.heads, block = blockIdx.x;  // (first: they take longer)
+    const int many = a.many.slots * a.c.heads, block = block_of();  // (first: they take longer)
     if (block < many)
         rows128_k::rows128<NG, PARTS>(a, block, (uint8_t *)lds);
     else
@@ -26,7 +26,7 @@ hipError_t mixed_launch(const AttnArgs &a, hipStream_t s) {
     constexpr size_t lds = std::max(rows16_k::lds_bytes(NG), rows128_k::lds_bytes(NG));
     const hipError_t e = set_max_lds_once((const void *)attn_mixed<NG, PARTS>, lds, done);
     if (e != hipSuccess) return e;
-    attn_mixed<NG, PARTS><<<dim3((unsigned)(a.many.slots + a.few.slots) * a.c.heads), 256, lds, s>>>(a);
+    attn_mixed<NG, PARTS><<<grid_of(((int64_t)a.many.slots + a.few.slots) * a.c.heads), 256, lds, s>>>(a);
     return hipGetLastError();
 }
 

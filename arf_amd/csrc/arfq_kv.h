@@ -48,6 +48,14 @@ inline KvLayout kv_layout(int page, int dim) {
     return {2 * ((int64_t)codes + scales), codes, 2 * codes, 2 * codes + scales};
 }
 
+// Workgroups of a launch, 256 threads each: a dimension of a grid has fewer than 2^32 threads, so from 2^23
+// workgroups on they lie in rows of that many (some of the last row have nothing to do).
+constexpr int GRID_ROW = 1 << 23;
+inline dim3 grid_of(int64_t blocks) {
+    return blocks <= GRID_ROW ? dim3((unsigned)blocks) : dim3(GRID_ROW, (unsigned)((blocks + GRID_ROW - 1) / GRID_ROW));
+}
+__device__ __forceinline__ int block_of() { return (int)(blockIdx.y * GRID_ROW + blockIdx.x); }
+
 // What every kernel of the cache takes: the cache and the batch.
 struct KvArgs {
     uint8_t *data;

@@ -228,7 +228,7 @@ template <int NG>
 __global__ __launch_bounds__(256) void kv_write_kernel(KvArgs a, const void *k, int64_t k_stride, const void *v,
                                                        int64_t v_stride, int f16, int rows) {
     constexpr int RL = row_lanes<NG>(), D = 32 * NG;
-    const int row0 = __builtin_amdgcn_readfirstlane((blockIdx.x * 4 + (threadIdx.x >> 6)) * (WAVE / RL));
+    const int row0 = __builtin_amdgcn_readfirstlane((block_of() * 4 + (threadIdx.x >> 6)) * (WAVE / RL));
     if (row0 >= rows) return;
     const Rows<RL, 1> r(a, row0, rows);
     const int u = threadIdx.x % RL, g = u >> 2, i = u & 3;
@@ -250,7 +250,7 @@ template <int NG, int S, bool F16, bool PAST>
 __global__ __launch_bounds__(256) void kv_read_kernel(KvArgs a, void *k, int64_t k_stride, void *v, int64_t v_stride,
                                                       int rows) {
     constexpr int RL = row_lanes<NG>(), D = 32 * NG;
-    const int row0 = __builtin_amdgcn_readfirstlane((blockIdx.x * 4 + (threadIdx.x >> 6)) * (WAVE / RL * S));
+    const int row0 = __builtin_amdgcn_readfirstlane((block_of() * 4 + (threadIdx.x >> 6)) * (WAVE / RL * S));
     if (row0 >= rows) return;
     const Rows<RL, S> r(a, row0, rows);
     const int u = threadIdx.x % RL, g = u >> 2, i = u & 3;
@@ -322,7 +322,7 @@ constexpr int SETS = 4;
 template <int NG, int S, class K, class... A>
 hipError_t rows_launch(K kernel, const KvArgs &a, hipStream_t s, A... args) {
     const int64_t rows = (int64_t)a.tokens * a.heads, per = 4 * S * (WAVE / row_lanes<NG>());
-    kernel<<<dim3((unsigned)((rows + per - 1) / per)), 256, 0, s>>>(a, args..., (int)rows);
+    kernel<<<grid_of((rows + per - 1) / per), 256, 0, s>>>(a, args..., (int)rows);
     return hipGetLastError();
 }
 template <int NG, class... A>

@@ -27,6 +27,8 @@ typedef enum { hipFuncAttributeMaxDynamicSharedMemorySize } hipFuncAttribute;
 hipError_t hipGetDevice(int *);
 hipError_t hipFuncSetAttribute(const void *, hipFuncAttribute, int);
 
+struct dim3 { unsigned x, y, z; dim3(unsigned x, unsigned y = 1, unsigned z = 1) : x(x), y(y), z(z) {} };
+extern const dim3 blockIdx;
 struct alignas(16) int4 { int x, y, z, w; };
 struct alignas(16) uint4 { unsigned x, y, z, w; };
 static inline int4 make_int4(int x, int y, int z, int w) { return {x, y, z, w}; }

@@ -74,3 +74,93 @@ def test_rows_written_and_read_where_start_decreases(gpu_ctx):
         zero = gpu_ctx.to_device(np.zeros((batch * 20, heads, dim), np.float32))
         gpu_ctx.kv_write(kv, whole, zero, zero)
     kv.free()
+
+
+# ---- the largest calls ----
+
+def _seqs(ctx, table, lens, start, tokens):
+    return arf_amd.KVSeqs(ctx.to_device(np.asarray(table, np.int32)), ctx.to_device(np.asarray(lens, np.int32)),
+                          ctx.to_device(np.asarray(start, np.int32)), tokens)
+
+
+@pytest.mark.parametrize("dim,heads", [(64, 1), (96, 2), (128, 1), (256, 4)])
+def test_as_many_rows_as_a_call_takes(gpu_ctx, dim, heads):
+    # 2^30 rows of k and v, all but the first few of no sequence (so there is no memory behind them):
+    # more threads than one dimension of a grid has
+    _say("2^30 rows", dim, heads)
+    rng = np.random.default_rng(dim)
+    L, h = arf_amd.load_library(), gpu_ctx.handle
+    kv = gpu_ctx.kv_cache(heads, dim, 16, 8)
+    seqs = _seqs(gpu_ctx, [[3, 1], [5, 0]], [20, 9], [2, 22, 31], 2 ** 30 // heads)
+    k, v = (_rows(rng, 31, heads, dim, np.float16) for _ in "kv")
+    dk, dv, w = gpu_ctx.to_device(k), gpu_ctx.to_device(v), heads * dim
+    assert L.arfq_kv_write(h, kv.handle, seqs.ref, dk.ptr, w, dv.ptr, w, 1) == arfq.ARFQ_OK, L.arfq_last_error(h)
+    for dtype, t in ((np.float32, 0), (np.float16, 1)):
+        ok, ov = (gpu_ctx.to_device(np.full((40, heads, dim), 5, dtype)) for _ in "kv")
+        assert L.arfq_kv_read(h, kv.handle, seqs.ref, ok.ptr, w, ov.ptr, w, t) == arfq.ARFQ_OK, L.arfq_last_error(h)
+        for got, x in ((ok.numpy(), k), (ov.numpy(), v)):
+            assert np.array_equal(got[2:31].astype(np.float64), kvref.held(x[2:])) and (got[:2] == 5).all() and (got[31:] == 5).all()
+    kv.free()
+
+
+def test_rows_behind_the_first_2_32_threads(gpu_ctx):
+    # the last rows of a write that takes more than 2^32 threads (k and v the same 64 GiB, most of it of no sequence)
+    _say("2^27 rows of 256")
+    dim, rows = 256, 2 ** 27 + 9
+    if gpu_ctx.memory()[1] < 100 * 2 ** 30:
+        pytest.skip("64 GiB of rows")
+    L, h = arf_amd.load_library(), gpu_ctx.handle
+    rng = np.random.default_rng(42)
+    kv = gpu_ctx.kv_cache(1, dim, 16, 2)
+    p = ctypes.c_void_p()
+    assert L.arfq_dev_malloc(h, rows * dim * 2, ctypes.byref(p)) == arfq.ARFQ_OK
+    try:
+        x = _rows(rng, 20, 1, dim, np.float16)
+        assert L.arfq_copy_h2d(h, p.value + (rows - 20) * dim * 2, x.ctypes.data, x.nbytes) == arfq.ARFQ_OK
+        seqs = _seqs(gpu_ctx, [[1, 0]], [20], [0, rows], rows)
+        assert L.arfq_kv_write(h, kv.handle, seqs.ref, p.value, dim, p.value, dim, 1) == arfq.ARFQ_OK, L.arfq_last_error(h)
+        dk, dv = (gpu_ctx.empty(x.shape, np.float32) for _ in "kv")
+        gpu_ctx.kv_read(kv, _seqs(gpu_ctx, [[1, 0]], [20], [0, 20], 20), dk, dv)
+        assert np.array_equal(dk.numpy().astype(np.float64), kvref.held(x)) and np.array_equal(dv.numpy(), dk.numpy())
+    finally:
+        L.arfq_dev_free(h, p.value)
+        kv.free()
+
+
+@pytest.mark.parametrize("dtype", [np.float16, np.float32])
+def test_as_many_workgroups_as_attention_takes(gpu_ctx, dtype):
+    # 1024 heads, 2048 sequences, 2^30 rows of q: a prompt, a token, and rows of no sequence
+    _say("2^30 rows of q", np.dtype(dtype).name)
+    heads, dim, batch = 1024, 64, 2048
+    rng = np.random.default_rng(43)
+    L, h = arf_amd.load_library(), gpu_ctx.handle
+    kv = gpu_ctx.kv_cache(heads, dim, 16, 8)
+    table = np.full((batch, 6), -1)
+    table[0], table[batch - 1, 0] = [4, 1, 7, 0, 2, 6], 3
+    lens = np.zeros(batch, np.int32)
+    lens[0], lens[-1] = 90, 12
+    start = np.full(batch + 1, 80)
+    start[0], start[-1] = 0, 81
+    filled = _seqs(gpu_ctx, table[[0, -1]], [90, 12], [0, 90, 102], 102)
+    k, v = (_rows(rng, 102, heads, dim, np.float16) for _ in "kv")
+    gpu_ctx.kv_write(kv, filled, gpu_ctx.to_device(k), gpu_ctx.to_device(v))
+    q = _rows(rng, 81, heads, dim, dtype)
+    dq, out = gpu_ctx.to_device(q), gpu_ctx.to_device(np.full((96, heads, dim), 9, dtype))
+    w, t = heads * dim, int(dtype == np.float16)
+    seqs = _seqs(gpu_ctx, table, lens, start, 2 ** 20)
+    assert L.arfq_kv_attention(h, kv.handle, seqs.ref, heads, dq.ptr, w, t, out.ptr, w, t, 0.125, 0.0, 0, 1,
+                               None, 0) == arfq.ARFQ_OK, L.arfq_last_error(h)
+    got = out.numpy()
+    assert (got[81:] == 9).all()
+    hk, hv = kvref.held_pair(k, v)
+    some = [0, 1, 500, 1023]  # heads
+
+    class One:
+        lens, news, start = [90, 12], [80, 1], [0, 80, 81]
+
+        @staticmethod
+        def cached(b):
+            return slice(0, 90) if b == 0 else slice(90, 102)
+
+    _check(One, np.ascontiguousarray(got[:81, some]), np.ascontiguousarray(q[:, some]), hk[:, some], hv[:, some], 0.125)
+    kv.free()
