@@ -177,8 +177,8 @@ __device__ __forceinline__ void rows128(const AttnArgs &a, int block, uint8_t *l
             }
         }
     }
-    constexpr float LOG2E = 1.4426950408889634f;
-    const float cap = a.softcap, x_of_s = fmaxf(cap > 0.0f ? sc / cap : sc * LOG2E, 1.1754944e-38f), x_of_t = cap * LOG2E;
+    const float cap = a.softcap;
+    const ScoreUnits of = score_units(sc, cap);
 
     f32x16 acc[NG];
     const f32x16 zero = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
@@ -203,10 +203,10 @@ __device__ __forceinline__ void rows128(const AttnArgs &a, int block, uint8_t *l
     f32x16 x = zero;
     auto step = [&](auto v, int k0, int odd) __attribute__((always_inline)) {
         const uint32_t was = in >> 2 * (AHEAD + (v ? 0 : 1));  // (of this step: as many loads ago)
-        float unit = x_of_s;
+        float unit = of.s;
         if (cap > 0.0f) {
 #pragma unroll
-            for (int i = 0; i < 16; i++) x[i] = tanh_of(x[i] * x_of_s) * x_of_t;
+            for (int i = 0; i < 16; i++) x[i] = tanh_of(x[i] * of.s) * of.t_of_tanh;
             unit = 1.0f;
         }
         if (k0 < inner_lo || k0 + STEP > inner_hi || (was & 3) != 3) {

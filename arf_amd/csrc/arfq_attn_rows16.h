@@ -104,11 +104,8 @@ __device__ __forceinline__ void rows16(const AttnArgs &a, int block, float *lds)
                 if constexpr (PARTS == 2) q[1][g][e] = (_Float16)(v - (float)t);
             }
     }
-    constexpr float LOG2E = 1.4426950408889634f;
-    // a product in the scores' log2, or in the cap (not below the smallest normal
-    // number, where products of it are 0 beside p's 24 bits: a masked score is -inf, and -inf * 0 would be NaN)
-    const float cap = a.softcap, x_of_s = fmaxf(cap > 0.0f ? sc / cap : sc * LOG2E, 1.1754944e-38f);
-    const float x_of_t = cap * LOG2E;
+    const float cap = a.softcap;
+    const ScoreUnits of = score_units(sc, cap);
 
     f32x4 acc[NT], sum = {0, 0, 0, 0};
 #pragma unroll
@@ -121,7 +118,7 @@ __device__ __forceinline__ void rows16(const AttnArgs &a, int block, float *lds)
 
     while (k0 < last) {
         const int k1 = k0 + NEXT;
-        float x[8], unit = x_of_s;  // scores; a unit of them in log2
+        float x[8], unit = of.s;  // scores; a unit of them in log2
 #pragma unroll
         for (int half = 0; half < 2; half++) {
             const f32x4 z = {0, 0, 0, 0};
@@ -143,7 +140,7 @@ __device__ __forceinline__ void rows16(const AttnArgs &a, int block, float *lds)
         if (k1 < last) load_ks();
         if (cap > 0.0f) {
 #pragma unroll
-            for (int i = 0; i < 8; i++) x[i] = tanh_of(x[i] * x_of_s) * x_of_t;
+            for (int i = 0; i < 8; i++) x[i] = tanh_of(x[i] * of.s) * of.t_of_tanh;
             unit = 1.0f;
         }
         if (k0 < inner_lo || k0 + STEP > inner_hi || !in0 || !in1) {

@@ -164,3 +164,51 @@ def test_as_many_workgroups_as_attention_takes(gpu_ctx, dtype):
 
     _check(One, np.ascontiguousarray(got[:81, some]), np.ascontiguousarray(q[:, some]), hk[:, some], hv[:, some], 0.125)
     kv.free()
+
+
+# ---- factors of the scores ----
+
+def _filled_batch(ctx, rng, dim):
+    batch = Batch(ctx, [300, 700, 20], [3, 40, 1], 16, rng)
+    kv = ctx.kv_cache(1, dim, 16, batch.n_pages)
+    return batch, kv, *_filled(ctx, kv, batch, rng)
+
+
+@pytest.mark.parametrize("dtype", [np.float16, np.float32])
+@pytest.mark.parametrize("cap", [1e25, 1e33, 1e35, 1e37, 2e38, 3.4028234e38])
+def test_caps_that_no_score_comes_near(gpu_ctx, dtype, cap):
+    # tanh(v) is v: the attention of no cap (kvref with none, within its tolerance of that)
+    _say("large cap", np.dtype(dtype).name, cap)
+    rng = np.random.default_rng(44)
+    batch, kv, hk, hv = _filled_batch(gpu_ctx, rng, 64)
+    q = _rows(rng, batch.tokens, 3, 64, dtype)
+    q[1, 0] = 0
+    for scale in (0.125, -3.0, 1e-30):
+        _check(batch, _attend(gpu_ctx, kv, batch, q, dtype, scale, softcap=cap), q, hk, hv, scale)
+    kv.free()
+
+
+@pytest.mark.parametrize("dtype", [np.float16, np.float32])
+@pytest.mark.parametrize("cap", [1e-45, 1e-40, 1e-38, 1e-20, 1e-3])
+def test_caps_that_leave_nothing(gpu_ctx, dtype, cap):
+    # every score within cap of 0: the mean of the values
+    _say("small cap", np.dtype(dtype).name, cap)
+    rng = np.random.default_rng(45)
+    batch, kv, hk, hv = _filled_batch(gpu_ctx, rng, 128)
+    q = _rows(rng, batch.tokens, 3, 128, dtype)
+    q[1, 0] = 0
+    for scale in (0.125, -1e30, 0.0):
+        _check(batch, _attend(gpu_ctx, kv, batch, q, dtype, scale, softcap=cap), q, hk, hv, scale, softcap=cap)
+    kv.free()
+
+
+@pytest.mark.parametrize("dtype", [np.float16, np.float32])
+@pytest.mark.parametrize("cap", [0.0, 1.0])
+def test_the_largest_scale_of_products_that_are_zero(gpu_ctx, dtype, cap):
+    _say("large scale", np.dtype(dtype).name, cap)
+    rng = np.random.default_rng(46)
+    batch, kv, hk, hv = _filled_batch(gpu_ctx, rng, 96)
+    q = np.zeros((batch.tokens, 3, 96), dtype)
+    for scale in (3.4e38, -3.4e38):
+        _check(batch, _attend(gpu_ctx, kv, batch, q, dtype, scale, softcap=cap), q, hk, hv, scale, softcap=cap)
+    kv.free()
