@@ -321,9 +321,13 @@ def _row_stride(a, tokens, width, stride, what):
 
 class Context:
     """One HIP device + one stream (GpuContext + CommandPass): the context's own, or the hipStream_t
-    `stream` (an address), which the caller keeps until the context is closed."""
+    `stream` (an address), which the caller keeps until the context is closed.  The default stream has
+    no address (0, as torch.cuda.current_stream().cuda_stream is at first): its work is not ordered with a
+    context's, and 0 is refused."""
 
     def __init__(self, device=0, stream=None):
+        if stream is not None and not stream:
+            raise ValueError("Context: stream 0 is the default stream; pass one that was created, or None")
         L = load_library()
         h = ctypes.c_void_p()
         st = L.arfq_ctx_create(int(device), stream, ctypes.byref(h))
