@@ -303,10 +303,11 @@ int arfq_ffn(arfq_ctx *ctx, const arfq_weight *gate, const arfq_weight *up, cons
  * head, head_dim values) is held in groups of 32: a scale d and 32 codes q in [-8, 7] that
  * stand for d * q, GGUF's Q4_0 values with a scale of 8 significant bits (4.5 bits a value).
  * With s the group's value of largest magnitude (the positive one of two alike),
- *     d = s / -8 rounded to 8 significant bits (ties to even) and to f16,
- *     q = x / d rounded to the nearest integer (ties to even), at most 7.
+ *     d = s / -8, at most 8160 in magnitude, rounded to 8 significant bits (ties to even) and to f16,
+ *     q = x / d rounded to the nearest integer (ties to even) in [-8, 7].
  * Every d * q is an f16, so what attention multiplies is what arfq_kv_read returns, to the bit.
- * Finite values beyond +-65280 are held as that.  A row of K or V with a NaN or an infinity
+ * So a finite value beyond 65280 of the sign of s is held as 65280 of that sign, one beyond 57120 of
+ * the other sign as 57120 of that.  A row of K or V with a NaN or an infinity
  * makes that token's key of that head NaN (K reads back as NaN, and a query row that attends
  * to it gives NaN) and each group of V with one zero.
  * Memory is allocated and cleared by arfq_kv_create, and reached through page tables: page p

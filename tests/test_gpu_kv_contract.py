@@ -212,3 +212,31 @@ def test_the_largest_scale_of_products_that_are_zero(gpu_ctx, dtype, cap):
     for scale in (3.4e38, -3.4e38):
         _check(batch, _attend(gpu_ctx, kv, batch, q, dtype, scale, softcap=cap), q, hk, hv, scale, softcap=cap)
     kv.free()
+
+
+# ---- the largest values ----
+
+@pytest.mark.parametrize("dim", [64, 96, 128, 256])
+def test_values_beyond_the_largest_scale(gpu_ctx, dim):
+    # of the sign of the group's extreme 65280, of the other 57120 (codes end at 7)
+    _say("largest values", dim)
+    batch = Batch(gpu_ctx, [4], [4], 16, np.random.default_rng(47))
+    kv = gpu_ctx.kv_cache(1, dim, 16, batch.n_pages)
+    x = np.zeros((4, 1, dim), np.float32)
+    x[0, 0, ::32], x[0, 0, 1::32] = 1e6, -1e6
+    x[1, 0, 2::32], x[1, 0, 3::32] = -2e6, 1e6
+    x[2, 0, 4::32], x[2, 0, 5::32] = 3e38, -65281
+    x[3, 0, 6::32], x[3, 0, 7::32] = -65280, 57121
+    want = np.zeros_like(x)
+    want[0, 0, ::32], want[0, 0, 1::32] = 65280, -57120
+    want[1, 0, 2::32], want[1, 0, 3::32] = -65280, 57120
+    want[2, 0, 4::32], want[2, 0, 5::32] = 65280, -57120
+    want[3, 0, 6::32], want[3, 0, 7::32] = -65280, 57120
+    assert np.array_equal(kvref.held(x), want)
+    d = gpu_ctx.to_device(x)
+    gpu_ctx.kv_write(kv, batch.seqs, d, d)
+    for dtype in (np.float32, np.float16):
+        dk, dv = gpu_ctx.empty(x.shape, dtype), gpu_ctx.empty(x.shape, dtype)
+        gpu_ctx.kv_read(kv, batch.seqs, dk, dv)
+        assert np.array_equal(dk.numpy(), want.astype(dtype)) and np.array_equal(dv.numpy(), want.astype(dtype))
+    kv.free()
