@@ -333,17 +333,17 @@ hipError_t write_launch(const KvArgs &a, hipStream_t s, A... args) {
 // there).  us past them and not: f16 43 MB 12.6 and 15.2, 107 MB 30.5 and 40.9, 578 MB 186 and 194; f32
 // 80 MB 18.5 and 18.9, 152 MB after their writing 92 and 82 with it, 214 MB 56 and 77, 428 MB 127 and 144.
 constexpr int64_t PAST_BYTES = (int64_t)192 << 20;
-template <int NG, bool F16, bool PAST, class... A>
-hipError_t read_launch(const KvArgs &a, hipStream_t s, A... args) {
-    const bool many = (int64_t)a.tokens * a.heads >= (int64_t)256 * 32 * SETS * (WAVE / row_lanes<NG>());
-    return many ? rows_launch<NG, SETS>(kv_read_kernel<NG, SETS, F16, PAST>, a, s, args...)
-                : rows_launch<NG, 1>(kv_read_kernel<NG, 1, F16, PAST>, a, s, args...);
-}
 template <int NG, class... A>
 hipError_t read_launch(const KvArgs &a, hipStream_t s, bool f16, A... args) {
-    if (f16) return read_launch<NG, true, true>(a, s, args...);
-    return (int64_t)a.tokens * a.heads * (2 * 32 * NG * 4) >= PAST_BYTES ? read_launch<NG, false, true>(a, s, args...)
-                                                                         : read_launch<NG, false, false>(a, s, args...);
+    constexpr int64_t MANY = (int64_t)256 * 32 * SETS * (WAVE / row_lanes<NG>()), F32_BYTES = 2 * 32 * NG * sizeof(float);
+    static_assert(MANY * F32_BYTES <= PAST_BYTES, "f32 rows that go past the caches are many");
+    const int64_t rows = (int64_t)a.tokens * a.heads;
+    if (f16)
+        return rows >= MANY ? rows_launch<NG, SETS>(kv_read_kernel<NG, SETS, true, true>, a, s, args...)
+                            : rows_launch<NG, 1>(kv_read_kernel<NG, 1, true, true>, a, s, args...);
+    if (rows * F32_BYTES >= PAST_BYTES) return rows_launch<NG, SETS>(kv_read_kernel<NG, SETS, false, true>, a, s, args...);
+    return rows >= MANY ? rows_launch<NG, SETS>(kv_read_kernel<NG, SETS, false, false>, a, s, args...)
+                        : rows_launch<NG, 1>(kv_read_kernel<NG, 1, false, false>, a, s, args...);
 }
 
 }  // namespace
