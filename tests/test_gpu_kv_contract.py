@@ -240,3 +240,96 @@ def test_values_beyond_the_largest_scale(gpu_ctx, dim):
         gpu_ctx.kv_read(kv, batch.seqs, dk, dv)
         assert np.array_equal(dk.numpy(), want.astype(dtype)) and np.array_equal(dv.numpy(), want.astype(dtype))
     kv.free()
+
+
+# ---- every variant that a size selects ----
+
+@pytest.mark.parametrize("dim,heads,rows", [(64, 7, 262144), (96, 3, 131072), (128, 5, 131072), (256, 3, 65536)])
+def test_reads_that_fill_the_chip(gpu_ctx, dim, heads, rows):
+    # from `rows` rows on a wave reads several sets of rows: just above it, ragged, an idle slot, an odd number of
+    # rows, both types; and f32 from 192 MiB on, where the stores pass the caches
+    _say("large reads", dim, heads)
+    rng = np.random.default_rng(dim + heads)
+    for least in (rows, (192 << 20) // (8 * dim)):
+        tokens = (least + heads - 1) // heads + 2
+        tokens += tokens % 2  # (odd with the idle slot's)
+        cuts = np.sort(rng.choice(np.arange(1, tokens), 9, replace=False))
+        lens = np.diff(np.concatenate([[0], cuts, [tokens]])).tolist()
+        lens[4:4] = [0]  # (its row is nobody's)
+        news = [max(1, n) for n in lens]
+        batch = Batch(gpu_ctx, lens, news, 48, rng)
+        kv = gpu_ctx.kv_cache(heads, dim, 48, batch.n_pages)
+        few = _rows(rng, 997, heads, dim, np.float16)
+        pick = rng.integers(0, 997, (2, batch.tokens))
+        dk, dv = (gpu_ctx.to_device(few[p]) for p in pick)
+        gpu_ctx.kv_write(kv, batch.seqs, dk, dv)
+        held = kvref.held(few)
+        nowhere = batch.start[4]
+        rest = np.arange(batch.tokens) != nowhere
+        for dtype in (np.float32, np.float16):
+            dk, dv = (gpu_ctx.to_device(np.full((batch.tokens, heads, dim), 5, dtype)) for _ in "kv")
+            gpu_ctx.kv_read(kv, batch.seqs, dk, dv)
+            for d, p in ((dk, pick[0]), (dv, pick[1])):
+                got = d.numpy()
+                assert (got[nowhere] == 5).all() and np.array_equal(got[rest], held.astype(dtype)[p[rest]])
+        kv.free()
+
+
+@pytest.mark.parametrize("dtype", [np.float16, np.float32])
+@pytest.mark.parametrize("n,length,kw", [(1153, 1153, {}), (2100, 2100, {}), (1100, 1400, dict(window=500)),
+                                         (1500, 1600, dict(causal=False))])
+def test_one_prompt_of_more_tiles_than_units(gpu_ctx, dtype, n, length, kw):
+    # 32 K/V heads: eight workgroups a head at a time, every other round of a prompt's tiles backwards
+    _say("tile rounds", np.dtype(dtype).name, n, length, kw)
+    rng = np.random.default_rng(n)
+    heads, dim, some = 32, 64, [0, 13, 31]
+    batch = Batch(gpu_ctx, [length], [n], 64, rng)
+    kv = gpu_ctx.kv_cache(heads, dim, 64, batch.n_pages)
+    hk, hv = _filled(gpu_ctx, kv, batch, rng)
+    q = _rows(rng, n, heads, dim, dtype)
+    got = _attend(gpu_ctx, kv, batch, q, dtype, 0.125, **kw)
+    assert np.isfinite(got).all() and (got != 7).any(-1).all()
+    _check(batch, np.ascontiguousarray(got[:, some]), np.ascontiguousarray(q[:, some]), hk[:, some], hv[:, some], 0.125, **kw)
+    kv.free()
+
+
+@pytest.mark.parametrize("dtype", [np.float16, np.float32])
+@pytest.mark.parametrize("dim", [64, 96, 128, 256])
+@pytest.mark.parametrize("page", [80, 112, 128, 240, 256])
+def test_attention_over_larger_pages(gpu_ctx, dtype, dim, page):
+    _say("pages", np.dtype(dtype).name, dim, page)
+    rng = np.random.default_rng(page + dim)
+    batch = Batch(gpu_ctx, [1, 700, 257, 0, 3000, page, page + 1], [1, 1, 2, 1, 1, 1, 90], page, rng, spare=3)
+    kv = gpu_ctx.kv_cache(2, dim, page, batch.n_pages)
+    hk, hv = _filled(gpu_ctx, kv, batch, rng)
+    q = _rows(rng, batch.tokens, 4, dim, dtype)
+    scale = dim ** -0.5
+    for kw in ({}, dict(window=130)):
+        _check(batch, _attend(gpu_ctx, kv, batch, q, dtype, scale, **kw), q, hk, hv, scale, **kw)
+    kv.free()
+
+
+@pytest.mark.parametrize("dtype", [np.float16, np.float32])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_a_cache_beyond_32_bits_of_bytes(gpu_ctx, dtype, dim):
+    # pages on both sides of 2^32 bytes, decode and a prompt
+    _say("large cache", np.dtype(dtype).name, dim)
+    rng = np.random.default_rng(48)
+    heads, page = 32, 256
+    bytes_of_page = heads * page * dim * 9 // 8
+    n_pages = 2 ** 32 // bytes_of_page + 9
+    kv = gpu_ctx.kv_cache(heads, dim, page, n_pages)
+    assert kv.bytes_num > 2 ** 32
+    batch = Batch(gpu_ctx, [700, 513, 300], [1, 1, 70], page, rng)
+    ids = np.concatenate([np.arange(4), n_pages - 1 - np.arange(4)])
+    ids = rng.permutation(ids)
+    batch.table = np.where(batch.table >= 0, ids[batch.table % 8], -1).astype(np.int32)
+    batch.d_table.upload(batch.table)
+    hk, hv = _filled(gpu_ctx, kv, batch, rng)
+    dk, dv = (gpu_ctx.empty(hk.shape, np.float16) for _ in "kv")
+    gpu_ctx.kv_read(kv, batch.whole, dk, dv)
+    assert np.array_equal(dk.numpy().astype(np.float64), hk) and np.array_equal(dv.numpy().astype(np.float64), hv)
+    q, some = _rows(rng, batch.tokens, heads, dim, dtype), [0, 17, 31]
+    got = _attend(gpu_ctx, kv, batch, q, dtype, 0.09)
+    _check(batch, np.ascontiguousarray(got[:, some]), np.ascontiguousarray(q[:, some]), hk[:, some], hv[:, some], 0.09)
+    kv.free()
