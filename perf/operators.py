@@ -225,16 +225,21 @@ _context = None
 
 
 def context():
-    """One context for the process, as a program keeps one per device."""
+    """One context for the process, as a program keeps one per device, on torch's current stream: what is
+    prepared, run and read of the results follows in order.  (torch's default stream has no address to
+    give: another is made the current one.)"""
     global _context
     if _context is None:
         import arf_amd
-        torch.cuda.init()
-        _context = arf_amd.Context(0)
+        stream = torch.cuda.Stream()
+        torch.cuda.set_stream(stream)
+        _context = arf_amd.Context(0, stream.cuda_stream)
     return _context
 
 
 def prepare(case, seed):
+    if own:
+        context()
     seqs = _order(case, seed)
     start, lens, pages, n_pages = _tables(case, seed, seqs)
     if case["op"] == "read":
@@ -265,7 +270,6 @@ def prepare(case, seed):
             s["out"] = [Buffer(torch.zeros(shape, device="cuda", dtype=t)) for _ in "kv"]
         if case["op"] != "write":  # the cache as earlier steps left it
             every = arf_amd.KVSeqs(buf["pages"], buf["lens"], Buffer(whole), k.shape[0])
-            torch.cuda.synchronize()  # the context has a stream of its own
             ctx.kv_write(s["kv"], every, Buffer(k), Buffer(v))
     else:
         d = case["dim"]
