@@ -95,11 +95,11 @@ __device__ __forceinline__ void kv_seq(const KvArgs &a, int b, int &t0, int &n) 
     n = t0 >= 0 && t1 > t0 && t1 <= a.tokens ? t1 - t0 : 0;
 }
 
-// The same for 64 sequences, b in each lane of a wave (0 tokens from a.batch on).  ended: start has decreased before
-// them; on return, among them too.
+// The same for 64 sequences, b in each lane of a wave (0 tokens from a.batch on; without a start a.tokens is no
+// more than it).  ended: start has decreased before them; on return, among them too.
 __device__ __forceinline__ void kv_seq64(const KvArgs &a, int b, bool &ended, int &t0, int &n) {
     t0 = b;
-    n = b < min(a.batch, a.tokens) ? 1 : 0;
+    n = b < a.tokens ? 1 : 0;
     if (!a.start) return;
     int t1 = t0 = 0;
     if (b < a.batch) {
