@@ -214,19 +214,12 @@ __device__ __forceinline__ RowScale row_scale(float top, float scale) {
             __builtin_bit_cast(float, (uint32_t)(127 - ex) << 23)};
 }
 
-// A row's products t of q and K (|t| < 2^40: 256 of q below 2^16 times K below 2^16) in scores: exp2's argument is
-// t * s, or tanh(t * s) * t_of_tanh with a cap.  sc: a product's score, above 0 here (a masked one is -inf, and
-// -inf * 0 would be NaN; below, scores are 0 beside p's 24 bits).  A cap beyond 2^100 sc is as good as that one:
-// |t s| is below 2^-60 with it, where tanh is its argument; and so is one beyond 2^126, as scores of f32
-// do not reach 4 of them.  Without these two, s or the cap's log2 would leave f32's normal numbers.
-struct ScoreUnits {
-    float s, t_of_tanh;
-};
-__device__ __forceinline__ ScoreUnits score_units(float sc, float cap) {
-    constexpr float LOG2E = 1.4426950408889634f, LEAST = 1.1754944e-38f, MOST = 3.4028235e38f;
-    sc = fminf(fmaxf(sc, LEAST), MOST);
-    const float c = fminf(fminf(cap, 0x1p126f), sc * 0x1p100f);
-    return {fminf(cap > 0.0f ? sc / c : sc * LOG2E, MOST), c * LOG2E};
+// What a row's products t of q and K are multiplied by: t * this is a score's log2, or tanh's argument where there
+// is a cap (below 2^64).  sc: a product's score.  Not below the smallest normal number (a masked score is -inf, and
+// -inf * 0 would be NaN): |t| is below 2^40, so what that makes of smaller scores stays below 2^-22.  Nor
+// beyond the largest (0 * inf).
+__device__ __forceinline__ float score_unit(float sc, float cap) {
+    return fminf(fmaxf(cap > 0.0f ? sc / cap : sc * 1.4426950408889634f, 1.1754944e-38f), 3.4028235e38f);
 }
 
 __device__ __forceinline__ float row_max(float v) {  // over the lanes of one matrix column

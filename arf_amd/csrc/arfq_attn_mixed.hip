@@ -10,8 +10,9 @@
 namespace arfq {
 namespace {
 
+// (at 64 values the registers leave room for a third workgroup of a compute unit, which the plan does not count on)
 template <int NG, int PARTS>
-__global__ __launch_bounds__(256, mixed_waves(NG)) void attn_mixed(AttnArgs a) {
+__global__ __launch_bounds__(256, NG <= 2 ? 3 : mixed_waves(NG)) void attn_mixed(AttnArgs a) {
     extern __shared__ float lds[];
     const int many = a.many.slots * a.c.heads, block = block_of();  // (first: they take longer)
     if (block < many)

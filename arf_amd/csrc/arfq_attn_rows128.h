@@ -178,7 +178,7 @@ __device__ __forceinline__ void rows128(const AttnArgs &a, int block, uint8_t *l
         }
     }
     const float cap = a.softcap;
-    const ScoreUnits of = score_units(sc, cap);
+    const float x_of_s = score_unit(sc, cap), x_of_t = cap * 1.4426950408889634f;
 
     f32x16 acc[NG];
     const f32x16 zero = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
@@ -203,10 +203,10 @@ __device__ __forceinline__ void rows128(const AttnArgs &a, int block, uint8_t *l
     f32x16 x = zero;
     auto step = [&](auto v, int k0, int odd) __attribute__((always_inline)) {
         const uint32_t was = in >> 2 * (AHEAD + (v ? 0 : 1));  // (of this step: as many loads ago)
-        float unit = of.s;
+        float unit = x_of_s;
         if (cap > 0.0f) {
 #pragma unroll
-            for (int i = 0; i < 16; i++) x[i] = tanh_of(x[i] * of.s) * of.t_of_tanh;
+            for (int i = 0; i < 16; i++) x[i] = tanh_of(x[i] * x_of_s) * x_of_t;
             unit = 1.0f;
         }
         if (k0 < inner_lo || k0 + STEP > inner_hi || (was & 3) != 3) {

@@ -105,7 +105,7 @@ __device__ __forceinline__ void rows16(const AttnArgs &a, int block, float *lds)
             }
     }
     const float cap = a.softcap;
-    const ScoreUnits of = score_units(sc, cap);
+    const float x_of_s = score_unit(sc, cap), x_of_t = cap * 1.4426950408889634f;
 
     f32x4 acc[NT], sum = {0, 0, 0, 0};
 #pragma unroll
@@ -120,7 +120,7 @@ __device__ __forceinline__ void rows16(const AttnArgs &a, int block, float *lds)
         // one token of each of 32 sequences of up to 4000, 16 x 256 on 8)
         const uint32_t magic = magic_1024();
         const int k1 = k0 + NEXT;
-        float x[8], unit = of.s;  // scores; a unit of them in log2
+        float x[8], unit = x_of_s;  // scores; a unit of them in log2
 #pragma unroll
         for (int half = 0; half < 2; half++) {
             const f32x4 z = {0, 0, 0, 0};
@@ -142,7 +142,7 @@ __device__ __forceinline__ void rows16(const AttnArgs &a, int block, float *lds)
         if (k1 < last) load_ks();
         if (cap > 0.0f) {
 #pragma unroll
-            for (int i = 0; i < 8; i++) x[i] = tanh_of(x[i] * of.s) * of.t_of_tanh;
+            for (int i = 0; i < 8; i++) x[i] = tanh_of(x[i] * x_of_s) * x_of_t;
             unit = 1.0f;
         }
         if (k0 < inner_lo || k0 + STEP > inner_hi || !in0 || !in1) {

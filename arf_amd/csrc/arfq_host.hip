@@ -639,7 +639,7 @@ int arfq_kv_attention(arfq_ctx *ctx, const arfq_kv *kv, const arfq_kv_seqs *seqs
     a.out_dtype = out_dtype;
     a.group = q_heads / kv->heads;
     a.scale = scale;
-    a.softcap = softcap;
+    a.softcap = softcap < 0x1p64f ? softcap : 0.0f;
     a.window = (int)std::min<int64_t>(window, INT32_MAX);
     a.causal = causal != 0;
     a.few_rows = plan.few_rows;

@@ -358,8 +358,9 @@ int arfq_kv_read(arfq_ctx *ctx, const arfq_kv *kv, const arfq_kv_seqs *seqs, voi
 /* out[t, h] = sum_j p_j v_j with p = softmax_j(c(scale * q[t, h] . k_j)), K/V head h / (q_heads /
  * heads), over the cached tokens j of row t's sequence with j <= its position (causal != 0) and,
  * where window > 0, j > its position - window.  c(s) = softcap * tanh(s / softcap), or s where
- * softcap is 0.  A row that attends to nothing gives zeros; rows of no sequence are left as
- * they were.  q and out [tokens, q_heads, head_dim], f32 or f16 each, with token strides as above.
+ * softcap is 0 or from 2^64 on (the same to f32's bits for |s| below 2^52).  A row that attends to
+ * nothing gives zeros; rows of no sequence are left as they were.  q and out [tokens, q_heads,
+ * head_dim], f32 or f16 each, with token strides as above.
  * Sums are f32; an f32 q and the weights p enter the matrix products as two f16 parts (22 bits),
  * one part (q exact, p 11 bits) where q and out are both f16.  Write the step's rows first:
  * a row's own token is among those that it attends to.
