@@ -106,9 +106,11 @@ __device__ __forceinline__ void kv_seq64(const KvArgs &a, int b, bool &ended, in
         t0 = a.start[b];
         t1 = a.start[b + 1];
     }
-    const uint64_t falls = __ballot(t1 < t0), before = ((uint64_t)2 << (threadIdx.x & 63)) - 1;  // (and itself)
-    n = !ended && !(falls & before) && t0 >= 0 && t1 > t0 && t1 <= a.tokens ? t1 - t0 : 0;
-    ended = ended || falls;
+    n = t0 >= 0 && t1 > t0 && t1 <= a.tokens ? t1 - t0 : 0;
+    const uint64_t falls = __ballot(t1 < t0);
+    if (!falls && !ended) return;
+    if (ended || (falls & (((uint64_t)2 << (threadIdx.x & 63)) - 1))) n = 0;  // (at this lane or one before)
+    ended = true;
 }
 
 hipError_t launch_kv_write(const KvArgs &a, int dim, const void *k, int64_t k_stride, const void *v, int64_t v_stride,

@@ -133,11 +133,12 @@ struct Rows {
             const int t0 = row0 / a.heads, t1 = min(row0 + S * R, rows) - 1;
             for (int b0 = 0; b0 < a.batch; b0 += WAVE) {
                 const bool mine = b0 + lane < a.batch;
-                const int u = mine ? a.start[b0 + lane] : 0, v = mine ? a.start[b0 + lane + 1] : INT32_MAX;
-                const uint64_t falls = __ballot(v < u), before = ((uint64_t)2 << lane) - 1;
-                const int end = falls & before ? INT32_MAX : v;
+                const int u = mine ? a.start[b0 + lane] : 0;
+                int v = mine ? a.start[b0 + lane + 1] : INT32_MAX;
+                const uint64_t falls = __ballot(v < u);
+                if (falls && (falls & (((uint64_t)2 << lane) - 1))) v = INT32_MAX;  // (at this lane or one before)
                 for (int t = t0; t <= t1 / a.heads; t++) {
-                    const int n = __popcll(__ballot(end <= t));
+                    const int n = __popcll(__ballot(v <= t));
 #pragma unroll
                     for (int s = 0; s < S; s++) b[s] += token[s] == t ? n : 0;
                 }
