@@ -333,3 +333,40 @@ def test_a_cache_beyond_32_bits_of_bytes(gpu_ctx, dtype, dim):
     got = _attend(gpu_ctx, kv, batch, q, dtype, 0.09)
     _check(batch, np.ascontiguousarray(got[:, some]), np.ascontiguousarray(q[:, some]), hk[:, some], hv[:, some], 0.09)
     kv.free()
+
+
+# ---- lengths beyond the table ----
+
+@pytest.mark.parametrize("dtype", [np.float16, np.float32])
+@pytest.mark.parametrize("causal", [True, False])
+def test_tokens_past_the_tables_end(gpu_ctx, dtype, causal):
+    # a length of more tokens than max_pages * page_size: those are not written, read or attended to
+    _say("past the table", np.dtype(dtype).name, causal)
+    rng = np.random.default_rng(49)
+    heads, dim, page, most = 2, 128, 16, 3
+    kv = gpu_ctx.kv_cache(heads, dim, page, 8)
+    table = [[5, 2, 7], [0, 4, 1]]
+    k, v = (_rows(rng, 96, heads, dim, np.float16) for _ in "kv")
+    gpu_ctx.kv_write(kv, _seqs(gpu_ctx, table, [48, 48], [0, 48, 96], 96), gpu_ctx.to_device(k), gpu_ctx.to_device(v))
+    hk, hv = kvref.held_pair(k, v)
+    # rows 0..59: of a sequence of 100 (its tokens 40 .. 99), rows 60..61 of one of 2^31 - 1
+    seqs = _seqs(gpu_ctx, table, [100, 2 ** 31 - 1], [0, 60, 62], 62)
+    nk, nv = (_rows(rng, 62, heads, dim, np.float16) for _ in "kv")
+    gpu_ctx.kv_write(kv, seqs, gpu_ctx.to_device(nk), gpu_ctx.to_device(nv))
+    new = kvref.held_pair(nk, nv)
+    for old, n in ((hk, new[0]), (hv, new[1])):
+        old[40:48] = n[:8]
+    dk, dv = (gpu_ctx.to_device(np.full((62, heads, dim), 5, np.float32)) for _ in "kv")
+    gpu_ctx.kv_read(kv, seqs, dk, dv)
+    assert np.array_equal(dk.numpy()[:8].astype(np.float64), new[0][:8]) and (dk.numpy()[8:] == 5).all()
+    assert np.array_equal(dv.numpy()[:8].astype(np.float64), new[1][:8]) and (dv.numpy()[8:] == 5).all()
+    q, out = _rows(rng, 62, 6, dim, dtype), gpu_ctx.empty((62, 6, dim), dtype)
+    gpu_ctx.kv_attention(kv, seqs, gpu_ctx.to_device(q), out, 6, 0.09, causal=causal)
+    got = out.numpy()
+    f16 = dtype == np.float16
+    for t in range(62):
+        # as the last token of what the table holds of it
+        n, at = (min(41 + t, 48) if causal else 48, 0) if t < 60 else (48, 48)
+        want, mag, eps, floor = kvref.attention(q[t:t + 1], hk[at:at + n], hv[at:at + n], 0.09)
+        assert (np.abs(got[t] - want[0]) <= kvref.tolerance(want, mag, eps, floor, n, f16)[0]).all(), t
+    kv.free()
