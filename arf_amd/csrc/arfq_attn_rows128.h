@@ -9,11 +9,12 @@
 // the order in which V goes to LDS.
 //
 // Bound by the matrix cores and the softmax beside them, two waves a SIMD (the accumulators and q take 128 registers
-// of 256 at D = 128 and one part, 192 at two).  Measured at 40 x 128 q heads on 8: 8192 tokens of f16 789 us
-// (871 TFLOP/s of the 1131 that a plain f16 product reaches), 2048 tokens 74 (580; its longest tile's
-// 64 steps one after another take 60); 512 f32 tokens after 32356 others 630 (543, that is 1086 of
-// f16 products, as f32's two parts double them; matrix cores and vector unit busy half the time each).
-// f16 24 x 96 on 8, seven prompts of up to 777 tokens: 53 (367).
+// of 256 at D = 128 and one part, 192 at two; 6 go to scratch).  Measured at 40 x 128 q heads on 8: 8192 tokens of f16
+// 776 us (885 TFLOP/s of the 1131 that a plain f16 product reaches), 2048 tokens 72 (597; its longest tile's
+// 64 steps one after another take 60, as none of more tiles than workgroups is cut); 512 f32 tokens after 32356 others
+// 622 to 656 (550 to 521, twice that of f16 products, as f32's two parts double them; matrix cores and vector unit busy
+// half the time each).  f16 24 x 96 on 8, seven prompts of up to 777 tokens: 51 to 58 (380 to 335): 47 steps of the longest
+// tile.  With a cap of scores 2048 tokens take 111, with a window of 512 57, with both 76.
 #pragma once
 #include <type_traits>
 

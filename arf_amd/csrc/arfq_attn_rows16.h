@@ -14,14 +14,17 @@ constexpr int WAVES = 4;  // of a workgroup
 // the layout of a result is the layout of the next product's operand (which keys a lane's
 // eight slots stand for is free, as V is loaded to match).  K's scales multiply the products of
 // a group (32 values: one MFMA), V's its codes; both straight from memory to registers, a step ahead.
-// PARTS: f16 parts of q and p (2: hi + lo, 22 bits, for f32 q or out).
+// PARTS: f16 parts of q and p (2: hi + lo, 22 bits, for f32 q or out; 1: an f16 q is exact in one, and p's 11
+// bits add to an f16 out's own rounding, 2.2e-4 to 2.4e-4 against 64 bits in all, for 2.05e-4 of rounding alone).
 //
 // Bound between memory and the vector unit: turning 4-bit codes into operands takes 4 instructions a key and
 // group, whatever the rows are.  Measured (the join's launch with it): 64 sequences of up to 8192 tokens, f32,
 // 32 x 128 q heads on 4: 45 us for 153 MB, 3.4 TB/s (the vector unit issues half of the time, a third of
 // a wave's time it waits for loads); one of 131071 tokens, 40 q heads on 8: 41 us, 3.7 TB/s; 16 of up
-// to 4097, f16, 32 x 64 heads ungrouped: 25.5 us, 3.0 TB/s; a window of 1024, f16, 16 x 256 on 8, 32
-// sequences: 27 us, 2.6 TB/s; 193 tokens of one: 7.3 us, all of it latency.
+// to 4097, f16, 32 x 64 heads ungrouped: 25.8 us, 3.0 TB/s; a window of 1024, f16, 16 x 256 on 8, 32
+// sequences: 27.7 us, 2.6 TB/s; 193 tokens of one: 7.3 us, all of it latency.  At 256 values and two parts 13 of the 256
+// registers go to scratch: 64 sequences of up to 8192, 32 x 256 on 4, f32, 152 us for 2.7 TB/s (f16, one part, 32 of
+// up to 4000, 16 x 256 on 8: 50 us, 4.1 TB/s; the same in f32 62, 3.0).
 // block: (item, head), head fastest.
 template <int NG, int PARTS>
 __device__ __forceinline__ void rows16(const AttnArgs &a, int block, float *lds) {

@@ -5,7 +5,11 @@
 // dependent loads in front of it (the row's sequence, its length, its page): f32 rows of three prompts,
 // 18552 tokens of 8 x 128, written in 52 us (173 MB, 3.3 TB/s; the codes' exact quotients are a third of
 // that time's vector work), read back in 32 (5.4 TB/s); 141000 tokens read as f16, 740 MB in
-// all, in 187 (4.0 TB/s; a plain copy reaches 4.8).
+// all, in 189 (3.9 TB/s; a plain copy reaches 4.8).
+// By width, 20700 tokens of 1536 values, at 64 / 96 / 128 / 256, us: f32 rows (290 MB with the codes) written in
+// 94 / 111 / 90 / 89, read in 70 / 70 / 81 / 81; f16 rows (163 MB) written in 92 / 114 / 89 / 86 (the quotients, not
+// the bytes), read in 38 / 37 / 31 / 31.  At 64 and 96 V goes byte by byte (VLane), at 96 a quarter of the
+// lanes idles besides.
 #include "arfq_kv.h"
 
 namespace arfq {
@@ -331,8 +335,12 @@ hipError_t write_launch(const KvArgs &a, hipStream_t s, A... args) {
     return rows_launch<NG, 1>(kv_write_kernel<NG>, a, s, args...);
 }
 // f16 goes past the caches, f32 from PAST_BYTES on (the last cache has 256 MB; below, what follows finds it
-// there).  us past them and not: f16 43 MB 12.6 and 15.2, 107 MB 30.5 and 40.9, 578 MB 186 and 194; f32
-// 80 MB 18.5 and 18.9, 152 MB after their writing 92 and 82 with it, 214 MB 56 and 77, 428 MB 127 and 144.
+// there).  us past them and not, 8 x 128, into three sets of rows in turn.  f16 alone: 2 MB 4.2 and 4.2, 20 MB 7.5
+// and 9.1, 107 MB 29 and 31, 214 MB 52 and 65, 428 MB 92 and 148; with copies of the rows after it 43 MB 31.2 and
+// 29.5, 107 MB 63 and 70.  f32 alone: 80 MB 23 and 20, 160 MB 52 and 34, 214 MB 67 and 48, 256 MB 79 and 78, 428 MB
+// 129 and 145; with copies after it 80 MB 53 and 44, 128 MB 80 and 82, 256 MB 177 and 177.  Into the same rows
+// again and again f32 gains from 214 MB on (56 and 77; 428 MB 127 and 144), which the border goes by; behind their
+// writing 152 MB take 92 and 82 with it.
 constexpr int64_t PAST_BYTES = (int64_t)192 << 20;
 template <int NG, class... A>
 hipError_t read_launch(const KvArgs &a, hipStream_t s, bool f16, A... args) {
