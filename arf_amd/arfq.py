@@ -112,6 +112,14 @@ _SIGS = {
     "arfq_kv_attention": (_int, [_vp, _vp, _vp, _int, _vp, _i64, _int, _vp, _i64, _int, ctypes.c_float,
                                  ctypes.c_float, _i64, _int, _vp, ctypes.c_size_t]),
     "arfq_kv_attention_workspace": (_int, [_vp, _vp, _i64, _i64, _i64, _int, ctypes.POINTER(ctypes.c_size_t)]),
+    "arfq_kv_plan": (_int, [_vp, _vp]),
+    "arfq_rope": (_int, [_vp, _vp, _vp, _i64, _i64, _int, _int, _vp, _i64, _int, _vp, _i64, _int, _int]),
+    "arfq_kv_bounds": (_int, [_vp, _vp, _vp, _vp]),
+    "arfq_kv_attention_blocks": (_int, [_vp, _vp, _vp, _vp, _int, _vp, _i64, _int, _vp, _i64, _int, ctypes.c_float,
+                                        ctypes.c_float, _i64, _i64, _i64, _vp, _vp, ctypes.c_size_t]),
+    "arfq_kv_attention_blocks_workspace": (_int, [_vp, _vp, _i64, _i64, _i64, _int, _i64, ctypes.POINTER(ctypes.c_size_t)]),
+    "arfq_lora_add": (_int, [_vp, _vp, _vp, _i64, _vp, _int, _vp, _i64, _vp, _i64, _vp, ctypes.c_size_t]),
+    "arfq_lora_workspace": (_int, [_vp, _vp, _i64, ctypes.POINTER(ctypes.c_size_t)]),
     "arfq_gguf_is_gguf": (_int, [ctypes.c_char_p]),
     "arfq_gguf_open": (_int, [ctypes.c_char_p, ctypes.POINTER(_vp)]),
     "arfq_gguf_close": (_int, [_vp]),
@@ -302,6 +310,108 @@ class KVCache:
             pass
 
 
+class _KVStepStruct(ctypes.Structure):
+    """arfq_kv_step"""
+    _fields_ = [("batch", _i64), ("max_pages", _i64), ("tokens", _i64), ("n_pages", _i64), ("page_size", _int),
+                ("add", _vp), ("held", _vp), ("held_next", _vp), ("pages", _vp), ("free_pages", _vp), ("n_free", _vp),
+                ("n_free_next", _vp), ("start", _vp), ("len", _vp), ("taken", _vp), ("freed", _vp), ("positions", _vp),
+                ("slots", _vp)]
+
+
+class KVStep:
+    """A step's bookkeeping (arfq_kv_step), device arrays throughout: `add`, `held` [batch] in, `held_next` [batch] out;
+    the tables `pages` [batch, max_pages]; the stack `free` [n_pages] with `n_free` [1] entries, `n_free_next` [1]; out
+    `start`, `taken`, `freed` [batch + 1], `lens` [batch], `positions`, `slots` [tokens].  All int32 but the int64
+    slots.  Keeps its arrays; `seqs` is the step's KVSeqs."""
+
+    def __init__(self, page_size, add, held, held_next, pages, free, n_free, n_free_next, start, lens, taken, freed,
+                 positions, slots):
+        arrays = dict(add=add, held=held, held_next=held_next, pages=pages, free=free, n_free=n_free, n_free_next=n_free_next,
+                      start=start, lens=lens, taken=taken, freed=freed, positions=positions, slots=slots)
+        for name, a in arrays.items():
+            if a.dtype != (np.int64 if name == "slots" else np.int32):
+                raise ValueError(f"KVStep: {name} is int{64 if name == 'slots' else 32}")
+        if len(pages.shape) != 2 or len(free.shape) != 1 or len(positions.shape) != 1:
+            raise ValueError("KVStep: want pages [batch, max_pages], free [n_pages] and positions [tokens]")
+        batch, most = (int(n) for n in pages.shape)
+        tokens = int(positions.shape[0])
+        for names, shape in ((("add", "held", "held_next", "lens"), (batch,)), (("start", "taken", "freed"), (batch + 1,)),
+                             (("n_free", "n_free_next"), (1,)), (("slots",), (tokens,))):
+            for name in names:
+                if tuple(arrays[name].shape) != shape:
+                    raise ValueError(f"KVStep: want {name} {list(shape)}, not {list(arrays[name].shape)}")
+        self.page_size, self.batch, self.tokens = int(page_size), batch, tokens
+        self.__dict__.update(arrays)
+        self.struct = _KVStepStruct(batch, most, tokens, int(free.shape[0]), self.page_size,
+                                    *(a.ptr for a in arrays.values()))
+        self.ref = ctypes.addressof(self.struct)
+        self.seqs = KVSeqs(pages, lens, start, tokens)
+
+
+class _RopeStruct(ctypes.Structure):
+    """arfq_rope_pairs"""
+    _fields_ = [("rot_dim", _int), ("pairs", _int), ("axes", _int), ("axis", _vp), ("freq", _vp), ("gain", ctypes.c_float)]
+
+
+class Rope:
+    """Rotary positions (arfq_rope_pairs): pair i turns by freqs[i] radians a position of axis axes[i] (one axis: None).
+    pairs: "halves" (i and i + rot_dim / 2) or "neighbours" (2i and 2i + 1); cosines and sines are multiplied by gain."""
+
+    def __init__(self, freqs, axes=None, pairs="halves", gain=1.0):
+        if pairs not in ("halves", "neighbours"):
+            raise ValueError(f"Rope: pairs {pairs!r} (want halves or neighbours)")
+        self._freqs = np.ascontiguousarray(freqs, dtype=np.float64).reshape(-1)
+        self._axes = None if axes is None else np.ascontiguousarray(axes, dtype=np.uint8).reshape(-1)
+        if self._axes is not None and self._axes.size != self._freqs.size:
+            raise ValueError("Rope: an axis for each frequency")
+        self.axes = 1 if self._axes is None or not self._axes.size else int(self._axes.max()) + 1
+        self.rot_dim = 2 * self._freqs.size
+        self.struct = _RopeStruct(self.rot_dim, 1 if pairs == "neighbours" else 0, self.axes,
+                                  None if self._axes is None else self._axes.ctypes.data, self._freqs.ctypes.data, gain)
+        self.ref = ctypes.addressof(self.struct)
+
+    @classmethod
+    def sections(cls, sections, base=10000.0, layout="chunks", pairs="halves", gain=1.0):
+        """Frequencies base^(-i / n) of n = sum(sections) pairs, sections[a] of them on axis a: `chunks`, one axis's after
+        another's; `cycle`, the axes in turn while they have pairs left; `own`, chunks of which each has frequencies of its own,
+        base^(-i / sections[a])."""
+        if layout not in ("chunks", "cycle", "own") or not sections or min(sections) < 0:
+            raise ValueError("Rope: want sections that are not negative, and layout chunks, cycle or own")
+        n = sum(sections)
+        if layout == "cycle":
+            turns = [(i, a) for a, s in enumerate(sections) for i in range(s)]
+            axes = [a for _, a in sorted(turns)]
+        else:
+            axes = [a for a, s in enumerate(sections) for _ in range(s)]
+        if layout == "own":
+            freqs = [float(base) ** (-i / s) for s in sections for i in range(s)]
+        else:
+            freqs = [float(base) ** (-i / n) for i in range(n)]
+        return cls(freqs, axes, pairs, gain)
+
+
+class _LoraStruct(ctypes.Structure):
+    """arfq_lora"""
+    _fields_ = [("adapters", _i64), ("n", _i64), ("k", _i64), ("rank", _i64), ("a", _vp), ("b", _vp), ("scale", _vp)]
+
+
+class Lora:
+    """Low-rank adapters (arfq_lora): device arrays a [adapters, rank, k] and b [adapters, n, rank], f16, and scale [adapters],
+    f32, or None for 1.  Keeps them."""
+
+    def __init__(self, a, b, scale=None):
+        if a.dtype != np.float16 or b.dtype != np.float16:
+            raise ValueError("Lora: a and b are f16")
+        if len(a.shape) != 3 or len(b.shape) != 3 or a.shape[0] != b.shape[0] or a.shape[1] != b.shape[2]:
+            raise ValueError("Lora: want a [adapters, rank, k] and b [adapters, n, rank]")
+        if scale is not None and (scale.dtype != np.float32 or tuple(scale.shape) != (a.shape[0],)):
+            raise ValueError("Lora: want scale [adapters], f32")
+        self.a, self.b, self.scale = a, b, scale
+        self.adapters, self.rank, self.k, self.n = int(a.shape[0]), int(a.shape[1]), int(a.shape[2]), int(b.shape[1])
+        self.struct = _LoraStruct(self.adapters, self.n, self.k, self.rank, a.ptr, b.ptr, None if scale is None else scale.ptr)
+        self.ref = ctypes.addressof(self.struct)
+
+
 def _float_type(a, what):
     """DType of a device array's elements."""
     if a.dtype == np.float32:
@@ -470,6 +580,77 @@ class Context:
         _check(self.handle, _lib.arfq_kv_attention(
             self.handle, kv.handle, seqs.ref, q_heads, q.ptr, qs, _float_type(q, "kv_attention: q"), out.ptr, os_,
             _float_type(out, "kv_attention: out"), scale, softcap, window, causal, ws[0], ws[1]))
+
+    def kv_plan(self, step):
+        """Write a step's tables, rows and lengths (arfq_kv_plan)."""
+        _check(self.handle, _lib.arfq_kv_plan(self.handle, step.ref))
+
+    def rope(self, rope, positions, x, out, tokens, heads, head_dim, x_stride=None, out_stride=None, inverse=False):
+        """Rotate the rows x [tokens, heads, head_dim] into out, which may be x (arfq_rope); positions: int32 [tokens], or
+        [axes, tokens or more]."""
+        if positions.dtype != np.int32 or len(positions.shape) not in (1, 2):
+            raise ValueError("rope: positions are int32 [axes, tokens]")
+        if len(positions.shape) == 2 and positions.shape[0] < rope.axes or len(positions.shape) == 1 and rope.axes > 1:
+            raise ValueError(f"rope: positions of {rope.axes} axes are wanted")
+        w = heads * head_dim
+        xs, os_ = _row_stride(x, tokens, w, x_stride, "rope: x"), _row_stride(out, tokens, w, out_stride, "rope: out")
+        _check(self.handle, _lib.arfq_rope(
+            self.handle, rope.ref, positions.ptr, int(positions.shape[-1]), tokens, heads, head_dim, x.ptr, xs,
+            _float_type(x, "rope: x"), out.ptr, os_, _float_type(out, "rope: out"), int(bool(inverse))))
+
+    def _kv_bounds_of(self, kv, bounds, what):
+        if bounds.dtype != np.float16 or bounds.nbytes < kv.n_pages * kv.heads * 4 * kv.head_dim:
+            raise ValueError(f"{what}: want bounds [n_pages, heads, 2, head_dim], f16")
+        return bounds.ptr
+
+    def kv_bounds(self, kv, seqs, bounds):
+        """Form the bounds [n_pages, heads, 2, head_dim] (f16) of the pages that the step's rows lie in (arfq_kv_bounds)."""
+        _check(self.handle, _lib.arfq_kv_bounds(self.handle, kv.handle, seqs.ref, self._kv_bounds_of(kv, bounds, "kv_bounds")))
+
+    def kv_attention_blocks(self, kv, seqs, bounds, q, out, q_heads, scale, count, first=0, last=1, softcap=0.0, chosen=None,
+                            q_stride=None, out_stride=None, workspace=None):
+        """out [tokens, q_heads, head_dim] = attention of q over the `count` blocks of the cache that each row chooses by
+        their bounds (arfq_kv_attention_blocks); chosen: None, or int32 [tokens, heads, count], which gets them;
+        `workspace`: a device array of kv_attention_blocks_workspace bytes, which a call under stream capture needs."""
+        what, w = "kv_attention_blocks", q_heads * kv.head_dim
+        qs, os_ = (_row_stride(a, seqs.tokens, w, s, f"{what}: {n}") for a, s, n in ((q, q_stride, "q"), (out, out_stride, "out")))
+        if chosen is not None and (chosen.dtype != np.int32 or chosen.nbytes < seqs.tokens * kv.heads * count * 4):
+            raise ValueError(f"{what}: want chosen [tokens, heads, count], int32")
+        ws = (None, 0) if workspace is None else (workspace.ptr, workspace.nbytes)
+        _check(self.handle, _lib.arfq_kv_attention_blocks(
+            self.handle, kv.handle, seqs.ref, self._kv_bounds_of(kv, bounds, what), q_heads, q.ptr, qs,
+            _float_type(q, f"{what}: q"), out.ptr, os_, _float_type(out, f"{what}: out"), scale, softcap, count, first, last,
+            None if chosen is None else chosen.ptr, ws[0], ws[1]))
+
+    def kv_attention_blocks_workspace(self, kv, seqs, q_heads, count):
+        """Bytes of kv_attention_blocks' workspace for such a batch (arfq_kv_attention_blocks_workspace)."""
+        sz = ctypes.c_size_t()
+        _check(self.handle, load_library().arfq_kv_attention_blocks_workspace(
+            self.handle, kv.handle, seqs.batch, seqs.tokens, int(seqs.pages.shape[1]), int(q_heads), int(count), ctypes.byref(sz)))
+        return sz.value
+
+    def lora_add(self, lora, ids, x, rows, out, base=None, out_stride=None, base_stride=None, workspace=None):
+        """out [rows, n] = base + each row's adapter of x [rows, k] (arfq_lora_add); ids: int32 [rows], -1 for none; base may be
+        out, None for zeros; `workspace`: a device array of lora_workspace bytes, which a call under stream capture
+        needs."""
+        if ids.dtype != np.int32 or ids.nbytes < rows * 4:
+            raise ValueError("lora_add: want ids [rows], int32")
+        if x.nbytes < rows * lora.k * x.dtype.itemsize:
+            raise ValueError("lora_add: x shape")
+        if out.dtype != np.float32 or (base is not None and base.dtype != np.float32):
+            raise ValueError("lora_add: base and out are f32")
+        os_ = _row_stride(out, rows, lora.n, out_stride, "lora_add: out")
+        bs = 0 if base is None else _row_stride(base, rows, lora.n, base_stride, "lora_add: base")
+        ws = (None, 0) if workspace is None else (workspace.ptr, workspace.nbytes)
+        _check(self.handle, _lib.arfq_lora_add(
+            self.handle, lora.ref, ids.ptr, rows, x.ptr, _float_type(x, "lora_add: x"), None if base is None else base.ptr, bs,
+            out.ptr, os_, ws[0], ws[1]))
+
+    def lora_workspace(self, lora, rows):
+        """Bytes of lora_add's workspace (arfq_lora_workspace)."""
+        sz = ctypes.c_size_t()
+        _check(self.handle, load_library().arfq_lora_workspace(self.handle, lora.ref, int(rows), ctypes.byref(sz)))
+        return sz.value
 
     def kv_attention_workspace(self, kv, seqs, q_heads):
         """Bytes of kv_attention's workspace for such a batch (arfq_kv_attention_workspace)."""

@@ -31,7 +31,7 @@ struct Steps {
     const int32_t *table;
     int first;  // the tile of lane 0
     uint32_t lo, hi, sub;  // sub: bit 31 where the page is not the cache's
-    // the wave's steps from key k0 on (k0 a multiple of 16; max_pages > 0)
+    // through the sequence of row b of the tables (k0 a multiple of 16; max_pages > 0)
     __device__ __forceinline__ Steps(const KvArgs &a, int b) : table(a.table + (int64_t)b * a.max_pages), first(INT32_MIN / 2) {
         lo = hi = sub = 0;
     }

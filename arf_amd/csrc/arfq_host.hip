@@ -10,6 +10,7 @@
 #include "arfq_common.h"
 #include "arfq_internal.h"
 #include "arfq_attn_list.h"
+#include "arfq_step.h"
 
 #include <algorithm>
 #include <cmath>
@@ -579,12 +580,32 @@ int arfq_kv_read(arfq_ctx *ctx, const arfq_kv *kv, const arfq_kv_seqs *seqs, voi
     return e == hipSuccess ? ARFQ_OK : hip_fail(ctx, e, "kv_read launch");
 }
 
-static int kv_q_heads(arfq_ctx *ctx, const arfq_kv *kv, int64_t batch, int64_t tokens, int q_heads) {
-    if (!kv) return fail(ctx, ARFQ_E_INVALID, "kv_attention: null argument");
+static int kv_q_heads(arfq_ctx *ctx, const arfq_kv *kv, int64_t batch, int64_t tokens, int q_heads,
+                      const char *what = "kv_attention") {
+    const std::string w = std::string(what) + ": ";
+    if (!kv) return fail(ctx, ARFQ_E_INVALID, w + "null argument");
     if (q_heads < 1 || q_heads % kv->heads)
-        return fail(ctx, ARFQ_E_SHAPE, "kv_attention: q_heads must be a multiple of the cache's heads");
+        return fail(ctx, ARFQ_E_SHAPE, w + "q_heads must be a multiple of the cache's heads");
     if (batch < 0 || batch > arfq::KV_BATCH_MAX || tokens < 0 || tokens > arfq::KV_ROWS_MAX / q_heads)
-        return fail(ctx, ARFQ_E_SHAPE, "kv_attention: batch above 16384, or tokens * q_heads above 2^30");
+        return fail(ctx, ARFQ_E_SHAPE, w + "batch above 16384, or tokens * q_heads above 2^30");
+    return ARFQ_OK;
+}
+
+// A call's workspace of `want` bytes: the caller's, or the context's scratch, which a captured graph cannot have.
+static int take_workspace(arfq_ctx *ctx, const char *what, size_t want, size_t bytes, void **workspace) {
+    const std::string w = std::string(what) + ": ";
+    if (*workspace) {
+        if (bytes < want || (uintptr_t)*workspace % 16)
+            return fail(ctx, ARFQ_E_SHAPE, w + "workspace of " + std::to_string(bytes) + " bytes, " + std::to_string(want) +
+                                               " (16-byte aligned) are wanted");
+    } else if (want) {
+        hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
+        HIP_TRY(ctx, hipStreamIsCapturing(ctx->stream, &cap));
+        if (cap != hipStreamCaptureStatusNone)
+            return fail(ctx, ARFQ_E_INVALID, w + "a call under stream capture needs a workspace");
+        if (int rc = ensure_scratch(ctx, want)) return rc;
+        *workspace = ctx->scratch;
+    }
     return ARFQ_OK;
 }
 
@@ -619,18 +640,7 @@ int arfq_kv_attention(arfq_ctx *ctx, const arfq_kv *kv, const arfq_kv_seqs *seqs
     if (int rc = use_device(ctx)) return rc;
     const arfq::AttnPlan plan = arfq::attn_plan(ctx->cus, kv->heads, kv->dim, seqs->batch, seqs->tokens, q_heads,
                                                     seqs->max_pages * kv->page, !seqs->start);
-    if (workspace) {
-        if (workspace_bytes < plan.ws_bytes || (uintptr_t)workspace % 16)
-            return fail(ctx, ARFQ_E_SHAPE, "kv_attention: workspace of " + std::to_string(workspace_bytes) + " bytes, " +
-                                               std::to_string(plan.ws_bytes) + " (16-byte aligned) are wanted");
-    } else if (plan.ws_bytes) {
-        hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
-        HIP_TRY(ctx, hipStreamIsCapturing(ctx->stream, &cap));
-        if (cap != hipStreamCaptureStatusNone)
-            return fail(ctx, ARFQ_E_INVALID, "kv_attention: a call under stream capture needs a workspace");
-        if (int rc = ensure_scratch(ctx, plan.ws_bytes)) return rc;
-        workspace = ctx->scratch;
-    }
+    if (int rc = take_workspace(ctx, "kv_attention", plan.ws_bytes, workspace_bytes, &workspace)) return rc;
     a.q = q;
     a.out = out;
     a.q_stride = q_stride;
@@ -652,6 +662,196 @@ int arfq_kv_attention(arfq_ctx *ctx, const arfq_kv *kv, const arfq_kv_seqs *seqs
     a.many = list(plan.many, plan.few.part_bytes, parts + plan.few.join_bytes);
     const hipError_t e = arfq::launch_attn(a, kv->dim, ctx->stream);
     return e == hipSuccess ? ARFQ_OK : hip_fail(ctx, e, "kv_attention launch");
+}
+
+// ------------------------------------------- a serving step around the cache ----
+
+int arfq_kv_plan(arfq_ctx *ctx, const arfq_kv_step *s) {
+    if (!ctx) return ARFQ_E_INVALID;
+    if (!s) return fail(ctx, ARFQ_E_INVALID, "kv_plan: null argument");
+    if (s->batch < 0 || s->tokens < 0 || s->max_pages < 0 || s->n_pages < 0)
+        return fail(ctx, ARFQ_E_SHAPE, "kv_plan: negative size");
+    if (s->page_size < 1 || s->page_size > arfq::PLAN_PAGE_MAX)
+        return fail(ctx, ARFQ_E_SHAPE, "kv_plan: page_size must be in [1, 65536]");
+    if (s->batch > arfq::KV_BATCH_MAX || s->max_pages > arfq::KV_KEYS_MAX / s->page_size)
+        return fail(ctx, ARFQ_E_SHAPE, "kv_plan: batch above 16384, or max_pages * page_size above 2^29");
+    if (s->tokens > arfq::KV_ROWS_MAX || s->n_pages > INT32_MAX || s->batch * s->max_pages > INT32_MAX)
+        return fail(ctx, ARFQ_E_SHAPE, "kv_plan: tokens above 2^30, or n_pages or batch * max_pages above 2^31 - 1");
+    if (!s->n_free || !s->n_free_next || !s->start || !s->taken || !s->freed)
+        return fail(ctx, ARFQ_E_INVALID, "kv_plan: null n_free, n_free_next, start, taken or freed");
+    if (s->batch > 0 && (!s->add || !s->held || !s->held_next || !s->len || (s->max_pages > 0 && !s->pages)))
+        return fail(ctx, ARFQ_E_INVALID, "kv_plan: null add, held, held_next, len or pages");
+    if ((s->tokens > 0 && (!s->positions || !s->slots)) || (s->n_pages > 0 && !s->free_pages))
+        return fail(ctx, ARFQ_E_INVALID, "kv_plan: null positions, slots or free_pages");
+    if (s->held_next == s->held || s->n_free_next == s->n_free)
+        return fail(ctx, ARFQ_E_INVALID, "kv_plan: held_next and n_free_next have places of their own");
+    if (int rc = use_device(ctx)) return rc;
+    const hipError_t e = arfq::launch_kv_plan(*s, ctx->stream);
+    return e == hipSuccess ? ARFQ_OK : hip_fail(ctx, e, "kv_plan launch");
+}
+
+int arfq_rope(arfq_ctx *ctx, const arfq_rope_pairs *rope, const int32_t *positions, int64_t position_stride,
+              int64_t tokens, int heads, int head_dim, const void *x, int64_t x_stride, int x_dtype, void *out,
+              int64_t out_stride, int out_dtype, int inverse) {
+    if (!ctx) return ARFQ_E_INVALID;
+    if (!rope || !rope->freq) return fail(ctx, ARFQ_E_INVALID, "rope: null argument");
+    if (tokens < 0 || heads < 1) return fail(ctx, ARFQ_E_SHAPE, "rope: negative tokens, or no heads");
+    if (head_dim < 1) return fail(ctx, ARFQ_E_SHAPE, "rope: head_dim must be positive");
+    if (head_dim % 8 || head_dim > arfq::ROPE_HEAD_MAX)
+        return fail(ctx, ARFQ_E_UNSUPPORTED, "rope: head_dim must be a multiple of 8 up to 1024");
+    if (rope->rot_dim < 8 || rope->rot_dim % 8 || rope->rot_dim > arfq::ROPE_DIM_MAX || rope->rot_dim > head_dim)
+        return fail(ctx, ARFQ_E_SHAPE, "rope: rot_dim must be a multiple of 8 up to 256 and head_dim");
+    if (rope->axes < 1 || rope->axes > arfq::ROPE_AXES_MAX) return fail(ctx, ARFQ_E_SHAPE, "rope: axes must be in [1, 4]");
+    if (rope->pairs != ARFQ_ROPE_HALVES && rope->pairs != ARFQ_ROPE_NEIGHBOURS)
+        return fail(ctx, ARFQ_E_INVALID, "rope: unknown pairs");
+    if (tokens > arfq::KV_ROWS_MAX / heads) return fail(ctx, ARFQ_E_SHAPE, "rope: tokens * heads above 2^30");
+    if (!std::isfinite(rope->gain)) return fail(ctx, ARFQ_E_INVALID, "rope: gain must be finite");
+    arfq::RopeArgs a;
+    for (int i = 0; i < rope->rot_dim / 2; i++) {
+        if (!std::isfinite(rope->freq[i])) return fail(ctx, ARFQ_E_INVALID, "rope: freq must be finite");
+        if (rope->axis && rope->axis[i] >= rope->axes) return fail(ctx, ARFQ_E_SHAPE, "rope: axis of a pair not below axes");
+        a.axis[i] = rope->axis ? rope->axis[i] : 0;
+        a.turns[i] = rope->freq[i] * (inverse ? -0.15915494309189535 : 0.15915494309189535);  // 1 / (2 pi)
+    }
+    if (tokens == 0) return ARFQ_OK;
+    if (!positions) return fail(ctx, ARFQ_E_INVALID, "rope: null positions");
+    if (position_stride < tokens || position_stride > (int64_t)1 << 40)
+        return fail(ctx, ARFQ_E_SHAPE, "rope: position_stride below tokens, or above 2^40");
+    if (int rc = kv_rows(ctx, "rope: x", x, x_stride, heads, head_dim, x_dtype)) return rc;
+    if (int rc = kv_rows(ctx, "rope: out", out, out_stride, heads, head_dim, out_dtype)) return rc;
+    if (x == out && (x_dtype != out_dtype || x_stride != out_stride))
+        return fail(ctx, ARFQ_E_INVALID, "rope: in place the types and strides of x and out are the same");
+    if (int rc = use_device(ctx)) return rc;
+    a.rot = rope->rot_dim;
+    a.dim = head_dim;
+    a.heads = heads;
+    a.tokens = (int)tokens;
+    a.positions = positions;
+    a.position_stride = position_stride;
+    a.x = x;
+    a.out = out;
+    a.x_stride = x_stride;
+    a.out_stride = out_stride;
+    a.gain = rope->gain;
+    a.neighbours = rope->pairs == ARFQ_ROPE_NEIGHBOURS;
+    a.x_f16 = x_dtype == ARFQ_F16;
+    a.out_f16 = out_dtype == ARFQ_F16;
+    const hipError_t e = arfq::launch_rope(a, ctx->cus, ctx->stream);
+    return e == hipSuccess ? ARFQ_OK : hip_fail(ctx, e, "rope launch");
+}
+
+int arfq_kv_bounds(arfq_ctx *ctx, const arfq_kv *kv, const arfq_kv_seqs *seqs, void *bounds) {
+    if (!ctx) return ARFQ_E_INVALID;
+    arfq::KvArgs a;
+    if (int rc = kv_args(ctx, kv, seqs, "kv_bounds", &a)) return rc;
+    if (a.tokens == 0 || a.batch == 0) return ARFQ_OK;
+    if (!bounds || (uintptr_t)bounds % 16) return fail(ctx, ARFQ_E_INVALID, "kv_bounds: null or unaligned bounds");
+    if (int rc = use_device(ctx)) return rc;
+    const hipError_t e = arfq::launch_kv_bounds(a, kv->dim, (_Float16 *)bounds, ctx->cus, ctx->stream);
+    return e == hipSuccess ? ARFQ_OK : hip_fail(ctx, e, "kv_bounds launch");
+}
+
+int arfq_kv_attention_blocks_workspace(arfq_ctx *ctx, const arfq_kv *kv, int64_t batch, int64_t tokens, int64_t max_pages,
+                                       int q_heads, int64_t count, size_t *bytes) {
+    if (!ctx) return ARFQ_E_INVALID;
+    if (!bytes) return fail(ctx, ARFQ_E_INVALID, "kv_attention_blocks_workspace: null argument");
+    if (int rc = kv_q_heads(ctx, kv, batch, tokens, q_heads, "kv_attention_blocks_workspace")) return rc;
+    if (max_pages < 0 || max_pages > arfq::KV_KEYS_MAX / kv->page)
+        return fail(ctx, ARFQ_E_SHAPE, "kv_attention_blocks_workspace: max_pages * page_size above 2^29");
+    if (count < 1 || count > arfq::BLOCKS_MAX)
+        return fail(ctx, ARFQ_E_SHAPE, "kv_attention_blocks_workspace: count must be in [1, 2^20]");
+    *bytes = tokens ? arfq::blocks_plan(ctx->cus, kv->heads, kv->dim, kv->page, tokens, q_heads, max_pages, count).ws_bytes : 0;
+    return ARFQ_OK;
+}
+
+int arfq_kv_attention_blocks(arfq_ctx *ctx, const arfq_kv *kv, const arfq_kv_seqs *seqs, const void *bounds, int q_heads,
+                             const void *q, int64_t q_stride, int q_dtype, void *out, int64_t out_stride, int out_dtype,
+                             float scale, float softcap, int64_t count, int64_t first, int64_t last, int32_t *chosen,
+                             void *workspace, size_t workspace_bytes) {
+    if (!ctx) return ARFQ_E_INVALID;
+    const char *const what = "kv_attention_blocks";
+    arfq::BlocksArgs b;
+    arfq::AttnArgs &a = b.a;
+    if (int rc = kv_args(ctx, kv, seqs, what, &a.c)) return rc;
+    if (int rc = kv_q_heads(ctx, kv, seqs->batch, seqs->tokens, q_heads, what)) return rc;
+    if (!std::isfinite(scale) || !std::isfinite(softcap) || softcap < 0.0f)
+        return fail(ctx, ARFQ_E_INVALID, "kv_attention_blocks: scale and softcap must be finite, softcap not negative");
+    if (count < 1 || count > arfq::BLOCKS_MAX || first < 0 || last < 1 || first > count - last)
+        return fail(ctx, ARFQ_E_SHAPE, "kv_attention_blocks: want count in [1, 2^20], first >= 0, last >= 1, first + last <= count");
+    if (a.c.tokens == 0 || a.c.batch == 0) return ARFQ_OK;
+    if (!bounds || (uintptr_t)bounds % 16) return fail(ctx, ARFQ_E_INVALID, "kv_attention_blocks: null or unaligned bounds");
+    if (int rc = kv_rows(ctx, "kv_attention_blocks: q", q, q_stride, q_heads, kv->dim, q_dtype)) return rc;
+    if (int rc = kv_rows(ctx, "kv_attention_blocks: out", out, out_stride, q_heads, kv->dim, out_dtype)) return rc;
+    if (int rc = use_device(ctx)) return rc;
+    const arfq::BlocksPlan plan = arfq::blocks_plan(ctx->cus, kv->heads, kv->dim, kv->page, seqs->tokens, q_heads,
+                                                    seqs->max_pages, count);
+    if (int rc = take_workspace(ctx, what, plan.ws_bytes, workspace_bytes, &workspace)) return rc;
+    a.q = q;
+    a.out = out;
+    a.q_stride = q_stride;
+    a.out_stride = out_stride;
+    a.q_dtype = q_dtype;
+    a.out_dtype = out_dtype;
+    a.group = q_heads / kv->heads;
+    a.scale = scale;
+    a.softcap = softcap < 0x1p64f ? softcap : 0.0f;
+    a.window = 0;
+    a.causal = 1;
+    a.few_rows = 0;
+    a.few = a.many = arfq::AttnList{1, 0, 0, 1, nullptr, nullptr};
+    b.bounds = (const _Float16 *)bounds;
+    b.count = (int)count;
+    b.first = (int)first;
+    b.last = (int)last;
+    b.chosen = chosen;
+    b.ws = (char *)workspace;
+    const hipError_t e = arfq::launch_blocks(b, kv->dim, plan, ctx->cus, ctx->stream);
+    return e == hipSuccess ? ARFQ_OK : hip_fail(ctx, e, "kv_attention_blocks launch");
+}
+
+static int lora_check(arfq_ctx *ctx, const arfq_lora *l, int64_t rows, const char *what) {
+    const std::string w = std::string(what) + ": ";
+    if (!l) return fail(ctx, ARFQ_E_INVALID, w + "null argument");
+    constexpr int64_t MOST = (int64_t)1 << 30;
+    if (rows < 0 || rows > arfq::LORA_ROWS_MAX) return fail(ctx, ARFQ_E_SHAPE, w + "rows must be in [0, 2^24]");
+    if (l->adapters < 1 || l->n < 1 || l->k < 1 || l->adapters > INT32_MAX || l->n > MOST || l->k > MOST)
+        return fail(ctx, ARFQ_E_SHAPE, w + "adapters, n and k must be positive, n and k at most 2^30");
+    if (l->k % 8) return fail(ctx, ARFQ_E_UNSUPPORTED, w + "k must be a multiple of 8");
+    if (l->rank < 1) return fail(ctx, ARFQ_E_SHAPE, w + "rank must be positive");
+    if (l->rank % 8 || l->rank > arfq::LORA_RANK_MAX)
+        return fail(ctx, ARFQ_E_UNSUPPORTED, w + "rank must be a multiple of 8 up to 256 (smaller ones: zeros behind them)");
+    return ARFQ_OK;
+}
+
+int arfq_lora_workspace(arfq_ctx *ctx, const arfq_lora *lora, int64_t rows, size_t *bytes) {
+    if (!ctx) return ARFQ_E_INVALID;
+    if (!bytes) return fail(ctx, ARFQ_E_INVALID, "lora_workspace: null argument");
+    if (int rc = lora_check(ctx, lora, rows, "lora_workspace")) return rc;
+    *bytes = rows ? arfq::lora_plan(ctx->cus, *lora, rows).ws_bytes : 0;
+    return ARFQ_OK;
+}
+
+int arfq_lora_add(arfq_ctx *ctx, const arfq_lora *lora, const int32_t *ids, int64_t rows, const void *x, int x_dtype,
+                  const float *base, int64_t base_stride, float *out, int64_t out_stride, void *workspace,
+                  size_t workspace_bytes) {
+    if (!ctx) return ARFQ_E_INVALID;
+    if (int rc = lora_check(ctx, lora, rows, "lora_add")) return rc;
+    if (x_dtype != ARFQ_F32 && x_dtype != ARFQ_F16) return fail(ctx, ARFQ_E_INVALID, "lora_add: unknown dtype");
+    if (rows == 0) return ARFQ_OK;
+    if (!lora->a || !lora->b || !ids || !x || !out) return fail(ctx, ARFQ_E_INVALID, "lora_add: null argument");
+    if ((uintptr_t)lora->a % 16 || (uintptr_t)lora->b % 16 || (uintptr_t)x % 16)
+        return fail(ctx, ARFQ_E_INVALID, "lora_add: a, b and x must be 16-byte aligned");
+    constexpr int64_t MOST = (int64_t)1 << 40;
+    if (out_stride < lora->n || out_stride > MOST || (base && (base_stride < lora->n || base_stride > MOST)))
+        return fail(ctx, ARFQ_E_SHAPE, "lora_add: row strides below n, or above 2^40");
+    if (base == out && base_stride != out_stride)
+        return fail(ctx, ARFQ_E_INVALID, "lora_add: in place the strides of base and out are the same");
+    if (int rc = use_device(ctx)) return rc;
+    const arfq::LoraPlan plan = arfq::lora_plan(ctx->cus, *lora, rows);
+    if (int rc = take_workspace(ctx, "lora_add", plan.ws_bytes, workspace_bytes, &workspace)) return rc;
+    const arfq::LoraArgs a = {*lora, ids, (int)rows, x, x_dtype == ARFQ_F16, base, out, base_stride, out_stride, (float *)workspace};
+    const hipError_t e = arfq::launch_lora(a, plan, ctx->stream);
+    return e == hipSuccess ? ARFQ_OK : hip_fail(ctx, e, "lora_add launch");
 }
 
 // -------------------------------------------------------------------- MoE ----

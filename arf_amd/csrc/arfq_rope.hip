@@ -1,0 +1,111 @@
+// arfq_rope.hip -- rotary positions of one to four axes.
+//
+// A thread has four pairs of a row (or eight of the values behind them) and goes over heads of its token, so that their
+// cosines are formed once for several heads; a workgroup's threads lie side by side on the heads of one token.  An
+// angle counts in turns: position times turns a position in 64 bits, of which the nearest quarter is taken off, and
+// what is left, at most an eighth of a turn, goes into the series of sine and cosine in 32 bits (the first terms left
+// out are below 2^-27 of a turn's radius).  Bound by memory.
+#include "arfq_step.h"
+
+namespace arfq {
+namespace {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+constexpr int THREADS = 256;
+
+struct Turn {
+    float c, s;
+};
+__device__ __forceinline__ Turn turn_of(double turns, float gain) {
+    const double quarter = rint(turns * 4.0);
+    const float a = (float)(turns - quarter * 0.25) * 6.283185307179586f, w = a * a;
+    const float c = 1.0f + w * (-1.0f / 2 + w * (1.0f / 24 + w * (-1.0f / 720 + w * (1.0f / 40320 + w * (-1.0f / 3628800)))));
+    const float s = a + a * w * (-1.0f / 6 + w * (1.0f / 120 + w * (-1.0f / 5040 + w * (1.0f / 362880))));
+    const int q = (int)((int64_t)quarter & 3);
+    const float x = q & 1 ? s : c, y = q & 1 ? c : s;
+    return {(q == 1 || q == 2 ? -x : x) * gain, (q >= 2 ? -y : y) * gain};
+}
+
+template <bool F16>
+__device__ __forceinline__ void load4(const void *p, int64_t i, float (&o)[4]) {
+    if constexpr (F16) {
+        const u32x2 w = *(const u32x2 *)((const _Float16 *)p + i);
+        o[0] = h2f(w.x); o[1] = h2f(w.x >> 16); o[2] = h2f(w.y); o[3] = h2f(w.y >> 16);
+    } else {
+        const f32x4 w = *(const f32x4 *)((const float *)p + i);
+        o[0] = w.x; o[1] = w.y; o[2] = w.z; o[3] = w.w;
+    }
+}
+template <bool F16>
+__device__ __forceinline__ void store4(void *p, int64_t i, const float (&o)[4]) {
+    if constexpr (F16)
+        *(u32x2 *)((_Float16 *)p + i) = u32x2{pack_f16x2(o[0], o[1]), pack_f16x2(o[2], o[3])};
+    else
+        *(f32x4 *)((float *)p + i) = f32x4{o[0], o[1], o[2], o[3]};
+}
+
+// lanes: threads of a row (dim / 8); slots: rows side by side in a workgroup; heads of a workgroup: `span`.
+template <bool XF16, bool OF16, bool NEIGHBOURS>
+__global__ __launch_bounds__(THREADS) void rope_kernel(RopeArgs a, int lanes, int slots, int span, int groups) {
+    const int slot = threadIdx.x / lanes, u = threadIdx.x - slot * lanes;
+    const int t = block_of() / groups, h0 = (block_of() - t * groups) * span, h1 = min(h0 + span, a.heads);
+    if (slot >= slots || t >= a.tokens) return;
+    // two runs of four values: a pair's halves, or eight neighbours
+    const bool turns = u < a.rot / 8;
+    if (!turns && a.x == a.out) return;
+    const int first = NEIGHBOURS || !turns ? 8 * u : 4 * u, second = first + (NEIGHBOURS || !turns ? 4 : a.rot / 2);
+    Turn w[4];
+    if (turns) {
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            w[i] = turn_of((double)a.positions[a.axis[4 * u + i] * a.position_stride + t] * a.turns[4 * u + i], a.gain);
+    }
+    for (int h = h0 + slot; h < h1; h += slots) {
+        const int64_t xo = t * a.x_stride + (int64_t)h * a.dim, oo = t * a.out_stride + (int64_t)h * a.dim;
+        float x[4], y[4];
+        load4<XF16>(a.x, xo + first, x);
+        load4<XF16>(a.x, xo + second, y);
+        if (turns) {
+            auto rotate = [&](int i, float &p, float &q) {
+                const float r = p * w[i].c - q * w[i].s;
+                q = p * w[i].s + q * w[i].c;
+                p = r;
+            };
+            if constexpr (NEIGHBOURS) {
+                rotate(0, x[0], x[1]);
+                rotate(1, x[2], x[3]);
+                rotate(2, y[0], y[1]);
+                rotate(3, y[2], y[3]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; i++) rotate(i, x[i], y[i]);
+            }
+        }
+        store4<OF16>(a.out, oo + first, x);
+        store4<OF16>(a.out, oo + second, y);
+    }
+}
+
+template <bool XF16, bool OF16, bool NEIGHBOURS>
+hipError_t rope_launch(const RopeArgs &a, int cus, hipStream_t s) {
+    const int lanes = a.dim / 8, slots = THREADS / lanes;
+    // heads of a workgroup: all of a token's, fewer where that leaves compute units idle
+    int span = a.heads;
+    while (span > slots && (int64_t)a.tokens * ((a.heads + span - 1) / span) < 4 * cus) span = (span + 1) / 2;
+    const int groups = (a.heads + span - 1) / span;
+    rope_kernel<XF16, OF16, NEIGHBOURS><<<grid_of((int64_t)a.tokens * groups), THREADS, 0, s>>>(a, lanes, slots, span, groups);
+    return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_rope(const RopeArgs &a, int cus, hipStream_t s) {
+    if (a.neighbours) {
+        if (a.x_f16) return a.out_f16 ? rope_launch<true, true, true>(a, cus, s) : rope_launch<true, false, true>(a, cus, s);
+        return a.out_f16 ? rope_launch<false, true, true>(a, cus, s) : rope_launch<false, false, true>(a, cus, s);
+    }
+    if (a.x_f16) return a.out_f16 ? rope_launch<true, true, false>(a, cus, s) : rope_launch<true, false, false>(a, cus, s);
+    return a.out_f16 ? rope_launch<false, true, false>(a, cus, s) : rope_launch<false, false, false>(a, cus, s);
+}
+
+}  // namespace arfq

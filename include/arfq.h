@@ -377,6 +377,114 @@ int arfq_kv_attention(arfq_ctx *ctx, const arfq_kv *kv, const arfq_kv_seqs *seqs
 int arfq_kv_attention_workspace(arfq_ctx *ctx, const arfq_kv *kv, int64_t batch, int64_t tokens, int64_t max_pages,
                                 int q_heads, size_t *bytes);
 
+/* ---- a serving step around the cache ------------------------------------------
+ * What stands between the quantised products and the cache in an attention block of many requests: the
+ * step's page tables, the requests' adapters, rotary positions, and attention over chosen blocks.  None has a
+ * counterpart in the reference's matmul path. */
+
+/* A step's bookkeeping, from the requests' lengths (host struct; its arrays are on the device, and are read and
+ * written when the work runs, so that a captured graph sees their values of the moment).  Sequence b holds held[b]
+ * tokens, in its pages pages[b * max_pages ..], and is to hold add[b] more (rows of the step), or -add[b] fewer
+ * (the last ones: rejected drafts; all of them at most: an ended request).  Whoever holds fewer gives back the
+ * pages that it then needs no more; whoever holds more takes what it lacks: first from the pages given back in
+ * this call (sequences in order, each one's pages in order), then from the top of the stack of free ones.  What is
+ * left of the pages given back goes onto the stack, the first of them topmost.
+ * A sequence gets nothing (held_next[b] = held[b], len[b] = 0, its rows' positions and slots -1) where its
+ * pages do not fit those free with the pages wanted before it counted (so none is overtaken; who wants no page is
+ * not refused for that), where they pass max_pages, where its rows pass `tokens`, or held[b] is not in
+ * [0, max_pages * page_size].
+ * With what it writes, { batch, tokens, start, len, pages, max_pages } is the step's arfq_kv_seqs, whose
+ * rows of refused sequences name nothing; positions are what arfq_rope takes.  Inputs are not changed (beyond
+ * pages' new entries and the stack's, above the free ones), so held and held_next, n_free and n_free_next change
+ * places from step to step. */
+typedef struct {
+    int64_t batch, max_pages;    /* at most 16384; max_pages * page_size <= 2^29 */
+    int64_t tokens;              /* places of positions and slots: the step's rows, or more; at most 2^30 */
+    int64_t n_pages;             /* places of the stack */
+    int page_size;               /* tokens of a page, 1..65536 */
+    const int32_t *add, *held;   /* [batch] */
+    int32_t *held_next;          /* [batch] */
+    int32_t *pages;              /* [batch, max_pages]: entries of new pages are written */
+    int32_t *free_pages;         /* [n_pages]: the stack, n_free entries from place 0 on */
+    const int32_t *n_free;       /* [1] (outside [0, n_pages]: the nearest of these) */
+    int32_t *n_free_next;        /* [1] */
+    int32_t *start;              /* [batch + 1]: running sum of the rows, at most `tokens` */
+    int32_t *len;                /* [batch]: held_next, or 0 where the sequence was refused */
+    int32_t *taken, *freed;      /* [batch + 1]: running sums of the pages taken and given back */
+    int32_t *positions;          /* [tokens]: a row's place in its sequence; -1: none */
+    int64_t *slots;              /* [tokens]: page id * page_size + place within the page; -1: none */
+} arfq_kv_step;
+int arfq_kv_plan(arfq_ctx *ctx, const arfq_kv_step *step);
+
+/* Rotary positions of one to four axes.  The rows of x and out are [tokens, heads, head_dim]; of a head's first rot_dim
+ * values, pair i, (x_i, x_(i + rot_dim / 2)) or with ARFQ_ROPE_NEIGHBOURS (x_2i, x_(2i + 1)), becomes
+ *     (a cos w - b sin w, a sin w + b cos w) * gain,  w = positions[axis[i] * position_stride + t] * freq[i]
+ * (-w with `inverse`: the rotation back, and what a gradient takes); the values behind rot_dim are copied.
+ * Angles are formed in 64 bits, cosines and products in 32.  Text: one axis (axis NULL), freq[i] =
+ * base^(-2i / rot_dim).  Images and video: axis[i] says whether pair i turns with time, height or width. */
+#define ARFQ_ROPE_HALVES 0
+#define ARFQ_ROPE_NEIGHBOURS 1
+typedef struct {
+    int rot_dim;           /* a multiple of 8 up to 256 */
+    int pairs;             /* ARFQ_ROPE_* */
+    int axes;              /* 1..4 */
+    const uint8_t *axis;   /* host, [rot_dim / 2], each below axes; NULL: 0 */
+    const double *freq;    /* host, [rot_dim / 2], finite: radians a position */
+    float gain;            /* finite */
+} arfq_rope_pairs;
+/* positions: device, int32, [axes][position_stride] (position_stride >= tokens).  x and out: device, f32 or f16 each,
+ * with the elements from one token to the next; pointers and strides multiples of 16 bytes; head_dim a multiple of 8
+ * up to 1024 (others: ARFQ_E_UNSUPPORTED).  out may be x where type and stride are the same (a fused qkv product's
+ * q and k columns are one call: heads = q's + k's); otherwise they do not overlap.  tokens * heads at most 2^30. */
+int arfq_rope(arfq_ctx *ctx, const arfq_rope_pairs *rope, const int32_t *positions, int64_t position_stride,
+              int64_t tokens, int heads, int head_dim, const void *x, int64_t x_stride, int x_dtype, void *out,
+              int64_t out_stride, int out_dtype, int inverse);
+
+/* Bounds of the cache's keys, [n_pages, heads, 2, head_dim] f16 (device, the caller's): of each channel of a page's keys of
+ * a head the largest and the smallest, as the cache holds them (exact; NaN where a key is NaN).  arfq_kv_bounds forms
+ * those of every page that the step's rows lie in, over the page's tokens below the sequence's length; after
+ * arfq_kv_write with the same seqs the bounds of a sequence are those of all that it holds.  (Tokens taken back
+ * leave the bounds as wide as they were until their page is written again.)  16-byte aligned. */
+int arfq_kv_bounds(arfq_ctx *ctx, const arfq_kv *kv, const arfq_kv_seqs *seqs, void *bounds);
+
+/* arfq_kv_attention (causal, no window) over at most `count` blocks of each row's sequence, which the row chooses for
+ * each K/V head.  A block is a page.  The row's position is in its last block; of the blocks up to there it takes
+ * the `last` latest, the `first` earliest, and of the others those with the largest
+ *     max over the K/V head's q heads of sum_d max(s q_d hi_d, s q_d lo_d),  s = 1, or -1 for a negative scale
+ * (64 bits; no product of scale, q and one of the block's keys is larger), the earlier one of two alike.  NaN comes first,
+ * pages that are not the cache's come last.  count 1..2^20, first >= 0, last >= 1, first + last <= count.
+ * chosen: NULL, or int32 [tokens, heads, count] on the device: the blocks' numbers within the sequence, ascending, then
+ * -1; all -1 for a row that attends to nothing; rows of no sequence are left as they were.
+ * q, out, rows that attend to nothing, arithmetic and workspace (arfq_kv_attention_blocks_workspace bytes) as in
+ * arfq_kv_attention. */
+int arfq_kv_attention_blocks(arfq_ctx *ctx, const arfq_kv *kv, const arfq_kv_seqs *seqs, const void *bounds, int q_heads,
+                             const void *q, int64_t q_stride, int q_dtype, void *out, int64_t out_stride, int out_dtype,
+                             float scale, float softcap, int64_t count, int64_t first, int64_t last, int32_t *chosen,
+                             void *workspace, size_t workspace_bytes);
+int arfq_kv_attention_blocks_workspace(arfq_ctx *ctx, const arfq_kv *kv, int64_t batch, int64_t tokens, int64_t max_pages,
+                                       int q_heads, int64_t count, size_t *bytes);
+
+/* Low-rank adapters of many requests beside a shared projection (arfq_matmul's y, of n values a row):
+ *     out[t] = base[t] + scale[e] * B_e (A_e x[t]),  e = ids[t];  out[t] = base[t] where e is not in [0, adapters).
+ * Adapters lie one after another: A_e [rank, k], B_e [n, rank], f16 (a smaller rank: zeros behind it).  Sums are f32:
+ * products of x and A are exact or rounded once to f32; A_e x enters the second product in f32 or as two f16
+ * parts (22 bits of the row's largest). */
+typedef struct {
+    int64_t adapters, n, k;  /* at least 1; k a multiple of 8 */
+    int64_t rank;            /* a multiple of 8 up to 256 */
+    const void *a;           /* device, f16 [adapters, rank, k], 16-byte aligned */
+    const void *b;           /* device, f16 [adapters, n, rank], 16-byte aligned */
+    const float *scale;      /* device, [adapters]; NULL: 1 */
+} arfq_lora;
+/* ids: device, int32 [rows].  x: [rows, k], f32 or f16, packed, 16-byte aligned.  base and out: f32 with the elements
+ * from one row to the next; base may be out (where the strides are the same too), or NULL for zeros.  Rows of one
+ * adapter need not lie together; in long batches they are fastest where they do.  At most 2^24 rows.  workspace
+ * (16-byte aligned, arfq_lora_workspace bytes): as in arfq_kv_attention. */
+int arfq_lora_add(arfq_ctx *ctx, const arfq_lora *lora, const int32_t *ids, int64_t rows, const void *x, int x_dtype,
+                  const float *base, int64_t base_stride, float *out, int64_t out_stride, void *workspace,
+                  size_t workspace_bytes);
+int arfq_lora_workspace(arfq_ctx *ctx, const arfq_lora *lora, int64_t rows, size_t *bytes);
+
 /* ---- GGUF reader ---------------------------------------------------------
  * A GGUF v3 file opened read-only and memory-mapped; tensors are read in place
  * (LazyGguf, crates/arf-core/src/model/gguf.rs:365-564).  Errors of
