@@ -12,11 +12,14 @@
 
 #include <math.h>
 
+#include <type_traits>
+
 namespace arfq {
 namespace {
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x8 __attribute__((ext_vector_type(8)));
 
 constexpr int K_PART = 512;  // values of k of a workgroup with one row: eight a lane
 
@@ -128,8 +131,25 @@ __global__ __launch_bounds__(256) void lora_rows_b(LoraArgs a, int splits, int p
 
 constexpr int TR = 16;  // rows of a tile: a matrix instruction's columns
 
-// The adapters that a tile's rows name, one after another (`mine`: this lane's row's; the same in all lanes of a row).
-// Returns the next one, or -2 behind the last; done: the lanes whose rows are served.
+// Workgroups go to the eight XCDs in turn: this numbering gives each of them a run of neighbouring items instead, so that an
+// adapter's A or B is fetched into few L2s.
+__device__ __forceinline__ int xcd_run(int block, int blocks) {
+    const int per = blocks / 8;
+    return block < 8 * per ? block % 8 * per + block / 8 : block;
+}
+
+// The adapters that the rows of tiles name, one after another (`mine`: those of this lane's rows; the same in all lanes of
+// a row; -1: none).  Returns the next one, or -2 behind the last; done: the lanes whose rows are served.
+template <int N>
+__device__ __forceinline__ int next_id(const int (&mine)[N], uint64_t (&done)[N]) {
+    int e = -2;
+#pragma unroll
+    for (int s = 0; s < N; s++)
+        if (e == -2 && done[s] != ~0ull) e = __builtin_amdgcn_readlane(mine[s], __ffsll((unsigned long long)~done[s]) - 1);
+#pragma unroll
+    for (int s = 0; s < N; s++) done[s] |= __ballot(mine[s] == e);
+    return e;
+}
 __device__ __forceinline__ int next_id(int mine, uint64_t &done) {
     if (done == ~0ull) return -2;
     const int e = __builtin_amdgcn_readlane(mine, __ffsll((unsigned long long)~done) - 1);
@@ -137,166 +157,224 @@ __device__ __forceinline__ int next_id(int mine, uint64_t &done) {
     return e;
 }
 
-// RT 16-rank tiles of h, TR rows, a part of k in four by the waves.
+// RT 16-rank tiles of h, two tiles of rows, a part of k in four by the waves, whose sums are added through LDS.  A step is
+// 32 values of k: eight neighbouring ones a lane.
+constexpr int A_WAVES = 4, A_TILES = 2;
+template <int RT, class X>
+struct Operands {
+    f16x8 w[RT];
+    X x[A_TILES];
+};
 template <int RT, bool F16>
-__global__ __launch_bounds__(256) void lora_tiles_a(LoraArgs a, int splits, int k_part, int ranks) {
-    __shared__ f32x4 sh[4][RT][64];
+__global__ __launch_bounds__(64 * A_WAVES, 2) void lora_tiles_a(LoraArgs a, int splits, int k_part, int ranks, int shares, int groups) {
+    __shared__ f32x4 sh[A_WAVES][A_TILES][RT][64];
     int block = block_of();
+    const int share = block / groups;  // (slowest: those with nothing to do come last)
+    block -= share * groups;
+    block = xcd_run(block, groups);
     const int rb = block % ranks;
     block /= ranks;
-    const int part = block % splits, t0 = block / splits * TR;
+    const int part = block % splits, t0 = block / splits * (A_TILES * TR);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
-    if (t0 >= a.rows) return;
-    const int rank = (int)a.l.rank, r0 = rb * RT * 16, t = min(t0 + c, a.rows - 1);
+    if (share >= shares) return;
+    const int rank = (int)a.l.rank, r0 = rb * RT * 16;
     const int64_t k = a.l.k;
     // the wave's range, in steps of 32: eight values a lane
-    const int64_t lo = (int64_t)part * k_part + (int64_t)wave * (k_part / 4), hi = min(lo + k_part / 4, k);
-    const int mine = t0 + c < a.rows ? id_of(a, t0 + c) : -1;
-    uint64_t done = 0;
-    for (int e; (e = next_id(mine, done)) != -2;) {
-        if (e < 0) continue;
-        f32x4 acc[RT];
+    const int64_t lo = (int64_t)part * k_part + (int64_t)wave * (k_part / A_WAVES), hi = min(lo + k_part / A_WAVES, k);
+    int mine[A_TILES];
 #pragma unroll
-        for (int i = 0; i < RT; i++) acc[i] = f32x4{0, 0, 0, 0};
+    for (int s = 0; s < A_TILES; s++) mine[s] = t0 + 16 * s + c < a.rows ? id_of(a, t0 + 16 * s + c) : -1;
+    using T = std::conditional_t<F16, _Float16, float>;
+    using X = std::conditional_t<F16, f16x8, f32x8>;
+    const T *xp[A_TILES];
+#pragma unroll
+    for (int s = 0; s < A_TILES; s++) xp[s] = (const T *)a.x + min(t0 + 16 * s + c, a.rows - 1) * k + lo + 8 * g;
+    uint64_t done[A_TILES] = {};
+    for (int e, turn = 0; (e = next_id(mine, done)) != -2;) {
+        if (e < 0 || turn++ % shares != share) continue;
+        f32x4 acc[A_TILES][RT];
+#pragma unroll
+        for (int s = 0; s < A_TILES; s++)
+#pragma unroll
+            for (int i = 0; i < RT; i++) acc[s][i] = f32x4{0, 0, 0, 0};
         const _Float16 *A = (const _Float16 *)a.l.a + (int64_t)e * rank * k;
-        for (int64_t k0 = lo; k0 < hi; k0 += 32) {
-            const int64_t kk = k0 + 8 * g;
-            const bool on = kk < hi;
-            f16x8 w[RT];
+        const _Float16 *wp[RT];
 #pragma unroll
-            for (int i = 0; i < RT; i++) w[i] = on ? *(const f16x8 *)(A + min(r0 + 16 * i + c, rank - 1) * k + kk) : zero8();
-            if constexpr (F16) {
-                const f16x8 x = on ? *(const f16x8 *)((const _Float16 *)a.x + t * k + kk) : zero8();
+        for (int i = 0; i < RT; i++) wp[i] = A + min(r0 + 16 * i + c, rank - 1) * k + lo + 8 * g;
+        constexpr int DEPTH = 4;
+        Operands<RT, X> ring[DEPTH];
+        auto load = [&](Operands<RT, X> &o, int64_t at, bool on) {
 #pragma unroll
-                for (int i = 0; i < RT; i++) acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[i], x, acc[i], 0, 0, 0);
-            } else {
-                float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-                if (on) load8<false>(a.x, t * k + kk, x);
+            for (int i = 0; i < RT; i++) o.w[i] = on ? *(const f16x8 *)(wp[i] + at) : zero8();
 #pragma unroll
-                for (int j = 0; j < 8; j++)
+            for (int s = 0; s < A_TILES; s++) o.x[s] = on ? *(const X *)(xp[s] + at) : X{};
+        };
+        auto add = [&](const Operands<RT, X> &o) {
 #pragma unroll
-                    for (int i = 0; i < RT; i++)
-                        acc[i] = __builtin_amdgcn_mfma_f32_16x16x4f32((float)w[i][j], x[j], acc[i], 0, 0, 0);
+            for (int i = 0; i < RT; i++)
+#pragma unroll
+                for (int s = 0; s < A_TILES; s++) {
+                    if constexpr (F16) {
+                        acc[s][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(o.w[i], o.x[s], acc[s][i], 0, 0, 0);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 8; j++)
+                            acc[s][i] = __builtin_amdgcn_mfma_f32_16x16x4f32((float)o.w[i][j], o.x[s][j], acc[s][i], 0, 0, 0);
+                    }
+                }
+        };
+        // loads DEPTH steps ahead of their use; the range's last, shorter step by itself
+        const int64_t whole = max(hi - lo, (int64_t)0) & ~(int64_t)31;
+#pragma unroll
+        for (int d = 0; d < DEPTH; d++)
+            if (32 * d < whole) load(ring[d], 32 * d, true);
+#pragma unroll 1
+        for (int64_t at = 0; at < whole; at += 32 * DEPTH) {
+#pragma unroll
+            for (int d = 0; d < DEPTH; d++) {
+                if (at + 32 * d < whole) add(ring[d]);
+                if (at + 32 * (d + DEPTH) < whole) load(ring[d], at + 32 * (d + DEPTH), true);
             }
         }
-#pragma unroll
-        for (int i = 0; i < RT; i++) sh[wave][i][lane] = acc[i];
-        __syncthreads();
-        // a lane's four results: ranks 4g .. +3 of a tile, row c
-        for (int i = wave; i < RT; i += 4) {
-            const f32x4 s = sh[0][i][lane] + sh[1][i][lane] + sh[2][i][lane] + sh[3][i][lane];
-            const int r = r0 + 16 * i + 4 * g;
-            if (mine == e && r < rank) *(f32x4 *)(a.h + ((int64_t)part * a.rows + t0 + c) * rank + r) = s;
+        if (lo + whole < hi) {
+            load(ring[0], whole, lo + whole + 8 * g < hi);
+            add(ring[0]);
         }
         __syncthreads();
+#pragma unroll
+        for (int s = 0; s < A_TILES; s++)
+#pragma unroll
+            for (int i = 0; i < RT; i++) sh[wave][s][i][lane] = acc[s][i];
+        __syncthreads();
+        // a lane's four results: ranks 4g .. +3 of a tile, row c
+#pragma unroll
+        for (int s = 0; s < A_TILES; s++)
+            for (int i = wave; i < RT; i += A_WAVES) {
+                f32x4 v = sh[0][s][i][lane];
+#pragma unroll
+                for (int u = 1; u < A_WAVES; u++) v += sh[u][s][i][lane];
+                const int r = r0 + 16 * i + 4 * g;
+                if (mine[s] == e && r < rank) *(f32x4 *)(a.h + ((int64_t)part * a.rows + t0 + 16 * s + c) * rank + r) = v;
+            }
     }
 }
 
-// A wave: CT tiles of rows, NT tiles of 16 outputs, ranks in runs of 64.
-constexpr int CT = 2, NT = 4;
-template <bool VEC>
-__global__ __launch_bounds__(256) void lora_tiles_b(LoraArgs a, int splits, int parts) {
-    const int block = block_of(), part = block % parts, t0 = block / parts * (CT * TR);
+// B_ROWS rows, of KS runs of 32 ranks.  Their h first, into LDS: the parts added, and as two f16 parts of it times a power of
+// two that puts a row's largest into [2^14, 2^15).  Then each wave has 16 NT outputs and goes over the rows' tiles: B_e
+// stays in registers while the adapter does, base is loaded a tile ahead.
+constexpr int B_WAVES = 4;
+template <int KS>
+struct TileB {
+    static constexpr int ROWS = KS <= 4 ? 64 : 32, NT = KS <= 4 ? 4 : 2, RANK = 32 * KS, LD = RANK + 8, OUT = B_WAVES * NT * 16;
+};
+template <int KS, bool VEC>
+__global__ __launch_bounds__(64 * B_WAVES) void lora_tiles_b(LoraArgs a, int splits, int parts) {
+    using T = TileB<KS>;
+    constexpr int NT = T::NT, ROWS = T::ROWS;
+    __shared__ __align__(16) _Float16 sh[2][ROWS][T::LD];
+    __shared__ float unit[ROWS];
+    __shared__ int ids[ROWS];
+    const int block = block_of(), part = block % parts, t0 = block / parts * ROWS;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
     if (t0 >= a.rows) return;
     const int rank = (int)a.l.rank;
-    const int64_t n = a.l.n, n0 = (int64_t)part * (4 * NT * 16) + wave * (NT * 16);
-    if (n0 >= n) return;
-    int mine[CT];
+    const int64_t n = a.l.n, n0 = (int64_t)part * T::OUT + wave * (NT * 16);
+    f32x4 next[NT];  // base of the tile to come
+    auto load_base = [&](int s) {
 #pragma unroll
-    for (int s = 0; s < CT; s++) mine[s] = t0 + 16 * s + c < a.rows ? id_of(a, t0 + 16 * s + c) : -1;
-    uint64_t done[CT] = {};
-    for (;;) {
-        // the next adapter, or none, that one of the tiles' rows is still to be served with
-        int e = -2;
-#pragma unroll
-        for (int s = 0; s < CT; s++)
-            if (e == -2 && done[s] != ~0ull) e = __builtin_amdgcn_readlane(mine[s], __ffsll((unsigned long long)~done[s]) - 1);
-        if (e == -2) break;
-#pragma unroll
-        for (int s = 0; s < CT; s++) done[s] |= __ballot(mine[s] == e);
-        f32x4 sum[CT][NT];
-#pragma unroll
-        for (int s = 0; s < CT; s++)
-#pragma unroll
-            for (int i = 0; i < NT; i++) sum[s][i] = f32x4{0, 0, 0, 0};
-        if (e >= 0) {
-            const _Float16 *B = (const _Float16 *)a.l.b + (int64_t)e * n * rank;
-            const float scale = a.l.scale ? a.l.scale[e] : 1.0f;
-            for (int r0 = 0; r0 < rank; r0 += 64) {
-                f16x8 w[NT][2];
-#pragma unroll
-                for (int i = 0; i < NT; i++)
-#pragma unroll
-                    for (int q = 0; q < 2; q++) {
-                        const int r = r0 + 32 * q + 8 * g;
-                        w[i][q] = r < rank ? *(const f16x8 *)(B + min(n0 + 16 * i + c, n - 1) * rank + r) : zero8();
-                    }
-#pragma unroll
-                for (int s = 0; s < CT; s++) {
-                    // h of the row: its parts added, and as two f16 parts of it times a power of two
-                    float h[2][8], top = 0.0f;
-#pragma unroll
-                    for (int q = 0; q < 2; q++) {
-                        const int r = r0 + 32 * q + 8 * g;
-#pragma unroll
-                        for (int j = 0; j < 8; j++) h[q][j] = 0.0f;
-                        if (mine[s] == e && r < rank)
-                            for (int p = 0; p < splits; p++) {
-                                float v[8];
-                                load8<false>(a.h, ((int64_t)p * a.rows + t0 + 16 * s + c) * rank + r, v);
-#pragma unroll
-                                for (int j = 0; j < 8; j++) h[q][j] += v[j];
-                            }
-#pragma unroll
-                        for (int j = 0; j < 8; j++) top = fmaxf(top, fabsf(h[q][j]));
-                    }
-                    top = fmaxf(top, __shfl_xor(top, 16));
-                    top = fmaxf(top, __shfl_xor(top, 32));
-                    const int ex = min(max(top > 0.0f ? 141 - (int)(__builtin_bit_cast(uint32_t, top) >> 23) : 0, -126), 126);
-                    const float up = __builtin_bit_cast(float, (uint32_t)(ex + 127) << 23);
-                    const float down = __builtin_bit_cast(float, (uint32_t)(127 - ex) << 23);
-                    f16x8 hi[2], lo[2];
-#pragma unroll
-                    for (int q = 0; q < 2; q++)
-#pragma unroll
-                        for (int j = 0; j < 8; j++) {
-                            const float v = h[q][j] * up;
-                            hi[q][j] = (_Float16)v;
-                            lo[q][j] = fabsf(v) == INFINITY ? (_Float16)0 : (_Float16)(v - (float)hi[q][j]);
-                        }
-#pragma unroll
-                    for (int i = 0; i < NT; i++) {
-                        f32x4 acc = {0, 0, 0, 0};
-#pragma unroll
-                        for (int q = 0; q < 2; q++) {
-                            acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[i][q], hi[q], acc, 0, 0, 0);
-                            acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[i][q], lo[q], acc, 0, 0, 0);
-                        }
-                        sum[s][i] += acc * (down * scale);
-                    }
-                }
-            }
+        for (int i = 0; i < NT; i++) {
+            const int64_t at = n0 + 16 * i + 4 * g;
+            next[i] = f32x4{0, 0, 0, 0};
+            if (VEC && a.base && at < n && t0 + 16 * s + c < a.rows)
+                next[i] = *(const f32x4 *)(a.base + (int64_t)(t0 + 16 * s + c) * a.base_stride + at);
         }
+    };
+    load_base(0);
+    constexpr int LANES = 4 * KS;  // of a row: eight ranks each
+    for (int i = threadIdx.x; i < ROWS * LANES; i += 64 * B_WAVES) {
+        const int row = i / LANES, u = i % LANES, t = t0 + row;
+        const int e = t < a.rows ? id_of(a, t) : -1;
+        float h[8] = {0, 0, 0, 0, 0, 0, 0, 0}, top = 0.0f;
+        if (e >= 0 && 8 * u < rank)
+#pragma unroll 4
+            for (int p = 0; p < splits; p++) {
+                float v[8];
+                load8<false>(a.h, ((int64_t)p * a.rows + t) * rank + 8 * u, v);
 #pragma unroll
-        for (int s = 0; s < CT; s++) {
-            const int t = t0 + 16 * s + c;
-            if (mine[s] != e || t >= a.rows) continue;
-            const float *base = a.base ? a.base + t * a.base_stride : nullptr;
-            float *out = a.out + t * a.out_stride;
-            if (e < 0 && base == out) continue;
+                for (int j = 0; j < 8; j++) h[j] += v[j];
+            }
+#pragma unroll
+        for (int j = 0; j < 8; j++) top = fmaxf(top, fabsf(h[j]));
+#pragma unroll
+        for (int d = 1; d < LANES; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
+        const int ex = min(max(top > 0.0f ? 141 - (int)(__builtin_bit_cast(uint32_t, top) >> 23) : 0, -126), 126);
+        const float up = __builtin_bit_cast(float, (uint32_t)(ex + 127) << 23);
+        f16x8 hi, lo;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const float v = h[j] * up;
+            hi[j] = (_Float16)v;
+            lo[j] = fabsf(v) == INFINITY ? (_Float16)0 : (_Float16)(v - (float)hi[j]);
+        }
+        *(f16x8 *)&sh[0][row][8 * u] = hi;
+        *(f16x8 *)&sh[1][row][8 * u] = lo;
+        if (u == 0) {
+            ids[row] = e;
+            unit[row] = __builtin_bit_cast(float, (uint32_t)(127 - ex) << 23) * (e >= 0 && a.l.scale ? a.l.scale[e] : 1.0f);
+        }
+    }
+    lds_barrier();
+    f16x8 w[NT][KS];
+    int loaded = -1;
+    if (n0 >= n) return;
+#pragma unroll 1
+    for (int s = 0; s < ROWS / 16 && t0 + 16 * s < a.rows; s++) {
+        f32x4 base[NT];
+#pragma unroll
+        for (int i = 0; i < NT; i++) base[i] = next[i];
+        if (s + 1 < ROWS / 16) load_base(s + 1);
+        const int t = t0 + 16 * s + c;
+        const int mine = ids[16 * s + c];
+        const float f = unit[16 * s + c];
+        float *out = a.out + (int64_t)t * a.out_stride;
+        const float *from = a.base ? a.base + (int64_t)t * a.base_stride : nullptr;
+        uint64_t done = 0;
+        for (int e; (e = next_id(mine, done)) != -2;) {
+            f32x4 acc[NT];
+#pragma unroll
+            for (int i = 0; i < NT; i++) acc[i] = f32x4{0, 0, 0, 0};
+            if (e >= 0) {
+                if (e != loaded) {
+                    const _Float16 *B = (const _Float16 *)a.l.b + (int64_t)e * n * rank;
+#pragma unroll
+                    for (int i = 0; i < NT; i++)
+#pragma unroll
+                        for (int q = 0; q < KS; q++)
+                            w[i][q] = 32 * q + 8 * g < rank ? *(const f16x8 *)(B + min(n0 + 16 * i + c, n - 1) * rank + 32 * q + 8 * g) : zero8();
+                    loaded = e;
+                }
+#pragma unroll
+                for (int q = 0; q < KS; q++)
+#pragma unroll
+                    for (int p = 0; p < 2; p++) {
+                        const f16x8 h = *(const f16x8 *)&sh[p][16 * s + c][32 * q + 8 * g];
+#pragma unroll
+                        for (int i = 0; i < NT; i++) acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[i][q], h, acc[i], 0, 0, 0);
+                    }
+            }
+            if (mine != e || t >= a.rows || (e < 0 && from == out)) continue;
 #pragma unroll
             for (int i = 0; i < NT; i++) {
                 const int64_t at = n0 + 16 * i + 4 * g;
                 if constexpr (VEC) {
-                    if (at >= n) continue;
-                    f32x4 v = sum[s][i];
-                    if (base) v += *(const f32x4 *)(base + at);
-                    *(f32x4 *)(out + at) = v;
+                    if (at < n) *(f32x4 *)(out + at) = e < 0 ? base[i] : base[i] + acc[i] * f;
                 } else {
 #pragma unroll
                     for (int j = 0; j < 4; j++)
-                        if (at + j < n) out[at + j] = (base ? base[at + j] : 0.0f) + sum[s][i][j];
+                        if (at + j < n) {
+                            const float v = from ? from[at + j] : 0.0f;
+                            out[at + j] = e < 0 ? v : v + acc[i][j] * f;
+                        }
                 }
             }
         }
@@ -316,9 +394,24 @@ hipError_t rows_b(const LoraArgs &a, const LoraPlan &p, hipStream_t s) {
 template <int RT>
 hipError_t tiles_a(const LoraArgs &a, const LoraPlan &p, hipStream_t s) {
     const int ranks = (int)((a.l.rank + RT * 16 - 1) / (RT * 16));
-    const dim3 grid = grid_of((int64_t)((a.rows + TR - 1) / TR) * p.splits * ranks);
-    if (a.x_f16) lora_tiles_a<RT, true><<<grid, 256, 0, s>>>(a, p.splits, p.k_part, ranks);
-    else lora_tiles_a<RT, false><<<grid, 256, 0, s>>>(a, p.splits, p.k_part, ranks);
+    const int64_t groups = (int64_t)((a.rows + A_TILES * TR - 1) / (A_TILES * TR)) * p.splits * ranks;
+    // a tile's adapters are shared by workgroups, two at least (those with nothing to do end at once): otherwise the tile in
+    // which one adapter's rows end and another's begin takes twice as long as any other
+    const int shares = (int)std::min<int64_t>(std::max<int64_t>(512 / groups, 2), A_TILES * TR);
+    const dim3 grid = grid_of(groups * shares);
+    if (a.x_f16) lora_tiles_a<RT, true><<<grid, 64 * A_WAVES, 0, s>>>(a, p.splits, p.k_part, ranks, shares, (int)groups);
+    else lora_tiles_a<RT, false><<<grid, 64 * A_WAVES, 0, s>>>(a, p.splits, p.k_part, ranks, shares, (int)groups);
+    return hipGetLastError();
+}
+
+template <int KS>
+hipError_t tiles_b(const LoraArgs &a, const LoraPlan &p, hipStream_t s) {
+    const int parts = (int)((a.l.n + TileB<KS>::OUT - 1) / TileB<KS>::OUT);
+    const dim3 grid = grid_of((int64_t)((a.rows + TileB<KS>::ROWS - 1) / TileB<KS>::ROWS) * parts);
+    const bool vec = a.l.n % 4 == 0 && a.out_stride % 4 == 0 && (uintptr_t)a.out % 16 == 0 &&
+                     (!a.base || (a.base_stride % 4 == 0 && (uintptr_t)a.base % 16 == 0));
+    if (vec) lora_tiles_b<KS, true><<<grid, 64 * B_WAVES, 0, s>>>(a, p.splits, parts);
+    else lora_tiles_b<KS, false><<<grid, 64 * B_WAVES, 0, s>>>(a, p.splits, parts);
     return hipGetLastError();
 }
 
@@ -328,11 +421,10 @@ LoraPlan lora_plan(int cus, const arfq_lora &l, int64_t rows) {
     LoraPlan p;
     p.tiles = rows > TILE_ROWS;
     if (p.tiles) {
-        // two workgroups a compute unit, and not fewer than 128 values of k a wave
-        const int64_t tiles = (rows + TR - 1) / TR;
-        const int64_t want = std::max<int64_t>(1, 2 * cus / tiles), most = std::max<int64_t>(1, l.k / 512);
-        const int64_t splits = std::min(want, most);
-        p.k_part = (int)(((l.k + splits - 1) / splits + 127) / 128 * 128);
+        // a workgroup a compute unit, and not fewer than four steps a wave
+        const int64_t tiles = (rows + A_TILES * TR - 1) / (A_TILES * TR);
+        const int64_t splits = std::max<int64_t>(1, std::min(cus / tiles, l.k / (4 * 32 * A_WAVES)));
+        p.k_part = (int)(((l.k + splits - 1) / splits + 32 * A_WAVES - 1) / (32 * A_WAVES) * (32 * A_WAVES));
         p.splits = (int)((l.k + p.k_part - 1) / p.k_part);
     } else {
         p.k_part = K_PART;
@@ -346,13 +438,8 @@ hipError_t launch_lora(const LoraArgs &a, const LoraPlan &p, hipStream_t s) {
     if (p.tiles) {
         hipError_t e = a.l.rank <= 16 ? tiles_a<1>(a, p, s) : a.l.rank <= 32 ? tiles_a<2>(a, p, s) : tiles_a<4>(a, p, s);
         if (e != hipSuccess) return e;
-        const int parts = (int)((a.l.n + 4 * NT * 16 - 1) / (4 * NT * 16));
-        const dim3 grid = grid_of((int64_t)((a.rows + CT * TR - 1) / (CT * TR)) * parts);
-        const bool vec = a.l.n % 4 == 0 && a.out_stride % 4 == 0 && (uintptr_t)a.out % 16 == 0 &&
-                         (!a.base || (a.base_stride % 4 == 0 && (uintptr_t)a.base % 16 == 0));
-        if (vec) lora_tiles_b<true><<<grid, 256, 0, s>>>(a, p.splits, parts);
-        else lora_tiles_b<false><<<grid, 256, 0, s>>>(a, p.splits, parts);
-        return hipGetLastError();
+        const int64_t runs = (a.l.rank + 31) / 32;
+        return runs <= 1 ? tiles_b<1>(a, p, s) : runs <= 2 ? tiles_b<2>(a, p, s) : runs <= 4 ? tiles_b<4>(a, p, s) : tiles_b<8>(a, p, s);
     }
     const dim3 grid = grid_of((int64_t)a.rows * p.splits);
     if (a.x_f16) lora_rows_a<true><<<grid, 256, 0, s>>>(a, p.splits);
