@@ -289,22 +289,49 @@ __global__ __launch_bounds__(64 * B_WAVES) void lora_tiles_b(LoraArgs a, int spl
                 next[i] = *(const f32x4 *)(a.base + (int64_t)(t0 + 16 * s + c) * a.base_stride + at);
         }
     };
+    f16x8 w[NT][KS];
+    auto load_b = [&](int e) {
+        const _Float16 *B = (const _Float16 *)a.l.b + (int64_t)e * n * rank;
+#pragma unroll
+        for (int i = 0; i < NT; i++)
+#pragma unroll
+            for (int q = 0; q < KS; q++)
+                w[i][q] = 32 * q + 8 * g < rank ? *(const f16x8 *)(B + min(n0 + 16 * i + c, n - 1) * rank + 32 * q + 8 * g) : zero8();
+    };
+    // (loads in the order of their use: ids, h, B of the first row, base)
+    constexpr int LANES = 4 * KS, ITEMS = ROWS * LANES / (64 * B_WAVES);  // eight ranks of a row
+    int of[ITEMS];
+    float h[ITEMS][8];
+    const int u = threadIdx.x % LANES, row0 = threadIdx.x / LANES;
+    constexpr int APART = 64 * B_WAVES / LANES;
+#pragma unroll
+    for (int it = 0; it < ITEMS; it++) {
+        of[it] = t0 + row0 + it * APART < a.rows ? id_of(a, t0 + row0 + it * APART) : -1;
+#pragma unroll
+        for (int j = 0; j < 8; j++) h[it][j] = 0.0f;
+    }
+    int loaded = id_of(a, t0);
+#pragma unroll 2
+    for (int p = 0; p < splits; p++)
+#pragma unroll
+        for (int it = 0; it < ITEMS; it++) {
+            float v[8];
+            load8<false>(a.h, ((int64_t)p * a.rows + min(t0 + row0 + it * APART, a.rows - 1)) * rank + min(8 * u, rank - 8), v);
+#pragma unroll
+            for (int j = 0; j < 8; j++) h[it][j] += v[j];
+        }
+    loaded = __builtin_amdgcn_readfirstlane(loaded);
+    if (loaded >= 0) load_b(loaded);
     load_base(0);
-    constexpr int LANES = 4 * KS;  // of a row: eight ranks each
-    for (int i = threadIdx.x; i < ROWS * LANES; i += 64 * B_WAVES) {
-        const int row = i / LANES, u = i % LANES, t = t0 + row;
-        const int e = t < a.rows ? id_of(a, t) : -1;
-        float h[8] = {0, 0, 0, 0, 0, 0, 0, 0}, top = 0.0f;
-        if (e >= 0 && 8 * u < rank)
-#pragma unroll 4
-            for (int p = 0; p < splits; p++) {
-                float v[8];
-                load8<false>(a.h, ((int64_t)p * a.rows + t) * rank + 8 * u, v);
 #pragma unroll
-                for (int j = 0; j < 8; j++) h[j] += v[j];
-            }
+    for (int it = 0; it < ITEMS; it++) {
+        const int row = row0 + it * APART, e = of[it];
+        float top = 0.0f;
 #pragma unroll
-        for (int j = 0; j < 8; j++) top = fmaxf(top, fabsf(h[j]));
+        for (int j = 0; j < 8; j++) {
+            if (e < 0 || 8 * u >= rank) h[it][j] = 0.0f;  // (what was loaded is not this row's)
+            top = fmaxf(top, fabsf(h[it][j]));
+        }
 #pragma unroll
         for (int d = 1; d < LANES; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
         const int ex = min(max(top > 0.0f ? 141 - (int)(__builtin_bit_cast(uint32_t, top) >> 23) : 0, -126), 126);
@@ -312,7 +339,7 @@ __global__ __launch_bounds__(64 * B_WAVES) void lora_tiles_b(LoraArgs a, int spl
         f16x8 hi, lo;
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-            const float v = h[j] * up;
+            const float v = h[it][j] * up;
             hi[j] = (_Float16)v;
             lo[j] = fabsf(v) == INFINITY ? (_Float16)0 : (_Float16)(v - (float)hi[j]);
         }
@@ -324,8 +351,6 @@ __global__ __launch_bounds__(64 * B_WAVES) void lora_tiles_b(LoraArgs a, int spl
         }
     }
     lds_barrier();
-    f16x8 w[NT][KS];
-    int loaded = -1;
     if (n0 >= n) return;
 #pragma unroll 1
     for (int s = 0; s < ROWS / 16 && t0 + 16 * s < a.rows; s++) {
@@ -344,15 +369,8 @@ __global__ __launch_bounds__(64 * B_WAVES) void lora_tiles_b(LoraArgs a, int spl
 #pragma unroll
             for (int i = 0; i < NT; i++) acc[i] = f32x4{0, 0, 0, 0};
             if (e >= 0) {
-                if (e != loaded) {
-                    const _Float16 *B = (const _Float16 *)a.l.b + (int64_t)e * n * rank;
-#pragma unroll
-                    for (int i = 0; i < NT; i++)
-#pragma unroll
-                        for (int q = 0; q < KS; q++)
-                            w[i][q] = 32 * q + 8 * g < rank ? *(const f16x8 *)(B + min(n0 + 16 * i + c, n - 1) * rank + 32 * q + 8 * g) : zero8();
-                    loaded = e;
-                }
+                if (e != loaded) load_b(e);
+                loaded = e;
 #pragma unroll
                 for (int q = 0; q < KS; q++)
 #pragma unroll
