@@ -91,6 +91,14 @@ def test_plan_refuses_what_does_not_fit(gpu_ctx, spare):
         _check_plan(gpu_ctx, 16, np.array(add, np.int32), np.array(h, np.int32), pages, free, n_free, tokens)
 
 
+def test_plan_pages_of_one_token(gpu_ctx):
+    # more pages wanted than 31 bits count
+    _say("plan pages of one")
+    pages, free = np.arange(12, dtype=np.int32).reshape(3, 4), np.arange(20, 28).astype(np.int32)
+    for add in ([1, 2 ** 31 - 1, 1], [2 ** 31 - 1, 1, 1], [-1, 2, -2 ** 31]):
+        _check_plan(gpu_ctx, 1, np.array(add, np.int32), np.array([2, 2, 3], np.int32), pages, free, 5, 1 << 20)
+
+
 def test_plan_of_nothing(gpu_ctx):
     _say("plan of nothing")
     none = np.zeros(0, np.int32)
