@@ -49,28 +49,40 @@ __device__ __forceinline__ void load8(const void *x, int64_t i, float (&o)[8]) {
 
 // ---- few rows ----
 
+template <int CTRL>
+__device__ __forceinline__ float dpp(float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, false));
+}
+// Sum over N neighbouring lanes, in each of them.
 template <int N>
-__device__ __forceinline__ float lanes_sum(float v) {  // over N neighbouring lanes
-#pragma unroll
-    for (int d = 1; d < N; d *= 2) v += __shfl_xor(v, d);
+__device__ __forceinline__ float lanes_sum(float v) {
+    if constexpr (N >= 2) v += dpp<0xb1>(v);    // quad_perm:[1,0,3,2]
+    if constexpr (N >= 4) v += dpp<0x4e>(v);    // quad_perm:[2,3,0,1]
+    if constexpr (N >= 8) v += dpp<0x141>(v);   // row_half_mirror
+    if constexpr (N >= 16) v += dpp<0x140>(v);  // row_mirror
+    if constexpr (N >= 32) v += __builtin_bit_cast(float, __builtin_amdgcn_ds_swizzle(__builtin_bit_cast(int, v), 0x401f));  // lane ^ 16
+    if constexpr (N == 64)
+        v = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 0)) +
+            __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 32));
     return v;
 }
 
 template <bool F16>
 __global__ __launch_bounds__(256) void lora_rows_a(LoraArgs a, int splits) {
     const int block = block_of(), t = block / splits, part = block - t * splits;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (t >= a.rows) return;
-    const int e = id_of(a, t);
-    if (e < 0) return;
     const int rank = (int)a.l.rank;
     const int64_t k = (int64_t)part * K_PART + 8 * lane;
     const bool on = k < a.l.k;
+    const int e = id_of(a, t);
     float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
     if (on) load8<F16>(a.x, t * a.l.k + k, x);
+    if (e < 0) return;
     const _Float16 *A = (const _Float16 *)a.l.a + (int64_t)e * rank * a.l.k + k;
     float *h = a.h + ((int64_t)part * a.rows + t) * rank;
     constexpr int U = 4;  // (a wave has every fourth run of as many ranks: 8 divides the rank)
+#pragma unroll 2
     for (int r0 = wave * U; r0 < rank; r0 += 4 * U) {
         f16x8 w[U];
 #pragma unroll
@@ -87,7 +99,7 @@ __global__ __launch_bounds__(256) void lora_rows_a(LoraArgs a, int splits) {
     }
 }
 
-// LP lanes have an output, eight ranks each.
+// LP lanes have an output, eight ranks each.  B and base are on their way while h's parts are added.
 constexpr int N_PART = 256;  // outputs of a workgroup
 template <int LP>
 __global__ __launch_bounds__(256) void lora_rows_b(LoraArgs a, int splits, int parts) {
@@ -103,27 +115,43 @@ __global__ __launch_bounds__(256) void lora_rows_b(LoraArgs a, int splits, int p
         if (n < a.l.n && base != out) out[n] = base ? base[n] : 0.0f;
         return;
     }
-    if ((int)threadIdx.x < rank) {
-        float s = 0.0f;
-        for (int p = 0; p < splits; p++) s += a.h[((int64_t)p * a.rows + t) * rank + threadIdx.x];
-        sh[threadIdx.x] = a.l.scale ? s * a.l.scale[e] : s;
-    }
-    __syncthreads();
     const int u = threadIdx.x % LP, r0 = 8 * u;
     const bool on = r0 < rank;
-    float h[8];
+    const _Float16 *B = (const _Float16 *)a.l.b + (int64_t)e * a.l.n * rank + r0;
+    constexpr int U = LP < 8 ? LP : 8, APART = 256 / LP;  // outputs of LP lanes at once; of a lane and the next
+    f16x8 w[U];
+    float own[U], h[8];
+    auto load = [&](int j0) {
+#pragma unroll
+        for (int j = 0; j < U; j++) {
+            const int64_t n = n0 + (j0 + j) * APART + threadIdx.x / LP;
+            w[j] = on && n < a.l.n ? *(const f16x8 *)(B + n * rank) : zero8();
+            own[j] = base && u == 0 && n < a.l.n ? base[n] : 0.0f;
+        }
+    };
+    float s = 0.0f;
+    if ((int)threadIdx.x < rank) {
+#pragma unroll 8
+        for (int p = 0; p < splits; p++) s += a.h[((int64_t)p * a.rows + t) * rank + threadIdx.x];
+        if (a.l.scale) s *= a.l.scale[e];
+    }
+    load(0);
+    if ((int)threadIdx.x < rank) sh[threadIdx.x] = s;
+    lds_barrier();
 #pragma unroll
     for (int i = 0; i < 8; i++) h[i] = on ? sh[r0 + i] : 0.0f;
-    const _Float16 *B = (const _Float16 *)a.l.b + (int64_t)e * a.l.n * rank + r0;
+#pragma unroll 1
+    for (int j0 = 0; j0 < LP; j0 += U) {
+        if (j0 > 0) load(j0);
 #pragma unroll
-    for (int j = 0; j < LP; j++) {
-        const int64_t n = n0 + j * (256 / LP) + threadIdx.x / LP;
-        const f16x8 w = on && n < a.l.n ? *(const f16x8 *)(B + n * rank) : zero8();
-        float s = 0.0f;
+        for (int j = 0; j < U; j++) {
+            float v = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 8; i++) s = __builtin_fmaf((float)w[i], h[i], s);
-        s = lanes_sum<LP>(s);
-        if (u == 0 && n < a.l.n) out[n] = (base ? base[n] : 0.0f) + s;
+            for (int i = 0; i < 8; i++) v = __builtin_fmaf((float)w[j][i], h[i], v);
+            v = lanes_sum<LP>(v);
+            const int64_t n = n0 + (j0 + j) * APART + threadIdx.x / LP;
+            if (u == 0 && n < a.l.n) out[n] = own[j] + v;
+        }
     }
 }
 
