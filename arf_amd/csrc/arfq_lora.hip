@@ -82,7 +82,6 @@ __global__ __launch_bounds__(256) void lora_rows_a(LoraArgs a, int splits) {
     const _Float16 *A = (const _Float16 *)a.l.a + (int64_t)e * rank * a.l.k + k;
     float *h = a.h + ((int64_t)part * a.rows + t) * rank;
     constexpr int U = 4;  // (a wave has every fourth run of as many ranks: 8 divides the rank)
-#pragma unroll 2
     for (int r0 = wave * U; r0 < rank; r0 += 4 * U) {
         f16x8 w[U];
 #pragma unroll
@@ -427,8 +426,11 @@ __global__ __launch_bounds__(64 * B_WAVES) void lora_tiles_b(LoraArgs a, int spl
     }
 }
 
-// Rows from which on tiles are faster.
-constexpr int64_t TILE_ROWS = 64;
+// rows * (k + n) from which on tiles are taken.  us one by one and in tiles, rows of two adapters in two runs / rows of 32 in any
+// order: rank 16, k + n = 12288, 256 rows 16.8 and 17.4 / 19 and 65, 512 rows 28 and 19 / 30 and 82; k + n = 22528, 128 rows
+// 17.7 and 17.7 / 19.6 and 55; rank 64, k + n = 12288, 256 rows 29 and 28 / 44 and 124; k + n = 1024, 1024 rows 11.6 and 21.
+// (The ids are on the device: the border leans to the side that loses less.)
+constexpr int64_t TILE_VALUES = 4 << 20;
 
 template <int LP>
 hipError_t rows_b(const LoraArgs &a, const LoraPlan &p, hipStream_t s) {
@@ -465,7 +467,7 @@ hipError_t tiles_b(const LoraArgs &a, const LoraPlan &p, hipStream_t s) {
 
 LoraPlan lora_plan(int cus, const arfq_lora &l, int64_t rows) {
     LoraPlan p;
-    p.tiles = rows > TILE_ROWS;
+    p.tiles = rows * (l.k + l.n) > TILE_VALUES;
     if (p.tiles) {
         // a workgroup a compute unit, and not fewer than four steps a wave
         const int64_t tiles = (rows + A_TILES * TR - 1) / (A_TILES * TR);

@@ -75,17 +75,17 @@ def rope_tolerance(out, mag, angle, f16):
 def lora(x, ids, a, b, scale, base):
     """Returns out and what its rounding goes by: sum_r |B| sum_k |A| |x|, sum_r |B| |h| and max |h| sum_r |B|, times
     |scale|."""
-    x, a, b = x.astype(np.float64), a.astype(np.float64), b.astype(np.float64)
-    rows, n = x.shape[0], b.shape[1]
+    ids, rows, n = np.asarray(ids), x.shape[0], b.shape[1]
     out = np.zeros((rows, n)) if base is None else base.astype(np.float64)
     mags = np.zeros((3, rows, n))
-    for t, e in enumerate(ids):
-        if 0 <= e < a.shape[0]:
-            s = 1.0 if scale is None else float(scale[e])
-            h, ab = a[e] @ x[t], np.abs(b[e])
-            out[t] = out[t] + s * (b[e] @ h)
-            mags[0, t], mags[1, t] = abs(s) * (ab @ (np.abs(a[e]) @ np.abs(x[t]))), abs(s) * (ab @ np.abs(h))
-            mags[2, t] = abs(s) * np.abs(h).max() * ab.sum(1)
+    for e in np.unique(ids[(ids >= 0) & (ids < a.shape[0])]):
+        t = np.flatnonzero(ids == e)
+        ae, be, xt = a[e].astype(np.float64), b[e].astype(np.float64), x[t].astype(np.float64)
+        s = 1.0 if scale is None else float(scale[e])
+        h, ab = xt @ ae.T, np.abs(be)
+        out[t] += s * (h @ be.T)
+        mags[0, t], mags[1, t] = abs(s) * (np.abs(xt) @ np.abs(ae).T @ ab.T), abs(s) * (np.abs(h) @ ab.T)
+        mags[2, t] = abs(s) * np.abs(h).max(1)[:, None] * ab.sum(1)
     return out, mags
 
 

@@ -257,6 +257,57 @@ def test_lora(gpu_ctx, xt, rank, rows, k, n):
     _lora_case(gpu_ctx, rng, rows, k, n, rank, adapters, ids, xt)
 
 
+def _runs(rng, rows, adapters):
+    """Adapters in runs of any length, from one row on; some rows with none."""
+    ids = np.concatenate([np.full(n, rng.integers(-1, adapters)) for n in rng.choice([1, 2, 15, 16, 33, 200], rows)])
+    return ids[:rows]
+
+
+# (products of so many rows that they are taken in tiles)
+@pytest.mark.parametrize("xt", [np.float32, np.float16])
+@pytest.mark.parametrize("rank", [8, 16, 24, 40, 64, 72, 136, 256])
+@pytest.mark.parametrize("k,n", [(2056, 2050), (5120, 321), (264, 7172)])
+def test_lora_many_rows(gpu_ctx, xt, rank, k, n):
+    rows = (4 << 20) // (k + n) + 19
+    _say("lora many", np.dtype(xt).name, rank, rows, k, n)
+    rng = np.random.default_rng(rank + rows + k)
+    _lora_case(gpu_ctx, rng, rows, k, n, rank, 4, _runs(rng, rows, 4), xt)
+
+
+@pytest.mark.parametrize("xt", [np.float32, np.float16])
+@pytest.mark.parametrize("scaled,based,strides", [(False, True, (0, 0)), (True, False, (0, 3)), (False, False, (0, 4)), (True, True, (8, 3)),
+                                                  (True, True, (4, 8))])
+def test_lora_many_rows_without_scale_or_base_and_with_strides(gpu_ctx, xt, scaled, based, strides):
+    _say("lora many forms", np.dtype(xt).name, scaled, based, strides)
+    rng = np.random.default_rng(5)
+    rows = (4 << 20) // (1032 + 1024) + 70
+    _lora_case(gpu_ctx, rng, rows, 1032, 1024, 16, 40, rng.integers(-2, 42, rows), xt, scaled, based, strides)
+
+
+@pytest.mark.parametrize("xt", [np.float32, np.float16])
+def test_lora_many_rows_not_finite_and_of_every_size(gpu_ctx, xt):
+    _say("lora many not finite", np.dtype(xt).name)
+    rng = np.random.default_rng(6)
+    k, n, rank, adapters = 520, 640, 16, 3
+    rows = (4 << 20) // (k + n) + 5
+    a = rng.standard_normal((adapters, rank, k)).astype(np.float16)
+    b = rng.standard_normal((adapters, n, rank)).astype(np.float16)
+    x = (rng.standard_normal((rows, k)) * 10.0 ** rng.integers(-4, 4, (rows, 1))).astype(xt)
+    ids = np.arange(rows) // 5 % adapters
+    lora = arf_amd.Lora(gpu_ctx.to_device(a), gpu_ctx.to_device(b))
+    out, d_ids = gpu_ctx.empty((rows, n), np.float32), gpu_ctx.to_device(ids.astype(np.int32))
+    gpu_ctx.lora_add(lora, d_ids, gpu_ctx.to_device(x), rows, out)
+    want, mags = stepref.lora(x, ids, a, b, None, None)
+    assert (np.abs(out.numpy() - want) <= stepref.lora_tolerance(want, mags, None, k, rank)).all()
+    a[1, 3, 5], b[2, 7, 1], x[3, 9] = np.nan, np.inf, np.inf  # (row 3 has adapter 0)
+    lora = arf_amd.Lora(gpu_ctx.to_device(a), gpu_ctx.to_device(b))
+    gpu_ctx.lora_add(lora, d_ids, gpu_ctx.to_device(x), rows, out)
+    got = out.numpy()
+    assert np.isfinite(got[(ids == 0) & (np.arange(rows) != 3)]).all() and np.isnan(got[ids == 1]).all() and not np.isfinite(got[3]).any()
+    rest = np.arange(n) != 7
+    assert np.isfinite(got[ids == 2][:, rest]).all() and not np.isfinite(got[ids == 2][:, 7]).any()
+
+
 @pytest.mark.parametrize("xt", [np.float32, np.float16])
 @pytest.mark.parametrize("rows,scaled,based,strides", [(4, False, True, (0, 0)), (4, True, False, (0, 3)), (200, False, False, (0, 4)),
                                                        (200, True, True, (8, 3)), (200, False, True, (1, 0)), (64, True, True, (5, 7))])
