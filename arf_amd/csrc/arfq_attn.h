@@ -31,10 +31,8 @@ struct Steps {
     const int32_t *table;
     int first;  // the tile of lane 0
     uint32_t lo, hi, sub;  // sub: bit 31 where the page is not the cache's
-    // through the sequence of row b of the tables (k0 a multiple of 16; max_pages > 0)
-    __device__ __forceinline__ Steps(const KvArgs &a, int b) : table(a.table + (int64_t)b * a.max_pages), first(INT32_MIN / 2) {
-        lo = hi = sub = 0;
-    }
+    // through the pages of a table, max_pages of them (k0 a multiple of 16; max_pages > 0)
+    __device__ __forceinline__ Steps(const int32_t *table) : table(table), first(INT32_MIN / 2) { lo = hi = sub = 0; }
     // The lane of the step's first tile.
     __device__ __forceinline__ int step(const KvArgs &a, int head, int k0) {
         const int t0 = k0 / KV_TILE, j = (t0 - first) / SS;

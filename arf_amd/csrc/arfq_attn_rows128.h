@@ -72,7 +72,7 @@ __device__ __forceinline__ void rows128(const AttnArgs &a, int block, uint8_t *l
     const int lo = row_lo(pos), hi = min(valid ? row_hi(pos) : 0, piece_hi);
 
     // ---- a step's K and V: from the cache to registers, and to LDS as f16 ----
-    Steps<STEP / KV_TILE> steps(a.c, it.b);
+    Steps<STEP / KV_TILE> steps(a.c.table + (int64_t)it.b * a.c.max_pages);
     const int half = wave >> 1;  // the wave's tile
     const bool is_v = wave & 1;
     const uint32_t x_off = lane * (4 * NG), s_off = is_v ? (lane >> 4) * (8 * NG) : (lane >> 2) * (2 * NG);

@@ -25,9 +25,9 @@ constexpr int WAVES = 4;  // of a workgroup
 // sequences: 27.7 us, 2.6 TB/s; 193 tokens of one: 7.3 us, all of it latency.  At 256 values and two parts 13 of the 256
 // registers go to scratch: 64 sequences of up to 8192, 32 x 256 on 4, f32, 152 us for 2.7 TB/s (f16, one part, 32 of
 // up to 4000, 16 x 256 on 8: 50 us, 4.1 TB/s; the same in f32 62, 3.0).
-// A tile's piece of K/V head `head`: it.b is the row of the tables that has its pages.
+// A tile's piece of K/V head `head`, whose pages are those of `table`.
 template <int NG, int PARTS>
-__device__ __forceinline__ void rows16_item(const AttnArgs &a, const Item &it, int head, float *lds) {
+__device__ __forceinline__ void rows16_item(const AttnArgs &a, const Item &it, const int32_t *table, int head, float *lds) {
     constexpr int D = 32 * NG, NT = 2 * NG;  // NT: 16-row tiles of O^T
     constexpr int OS = D + 4;                // LDS floats of a row of O: [WAVES][16][OS], then [WAVES][16][2]
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, h = lane >> 4;
@@ -50,7 +50,7 @@ __device__ __forceinline__ void rows16_item(const AttnArgs &a, const Item &it, i
     const int lo = row_lo(pos), hi = min(valid ? row_hi(pos) : 0, piece_hi);
 
     constexpr int NEXT = WAVES * STEP;
-    Steps<NEXT / KV_TILE> steps(a.c, it.b);
+    Steps<NEXT / KV_TILE> steps(table);
     const Offs<NG> offs = lane_offs<NG>();
     Raw<NG> r;
     int k0 = first + wave * STEP;
@@ -252,7 +252,8 @@ __device__ __forceinline__ void rows16_item(const AttnArgs &a, const Item &it, i
 template <int NG, int PARTS>
 __device__ __forceinline__ void rows16(const AttnArgs &a, int block, float *lds) {
     Item it;
-    if (take_item<TR>(a, block, it)) rows16_item<NG, PARTS>(a, it, block % a.c.heads, lds);
+    if (take_item<TR>(a, block, it))
+        rows16_item<NG, PARTS>(a, it, a.c.table + (int64_t)it.b * a.c.max_pages, block % a.c.heads, lds);
 }
 
 constexpr size_t lds_bytes(int ng) { return (size_t)WAVES * TR * (32 * ng + 4 + 2) * sizeof(float); }

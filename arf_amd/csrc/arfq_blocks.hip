@@ -13,6 +13,10 @@
 namespace arfq {
 namespace {
 
+// Chosen pages, and blocks to choose them from, up to which the attention's workgroups choose by themselves: a launch and a
+// table's way through memory less, but every piece of a row's keys looks through all of the row's blocks.
+constexpr int WIDTH_LDS = 2048, BLOCKS_LDS = 16384;
+
 // ---- rows ------------------------------------------------------------------------------------
 
 // The sequence of row t (the same in all lanes), a.batch behind the last; none of it has rows from where start
@@ -37,82 +41,113 @@ __device__ __forceinline__ int seq_of_row(const KvArgs &a, int t) {
 struct Row {
     int b, seen, end;
 };
+// Rows one after another: those of one sequence are found by its first.
+struct Rows {
+    int b = 0, t0 = 0, n = 0, len = 0;
+    __device__ __forceinline__ Row operator()(const KvArgs &a, int t) {
+        if (t < t0 || t >= t0 + n) {
+            n = 0;
+            b = seq_of_row(a, t);
+            if (b < a.batch) {
+                len = a.len[b];
+                kv_seq(a, b, t0, n);
+            }
+            if (t < t0 || t >= t0 + n) return {-1, 0, 0};
+        }
+        const int64_t pos = (int64_t)len - ((int64_t)t0 + n - t);
+        const int end = pos < 0 ? 0 : (int)min(pos + 1, (int64_t)a.max_pages * a.page);
+        return {b, (end + a.page - 1) / a.page, end};
+    }
+};
 __device__ __forceinline__ Row row_of(const KvArgs &a, int t) {
-    Row r = {-1, 0, 0};
-    const int b = seq_of_row(a, t);
-    if (b >= a.batch) return r;
-    int t0, n;
-    kv_seq(a, b, t0, n);
-    if (t < t0 || t >= t0 + n) return r;
-    r.b = b;
-    const int64_t pos = (int64_t)a.len[b] - ((int64_t)t0 + n - t);
-    r.end = pos < 0 ? 0 : (int)min(pos + 1, (int64_t)a.max_pages * a.page);
-    r.seen = (r.end + a.page - 1) / a.page;
-    return r;
+    Rows rows;
+    return rows(a, t);
 }
 
 // ---- bounds ----------------------------------------------------------------------------------
 
-// One page of a head: a lane has a dword column of K's codes (eight values of a key), 64 / (4 NG) keys side by side.
+// Keys [k0, k1) of a page of a head: a lane has a dword column of K's codes (eight values of a key), 64 / (4 NG) keys side by
+// side, and of those every one behind the last again (no branch: an extreme does not mind).  The result is in the first
+// 4 NG lanes.
 template <int NG>
-__device__ __forceinline__ void page_bounds(const KvArgs &a, int id, int head, int keys, _Float16 *bounds) {
-    constexpr int D = 32 * NG, COLS = 4 * NG, KL = WAVE / COLS;
-    const int lane = threadIdx.x & 63, kk = lane / COLS, col = lane - kk * COLS, g = col % NG, h = col / NG;
-    const uint8_t *reg = a.data + ((int64_t)id * a.heads + head) * a.region;
-    const uint32_t *codes = (const uint32_t *)reg + col;
-    const uint16_t *scales = (const uint16_t *)(reg + a.off_ks) + g;
+struct Extremes {
+    static constexpr int COLS = 4 * NG, KL = WAVE / COLS;
     float hi[8], lo[8];
-    bool nan = false;
-#pragma unroll
-    for (int e = 0; e < 8; e++) {
-        hi[e] = -INFINITY;
-        lo[e] = INFINITY;
-    }
-    if (kk < KL) {
-#pragma unroll 4
-        for (int key = kk; key < keys; key += KL) {
-            const uint32_t w = codes[key * COLS];
-            const float d = h2f(scales[key * NG]);
-            nan |= d != d;
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const float v = d * (float)((int)(w >> (4 * ((e >> 1) + 4 * (e & 1))) & 15u) - 8);
-                hi[e] = fmaxf(hi[e], v);
-                lo[e] = fminf(lo[e], v);
-            }
-        }
-    }
-    // over the keys side by side: a tree over any number of them
-    int bad = nan;
-    for (int s = KL; s > 1;) {
-        const int half = (s + 1) / 2;
-        const bool in = kk + half < s;
-        const int from = in ? lane + half * COLS : lane;
-        bad |= __shfl(bad, from);
+    int bad;  // a key that is NaN
+    __device__ __forceinline__ void add(const float (&h)[8], const float (&l)[8], int b) {
+        bad |= b;
 #pragma unroll
         for (int e = 0; e < 8; e++) {
-            hi[e] = fmaxf(hi[e], __shfl(hi[e], from));
-            lo[e] = fminf(lo[e], __shfl(lo[e], from));
+            hi[e] = fmaxf(hi[e], h[e]);
+            lo[e] = fminf(lo[e], l[e]);
         }
-        s = half;
     }
-    if (kk != 0) return;
-    _Float16 *o = bounds + ((int64_t)id * a.heads + head) * (2 * D) + 32 * g + 8 * h;
-    f16x8 vh, vl;
+    __device__ __forceinline__ Extremes(const uint8_t *reg, const KvArgs &a, int k0, int k1) : bad(0) {
+        const int lane = threadIdx.x & 63, kk = min(lane / COLS, KL - 1), col = lane % COLS, g = col % NG;
+        const uint32_t *codes = (const uint32_t *)reg + col;
+        const uint16_t *scales = (const uint16_t *)(reg + a.off_ks) + g;
 #pragma unroll
-    for (int e = 0; e < 8; e++) {
-        vh[e] = (_Float16)(bad ? NAN : hi[e]);
-        vl[e] = (_Float16)(bad ? NAN : lo[e]);
+        for (int e = 0; e < 8; e++) {
+            hi[e] = -INFINITY;
+            lo[e] = INFINITY;
+        }
+        constexpr int U = 8;
+        for (int key = k0 + kk; key < k1 + kk; key += U * KL) {
+            uint32_t w[U];
+            uint16_t d[U];
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const int at = min(key + u * KL, k1 - 1);
+                w[u] = codes[at * COLS];
+                d[u] = scales[at * NG];
+            }
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const float f = h2f(d[u]);
+                bad |= f != f;
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const float v = f * (float)((int)(w[u] >> (4 * ((e >> 1) + 4 * (e & 1))) & 15u) - 8);
+                    hi[e] = fmaxf(hi[e], v);
+                    lo[e] = fminf(lo[e], v);
+                }
+            }
+        }
+        // over the keys side by side: a tree over any number of them
+#pragma unroll
+        for (int s = KL; s > 1;) {
+            const int half = (s + 1) / 2, from = kk + half < s ? lane + half * COLS : lane;
+            float h[8], l[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                h[e] = __shfl(hi[e], from);
+                l[e] = __shfl(lo[e], from);
+            }
+            add(h, l, __shfl(bad, from));
+            s = half;
+        }
     }
-    *(f16x8 *)o = vh;
-    *(f16x8 *)(o + D) = vl;
-}
+    __device__ __forceinline__ void store(_Float16 *bounds) const {
+        const int lane = threadIdx.x & 63, g = lane % NG, h = lane / NG;
+        f16x8 vh, vl;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            vh[e] = (_Float16)(bad ? NAN : hi[e]);
+            vl[e] = (_Float16)(bad ? NAN : lo[e]);
+        }
+        *(f16x8 *)(bounds + 32 * g + 8 * h) = vh;
+        *(f16x8 *)(bounds + 32 * NG + 32 * g + 8 * h) = vl;
+    }
+};
 
-// A wave: `per` rows of a head, and of those the pages that begin with one of them, or in which a sequence's first one
-// lies.
-template <int NG>
+// `per` rows of a head, and of those the pages that begin with one of them, or in which a sequence's first one lies.  By a
+// wave, or (WIDE) by a workgroup whose waves share a page's keys.
+template <int NG, bool WIDE>
 __global__ __launch_bounds__(256) void kv_bounds_kernel(KvArgs a, _Float16 *bounds, int per, int items) {
-    const int item = __builtin_amdgcn_readfirstlane(block_of() * 4 + (int)(threadIdx.x >> 6));
+    constexpr int COLS = 4 * NG;
+    __shared__ float sh[WIDE ? 3 : 1][COLS][17];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const int item = WIDE ? block_of() : block_of() * 4 + wave;
     if (item >= items) return;
     const int head = item % a.heads, row0 = item / a.heads * per, row1 = min(row0 + per, a.tokens);
     for (int b = seq_of_row(a, row0); b < a.batch; b++) {
@@ -126,18 +161,55 @@ __global__ __launch_bounds__(256) void kv_bounds_kernel(KvArgs a, _Float16 *boun
         const int64_t p1 = pos1 < 0 ? -1 : min(pos1 / a.page, (int64_t)a.max_pages - 1);
         for (int64_t p = p0; p <= p1; p++) {
             const int id = a.table[(int64_t)b * a.max_pages + p];
-            if ((uint32_t)id < (uint32_t)a.n_pages) page_bounds<NG>(a, id, head, (int)min((int64_t)a.page, len - p * a.page), bounds);
+            if ((uint32_t)id >= (uint32_t)a.n_pages) continue;
+            const uint8_t *reg = a.data + ((int64_t)id * a.heads + head) * a.region;
+            _Float16 *out = bounds + ((int64_t)id * a.heads + head) * (64 * NG);
+            const int keys = (int)min((int64_t)a.page, len - p * a.page);
+            if constexpr (WIDE) {
+                const int share = a.page / 4, k0 = min(wave * share, keys - 1);
+                Extremes<NG> x(reg, a, k0, min(k0 + share, keys));
+                if (wave && lane < COLS) {
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        sh[wave - 1][lane][e] = x.hi[e];
+                        sh[wave - 1][lane][8 + e] = x.lo[e];
+                    }
+                    sh[wave - 1][lane][16] = (float)x.bad;
+                }
+                __syncthreads();
+                if (wave == 0 && lane < COLS) {
+#pragma unroll
+                    for (int w = 0; w < 3; w++) {
+                        float h[8], l[8];
+#pragma unroll
+                        for (int e = 0; e < 8; e++) {
+                            h[e] = sh[w][lane][e];
+                            l[e] = sh[w][lane][8 + e];
+                        }
+                        x.add(h, l, sh[w][lane][16] != 0.0f);
+                    }
+                    x.store(out);
+                }
+                __syncthreads();
+            } else {
+                const Extremes<NG> x(reg, a, 0, keys);
+                if (lane < COLS) x.store(out);
+            }
         }
     }
 }
 
 template <int NG>
 hipError_t bounds_launch(const KvArgs &a, _Float16 *bounds, int cus, hipStream_t s) {
-    // rows of a wave: one while that does not fill the chip several times over
     const int64_t rows = (int64_t)a.tokens * a.heads;
+    if (rows <= 2 * (int64_t)cus) {
+        kv_bounds_kernel<NG, true><<<grid_of(rows), 256, 0, s>>>(a, bounds, 1, (int)rows);
+        return hipGetLastError();
+    }
+    // rows of a wave: one while that does not fill the chip several times over
     const int per = (int)std::min<int64_t>(std::max<int64_t>(rows / (64 * (int64_t)cus), 1), 64);
     const int64_t items = ((int64_t)a.tokens + per - 1) / per * a.heads;
-    kv_bounds_kernel<NG><<<grid_of((items + 3) / 4), 256, 0, s>>>(a, bounds, per, (int)items);
+    kv_bounds_kernel<NG, false><<<grid_of((items + 3) / 4), 256, 0, s>>>(a, bounds, per, (int)items);
     return hipGetLastError();
 }
 
@@ -189,8 +261,9 @@ __global__ __launch_bounds__(256) void blocks_score(ScoreArgs a) {
     const int rt = c / a.group;  // (0 where the group has more than 16 heads)
     Row mine = {-1, 0, 0};
     int most = 0;  // blocks of the tile's rows
+    Rows rows;
     for (int r = 0; r < a.per_tile && row0 + r < a.rows; r++) {
-        const Row x = row_of(kv, a.row0 + row0 + r);
+        const Row x = rows(kv, a.row0 + row0 + r);
         if (rt == r) mine = x;
         if (x.seen > a.count) most = max(most, x.seen);
     }
@@ -235,25 +308,40 @@ __global__ __launch_bounds__(256) void blocks_score(ScoreArgs a) {
 #pragma unroll
                     for (int i = 0; i < DL; i++) q[i] = -q[i];
             }
-            for (int j = j0; j < last; j += 16) {
-                const int id = j + c < last ? table[j + c] : -1;
+            // bounds a tile ahead of their use, pages two (at 256 channels the registers leave no room for it)
+            constexpr bool AHEAD = NG <= 4;
+            f16x8 hi[DL / 8], lo[DL / 8];
+            auto page_of = [&](int j) { return table[min(j + c, last - 1)]; };
+            auto load = [&](int id) {
                 const bool page = (uint32_t)id < (uint32_t)kv.n_pages;
                 const _Float16 *p = a.bounds + ((int64_t)(page ? id : 0) * kv.heads + head) * (2 * D) + DL * kg;
-                f64x4 up = {0, 0, 0, 0}, down = {0, 0, 0, 0};
 #pragma unroll
-                for (int i = 0; i < DL; i += 8) {
-                    f16x8 hi = {0, 0, 0, 0, 0, 0, 0, 0}, lo = hi;
-                    if (page) {
-                        hi = *(const f16x8 *)(p + i);
-                        lo = *(const f16x8 *)(p + D + i);
-                    }
-#pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        const float v = q[i + e];  // (NaN goes into the first)
-                        up = __builtin_amdgcn_mfma_f64_16x16x4f64((double)(float)hi[e], (double)(v < 0.0f ? 0.0f : v), up, 0, 0, 0);
-                        down = __builtin_amdgcn_mfma_f64_16x16x4f64((double)(float)lo[e], (double)(v < 0.0f ? v : 0.0f), down, 0, 0, 0);
-                    }
+                for (int i = 0; i < DL / 8; i++) {
+                    hi[i] = *(const f16x8 *)(p + 8 * i);
+                    lo[i] = *(const f16x8 *)(p + D + 8 * i);
                 }
+            };
+            int id = page_of(j0), id1 = page_of(j0 + 16);
+            load(id);
+            for (int j = j0; j < last; j += 16) {
+                const bool page = (uint32_t)id < (uint32_t)kv.n_pages;
+                f64x4 up = {0, 0, 0, 0}, down = {0, 0, 0, 0};
+                f16x8 h[DL / 8], l[DL / 8];
+#pragma unroll
+                for (int i = 0; i < DL / 8; i++) {
+                    h[i] = hi[i];
+                    l[i] = lo[i];
+                }
+                if (AHEAD && j + 16 < last) load(id1);
+                id = id1;
+                id1 = page_of(j + 32);
+#pragma unroll
+                for (int i = 0; i < DL; i++) {
+                    const float v = q[i];  // (NaN goes into the first)
+                    up = __builtin_amdgcn_mfma_f64_16x16x4f64((double)(float)h[i / 8][i % 8], (double)(v < 0.0f ? 0.0f : v), up, 0, 0, 0);
+                    down = __builtin_amdgcn_mfma_f64_16x16x4f64((double)(float)l[i / 8][i % 8], (double)(v < 0.0f ? v : 0.0f), down, 0, 0, 0);
+                }
+                if (!AHEAD && j + 16 < last) load(id);
                 // a lane's four results: blocks kg, kg + 4, .. of the 16, its column
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
@@ -278,210 +366,273 @@ __global__ __launch_bounds__(256) void blocks_score(ScoreArgs a) {
 
 // ---- choice ----------------------------------------------------------------------------------
 
-struct SelectArgs {
-    KvArgs c;
-    int row0, rows, count, first, last, width;
-    const uint64_t *keys;
-    int32_t *table;   // [rows][heads][width]: pages
-    int32_t *chosen;  // of the whole call, or null
+constexpr int SEL = 256, SEL_WAVES = SEL / WAVE;
+struct SelLds {
+    uint32_t bins[256], found[3], sums[2][SEL_WAVES];
 };
 
-constexpr int SEL = 256, SEL_WAVES = SEL / WAVE;
-
-template <class T, class F>
-__device__ __forceinline__ T wave_all(T v, F f) {
-#pragma unroll
-    for (int d = 1; d < WAVE; d *= 2) v = f(v, (T)__shfl_xor(v, d));
-    return v;
+// Largest value and running sum over a wave's lanes, and over the workgroup's threads (sh is free again behind the next
+// barrier).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t lane_of(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false);
 }
+template <class F>
+__device__ __forceinline__ uint32_t wave_run(uint32_t v, F f) {
+    v = f(v, lane_of<0x111, 0xf>(v));  // row_shr:1, 2, 4, 8
+    v = f(v, lane_of<0x112, 0xf>(v));
+    v = f(v, lane_of<0x114, 0xf>(v));
+    v = f(v, lane_of<0x118, 0xf>(v));
+    v = f(v, lane_of<0x142, 0xa>(v));  // row_bcast:15 into rows 1 and 3
+    return f(v, lane_of<0x143, 0xc>(v));  // row_bcast:31 into rows 2 and 3
+}
+__device__ __forceinline__ uint32_t run_sum(uint32_t v) { return wave_run(v, [](uint32_t x, uint32_t y) { return x + y; }); }
+__device__ __forceinline__ uint32_t run_max(uint32_t v) { return wave_run(v, [](uint32_t x, uint32_t y) { return max(x, y); }); }
 
-// A workgroup: a row and K/V head.  A thread has a run of neighbouring blocks.  The keys' range [lo, hi] that the
-// last chosen one lies in is cut into 256 parts and counted, until a part's keys are all chosen or all alike.
-__global__ __launch_bounds__(SEL) void blocks_select(SelectArgs a) {
-    __shared__ uint32_t bins[256];
-    __shared__ unsigned long long wlo[SEL_WAVES], whi[SEL_WAVES];
-    __shared__ uint32_t found[3], sums[2][SEL_WAVES];
-    const KvArgs &kv = a.c;
-    const int block = block_of(), head = block % kv.heads, row = block / kv.heads, tid = threadIdx.x;
-    if (row >= a.rows) return;
-    const Row r = row_of(kv, a.row0 + row);
-    if (r.b < 0) return;
-    const int32_t *pages = kv.table + (int64_t)r.b * kv.max_pages;
-    const int64_t at = (int64_t)row * kv.heads + head;
-    int32_t *table = a.table + at * a.width;
-    int32_t *chosen = a.chosen ? a.chosen + (((int64_t)a.row0 + row) * kv.heads + head) * a.count : nullptr;
-    const int n = r.seen, most = min(n, a.count);
-    auto take = [&](int rank, int j) {
-        table[rank] = pages[j];
-        if (chosen) chosen[rank] = j;
-    };
-    if (chosen)
-        for (int i = most + tid; i < a.count; i += SEL) chosen[i] = -1;
-    if (n <= a.count) {
-        for (int j = tid; j < n; j += SEL) take(j, j);
-        return;
-    }
-    const uint64_t *keys = a.keys + at * kv.max_pages;
-    const int per = (n + SEL - 1) / SEL, j0 = min(tid * per, n), j1 = min(j0 + per, n);
-    const int f0 = a.first, f1 = n - a.last;  // blocks [f0, f1) go by their scores
-    constexpr int KEPT = 8;  // keys in registers
-    uint64_t kept[KEPT];
+// The `count` blocks of n that are chosen: the `first` earliest, the `last` latest, and of the others those with the largest
+// keys, the earlier one of two alike; in their order.  A thread has a run of neighbouring blocks.  The
+// range of the keys' upper halves that the last chosen one lies in is cut into 256 parts and counted, until a
+// part's keys are all chosen or all alike; then, where they are alike, that of their lower halves.  (n > count, the
+// workgroup's threads all come here.)  take(rank, block, page).
+// most: places of keys and pages.
+constexpr int KEPT = 8;  // keys of a thread in registers
+struct Kept {
+    uint64_t key[KEPT];
+    // (before n is known: the loads do not wait for it)
+    __device__ __forceinline__ Kept(const uint64_t *keys, int most) {
+        if (most == 0) return;  // (all blocks are chosen)
+        const int j0 = threadIdx.x * ((most + SEL - 1) / SEL);
 #pragma unroll
-    for (int i = 0; i < KEPT; i++) kept[i] = j0 + i < j1 ? keys[j0 + i] : 0;
+        for (int i = 0; i < KEPT; i++) key[i] = keys[min(j0 + i, most - 1)];
+    }
+};
+template <class Take>
+__device__ __forceinline__ void choose(const uint64_t *keys, const Kept &kept, const int32_t *pages, int most, int n, int count,
+                                       int first, int last, SelLds &sh, Take take) {
+    const int tid = threadIdx.x, wave = tid >> 6;
+    const int per = (most + SEL - 1) / SEL, j0 = min(tid * per, n), j1 = min(j0 + per, n);
+    const int f0 = first, f1 = n - last;  // blocks [f0, f1) go by their keys
+    int32_t page[KEPT];
+#pragma unroll
+    for (int i = 0; i < KEPT; i++) page[i] = pages[min(j0 + i, n - 1)];
     auto each = [&](auto f) {  // f(block, key)
 #pragma unroll
         for (int i = 0; i < KEPT; i++)
-            if (j0 + i < j1) f(j0 + i, kept[i]);
+            if (j0 + i < j1) f(j0 + i, kept.key[i]);
         for (int j = j0 + KEPT; j < j1; j++) f(j, keys[j]);
     };
-    unsigned long long lo = ~0ull, hi = 0;
-    each([&](int j, uint64_t key) {
-        if (j < f0 || j >= f1) return;
-        lo = min(lo, (unsigned long long)key);
-        hi = max(hi, (unsigned long long)key);
-    });
-    lo = wave_all(lo, [](unsigned long long x, unsigned long long y) { return min(x, y); });
-    hi = wave_all(hi, [](unsigned long long x, unsigned long long y) { return max(x, y); });
-    if ((tid & 63) == 0) {
-        wlo[tid >> 6] = lo;
-        whi[tid >> 6] = hi;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < SEL_WAVES; w++) {
-        lo = min(lo, wlo[w]);
-        hi = max(hi, whi[w]);
-    }
-    // the `need` largest of the keys in [lo, hi]; those above hi are chosen
-    uint32_t need = (uint32_t)(a.count - a.first - a.last);
-    bool all = need == 0;
-    while (need > 0 && lo < hi) {
-        const int bits = 64 - __clzll((long long)(hi - lo)), shift = max(bits - 8, 0);
-        bins[tid] = 0;
-        __syncthreads();
+    sh.bins[tid] = 0;
+    // The `need` largest of the candidates' words: all from `at` on (true), or those above `at` and `need` more of those that
+    // are `at`.
+    auto narrow = [&](auto word, auto candidate, uint32_t &need, uint32_t &at) {
+        uint32_t hi = 0, not_lo = 0;
         each([&](int j, uint64_t key) {
-            if (j >= f0 && j < f1 && key >= lo && key <= hi) atomicAdd(&bins[(key - lo) >> shift], 1u);
+            if (!candidate(j, key)) return;
+            hi = max(hi, word(key));
+            not_lo = max(not_lo, ~word(key));
         });
+        hi = run_max(hi);
+        not_lo = run_max(not_lo);
+        if ((tid & 63) == 63) {
+            sh.sums[0][wave] = hi;
+            sh.sums[1][wave] = not_lo;
+        }
         __syncthreads();
-        // the part that the last chosen key lies in: 256 counts summed from the top
-        const uint32_t mine = bins[255 - tid];
-        uint32_t inc = mine;
+        hi = not_lo = 0;
 #pragma unroll
-        for (int d = 1; d < WAVE; d *= 2) {
-            const uint32_t u = __shfl_up(inc, d);
-            if ((tid & 63) >= d) inc += u;
+        for (int w = 0; w < SEL_WAVES; w++) {
+            hi = max(hi, sh.sums[0][w]);
+            not_lo = max(not_lo, sh.sums[1][w]);
         }
-        if ((tid & 63) == 63) sums[0][tid >> 6] = inc;
-        __syncthreads();
-        for (int w = 0; w < (tid >> 6); w++) inc += sums[0][w];
-        if (inc >= need && inc - mine < need) {
-            found[0] = 255 - tid;
-            found[1] = need - (inc - mine);
-            found[2] = mine;
+        uint32_t lo = ~not_lo;
+        bool all = false;
+        while (lo < hi) {
+            const int shift = max(24 - __clz((int)(hi - lo)), 0);
+            each([&](int j, uint64_t key) {
+                if (candidate(j, key) && word(key) >= lo && word(key) <= hi) atomicAdd(&sh.bins[(word(key) - lo) >> shift], 1u);
+            });
+            __syncthreads();
+            // the part that the last chosen one lies in: 256 counts summed from the top
+            const uint32_t mine = sh.bins[255 - tid];
+            sh.bins[255 - tid] = 0;
+            uint32_t upto = run_sum(mine);
+            if ((tid & 63) == 63) sh.sums[0][wave] = upto;
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < SEL_WAVES - 1; w++) upto += w < wave ? sh.sums[0][w] : 0;
+            if (upto >= need && upto - mine < need) {
+                sh.found[0] = 255 - tid;
+                sh.found[1] = need - (upto - mine);
+                sh.found[2] = mine;
+            }
+            __syncthreads();
+            const uint32_t wide = (1u << shift) - 1;
+            need = sh.found[1];
+            lo += sh.found[0] << shift;
+            if (hi - lo > wide) hi = lo + wide;
+            all = sh.found[2] == need;
+            if (all) break;
         }
-        __syncthreads();
-        const unsigned long long part = found[0];
-        need = found[1];
-        all = found[2] == need;
-        lo += part << shift;
-        const unsigned long long wide = (1ull << shift) - 1;
-        if (hi - lo > wide) hi = lo + wide;
-        if (all) break;
+        at = lo;
+        return all;
+    };
+    auto upper = [](uint64_t key) { return (uint32_t)(key >> 32); };
+    auto lower = [](uint64_t key) { return (uint32_t)key; };
+    uint32_t need = (uint32_t)(count - first - last), at = ~0u, at_lower = ~0u;
+    bool all = false, all_lower = false;
+    if (need > 0) {
+        all = narrow(upper, [&](int j, uint64_t) { return j >= f0 && j < f1; }, need, at);
+        if (!all) {
+            __syncthreads();  // (the sums' places)
+            all_lower = narrow(lower, [&](int j, uint64_t key) { return j >= f0 && j < f1 && upper(key) == at; }, need, at_lower);
+        }
     }
-    // chosen: by rule, keys above hi, with `all` those from lo on, otherwise the `need` first of those that are lo
+    auto is_sure = [&](int j, uint64_t key) {
+        const uint32_t u = upper(key), l = lower(key);
+        return j < f0 || j >= f1 || u > at || (u == at && (all || l > at_lower || (all_lower && l == at_lower)));
+    };
+    auto is_tie = [&](int j, uint64_t key) {
+        return j >= f0 && j < f1 && !all && !all_lower && upper(key) == at && lower(key) == at_lower;
+    };
     uint32_t sure = 0, ties = 0;
-    auto is_sure = [&](int j, uint64_t key) { return j < f0 || j >= f1 || key > hi || (all && need > 0 && key >= lo); };
-    auto is_tie = [&](int j, uint64_t key) { return !all && j >= f0 && j < f1 && key == lo; };
     each([&](int j, uint64_t key) {
         sure += is_sure(j, key);
         ties += is_tie(j, key);
     });
-    uint32_t sure_inc = sure, ties_inc = ties;
-#pragma unroll
-    for (int d = 1; d < WAVE; d *= 2) {
-        const uint32_t u = __shfl_up(sure_inc, d), v = __shfl_up(ties_inc, d);
-        if ((tid & 63) >= d) {
-            sure_inc += u;
-            ties_inc += v;
-        }
-    }
+    uint32_t before = run_sum(sure), tie = run_sum(ties);
     __syncthreads();
     if ((tid & 63) == 63) {
-        sums[0][tid >> 6] = sure_inc;
-        sums[1][tid >> 6] = ties_inc;
+        sh.sums[0][wave] = before;
+        sh.sums[1][wave] = tie;
     }
     __syncthreads();
-    for (int w = 0; w < (tid >> 6); w++) {
-        sure_inc += sums[0][w];
-        ties_inc += sums[1][w];
+#pragma unroll
+    for (int w = 0; w < SEL_WAVES - 1; w++) {
+        before += w < wave ? sh.sums[0][w] : 0;
+        tie += w < wave ? sh.sums[1][w] : 0;
     }
-    uint32_t before = sure_inc - sure, tie = ties_inc - ties;
-    each([&](int j, uint64_t key) {
+    before -= sure;
+    tie -= ties;
+    auto step = [&](int j, uint64_t key, auto page) {
         const bool s = is_sure(j, key), e = is_tie(j, key);
         const uint32_t rank = before + min(tie, need);
-        if ((s || (e && tie < need)) && rank < (uint32_t)most) take((int)rank, j);
+        if ((s || (e && tie < need)) && rank < (uint32_t)count) take((int)rank, j, page());
         before += s;
         tie += e;
-    });
+    };
+#pragma unroll
+    for (int i = 0; i < KEPT; i++)
+        if (j0 + i < j1) step(j0 + i, kept.key[i], [&] { return page[i]; });
+    for (int j = j0 + KEPT; j < j1; j++) step(j, keys[j], [&] { return pages[j]; });
+}
+
+// What a row chooses.  A row's pages of a K/V head are put into `table` (LDS or memory); `write`: its blocks into chosen, too.
+struct ChooseArgs {
+    KvArgs c;
+    const uint64_t *keys;  // [rows][heads][max_pages] of the chunk
+    int32_t *table;        // [rows][heads][width], or null: in the workgroups' LDS
+    int32_t *chosen;       // [tokens][heads][count] of the call, or null
+    int row0, rows, count, first, last, width;
+};
+__device__ __forceinline__ const uint64_t *keys_of(const ChooseArgs &a, int row, int head) {
+    return a.keys + ((int64_t)row * a.c.heads + head) * a.c.max_pages;
+}
+__device__ __forceinline__ void choose_row(const ChooseArgs &a, const Row &r, const Kept &kept, int row, int head, int32_t *table,
+                                           bool write, SelLds &sh) {
+    const int32_t *pages = a.c.table + (int64_t)r.b * a.c.max_pages;
+    int32_t *chosen = a.chosen && write ? a.chosen + (((int64_t)a.row0 + row) * a.c.heads + head) * a.count : nullptr;
+    auto take = [&](int rank, int j, int32_t page) {
+        table[rank] = page;
+        if (chosen) chosen[rank] = j;
+    };
+    if (r.seen <= a.count) {
+        for (int j = threadIdx.x; j < r.seen; j += SEL) take(j, j, pages[j]);
+    } else {
+        choose(keys_of(a, row, head), kept, pages, a.c.max_pages, r.seen, a.count, a.first, a.last, sh, take);
+    }
+    if (chosen)
+        for (int i = min(r.seen, a.count) + (int)threadIdx.x; i < a.count; i += SEL) chosen[i] = -1;
+}
+
+__global__ __launch_bounds__(SEL) void blocks_select(ChooseArgs a) {
+    __shared__ SelLds sh;
+    const int block = block_of(), head = block % a.c.heads, row = block / a.c.heads;
+    if (row >= a.rows) return;
+    const Kept kept(keys_of(a, row, head), a.c.max_pages > a.count ? a.c.max_pages : 0);
+    const Row r = row_of(a.c, a.row0 + row);
+    if (r.b < 0) return;
+    choose_row(a, r, kept, row, head, a.table + ((int64_t)row * a.c.heads + head) * a.width, true, sh);
 }
 
 // ---- attention -------------------------------------------------------------------------------
 
-// A row as a sequence of its own, whose pages are the chosen ones: all but its own are whole.
+// A row is a sequence of its own, whose pages are the chosen ones: all but its own, the last, are whole.
 struct RowsArgs {
-    AttnArgs a;   // c.table and c.max_pages: the chosen pages
-    int most;     // of the call's tables: max_pages
-    int count, row0, rows, tiles, pieces;
+    AttnArgs a;       // max_pages: chosen pages
+    ChooseArgs ch;
+    int tiles, pieces;
 };
-__device__ __forceinline__ int chosen_keys(const RowsArgs &r, int t) {
-    KvArgs c = r.a.c;
-    c.max_pages = r.most;
-    const Row x = row_of(c, t);
-    if (x.b < 0) return -1;
-    return x.end - max(x.seen - r.count, 0) * c.page;
-}
-__device__ __forceinline__ int pieces_of(const RowsArgs &r, int keys) { return max(1, min(r.pieces, (keys + MIN_PIECE - 1) / MIN_PIECE)); }
+struct RowItem {
+    Row r;
+    int row, tile, piece, pieces, keys, part;
+    __device__ __forceinline__ RowItem(const RowsArgs &a, int slot) : part(slot) {
+        piece = slot % a.pieces;
+        tile = slot / a.pieces % a.tiles;
+        row = slot / a.pieces / a.tiles;
+        r = {-1, 0, 0};
+        if (row < a.ch.rows) r = row_of(a.ch.c, a.ch.row0 + row);
+        keys = r.end - max(r.seen - a.ch.count, 0) * a.ch.c.page;
+        pieces = max(1, min(a.pieces, (keys + MIN_PIECE - 1) / MIN_PIECE));
+    }
+    __device__ __forceinline__ bool none() const { return r.b < 0 || piece >= pieces; }
+};
 
-template <int NG, int PARTS>
+// CHOOSE: every workgroup chooses for itself, into its LDS (behind the tile's).
+template <int NG, int PARTS, bool CHOOSE>
 __global__ __launch_bounds__(256, rows16_waves(NG)) void blocks_attend(RowsArgs r) {
     extern __shared__ float lds[];
-    int block = block_of();
-    const int head = block % r.a.c.heads;
-    block /= r.a.c.heads;
-    const int piece = block % r.pieces, tile = block / r.pieces % r.tiles, row = block / r.pieces / r.tiles;
-    if (row >= r.rows) return;
-    const int keys = chosen_keys(r, r.row0 + row);
+    __shared__ SelLds sh;
+    const int block = block_of(), head = block % r.a.c.heads, slot = block / r.a.c.heads;
+    const Kept kept(keys_of(r.ch, min(slot / r.pieces / r.tiles, r.ch.rows - 1), head), CHOOSE && r.ch.c.max_pages > r.ch.count ? r.ch.c.max_pages : 0);
+    const RowItem x(r, slot);
+    if (x.none()) return;
+    const int32_t *table;
+    if constexpr (CHOOSE) {
+        int32_t *own = (int32_t *)((uint8_t *)lds + rows16_k::lds_bytes(NG));
+        choose_row(r.ch, x.r, kept, x.row, head, own, x.tile == 0 && x.piece == 0, sh);
+        __syncthreads();
+        table = own;
+    } else {
+        table = r.ch.table + ((int64_t)x.row * r.a.c.heads + head) * r.ch.width;
+    }
     Item it;
-    it.pieces = pieces_of(r, keys);
-    if (keys < 0 || piece >= it.pieces) return;
-    it.s = {r.row0 + row, 1, keys, 0, keys, r.tiles};
-    it.b = row * r.a.c.heads + head;
-    it.tile = tile;
-    it.piece = piece;
-    it.keys = ((keys + STEP - 1) / STEP + it.pieces - 1) / it.pieces * STEP;
-    it.cut = 0;
-    it.part = (row * r.tiles + tile) * r.pieces + piece;
-    rows16_k::rows16_item<NG, PARTS>(r.a, it, head, lds);
+    it.s = {r.ch.row0 + x.row, 1, x.keys, 0, x.keys, r.tiles};
+    it.b = it.cut = 0;
+    it.tile = x.tile;
+    it.piece = x.piece;
+    it.pieces = x.pieces;
+    it.keys = ((x.keys + STEP - 1) / STEP + x.pieces - 1) / x.pieces * STEP;
+    it.part = x.part;
+    rows16_k::rows16_item<NG, PARTS>(r.a, it, table, head, lds);
 }
 
 template <int NG>
 __global__ __launch_bounds__(256) void blocks_join(RowsArgs r) {
     __shared__ JoinLds<NG> sh;
     const int block = block_of(), head = block % r.a.c.heads, slot = block / r.a.c.heads;
-    const int piece = slot % r.pieces, tile = slot / r.pieces % r.tiles, row = slot / r.pieces / r.tiles;
-    if (row >= r.rows) return;
-    const int keys = chosen_keys(r, r.row0 + row), pieces = pieces_of(r, keys);
-    if (keys < 0 || pieces == 1 || piece >= pieces) return;
-    join_tile<NG, 16>(r.a, r.a.few, make_int4(pieces | piece << 16, tile * 16, r.a.group, r.row0 + row), slot, head, sh);
+    const RowItem x(r, slot);
+    if (x.none() || x.pieces == 1) return;
+    join_tile<NG, 16>(r.a, r.a.few, make_int4(x.pieces | x.piece << 16, x.tile * 16, r.a.group, r.ch.row0 + x.row), slot, head, sh);
 }
 
-template <int NG, int PARTS>
+template <int NG, int PARTS, bool CHOOSE>
 hipError_t attend_launch(const RowsArgs &r, hipStream_t s) {
     static std::atomic<uint64_t> done{0};
     constexpr size_t lds = rows16_k::lds_bytes(NG);
-    const hipError_t e = set_max_lds_once((const void *)blocks_attend<NG, PARTS>, lds, done);
+    const size_t all = lds + (CHOOSE ? (size_t)r.ch.width * sizeof(int32_t) : 0);
+    const hipError_t e = set_max_lds_once((const void *)blocks_attend<NG, PARTS, CHOOSE>, lds + (CHOOSE ? WIDTH_LDS * sizeof(int32_t) : 0), done);
     if (e != hipSuccess) return e;
-    blocks_attend<NG, PARTS><<<grid_of((int64_t)r.rows * r.tiles * r.pieces * r.a.c.heads), 256, lds, s>>>(r);
+    blocks_attend<NG, PARTS, CHOOSE><<<grid_of((int64_t)r.ch.rows * r.tiles * r.pieces * r.a.c.heads), 256, all, s>>>(r);
     return hipGetLastError();
 }
 
@@ -496,7 +647,6 @@ template <int NG>
 hipError_t dim_launch(const BlocksArgs &b, const BlocksPlan &p, int cus, hipStream_t s) {
     const KvArgs &c = b.a.c;
     uint64_t *keys = (uint64_t *)b.ws;
-    int32_t *table = (int32_t *)(b.ws + p.off_table);
     const bool f16 = b.a.q_dtype == ARFQ_F16 && b.a.out_dtype == ARFQ_F16;
     for (int row0 = 0; row0 < c.tokens; row0 += p.rows) {
         const int rows = std::min(p.rows, c.tokens - row0);
@@ -511,16 +661,16 @@ hipError_t dim_launch(const BlocksArgs &b, const BlocksPlan &p, int cus, hipStre
             blocks_score<NG><<<grid_of(tiles * parts), 256, 0, s>>>(sc);
             if ((e = hipGetLastError()) != hipSuccess) return e;
         }
-        const SelectArgs sel = {c, row0, rows, b.count, b.first, b.last, p.width, keys, table, b.chosen};
-        blocks_select<<<grid_of((int64_t)rows * c.heads), SEL, 0, s>>>(sel);
-        if ((e = hipGetLastError()) != hipSuccess) return e;
-        RowsArgs r = {b.a, c.max_pages, b.count, row0, rows, p.tiles, p.pieces};
-        r.a.c.table = table;
+        const ChooseArgs ch = {c, keys, p.in_lds ? nullptr : (int32_t *)(b.ws + p.off_table), b.chosen, row0, rows, b.count, b.first, b.last, p.width};
+        if (!p.in_lds) {
+            blocks_select<<<grid_of((int64_t)rows * c.heads), SEL, 0, s>>>(ch);
+            if ((e = hipGetLastError()) != hipSuccess) return e;
+        }
+        RowsArgs r = {b.a, ch, p.tiles, p.pieces};
         r.a.c.max_pages = p.width;
-        r.a.causal = 1;
-        r.a.window = 0;
         r.a.few = {1, 0, rows * p.tiles * p.pieces, 1, (float *)(b.ws + p.off_part), nullptr};
-        e = f16 ? attend_launch<NG, 1>(r, s) : attend_launch<NG, 2>(r, s);
+        e = p.in_lds ? f16 ? attend_launch<NG, 1, true>(r, s) : attend_launch<NG, 2, true>(r, s)
+                     : f16 ? attend_launch<NG, 1, false>(r, s) : attend_launch<NG, 2, false>(r, s);
         if (e != hipSuccess) return e;
         if (p.pieces > 1) {
             blocks_join<NG><<<grid_of((int64_t)rows * p.tiles * p.pieces * c.heads), 256, 0, s>>>(r);
@@ -550,8 +700,9 @@ BlocksPlan blocks_plan(int cus, int heads, int dim, int page, int64_t tokens, in
     const int64_t group = q_heads / heads;
     p.tiles = (int)((group + 15) / 16);
     p.width = (int)std::max<int64_t>(1, std::min(count, max_pages));
-    const int64_t keys = max_pages > count ? heads * max_pages * 8 : 0, table = (int64_t)heads * p.width * 4;
-    p.rows = (int)std::min<int64_t>(std::max<int64_t>(CHUNK_BYTES / (keys + table), 1), std::max<int64_t>(tokens, 1));
+    p.in_lds = p.width <= WIDTH_LDS && max_pages <= BLOCKS_LDS;
+    const int64_t keys = max_pages > count ? heads * max_pages * 8 : 0, table = p.in_lds ? 0 : (int64_t)heads * p.width * 4;
+    p.rows = (int)std::min<int64_t>(keys + table ? std::max<int64_t>(CHUNK_BYTES / (keys + table), 1) : INT32_MAX, std::max<int64_t>(tokens, 1));
     const int64_t items = (int64_t)p.rows * heads * p.tiles, target = (int64_t)rows16_waves(dim / KV_GROUP) * cus;
     const int64_t most = std::min((p.width * (int64_t)page + MIN_PIECE - 1) / MIN_PIECE, (int64_t)0x7fff);
     p.pieces = (int)std::min(std::max<int64_t>(target / items, 1), most);

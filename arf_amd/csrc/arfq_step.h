@@ -58,6 +58,7 @@ struct BlocksPlan {
     int tiles = 1;    // 16-row tiles of a row's group of q heads
     int pieces = 1;   // of a row's keys, at most
     int width = 0;    // chosen blocks of a row: min(count, max_pages)
+    bool in_lds = false;  // the attention's workgroups choose, each for itself
     size_t off_table = 0, off_part = 0, ws_bytes = 0;
 };
 BlocksPlan blocks_plan(int cus, int heads, int dim, int page, int64_t tokens, int q_heads, int64_t max_pages, int64_t count);
