@@ -215,6 +215,7 @@ hipError_t bounds_launch(const KvArgs &a, _Float16 *bounds, int cus, hipStream_t
 
 // ---- scores ----------------------------------------------------------------------------------
 
+typedef double f64x2 __attribute__((ext_vector_type(2)));
 typedef double f64x4 __attribute__((ext_vector_type(4)));
 
 // Scores as whole numbers in their order.  Those of chosen blocks by rule are never formed; NaN comes first, pages
@@ -245,17 +246,22 @@ struct ScoreArgs {
 // 16 blocks by 16 columns with v_mfma_f64_16x16x4_f64: a column is a (row, q head of the K/V head), and the sum runs
 // over [max(q, 0), min(q, 0)] times [hi, lo].  The products of an f32 and an f16 are exact in 64 bits, so that nothing but the
 // order of the sum's last bits is left to chance: blocks' order is that of their scores.  A lane of the operands has
-// the channels D / 4 * (lane / 16) .. of its block or column.
+// the channels D / 4 * (lane / 16) .. of its block or column.  The workgroup's waves have other blocks of the same columns,
+// whose q is in LDS as the products take it: the vector unit's conversions do not overlap with these products (256 rows of 520
+// blocks, 32 x 64 on 8: 37 us with q converted beside each product, 29 so).
+// Waves of a SIMD.
+constexpr int score_waves(int ng) { return ng <= 4 ? 2 : 1; }
 template <int NG>
-__global__ __launch_bounds__(256) void blocks_score(ScoreArgs a) {
+__global__ __launch_bounds__(256, score_waves(NG)) void blocks_score(ScoreArgs a) {
     constexpr int D = 32 * NG, DL = D / 4;
+    __shared__ f64x2 qs[DL][WAVE];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, kg = lane >> 4;
     const KvArgs &kv = a.c;
     const int parts = (kv.max_pages + 4 * a.blocks - 1) / (4 * a.blocks);
     int block = block_of();
     const int head = block % kv.heads;
     block /= kv.heads;
-    const int j0 = (block % parts * 4 + wave) * a.blocks, row0 = block / parts * a.per_tile;
+    const int part = block % parts, j0 = (part * 4 + wave) * a.blocks, row0 = block / parts * a.per_tile;
     if (row0 >= a.rows) return;
     // this lane's column
     const int rt = c / a.group;  // (0 where the group has more than 16 heads)
@@ -267,52 +273,58 @@ __global__ __launch_bounds__(256) void blocks_score(ScoreArgs a) {
         if (rt == r) mine = x;
         if (x.seen > a.count) most = max(most, x.seen);
     }
-    if (j0 >= most) return;
+    if (part * 4 * a.blocks >= most) return;
     if (mine.seen <= a.count) mine.b = -1;  // (its blocks are all chosen)
     const int64_t t = (int64_t)a.row0 + row0 + rt;
-    uint64_t done = __ballot(mine.b < 0);
-    while (done != ~0ull) {
-        const int b = __builtin_amdgcn_readlane(mine.b, __ffsll((unsigned long long)~done) - 1);
-        const uint64_t same = __ballot(mine.b == b);
-        done |= same;
-        int last = mine.b == b ? mine.seen : 0;
-#pragma unroll
-        for (int d = 1; d < 16; d *= 2) last = max(last, __shfl_xor(last, d));
-        last = min(__builtin_amdgcn_readfirstlane(last), j0 + a.blocks);
-        const int32_t *table = kv.table + (int64_t)b * kv.max_pages;
-        // (one pass over the columns, unless the group has more than 16 heads: then the blocks' loop is inside)
-        for (int g0 = 0; g0 < a.group; g0 += 16) {
-            const int gh = g0 + (a.group > 16 ? c : c - rt * a.group);
-            const bool on = mine.b == b && gh < a.group;
-            float q[DL];
-#pragma unroll
-            for (int i = 0; i < DL; i++) q[i] = 0.0f;
+    // (one pass, unless the group has more than 16 heads)
+    for (int g0 = 0; g0 < a.group; g0 += 16) {
+        const int gh = g0 + (a.group > 16 ? c : c - rt * a.group);
+        const bool on = mine.b >= 0 && gh < a.group;
+        if (g0) __syncthreads();
+        for (int ch = wave; ch < DL / 8; ch += 4) {
+            float q[8] = {0, 0, 0, 0, 0, 0, 0, 0};
             if (on) {
-                const int64_t at = t * a.q_stride + (int64_t)(head * a.group + gh) * D + DL * kg;
+                const int64_t at = t * a.q_stride + (int64_t)(head * a.group + gh) * D + DL * kg + 8 * ch;
+                if (a.q_f16) {
+                    const f16x8 v = *(const f16x8 *)((const _Float16 *)a.q + at);
 #pragma unroll
-                for (int i = 0; i < DL; i += 8) {
-                    if (a.q_f16) {
-                        const f16x8 v = *(const f16x8 *)((const _Float16 *)a.q + at + i);
+                    for (int e = 0; e < 8; e++) q[e] = (float)v[e];
+                } else {
+                    const f32x4 v = *(const f32x4 *)((const float *)a.q + at), w = *(const f32x4 *)((const float *)a.q + at + 4);
 #pragma unroll
-                        for (int e = 0; e < 8; e++) q[i + e] = (float)v[e];
-                    } else {
-                        const f32x4 v = *(const f32x4 *)((const float *)a.q + at + i), w = *(const f32x4 *)((const float *)a.q + at + i + 4);
-#pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            q[i + e] = v[e];
-                            q[i + 4 + e] = w[e];
-                        }
+                    for (int e = 0; e < 4; e++) {
+                        q[e] = v[e];
+                        q[4 + e] = w[e];
                     }
                 }
-                if (a.negative)
-#pragma unroll
-                    for (int i = 0; i < DL; i++) q[i] = -q[i];
             }
-            // bounds a tile ahead of their use, pages two (at 256 channels the registers leave no room for it)
-            constexpr bool AHEAD = NG <= 4;
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const float v = a.negative ? -q[e] : q[e];  // (NaN goes into the first)
+                qs[8 * ch + e][lane] = f64x2{v < 0.0f ? 0.0 : (double)v, v < 0.0f ? (double)v : 0.0};
+            }
+        }
+        __syncthreads();
+        uint64_t done = __ballot(mine.b < 0);
+        while (done != ~0ull) {
+            const int b = __builtin_amdgcn_readlane(mine.b, __ffsll((unsigned long long)~done) - 1);
+            done |= __ballot(mine.b == b);
+            int last = mine.b == b ? mine.seen : 0;
+#pragma unroll
+            for (int d = 1; d < 16; d *= 2) last = max(last, __shfl_xor(last, d));
+            last = min(__builtin_amdgcn_readfirstlane(last), j0 + a.blocks);
+            if (j0 >= last) continue;
+            const int32_t *table = kv.table + (int64_t)b * kv.max_pages;
+            // bounds a tile ahead of their use, pages 64 blocks at a time; keys are stored a tile later, so that no load's
+            // wait is for a store
             f16x8 hi[DL / 8], lo[DL / 8];
-            auto page_of = [&](int j) { return table[min(j + c, last - 1)]; };
-            auto load = [&](int id) {
+            int ids = 0, from = j0 - WAVE;
+            auto load = [&](int j) -> bool {  // (a tile lies in one 64: the waves' blocks are a multiple of 16)
+                if (j >= from + WAVE) {
+                    from += WAVE;
+                    ids = table[min(from + lane, last - 1)];
+                }
+                const int id = __shfl(ids, j - from + c);
                 const bool page = (uint32_t)id < (uint32_t)kv.n_pages;
                 const _Float16 *p = a.bounds + ((int64_t)(page ? id : 0) * kv.heads + head) * (2 * D) + DL * kg;
 #pragma unroll
@@ -320,11 +332,21 @@ __global__ __launch_bounds__(256) void blocks_score(ScoreArgs a) {
                     hi[i] = *(const f16x8 *)(p + 8 * i);
                     lo[i] = *(const f16x8 *)(p + D + 8 * i);
                 }
+                return page;
             };
-            int id = page_of(j0), id1 = page_of(j0 + 16);
-            load(id);
+            const int heads = a.group > 16 ? 16 : a.group, h0 = a.group > 16 ? c : c - rt * a.group;
+            const bool first = h0 == 0 && mine.b == b;
+            uint64_t *out = a.keys + ((int64_t)(row0 + rt) * kv.heads + head) * kv.max_pages;
+            uint64_t key[4];
+            auto store = [&](int j) {  // a lane's four results: blocks kg, kg + 4, .. of the 16, its column
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int jj = j + kg + 4 * i;
+                    if (first && jj < min(mine.seen, last)) out[jj] = g0 == 0 ? key[i] : max(key[i], out[jj]);
+                }
+            };
+            bool page = load(j0);
             for (int j = j0; j < last; j += 16) {
-                const bool page = (uint32_t)id < (uint32_t)kv.n_pages;
                 f64x4 up = {0, 0, 0, 0}, down = {0, 0, 0, 0};
                 f16x8 h[DL / 8], l[DL / 8];
 #pragma unroll
@@ -332,34 +354,29 @@ __global__ __launch_bounds__(256) void blocks_score(ScoreArgs a) {
                     h[i] = hi[i];
                     l[i] = lo[i];
                 }
-                if (AHEAD && j + 16 < last) load(id1);
-                id = id1;
-                id1 = page_of(j + 32);
+                const bool there = page;
+                if (j + 16 < last) page = load(j + 16);
+                if (j > j0) store(j - 16);
 #pragma unroll
                 for (int i = 0; i < DL; i++) {
-                    const float v = q[i];  // (NaN goes into the first)
-                    up = __builtin_amdgcn_mfma_f64_16x16x4f64((double)(float)h[i / 8][i % 8], (double)(v < 0.0f ? 0.0f : v), up, 0, 0, 0);
-                    down = __builtin_amdgcn_mfma_f64_16x16x4f64((double)(float)l[i / 8][i % 8], (double)(v < 0.0f ? v : 0.0f), down, 0, 0, 0);
+                    const f64x2 q = qs[i][lane];
+                    up = __builtin_amdgcn_mfma_f64_16x16x4f64((double)(float)h[i / 8][i % 8], q.x, up, 0, 0, 0);
+                    down = __builtin_amdgcn_mfma_f64_16x16x4f64((double)(float)l[i / 8][i % 8], q.y, down, 0, 0, 0);
                 }
-                if (!AHEAD && j + 16 < last) load(id);
-                // a lane's four results: blocks kg, kg + 4, .. of the 16, its column
+                const uint64_t pages = __ballot(there);  // (lane n has block n's page)
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const int jj = j + kg + 4 * i;
-                    const bool there = __shfl(page, kg + 4 * i) != 0;  // (lane n has block n's page)
-                    uint64_t key = on && there ? key_of(up[i] + down[i]) : KEY_NONE;
-                    // the largest of the row's heads, at the first of them
-                    const int heads = a.group > 16 ? 16 : a.group, h = a.group > 16 ? c : c - rt * a.group;
-                    for (int d = 1; d < heads; d *= 2) {
-                        const uint64_t other = shfl64(key, (lane & 48) | ((c + d) & 15));
-                        if (h + d < heads) key = max(key, other);
-                    }
-                    if (h == 0 && mine.b == b && jj < min(mine.seen, last)) {
-                        uint64_t *o = a.keys + ((int64_t)(row0 + rt) * kv.heads + head) * kv.max_pages + jj;
-                        *o = g0 == 0 ? key : max(key, *o);
+                for (int i = 0; i < 4; i++) key[i] = on && (pages >> (kg + 4 * i) & 1) ? key_of(up[i] + down[i]) : KEY_NONE;
+                // the largest of the row's heads, at the first of them
+                for (int d = 1; d < heads; d *= 2) {
+                    const int other = (lane & 48) | ((c + d) & 15);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const uint64_t k = shfl64(key[i], other);
+                        if (h0 + d < heads) key[i] = max(key[i], k);
                     }
                 }
             }
+            store(j0 + (last - 1 - j0) / 16 * 16);
         }
     }
 }
@@ -637,8 +654,8 @@ hipError_t attend_launch(const RowsArgs &r, hipStream_t s) {
 }
 
 // Blocks that a wave scores: all of a short sequence's; of long ones so many that the chip is filled.
-int score_blocks(int cus, int64_t tiles, int max_pages) {
-    const int64_t want = 16 * (int64_t)cus / std::max<int64_t>(tiles, 1);  // waves of a tile
+int score_blocks(int cus, int waves, int64_t tiles, int max_pages) {
+    const int64_t want = 4 * waves * (int64_t)cus / std::max<int64_t>(tiles, 1);  // waves of a tile
     int64_t n = (max_pages + std::max<int64_t>(want, 4) - 1) / std::max<int64_t>(want, 4);
     return (int)((n + 15) / 16 * 16);
 }
@@ -656,7 +673,7 @@ hipError_t dim_launch(const BlocksArgs &b, const BlocksPlan &p, int cus, hipStre
                             std::max(1, 16 / b.a.group), 0, keys};
             if (!c.start) sc.per_tile = 1;  // (no two rows have blocks in common)
             const int64_t tiles = (int64_t)((rows + sc.per_tile - 1) / sc.per_tile) * c.heads;
-            sc.blocks = score_blocks(cus, tiles, c.max_pages);
+            sc.blocks = score_blocks(cus, score_waves(NG), tiles, c.max_pages);
             const int64_t parts = (c.max_pages + 4 * (int64_t)sc.blocks - 1) / (4 * (int64_t)sc.blocks);
             blocks_score<NG><<<grid_of(tiles * parts), 256, 0, s>>>(sc);
             if ((e = hipGetLastError()) != hipSuccess) return e;
