@@ -1,7 +1,7 @@
 // arfq_rope.hip -- rotary positions of one to four axes.
 //
-// A thread has four pairs of a row (or eight of the values behind them) and goes over heads of its token, so that their
-// cosines are formed once for several heads; a workgroup's threads lie side by side on the heads of one token.  An
+// A workgroup forms the cosines of one to eight tokens once, in LDS, for all of its heads; a thread has four pairs of a row
+// (or eight of the values behind them), its first row's on the way meanwhile.  An
 // angle counts in turns: position times turns a position in 64 bits, of which the nearest quarter is taken off, and
 // what is left, at most an eighth of a turn, goes into the series of sine and cosine in 32 bits (the first terms left
 // out are below 2^-27 of a turn's radius).  Bound by memory.
@@ -11,7 +11,7 @@ namespace arfq {
 namespace {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
-constexpr int THREADS = 256;
+constexpr int THREADS = 256, DEEP_MAX = 8, ROWS_THREAD = 4;
 
 struct Turn {
     float c, s;
@@ -44,28 +44,35 @@ __device__ __forceinline__ void store4(void *p, int64_t i, const float (&o)[4]) 
         *(f32x4 *)((float *)p + i) = f32x4{o[0], o[1], o[2], o[3]};
 }
 
-// lanes: threads of a row (dim / 8); slots: rows side by side in a workgroup; heads of a workgroup: `span`.
+// A workgroup: `deep` tokens, `span` heads of each.  lanes: threads of a row (dim / 8); slots: rows side by side.
 template <bool XF16, bool OF16, bool NEIGHBOURS>
-__global__ __launch_bounds__(THREADS) void rope_kernel(RopeArgs a, int lanes, int slots, int span, int groups) {
-    const int slot = threadIdx.x / lanes, u = threadIdx.x - slot * lanes;
-    const int t = block_of() / groups, h0 = (block_of() - t * groups) * span, h1 = min(h0 + span, a.heads);
-    if (slot >= slots || t >= a.tokens) return;
+__global__ __launch_bounds__(THREADS) void rope_kernel(RopeArgs a, int lanes, int slots, int deep, int span, int groups) {
+    __shared__ Turn turns[DEEP_MAX * ROPE_DIM_MAX / 2];
+    const int slot = threadIdx.x / lanes, u = threadIdx.x - slot * lanes, half = a.rot / 2;
+    const int tile = block_of() / groups, t0 = tile * deep, h0 = (block_of() - tile * groups) * span;
+    if (t0 >= a.tokens) return;
+    deep = min(deep, a.tokens - t0);
+    span = min(span, a.heads - h0);
     // two runs of four values: a pair's halves, or eight neighbours
-    const bool turns = u < a.rot / 8;
-    if (!turns && a.x == a.out) return;
-    const int first = NEIGHBOURS || !turns ? 8 * u : 4 * u, second = first + (NEIGHBOURS || !turns ? 4 : a.rot / 2);
-    Turn w[4];
-    if (turns) {
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-            w[i] = turn_of((double)a.positions[a.axis[4 * u + i] * a.position_stride + t] * a.turns[4 * u + i], a.gain);
+    const bool turned = u < a.rot / 8;
+    const int first = NEIGHBOURS || !turned ? 8 * u : 4 * u, second = first + (NEIGHBOURS || !turned ? 4 : half);
+    const int rows = slot < slots && (turned || a.x != a.out) ? deep * span : 0;
+    float x[4], y[4];
+    int row = slot, tok = row / span;
+    auto load = [&] {
+        const int64_t o = (t0 + tok) * a.x_stride + (int64_t)(h0 + row - tok * span) * a.dim;
+        load4<XF16>(a.x, o + first, x);
+        load4<XF16>(a.x, o + second, y);
+    };
+    if (row < rows) load();
+    for (int i = threadIdx.x; i < deep * half; i += THREADS) {
+        const int t = i / half, p = i - t * half;
+        turns[i] = turn_of((double)a.positions[a.axis[p] * a.position_stride + t0 + t] * a.turns[p], a.gain);
     }
-    for (int h = h0 + slot; h < h1; h += slots) {
-        const int64_t xo = t * a.x_stride + (int64_t)h * a.dim, oo = t * a.out_stride + (int64_t)h * a.dim;
-        float x[4], y[4];
-        load4<XF16>(a.x, xo + first, x);
-        load4<XF16>(a.x, xo + second, y);
-        if (turns) {
+    lds_barrier();
+    while (row < rows) {
+        if (turned) {
+            const Turn *w = turns + tok * half + 4 * u;
             auto rotate = [&](int i, float &p, float &q) {
                 const float r = p * w[i].c - q * w[i].s;
                 q = p * w[i].s + q * w[i].c;
@@ -81,19 +88,28 @@ __global__ __launch_bounds__(THREADS) void rope_kernel(RopeArgs a, int lanes, in
                 for (int i = 0; i < 4; i++) rotate(i, x[i], y[i]);
             }
         }
-        store4<OF16>(a.out, oo + first, x);
-        store4<OF16>(a.out, oo + second, y);
+        const int64_t o = (t0 + tok) * a.out_stride + (int64_t)(h0 + row - tok * span) * a.dim;
+        store4<OF16>(a.out, o + first, x);
+        store4<OF16>(a.out, o + second, y);
+        row += slots;
+        if (row >= rows) break;
+        tok = row / span;
+        load();
     }
 }
 
 template <bool XF16, bool OF16, bool NEIGHBOURS>
 hipError_t rope_launch(const RopeArgs &a, int cus, hipStream_t s) {
     const int lanes = a.dim / 8, slots = THREADS / lanes;
-    // heads of a workgroup: all of a token's, fewer where that leaves compute units idle
+    // heads of a workgroup: all of a token's, fewer where that leaves compute units idle; then tokens, so that a
+    // thread has about four rows
     int span = a.heads;
     while (span > slots && (int64_t)a.tokens * ((a.heads + span - 1) / span) < 4 * cus) span = (span + 1) / 2;
     const int groups = (a.heads + span - 1) / span;
-    rope_kernel<XF16, OF16, NEIGHBOURS><<<grid_of((int64_t)a.tokens * groups), THREADS, 0, s>>>(a, lanes, slots, span, groups);
+    int deep = 1;
+    while (deep < DEEP_MAX && 2 * deep * span <= ROWS_THREAD * slots && (int64_t)a.tokens / (2 * deep) * groups >= 4 * cus) deep *= 2;
+    const int64_t blocks = ((int64_t)a.tokens + deep - 1) / deep * groups;
+    rope_kernel<XF16, OF16, NEIGHBOURS><<<grid_of(blocks), THREADS, 0, s>>>(a, lanes, slots, deep, span, groups);
     return hipGetLastError();
 }
 
