@@ -1,9 +1,9 @@
 // arfq_lora.hip -- low-rank adapters of many requests beside a shared projection:
 // out[t] = base[t] + scale_e B_e (A_e x[t]), e = ids[t].
 //
-// Two launches.  The first forms parts of h = A_e x over ranges of k, [splits][rows][rank] in f32; the second adds the
-// parts in order, and B_e h to base.  Few rows: a workgroup has one row (and a range of k, or of n) on the vector unit,
-// products in f32.  Many rows: tiles of 16 or 32 neighbouring rows on the matrix cores, once for each adapter that the
+// Two launches, where A_e x takes little one.  The first forms parts of h = A_e x over ranges of k, [splits][rows][rank] in
+// f32; the second adds the parts in order, and B_e h to base.  Few rows: a workgroup has one row (and a range of k, or of n)
+// on the vector unit, products in f32.  Many rows: tiles of neighbouring rows on the matrix cores, once for each adapter that the
 // tile's rows name; an f32 x goes through v_mfma_f32_16x16x4_f32 as it is, an f16 x is exact in f16 operands, and h
 // enters the second product as two f16 parts of 22 bits of the row's largest.  Every adapter has accumulators of its
 // own: a NaN in one does not reach another's rows.  Bound by memory: the adapters' bytes for few rows, base and out for
@@ -98,60 +98,125 @@ __global__ __launch_bounds__(256) void lora_rows_a(LoraArgs a, int splits) {
     }
 }
 
-// LP lanes have an output, eight ranks each.  B and base are on their way while h's parts are added.
-constexpr int N_PART = 256;  // outputs of a workgroup
+// Outputs n0 .. of a row, 64 W of them: LP lanes have an output, eight ranks each.  B and base of the first eight that a lane
+// has a part in are loaded by begin(), before h is known.
+template <int LP, int W>
+struct Outputs {
+    static constexpr int U = LP < 8 ? LP : 8, APART = 64 * W / LP;  // outputs of LP lanes at once; of a lane and the next
+    const float *base;
+    float *out;
+    const _Float16 *B;
+    int64_t n, n0;
+    int rank, u;
+    bool on;
+    f16x8 w[U];
+    float own[U];
+    __device__ __forceinline__ void load(int j0) {
+#pragma unroll
+        for (int j = 0; j < U; j++) {
+            const int64_t at = n0 + (j0 + j) * APART + threadIdx.x / LP;
+            w[j] = on && at < n ? *(const f16x8 *)(B + at * rank) : zero8();
+            own[j] = base && u == 0 && at < n ? base[at] : 0.0f;
+        }
+    }
+    __device__ __forceinline__ Outputs(const LoraArgs &a, int t, int e, int64_t n0)
+        : base(a.base ? a.base + t * a.base_stride : nullptr), out(a.out + t * a.out_stride), n(a.l.n), n0(n0), rank((int)a.l.rank),
+          u(threadIdx.x % LP), on(8 * u < rank) {
+        B = (const _Float16 *)a.l.b + (int64_t)e * n * rank + 8 * u;
+    }
+    // (a row without an adapter)
+    __device__ __forceinline__ void copy() {
+        const int64_t at = n0 + threadIdx.x;
+        if (at < n && base != out) out[at] = base ? base[at] : 0.0f;
+    }
+    __device__ __forceinline__ void finish(const float *sh) {
+        float h[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) h[i] = on ? sh[8 * u + i] : 0.0f;
+#pragma unroll 1
+        for (int j0 = 0; j0 < LP; j0 += U) {
+            if (j0 > 0) load(j0);
+#pragma unroll
+            for (int j = 0; j < U; j++) {
+                float v = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 8; i++) v = __builtin_fmaf((float)w[j][i], h[i], v);
+                v = lanes_sum<LP>(v);
+                const int64_t at = n0 + (j0 + j) * APART + threadIdx.x / LP;
+                if (u == 0 && at < n) out[at] = own[j] + v;
+            }
+        }
+    }
+};
+
 template <int LP>
 __global__ __launch_bounds__(256) void lora_rows_b(LoraArgs a, int splits, int parts) {
     __shared__ float sh[LORA_RANK_MAX];
     const int block = block_of(), t = block / parts, part = block - t * parts;
     if (t >= a.rows) return;
     const int e = id_of(a, t), rank = (int)a.l.rank;
-    const float *base = a.base ? a.base + t * a.base_stride : nullptr;
-    float *out = a.out + t * a.out_stride;
-    const int64_t n0 = (int64_t)part * N_PART;
-    if (e < 0) {
-        const int64_t n = n0 + threadIdx.x;
-        if (n < a.l.n && base != out) out[n] = base ? base[n] : 0.0f;
-        return;
-    }
-    const int u = threadIdx.x % LP, r0 = 8 * u;
-    const bool on = r0 < rank;
-    const _Float16 *B = (const _Float16 *)a.l.b + (int64_t)e * a.l.n * rank + r0;
-    constexpr int U = LP < 8 ? LP : 8, APART = 256 / LP;  // outputs of LP lanes at once; of a lane and the next
-    f16x8 w[U];
-    float own[U], h[8];
-    auto load = [&](int j0) {
-#pragma unroll
-        for (int j = 0; j < U; j++) {
-            const int64_t n = n0 + (j0 + j) * APART + threadIdx.x / LP;
-            w[j] = on && n < a.l.n ? *(const f16x8 *)(B + n * rank) : zero8();
-            own[j] = base && u == 0 && n < a.l.n ? base[n] : 0.0f;
-        }
-    };
+    Outputs<LP, 4> o(a, t, e, (int64_t)part * 256);
+    if (e < 0) return o.copy();
     float s = 0.0f;
     if ((int)threadIdx.x < rank) {
 #pragma unroll 8
         for (int p = 0; p < splits; p++) s += a.h[((int64_t)p * a.rows + t) * rank + threadIdx.x];
         if (a.l.scale) s *= a.l.scale[e];
     }
-    load(0);
+    o.load(0);
     if ((int)threadIdx.x < rank) sh[threadIdx.x] = s;
     lds_barrier();
+    o.finish(sh);
+}
+
+// Both products in one launch, where A_e x takes little: each workgroup forms it for itself.  The waves share the ranks, four
+// a wave, and where these are fewer, k.  (Four waves for sixteen: 0.1 us slower at the smallest sizes, twice the time at the
+// largest.)
+constexpr int ONE_WAVES = 16, ONE_OUT = 64 * ONE_WAVES;  // outputs of a workgroup
+template <int LP>
+__global__ __launch_bounds__(64 * ONE_WAVES) void lora_rows_ab(LoraArgs a, int parts) {
+    constexpr int W = ONE_WAVES;
+    constexpr int R = 2 * LP < W ? 2 * LP : W;  // waves side by side on ranks (LP lanes: 8 LP ranks at most)
+    constexpr int K = W / R;
+    __shared__ __align__(16) float sh[K][LORA_RANK_MAX];
+    const int block = block_of(), t = block / parts, part = block - t * parts;
+    if (t >= a.rows) return;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), rw = wave % R, kw = wave / R;
+    const int e = id_of(a, t), rank = (int)a.l.rank;
+    Outputs<LP, W> o(a, t, e, (int64_t)part * 64 * W);
+    if (e < 0) return o.copy();
+    const _Float16 *A = (const _Float16 *)a.l.a + (int64_t)e * rank * a.l.k;
+    const float scale = a.l.scale ? a.l.scale[e] : 1.0f;
+    o.load(0);
+    constexpr int U = 4;
+    for (int r0 = rw * U; r0 < rank; r0 += R * U) {
+        float s[U] = {0, 0, 0, 0};
+#pragma unroll 2
+        for (int64_t k = 512 * kw + 8 * lane; k < a.l.k; k += 512 * K) {
+            float x[8];
+            if (a.x_f16) load8<true>(a.x, t * a.l.k + k, x);
+            else load8<false>(a.x, t * a.l.k + k, x);
+            f16x8 w[U];
 #pragma unroll
-    for (int i = 0; i < 8; i++) h[i] = on ? sh[r0 + i] : 0.0f;
-#pragma unroll 1
-    for (int j0 = 0; j0 < LP; j0 += U) {
-        if (j0 > 0) load(j0);
+            for (int u = 0; u < U; u++) w[u] = *(const f16x8 *)(A + (r0 + u) * a.l.k + k);
 #pragma unroll
-        for (int j = 0; j < U; j++) {
-            float v = 0.0f;
+            for (int u = 0; u < U; u++)
 #pragma unroll
-            for (int i = 0; i < 8; i++) v = __builtin_fmaf((float)w[j][i], h[i], v);
-            v = lanes_sum<LP>(v);
-            const int64_t n = n0 + (j0 + j) * APART + threadIdx.x / LP;
-            if (u == 0 && n < a.l.n) out[n] = own[j] + v;
+                for (int i = 0; i < 8; i++) s[u] = __builtin_fmaf((float)w[u][i], x[i], s[u]);
         }
+#pragma unroll
+        for (int u = 0; u < U; u++) s[u] = lanes_sum<64>(s[u]);
+        if (lane == 0) *(f32x4 *)&sh[kw][r0] = f32x4{s[0], s[1], s[2], s[3]};
     }
+    lds_barrier();
+    if ((int)threadIdx.x < rank) {
+        float s = sh[0][threadIdx.x];
+#pragma unroll
+        for (int i = 1; i < K; i++) s += sh[i][threadIdx.x];
+        sh[0][threadIdx.x] = s * scale;
+    }
+    lds_barrier();
+    o.finish(sh[0]);
 }
 
 // ---- many rows ----
@@ -432,10 +497,18 @@ __global__ __launch_bounds__(64 * B_WAVES) void lora_tiles_b(LoraArgs a, int spl
 // (The ids are on the device: the border leans to the side that loses less.)
 constexpr int64_t TILE_VALUES = 4 << 20;
 
+// Values of A_e, and of it over all workgroups, up to which both products of rows one by one are one launch.  us in one and
+// in two: k = n = 512, rank 16, any rows up to 256 4.3 and 6.8; k = n = 2048, rank 64 (2^17 of A), one row 7.1 and 8.2;
+// k = 5120, n = 17408, rank 16, 8 rows (11 M) 5.4 and 6.6; k = n = 2048, rank 64, 64 rows (17 M) 9.1 and 8.8; k = 1024,
+// n = 4096, rank 16, 256 rows (17 M) 12.3 and 9.6; k = 17408, rank 16 (2^18), one row 8.7 and 6.7.
+constexpr int64_t ONE_A = 1 << 17, ONE_READ = 12 << 20;
+
 template <int LP>
 hipError_t rows_b(const LoraArgs &a, const LoraPlan &p, hipStream_t s) {
-    const int parts = (int)((a.l.n + N_PART - 1) / N_PART);
-    lora_rows_b<LP><<<grid_of((int64_t)a.rows * parts), 256, 0, s>>>(a, p.splits, parts);
+    const int64_t parts = (a.l.n + (p.one ? ONE_OUT : 256) - 1) / (p.one ? ONE_OUT : 256);
+    const dim3 grid = grid_of(a.rows * parts);
+    if (p.one) lora_rows_ab<LP><<<grid, 64 * ONE_WAVES, 0, s>>>(a, (int)parts);
+    else lora_rows_b<LP><<<grid, 256, 0, s>>>(a, p.splits, (int)parts);
     return hipGetLastError();
 }
 
@@ -477,8 +550,9 @@ LoraPlan lora_plan(int cus, const arfq_lora &l, int64_t rows) {
     } else {
         p.k_part = K_PART;
         p.splits = (int)((l.k + K_PART - 1) / K_PART);
+        p.one = l.k * l.rank <= ONE_A && rows * ((l.n + ONE_OUT - 1) / ONE_OUT) * l.k * l.rank <= ONE_READ;
     }
-    p.ws_bytes = (size_t)p.splits * rows * l.rank * sizeof(float);
+    p.ws_bytes = p.one ? 0 : (size_t)p.splits * rows * l.rank * sizeof(float);
     return p;
 }
 
@@ -489,11 +563,13 @@ hipError_t launch_lora(const LoraArgs &a, const LoraPlan &p, hipStream_t s) {
         const int64_t runs = (a.l.rank + 31) / 32;
         return runs <= 1 ? tiles_b<1>(a, p, s) : runs <= 2 ? tiles_b<2>(a, p, s) : runs <= 4 ? tiles_b<4>(a, p, s) : tiles_b<8>(a, p, s);
     }
-    const dim3 grid = grid_of((int64_t)a.rows * p.splits);
-    if (a.x_f16) lora_rows_a<true><<<grid, 256, 0, s>>>(a, p.splits);
-    else lora_rows_a<false><<<grid, 256, 0, s>>>(a, p.splits);
-    hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
+    if (!p.one) {
+        const dim3 grid = grid_of((int64_t)a.rows * p.splits);
+        if (a.x_f16) lora_rows_a<true><<<grid, 256, 0, s>>>(a, p.splits);
+        else lora_rows_a<false><<<grid, 256, 0, s>>>(a, p.splits);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
     const int64_t lanes = a.l.rank / 8;
     return lanes <= 1 ? rows_b<1>(a, p, s) : lanes <= 2 ? rows_b<2>(a, p, s) : lanes <= 4 ? rows_b<4>(a, p, s) :
            lanes <= 8 ? rows_b<8>(a, p, s) : lanes <= 16 ? rows_b<16>(a, p, s) : rows_b<32>(a, p, s);

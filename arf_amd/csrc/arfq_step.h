@@ -29,6 +29,7 @@ hipError_t launch_rope(const RopeArgs &a, int cus, hipStream_t stream);
 constexpr int64_t LORA_RANK_MAX = 256, LORA_ROWS_MAX = (int64_t)1 << 24;
 struct LoraPlan {
     bool tiles = false;  // rows in tiles on the matrix cores; one by one on the vector unit otherwise
+    bool one = false;    // rows one by one, both products in one launch
     int splits = 1;      // parts of k
     int k_part = 0;      // values of a part
     size_t ws_bytes = 0; // [splits][rows][rank] f32

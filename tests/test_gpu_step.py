@@ -687,10 +687,11 @@ def test_refusals(gpu_ctx):
             gpu_ctx.lora_add(arf_amd.Lora(up(np.zeros(la, np.float16)), up(np.zeros(lb, np.float16))), i32(3), lx, 3, y)
         assert e.value.status == arfq.ARFQ_E_UNSUPPORTED
     lora = arf_amd.Lora(a, b)
+    big = arf_amd.Lora(up(np.zeros((1, 8, 16392), np.float16)), up(np.zeros((1, 5, 8), np.float16)))  # (in two launches)
     for bad in (lambda: arf_amd.Lora(a, a), lambda: arf_amd.Lora(lx, b), lambda: arf_amd.Lora(a, b, i32(2)),
                 lambda: gpu_ctx.lora_add(lora, i32(2), lx, 3, y), lambda: gpu_ctx.lora_add(lora, i32(4), lx, 4, y),
                 lambda: gpu_ctx.lora_add(lora, i32(3), lx, 3, y, out_stride=6), lambda: gpu_ctx.lora_add(lora, i32(3), lx, 3, lx, base_stride=4, base=y),
-                lambda: gpu_ctx.lora_add(lora, i32(3), lx, 3, y, workspace=up(np.zeros(4, np.uint8)))):
+                lambda: gpu_ctx.lora_add(big, i32(1), up(np.zeros((1, 16392), np.float32)), 1, y, workspace=up(np.zeros(4, np.uint8)))):
         with pytest.raises(ValueError):
             bad()
     with pytest.raises(arf_amd.ArfqError, match="in place"):

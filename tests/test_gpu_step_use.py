@@ -148,7 +148,10 @@ def test_captured_and_replayed(dtype):
             return s
         s, t = program(ctx, True), program(other, False)
         with pytest.raises(arf_amd.ArfqError, match="needs a workspace"):
-            Graph(stream, lambda: ctx.lora_add(s.lora, s.ids, s.x, tokens, s.qkv))
+            big = arf_amd.Lora(ctx.to_device(np.zeros((1, 8, 16392), np.float16)), ctx.to_device(np.zeros((1, 8, 8), np.float16)))
+            wide = ctx.to_device(np.zeros((1, 16392), np.float32))
+            assert ctx.lora_workspace(big, 1) > 0
+            Graph(stream, lambda: ctx.lora_add(big, s.ids, wide, 1, s.qkv))
         with pytest.raises(arf_amd.ArfqError, match="needs a workspace"):
             Graph(stream, lambda: ctx.kv_attention_blocks(s.kv, s.steps[0].seqs, s.bounds, s.rows, s.out[0], hq, 0.125, count))
         graph = Graph(stream, s.run)
