@@ -543,14 +543,14 @@ static int kv_args(arfq_ctx *ctx, const arfq_kv *kv, const arfq_kv_seqs *s, cons
 
 // A [tokens, heads, dim] array of a call.
 static int kv_rows(arfq_ctx *ctx, const char *what, const void *p, int64_t stride, int64_t heads, int dim, int dtype) {
-    const std::string w = std::string(what) + ": ";
-    if (dtype != ARFQ_F32 && dtype != ARFQ_F16) return fail(ctx, ARFQ_E_INVALID, w + "unknown dtype");
-    if (!p) return fail(ctx, ARFQ_E_INVALID, w + "null argument");
+    auto refuse = [&](int rc, const std::string &why) { return fail(ctx, rc, std::string(what) + ": " + why); };
+    if (dtype != ARFQ_F32 && dtype != ARFQ_F16) return refuse(ARFQ_E_INVALID, "unknown dtype");
+    if (!p) return refuse(ARFQ_E_INVALID, "null argument");
     if (stride < heads * dim || stride > (int64_t)1 << 40)
-        return fail(ctx, ARFQ_E_SHAPE, w + "token stride " + std::to_string(stride) + " below heads * head_dim = " +
-                                           std::to_string(heads * dim) + ", or above 2^40");
+        return refuse(ARFQ_E_SHAPE, "token stride " + std::to_string(stride) + " below heads * head_dim = " +
+                                        std::to_string(heads * dim) + ", or above 2^40");
     if ((uintptr_t)p % 16 || stride % (dtype == ARFQ_F16 ? 8 : 4))
-        return fail(ctx, ARFQ_E_INVALID, w + "pointers and token strides must be multiples of 16 bytes");
+        return refuse(ARFQ_E_INVALID, "pointers and token strides must be multiples of 16 bytes");
     return ARFQ_OK;
 }
 
@@ -706,12 +706,13 @@ int arfq_rope(arfq_ctx *ctx, const arfq_rope_pairs *rope, const int32_t *positio
         return fail(ctx, ARFQ_E_INVALID, "rope: unknown pairs");
     if (tokens > arfq::KV_ROWS_MAX / heads) return fail(ctx, ARFQ_E_SHAPE, "rope: tokens * heads above 2^30");
     if (!std::isfinite(rope->gain)) return fail(ctx, ARFQ_E_INVALID, "rope: gain must be finite");
+    arfq::RopePairs pairs;
     arfq::RopeArgs a;
     for (int i = 0; i < rope->rot_dim / 2; i++) {
         if (!std::isfinite(rope->freq[i])) return fail(ctx, ARFQ_E_INVALID, "rope: freq must be finite");
         if (rope->axis && rope->axis[i] >= rope->axes) return fail(ctx, ARFQ_E_SHAPE, "rope: axis of a pair not below axes");
-        a.axis[i] = rope->axis ? rope->axis[i] : 0;
-        a.turns[i] = rope->freq[i] * (inverse ? -0.15915494309189535 : 0.15915494309189535);  // 1 / (2 pi)
+        pairs.axis[i] = rope->axis ? rope->axis[i] : 0;
+        pairs.turns[i] = rope->freq[i] * (inverse ? -0.15915494309189535 : 0.15915494309189535);  // 1 / (2 pi)
     }
     if (tokens == 0) return ARFQ_OK;
     if (!positions) return fail(ctx, ARFQ_E_INVALID, "rope: null positions");
@@ -736,7 +737,7 @@ int arfq_rope(arfq_ctx *ctx, const arfq_rope_pairs *rope, const int32_t *positio
     a.neighbours = rope->pairs == ARFQ_ROPE_NEIGHBOURS;
     a.x_f16 = x_dtype == ARFQ_F16;
     a.out_f16 = out_dtype == ARFQ_F16;
-    const hipError_t e = arfq::launch_rope(a, ctx->cus, ctx->stream);
+    const hipError_t e = arfq::launch_rope(a, pairs, ctx->cus, ctx->stream);
     return e == hipSuccess ? ARFQ_OK : hip_fail(ctx, e, "rope launch");
 }
 

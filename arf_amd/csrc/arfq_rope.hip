@@ -5,6 +5,8 @@
 // angle counts in turns: position times turns a position in 64 bits, of which the nearest quarter is taken off, and
 // what is left, at most an eighth of a turn, goes into the series of sine and cosine in 32 bits (the first terms left
 // out are below 2^-27 of a turn's radius).  Bound by memory.
+#include <string.h>
+
 #include "arfq_step.h"
 
 namespace arfq {
@@ -45,9 +47,10 @@ __device__ __forceinline__ void store4(void *p, int64_t i, const float (&o)[4]) 
 }
 
 // A workgroup: `deep` tokens, `span` heads of each.  lanes: threads of a row (dim / 8); slots: rows side by side.
-template <bool XF16, bool OF16, bool NEIGHBOURS>
-__global__ __launch_bounds__(THREADS) void rope_kernel(RopeArgs a, int lanes, int slots, int deep, int span, int groups) {
-    __shared__ Turn turns[DEEP_MAX * ROPE_DIM_MAX / 2];
+// PAIRS at most: the host copies a launch's arguments (64 rows a call with room for 128 pairs 5.4 us, for 64 5.2).
+template <bool XF16, bool OF16, bool NEIGHBOURS, int PAIRS>
+__global__ __launch_bounds__(THREADS) void rope_kernel(RopeArgs a, RopePairsOf<PAIRS> pairs, int lanes, int slots, int deep, int span, int groups) {
+    __shared__ Turn turns[DEEP_MAX * PAIRS];
     const int slot = threadIdx.x / lanes, u = threadIdx.x - slot * lanes, half = a.rot / 2;
     const int tile = block_of() / groups, t0 = tile * deep, h0 = (block_of() - tile * groups) * span;
     if (t0 >= a.tokens) return;
@@ -67,7 +70,7 @@ __global__ __launch_bounds__(THREADS) void rope_kernel(RopeArgs a, int lanes, in
     if (row < rows) load();
     for (int i = threadIdx.x; i < deep * half; i += THREADS) {
         const int t = i / half, p = i - t * half;
-        turns[i] = turn_of((double)a.positions[a.axis[p] * a.position_stride + t0 + t] * a.turns[p], a.gain);
+        turns[i] = turn_of((double)a.positions[pairs.axis[p] * a.position_stride + t0 + t] * pairs.turns[p], a.gain);
     }
     lds_barrier();
     while (row < rows) {
@@ -98,8 +101,11 @@ __global__ __launch_bounds__(THREADS) void rope_kernel(RopeArgs a, int lanes, in
     }
 }
 
-template <bool XF16, bool OF16, bool NEIGHBOURS>
-hipError_t rope_launch(const RopeArgs &a, int cus, hipStream_t s) {
+template <bool XF16, bool OF16, bool NEIGHBOURS, int PAIRS>
+hipError_t rope_launch(const RopeArgs &a, const RopePairs &all, int cus, hipStream_t s) {
+    RopePairsOf<PAIRS> pairs;
+    memcpy(pairs.turns, all.turns, sizeof(pairs.turns));
+    memcpy(pairs.axis, all.axis, sizeof(pairs.axis));
     const int lanes = a.dim / 8, slots = THREADS / lanes;
     // heads of a workgroup: all of a token's, fewer where that leaves compute units idle; then tokens, so that a
     // thread has about four rows
@@ -109,19 +115,25 @@ hipError_t rope_launch(const RopeArgs &a, int cus, hipStream_t s) {
     int deep = 1;
     while (deep < DEEP_MAX && 2 * deep * span <= ROWS_THREAD * slots && (int64_t)a.tokens / (2 * deep) * groups >= 4 * cus) deep *= 2;
     const int64_t blocks = ((int64_t)a.tokens + deep - 1) / deep * groups;
-    rope_kernel<XF16, OF16, NEIGHBOURS><<<grid_of(blocks), THREADS, 0, s>>>(a, lanes, slots, deep, span, groups);
+    rope_kernel<XF16, OF16, NEIGHBOURS, PAIRS><<<grid_of(blocks), THREADS, 0, s>>>(a, pairs, lanes, slots, deep, span, groups);
     return hipGetLastError();
+}
+
+template <bool XF16, bool OF16>
+hipError_t types_launch(const RopeArgs &a, const RopePairs &p, int cus, hipStream_t s) {
+    constexpr int FEW = 32, MANY = ROPE_DIM_MAX / 2;
+    if (a.neighbours)
+        return a.rot <= 2 * FEW ? rope_launch<XF16, OF16, true, FEW>(a, p, cus, s) : a.rot <= 4 * FEW ? rope_launch<XF16, OF16, true, 2 * FEW>(a, p, cus, s)
+                                                                                               : rope_launch<XF16, OF16, true, MANY>(a, p, cus, s);
+    return a.rot <= 2 * FEW ? rope_launch<XF16, OF16, false, FEW>(a, p, cus, s) : a.rot <= 4 * FEW ? rope_launch<XF16, OF16, false, 2 * FEW>(a, p, cus, s)
+                                                                                            : rope_launch<XF16, OF16, false, MANY>(a, p, cus, s);
 }
 
 }  // namespace
 
-hipError_t launch_rope(const RopeArgs &a, int cus, hipStream_t s) {
-    if (a.neighbours) {
-        if (a.x_f16) return a.out_f16 ? rope_launch<true, true, true>(a, cus, s) : rope_launch<true, false, true>(a, cus, s);
-        return a.out_f16 ? rope_launch<false, true, true>(a, cus, s) : rope_launch<false, false, true>(a, cus, s);
-    }
-    if (a.x_f16) return a.out_f16 ? rope_launch<true, true, false>(a, cus, s) : rope_launch<true, false, false>(a, cus, s);
-    return a.out_f16 ? rope_launch<false, true, false>(a, cus, s) : rope_launch<false, false, false>(a, cus, s);
+hipError_t launch_rope(const RopeArgs &a, const RopePairs &p, int cus, hipStream_t s) {
+    if (a.x_f16) return a.out_f16 ? types_launch<true, true>(a, p, cus, s) : types_launch<true, false>(a, p, cus, s);
+    return a.out_f16 ? types_launch<false, true>(a, p, cus, s) : types_launch<false, false>(a, p, cus, s);
 }
 
 }  // namespace arfq

@@ -11,9 +11,13 @@ hipError_t launch_kv_plan(const arfq_kv_step &s, hipStream_t stream);
 
 // ---- arfq_rope.hip ----
 constexpr int ROPE_DIM_MAX = 256, ROPE_HEAD_MAX = 1024, ROPE_AXES_MAX = 4;
+template <int PAIRS>
+struct RopePairsOf {
+    double turns[PAIRS];  // of a pair, a position: freq / (2 pi), negative for the way back
+    uint8_t axis[PAIRS];
+};
+using RopePairs = RopePairsOf<ROPE_DIM_MAX / 2>;
 struct RopeArgs {
-    double turns[ROPE_DIM_MAX / 2];     // of a pair, a position: freq / (2 pi), negative for the way back
-    uint8_t axis[ROPE_DIM_MAX / 2];
     int rot, dim, heads, tokens;
     const int32_t *positions;
     int64_t position_stride;
@@ -23,7 +27,7 @@ struct RopeArgs {
     float gain;
     bool neighbours, x_f16, out_f16;
 };
-hipError_t launch_rope(const RopeArgs &a, int cus, hipStream_t stream);
+hipError_t launch_rope(const RopeArgs &a, const RopePairs &pairs, int cus, hipStream_t stream);
 
 // ---- arfq_lora.hip ----
 constexpr int64_t LORA_RANK_MAX = 256, LORA_ROWS_MAX = (int64_t)1 << 24;
