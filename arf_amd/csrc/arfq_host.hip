@@ -683,8 +683,12 @@ int arfq_kv_plan(arfq_ctx *ctx, const arfq_kv_step *s) {
         return fail(ctx, ARFQ_E_INVALID, "kv_plan: null add, held, held_next, len or pages");
     if ((s->tokens > 0 && (!s->positions || !s->slots)) || (s->n_pages > 0 && !s->free_pages))
         return fail(ctx, ARFQ_E_INVALID, "kv_plan: null positions, slots or free_pages");
-    if (s->held_next == s->held || s->n_free_next == s->n_free)
-        return fail(ctx, ARFQ_E_INVALID, "kv_plan: held_next and n_free_next have places of their own");
+    // what is written, and then what is only read
+    const void *const at[] = {s->n_free_next, s->start, s->taken, s->freed, s->held_next, s->len, s->pages, s->free_pages,
+                              s->positions, s->slots, s->n_free, s->add, s->held};
+    for (int i = 0; i < 10; i++)
+        for (int j = i + 1; j < 13; j++)
+            if (at[i] && at[i] == at[j]) return fail(ctx, ARFQ_E_INVALID, "kv_plan: arrays that are written have places of their own");
     if (int rc = use_device(ctx)) return rc;
     const hipError_t e = arfq::launch_kv_plan(*s, ctx->stream);
     return e == hipSuccess ? ARFQ_OK : hip_fail(ctx, e, "kv_plan launch");

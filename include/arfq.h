@@ -396,7 +396,7 @@ int arfq_kv_attention_workspace(arfq_ctx *ctx, const arfq_kv *kv, int64_t batch,
  * With what it writes, { batch, tokens, start, len, pages, max_pages } is the step's arfq_kv_seqs, whose
  * rows of refused sequences name nothing; positions are what arfq_rope takes.  Inputs are not changed (beyond
  * pages' new entries and the stack's, above the free ones), so held and held_next, n_free and n_free_next change
- * places from step to step. */
+ * places from step to step; no array that is written may be another of the call's. */
 typedef struct {
     int64_t batch, max_pages;    /* at most 16384; max_pages * page_size <= 2^29 */
     int64_t tokens;              /* places of positions and slots: the step's rows, or more; at most 2^30 */

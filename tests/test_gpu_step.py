@@ -598,6 +598,28 @@ def test_rows_in_several_chunks(gpu_ctx):
     assert np.array_equal(out.numpy(), got)
 
 
+@pytest.mark.parametrize("dtype", [np.float16, np.float32])
+@pytest.mark.parametrize("lens,count,width", [([40005, 100], 2100, 0), ([9000, 2000, 400], 20, 17000), ([40005], 2300, 17000)])
+def test_choices_in_a_launch_of_their_own(gpu_ctx, dtype, lens, count, width):
+    # more chosen blocks than the attention's workgroups keep, and tables wider than they look through
+    _say("blocks wide", np.dtype(dtype).name, lens, count, width)
+    rng = np.random.default_rng(count + width)
+    page, heads, dim, group = 16, 2, 64, 3
+    batch = Batch(gpu_ctx, lens, [2] * len(lens), page, rng)
+    if width:
+        wide = np.full((len(lens), width), -1, np.int32)
+        wide[:, :batch.table.shape[1]] = batch.table
+        batch.d_table = gpu_ctx.to_device(wide)
+        batch.seqs = arf_amd.KVSeqs(batch.d_table, batch.d_len, batch.d_start, batch.tokens)
+        batch.whole = arf_amd.KVSeqs(batch.d_table, batch.d_len, batch.d_whole, int(batch.whole_start[-1]))
+    kv = gpu_ctx.kv_cache(heads, dim, page, batch.n_pages)
+    hk, hv = _filled(gpu_ctx, kv, batch, rng)
+    q = _rows(rng, batch.tokens, heads * group, dim, dtype, False)
+    kw = dict(count=count, first=2, last=3)
+    got, chosen = _attend(gpu_ctx, kv, batch, _bounds(gpu_ctx, kv, batch), q, dtype, 0.125, **kw)
+    _check(batch, got, chosen, q, hk, hv, 0.125, **kw)
+
+
 def test_all_blocks_are_what_attention_takes(gpu_ctx):
     # count from the table's width on: kv_attention's rows
     _say("blocks all")
@@ -644,9 +666,11 @@ def test_refusals(gpu_ctx):
                dict(positions=up(np.zeros(5, np.float32)))):
         with pytest.raises(ValueError):
             gpu_ctx.kv_plan(step(**kw))
-    same = i32(2)
-    with pytest.raises(arf_amd.ArfqError, match="places of their own"):
-        gpu_ctx.kv_plan(step(held=same, held_next=same))
+    same, wider, one = i32(2), i32(3), i32(1)
+    for kw in (dict(held=same, held_next=same), dict(add=same, lens=same), dict(lens=same, held_next=same), dict(start=wider, freed=wider),
+               dict(taken=wider, freed=wider), dict(n_free=one, n_free_next=one)):
+        with pytest.raises(arf_amd.ArfqError, match="places of their own"):
+            gpu_ctx.kv_plan(step(**kw))
     bad = step()
     for field, value, status in (("tokens", -1, arfq.ARFQ_E_SHAPE), ("tokens", (1 << 30) + 1, arfq.ARFQ_E_SHAPE), ("batch", 16385, arfq.ARFQ_E_SHAPE),
                                  ("max_pages", 1 << 30, arfq.ARFQ_E_SHAPE), ("n_pages", 1 << 31, arfq.ARFQ_E_SHAPE), ("add", None, arfq.ARFQ_E_INVALID),
