@@ -2,8 +2,11 @@
 //
 // Bounds: of each channel of a page's keys the largest and smallest (arfq_kv_bounds), f16 and exact, as keys are.
 // A call: the scores' keys of all blocks (blocks_score), the best of them for each row and K/V head and their pages
-// (blocks_select), attention with those pages as the row's table (the tile of arfq_attn_rows16.h, a row a sequence
-// of its own), and the joining of rows whose keys were cut into pieces.
+// (blocks_select, or choose() within the next), attention with those pages as the row's table (blocks_attend: the tile of
+// arfq_attn_rows16.h, a row a sequence of its own), and the joining of rows whose keys were cut into pieces.
+// One token at 131071, 64 of 2048 blocks of 64, 40 x 128 on 8, f32: bounds 4, scores 8, attention 13 (6 of it the choice), join
+// 4 us: latency.  256 rows of a prompt, 32 of 520 blocks of 32, 32 x 64 on 8, f16: 5, 34 and 46 (four rows of 16 in a tile's
+// products, whose operands are made for every row anew).
 #include <math.h>
 
 #include "arfq_attn_join.h"
@@ -14,7 +17,8 @@ namespace arfq {
 namespace {
 
 // Chosen pages, and blocks to choose them from, up to which the attention's workgroups choose by themselves: a launch and a
-// table's way through memory less, but every piece of a row's keys looks through all of the row's blocks.
+// table's way through memory less (the long document 30.8 us for 36.7, 32 sequences 40 for 45), but every piece of a row's keys
+// looks through all of the row's blocks, and its LDS holds the pages.
 constexpr int WIDTH_LDS = 2048, BLOCKS_LDS = 16384;
 
 // ---- rows ------------------------------------------------------------------------------------
@@ -202,6 +206,7 @@ __global__ __launch_bounds__(256) void kv_bounds_kernel(KvArgs a, _Float16 *boun
 template <int NG>
 hipError_t bounds_launch(const KvArgs &a, _Float16 *bounds, int cus, hipStream_t s) {
     const int64_t rows = (int64_t)a.tokens * a.heads;
+    // (a workgroup a page: 8 rows of 64 keys 3.6 us for 5.8 by a wave; 2048 rows, of which 64 have a page, 8.6 for 5.2)
     if (rows <= 2 * (int64_t)cus) {
         kv_bounds_kernel<NG, true><<<grid_of(rows), 256, 0, s>>>(a, bounds, 1, (int)rows);
         return hipGetLastError();
@@ -247,9 +252,9 @@ struct ScoreArgs {
 // over [max(q, 0), min(q, 0)] times [hi, lo].  The products of an f32 and an f16 are exact in 64 bits, so that nothing but the
 // order of the sum's last bits is left to chance: blocks' order is that of their scores.  A lane of the operands has
 // the channels D / 4 * (lane / 16) .. of its block or column.  The workgroup's waves have other blocks of the same columns,
-// whose q is in LDS as the products take it: the vector unit's conversions do not overlap with these products (256 rows of 520
-// blocks, 32 x 64 on 8: 37 us with q converted beside each product, 29 so).
-// Waves of a SIMD.
+// whose q is in LDS as the products take it.  256 rows of 520 blocks, 32 x 64 on 8: 34 us, the matrix cores busy half of a wave's
+// time (14 us of 64-cycle instructions); one row of 2048 blocks, 40 x 128 on 8: 8, of which a tile's products are 1.7.
+// Waves of a SIMD, which the split of the blocks counts on.  (Three / four of them at 64 channels 43 and 44 us for 34.)
 constexpr int score_waves(int ng) { return ng <= 4 ? 2 : 1; }
 template <int NG>
 __global__ __launch_bounds__(256, score_waves(NG)) void blocks_score(ScoreArgs a) {
@@ -653,7 +658,7 @@ hipError_t attend_launch(const RowsArgs &r, hipStream_t s) {
     return hipGetLastError();
 }
 
-// Blocks that a wave scores: all of a short sequence's; of long ones so many that the chip is filled.
+// Blocks that a wave scores: a workgroup's four waves share a tile's, several workgroups where that leaves SIMDs without their waves.
 int score_blocks(int cus, int waves, int64_t tiles, int max_pages) {
     const int64_t want = 4 * waves * (int64_t)cus / std::max<int64_t>(tiles, 1);  // waves of a tile
     int64_t n = (max_pages + std::max<int64_t>(want, 4) - 1) / std::max<int64_t>(want, 4);

@@ -5,9 +5,10 @@
 // f32; the second adds the parts in order, and B_e h to base.  Few rows: a workgroup has one row (and a range of k, or of n)
 // on the vector unit, products in f32.  Many rows: tiles of neighbouring rows on the matrix cores, once for each adapter that the
 // tile's rows name; an f32 x goes through v_mfma_f32_16x16x4_f32 as it is, an f16 x is exact in f16 operands, and h
-// enters the second product as two f16 parts of 22 bits of the row's largest.  Every adapter has accumulators of its
-// own: a NaN in one does not reach another's rows.  Bound by memory: the adapters' bytes for few rows, base and out for
-// many.
+// enters the second product as two f16 parts of 22 bits of the row's largest.  Every adapter has accumulators of its own: a NaN
+// in one does not reach another's rows.  Bound by memory and latency: 64 rows of 32 adapters, 5120 x 7168, rank 16, 17.6 MB
+// in 8.6 us (4.1 and 5.2 of it on the device: the row's id, then what it names); 2048 rows of four, 5120 x 17408, rank 64,
+// f16, 318 MB in 98: 21, of which the f16 products are 3, and 78 for base and out at 3.7 TB/s (rank 16: 13 and 66).
 #include "arfq_step.h"
 
 #include <math.h>
