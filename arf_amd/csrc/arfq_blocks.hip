@@ -5,7 +5,7 @@
 // (blocks_select, or choose() within the next), attention with those pages as the row's table (blocks_attend: the tile of
 // arfq_attn_rows16.h, a row a sequence of its own), and the joining of rows whose keys were cut into pieces.
 // One token at 131071, 64 of 2048 blocks of 64, 40 x 128 on 8, f32: bounds 4, scores 8, attention 13 (6 of it the choice), join
-// 4 us: latency.  256 rows of a prompt, 32 of 520 blocks of 32, 32 x 64 on 8, f16: 5, 34 and 46 (four rows of 16 in a tile's
+// 4 us: latency.  256 rows of a prompt, 32 of 520 blocks of 32, 32 x 64 on 8, f16: 5, 30 and 44 (four rows of 16 in a tile's
 // products, whose operands are made for every row anew).
 #include <math.h>
 
@@ -226,13 +226,19 @@ typedef double f64x4 __attribute__((ext_vector_type(4)));
 // Scores as whole numbers in their order.  Those of chosen blocks by rule are never formed; NaN comes first, pages
 // that are not the cache's last.
 constexpr uint64_t KEY_NAN = ~0ull, KEY_NONE = 0;
-__device__ __forceinline__ uint64_t key_of(double v) {
-    if (v != v) return KEY_NAN;
+__device__ __forceinline__ uint64_t key_of(double v, bool number) {
+    if (!number && v != v) return KEY_NAN;
     const uint64_t u = __builtin_bit_cast(uint64_t, v + 0.0);  // (-0 as 0)
-    return u >> 63 ? ~u : u | 1ull << 63;
+    const uint32_t hi = (uint32_t)(u >> 32), sign = (uint32_t)((int32_t)hi >> 31);
+    return (uint64_t)(hi ^ (sign | 0x80000000u)) << 32 | ((uint32_t)u ^ sign);
 }
-__device__ __forceinline__ uint64_t shfl64(uint64_t v, int lane) {
-    return (uint64_t)(uint32_t)__shfl((int)(v >> 32), lane) << 32 | (uint32_t)__shfl((int)v, lane);
+// Of the lane N further on in the 16 lanes of a row, around its end.
+template <int N, class T>
+__device__ __forceinline__ T lane_on(T t) {
+    constexpr int ror = 0x120 + 16 - N;
+    const uint64_t v = __builtin_bit_cast(uint64_t, t);
+    return __builtin_bit_cast(T, (uint64_t)(uint32_t)__builtin_amdgcn_update_dpp(0, (int)(v >> 32), ror, 0xf, 0xf, false) << 32 |
+                                     (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, ror, 0xf, 0xf, false));
 }
 
 struct ScoreArgs {
@@ -244,7 +250,8 @@ struct ScoreArgs {
     int group, count;
     int row0, rows;       // of the chunk
     int per_tile;         // rows of a tile
-    int blocks;           // of a wave
+    int parts;            // workgroups of a tile's blocks
+    int second;           // workgroups from this one on are likely the second ones of their compute units
     uint64_t *keys;       // [rows][heads][max_pages]
 };
 
@@ -252,9 +259,11 @@ struct ScoreArgs {
 // over [max(q, 0), min(q, 0)] times [hi, lo].  The products of an f32 and an f16 are exact in 64 bits, so that nothing but the
 // order of the sum's last bits is left to chance: blocks' order is that of their scores.  A lane of the operands has
 // the channels D / 4 * (lane / 16) .. of its block or column.  The workgroup's waves have other blocks of the same columns,
-// whose q is in LDS as the products take it.  256 rows of 520 blocks, 32 x 64 on 8: 34 us, the matrix cores busy half of a wave's
-// time (14 us of 64-cycle instructions); one row of 2048 blocks, 40 x 128 on 8: 8, of which a tile's products are 1.7.
-// Waves of a SIMD, which the split of the blocks counts on.  (Three / four of them at 64 channels 43 and 44 us for 34.)
+// whose q is in LDS as the products take it.  The vector unit's instructions do not overlap with these products (two waves
+// a SIMD: 69 cycles a product alone, 85 with three of them between), so what is not a product is kept short: 256 rows of 520
+// blocks, 32 x 64 on 8: 29.7 us, 14 of them products at 64 cycles (34.2 with operands made product by product, and keys of
+// every column compared as whole numbers); one row of 2048 blocks, 40 x 128 on 8: 8, of which a tile's products are 1.7.
+// Waves of a SIMD, which the split of the blocks counts on.  (Three / four of them at 64 channels a quarter slower.)
 constexpr int score_waves(int ng) { return ng <= 4 ? 2 : 1; }
 template <int NG>
 __global__ __launch_bounds__(256, score_waves(NG)) void blocks_score(ScoreArgs a) {
@@ -262,11 +271,10 @@ __global__ __launch_bounds__(256, score_waves(NG)) void blocks_score(ScoreArgs a
     __shared__ f64x2 qs[DL][WAVE];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, kg = lane >> 4;
     const KvArgs &kv = a.c;
-    const int parts = (kv.max_pages + 4 * a.blocks - 1) / (4 * a.blocks);
     int block = block_of();
     const int head = block % kv.heads;
     block /= kv.heads;
-    const int part = block % parts, j0 = (part * 4 + wave) * a.blocks, row0 = block / parts * a.per_tile;
+    const int part = block % a.parts, row0 = block / a.parts * a.per_tile;
     if (row0 >= a.rows) return;
     // this lane's column
     const int rt = c / a.group;  // (0 where the group has more than 16 heads)
@@ -278,7 +286,12 @@ __global__ __launch_bounds__(256, score_waves(NG)) void blocks_score(ScoreArgs a
         if (rt == r) mine = x;
         if (x.seen > a.count) most = max(most, x.seen);
     }
-    if (part * 4 * a.blocks >= most) return;
+    // this wave's blocks [j0, j1): shares of whole sixteens, one more for the last ones where they do not come out even (the
+    // first ones of a second workgroup: a SIMD has both workgroups' wave of a number)
+    const int sixteens = (most + 15) / 16, share = sixteens / (4 * a.parts), odd = 4 * a.parts - sixteens % (4 * a.parts);
+    auto share_of = [&](int w) { return 16 * (w * share + max(w - odd, 0)); };
+    if (share_of(4 * part) == share_of(4 * part + 4)) return;
+    const int of = 4 * part + ((int)blockIdx.x >= a.second ? 3 - wave : wave), j0 = share_of(of), j1 = share_of(of + 1);
     if (mine.seen <= a.count) mine.b = -1;  // (its blocks are all chosen)
     const int64_t t = (int64_t)a.row0 + row0 + rt;
     // (one pass, unless the group has more than 16 heads)
@@ -317,7 +330,7 @@ __global__ __launch_bounds__(256, score_waves(NG)) void blocks_score(ScoreArgs a
             int last = mine.b == b ? mine.seen : 0;
 #pragma unroll
             for (int d = 1; d < 16; d *= 2) last = max(last, __shfl_xor(last, d));
-            last = min(__builtin_amdgcn_readfirstlane(last), j0 + a.blocks);
+            last = min(__builtin_amdgcn_readfirstlane(last), j1);
             if (j0 >= last) continue;
             const int32_t *table = kv.table + (int64_t)b * kv.max_pages;
             // bounds a tile ahead of their use, pages 64 blocks at a time; keys are stored a tile later, so that no load's
@@ -341,14 +354,15 @@ __global__ __launch_bounds__(256, score_waves(NG)) void blocks_score(ScoreArgs a
             };
             const int heads = a.group > 16 ? 16 : a.group, h0 = a.group > 16 ? c : c - rt * a.group;
             const bool first = h0 == 0 && mine.b == b;
+            const bool plain = a.group <= 16 || g0 + 16 <= a.group;  // every column of a row is one of its heads
             uint64_t *out = a.keys + ((int64_t)(row0 + rt) * kv.heads + head) * kv.max_pages;
             uint64_t key[4];
+            const int to = first ? min(mine.seen, last) - kg : 0;
             auto store = [&](int j) {  // a lane's four results: blocks kg, kg + 4, .. of the 16, its column
+                uint64_t *o = out + j + kg;
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const int jj = j + kg + 4 * i;
-                    if (first && jj < min(mine.seen, last)) out[jj] = g0 == 0 ? key[i] : max(key[i], out[jj]);
-                }
+                for (int i = 0; i < 4; i++)
+                    if (j + 4 * i < to) o[4 * i] = g0 == 0 ? key[i] : max(key[i], o[4 * i]);
             };
             bool page = load(j0);
             for (int j = j0; j < last; j += 16) {
@@ -362,23 +376,54 @@ __global__ __launch_bounds__(256, score_waves(NG)) void blocks_score(ScoreArgs a
                 const bool there = page;
                 if (j + 16 < last) page = load(j + 16);
                 if (j > j0) store(j - 16);
+                // (operands of eight channels made together: each change between the two units costs some cycles more)
 #pragma unroll
-                for (int i = 0; i < DL; i++) {
-                    const f64x2 q = qs[i][lane];
-                    up = __builtin_amdgcn_mfma_f64_16x16x4f64((double)(float)h[i / 8][i % 8], q.x, up, 0, 0, 0);
-                    down = __builtin_amdgcn_mfma_f64_16x16x4f64((double)(float)l[i / 8][i % 8], q.y, down, 0, 0, 0);
-                }
-                const uint64_t pages = __ballot(there);  // (lane n has block n's page)
+                for (int ch = 0; ch < DL / 8; ch++) {
+                    f64x2 q[8];
+                    double x[8], y[8];
 #pragma unroll
-                for (int i = 0; i < 4; i++) key[i] = on && (pages >> (kg + 4 * i) & 1) ? key_of(up[i] + down[i]) : KEY_NONE;
-                // the largest of the row's heads, at the first of them
-                for (int d = 1; d < heads; d *= 2) {
-                    const int other = (lane & 48) | ((c + d) & 15);
+                    for (int e = 0; e < 8; e++) q[e] = qs[8 * ch + e][lane];
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const uint64_t k = shfl64(key[i], other);
-                        if (h0 + d < heads) key[i] = max(key[i], k);
+                    for (int e = 0; e < 8; e++) {
+                        x[e] = (double)(float)h[ch][e];
+                        y[e] = (double)(float)l[ch][e];
                     }
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        up = __builtin_amdgcn_mfma_f64_16x16x4f64(x[e], q[e].x, up, 0, 0, 0);
+                        down = __builtin_amdgcn_mfma_f64_16x16x4f64(y[e], q[e].y, down, 0, 0, 0);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                // the largest of the row's heads, at the first of them (of its lanes alone the results are stored)
+                double v[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) v[i] = up[i] + down[i];
+                const double all = (v[0] + v[1]) + (v[2] + v[3]);
+                const uint64_t pages = __ballot(there);  // (lane n has block n's page)
+                auto heads_max = [&](auto &best) {
+                    auto wider = [&](auto step) {
+                        constexpr int N = decltype(step)::value;
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const auto k = lane_on<N>(best[i]);
+                            if (h0 + N < heads && k > best[i]) best[i] = k;
+                        }
+                    };
+                    if (heads > 1) wider(std::integral_constant<int, 1>());
+                    if (heads > 2) wider(std::integral_constant<int, 2>());
+                    if (heads > 4) wider(std::integral_constant<int, 4>());
+                    if (heads > 8) wider(std::integral_constant<int, 8>());
+                };
+                if (plain && pages == ~0ull && __ballot(all != all) == 0) {  // numbers throughout
+                    heads_max(v);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) key[i] = key_of(v[i], true);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; i++) key[i] = on && (pages >> (kg + 4 * i) & 1) ? key_of(v[i], false) : KEY_NONE;
+                    heads_max(key);
                 }
             }
             store(j0 + (last - 1 - j0) / 16 * 16);
@@ -609,9 +654,12 @@ struct RowItem {
     __device__ __forceinline__ bool none() const { return r.b < 0 || piece >= pieces; }
 };
 
+// Waves of a SIMD that the registers are for: five at 64 channels and one part (256 rows of 32 chosen blocks 44.2 us, 45.6 with
+// four; two parts would go to scratch).
+constexpr int attend_waves(int ng, int parts) { return ng == 2 && parts == 1 ? 5 : rows16_waves(ng); }
 // CHOOSE: every workgroup chooses for itself, into its LDS (behind the tile's).
 template <int NG, int PARTS, bool CHOOSE>
-__global__ __launch_bounds__(256, rows16_waves(NG)) void blocks_attend(RowsArgs r) {
+__global__ __launch_bounds__(256, attend_waves(NG, PARTS)) void blocks_attend(RowsArgs r) {
     extern __shared__ float lds[];
     __shared__ SelLds sh;
     const int block = block_of(), head = block % r.a.c.heads, slot = block / r.a.c.heads;
@@ -658,11 +706,10 @@ hipError_t attend_launch(const RowsArgs &r, hipStream_t s) {
     return hipGetLastError();
 }
 
-// Blocks that a wave scores: a workgroup's four waves share a tile's, several workgroups where that leaves SIMDs without their waves.
-int score_blocks(int cus, int waves, int64_t tiles, int max_pages) {
-    const int64_t want = 4 * waves * (int64_t)cus / std::max<int64_t>(tiles, 1);  // waves of a tile
-    int64_t n = (max_pages + std::max<int64_t>(want, 4) - 1) / std::max<int64_t>(want, 4);
-    return (int)((n + 15) / 16 * 16);
+// Workgroups of a tile's blocks, which its four waves share: several where one leaves SIMDs without their waves, as far as there
+// are sixteen blocks for a wave.
+int score_parts(int cus, int waves, int64_t tiles, int max_pages) {
+    return (int)std::max<int64_t>(1, std::min(waves * (int64_t)cus / std::max<int64_t>(tiles, 1), ((int64_t)max_pages + 63) / 64));
 }
 
 template <int NG>
@@ -675,12 +722,11 @@ hipError_t dim_launch(const BlocksArgs &b, const BlocksPlan &p, int cus, hipStre
         hipError_t e;
         if (c.max_pages > b.count) {
             ScoreArgs sc = {c, b.bounds, b.a.q, b.a.q_stride, b.a.q_dtype == ARFQ_F16, b.a.scale < 0.0f, b.a.group, b.count, row0, rows,
-                            std::max(1, 16 / b.a.group), 0, keys};
+                            std::max(1, 16 / b.a.group), 1, cus, keys};
             if (!c.start) sc.per_tile = 1;  // (no two rows have blocks in common)
             const int64_t tiles = (int64_t)((rows + sc.per_tile - 1) / sc.per_tile) * c.heads;
-            sc.blocks = score_blocks(cus, score_waves(NG), tiles, c.max_pages);
-            const int64_t parts = (c.max_pages + 4 * (int64_t)sc.blocks - 1) / (4 * (int64_t)sc.blocks);
-            blocks_score<NG><<<grid_of(tiles * parts), 256, 0, s>>>(sc);
+            sc.parts = score_parts(cus, score_waves(NG), tiles, c.max_pages);
+            blocks_score<NG><<<grid_of(tiles * sc.parts), 256, 0, s>>>(sc);
             if ((e = hipGetLastError()) != hipSuccess) return e;
         }
         const ChooseArgs ch = {c, keys, p.in_lds ? nullptr : (int32_t *)(b.ws + p.off_table), b.chosen, row0, rows, b.count, b.first, b.last, p.width};

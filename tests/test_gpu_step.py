@@ -485,6 +485,21 @@ def test_long_sequences(gpu_ctx, dtype, lens, count, page, heads, group, dim):
     _check(batch, got, chosen, q, hk, hv, dim ** -0.5, **kw)
 
 
+@pytest.mark.parametrize("heads,group,dim,lens,news", [(8, 4, 64, [1700, 900], [300, 250]), (16, 3, 96, [700, 2100], [130, 131]),
+                                                       (40, 2, 128, [1337], [70])])
+def test_prompts_of_more_tiles_than_compute_units(gpu_ctx, heads, group, dim, lens, news):
+    # (waves' shares of the blocks that do not come out even; a tile with rows of two sequences)
+    _say("blocks of prompts", heads, group, dim, lens, news)
+    rng = np.random.default_rng(heads)
+    batch = Batch(gpu_ctx, lens, news, 16, rng)
+    kv = gpu_ctx.kv_cache(heads, dim, 16, batch.n_pages)
+    hk, hv = _filled(gpu_ctx, kv, batch, rng)
+    q = _rows(rng, batch.tokens, heads * group, dim, np.float16, False)
+    kw = dict(count=10, first=1, last=2)
+    got, chosen = _attend(gpu_ctx, kv, batch, _bounds(gpu_ctx, kv, batch), q, np.float16, dim ** -0.5, **kw)
+    _check(batch, got, chosen, q, hk, hv, dim ** -0.5, rows=[0, 1, 2, 3, 66, 127, 129, 130, 249, 298, 299], **kw)
+
+
 def test_alike_blocks_the_earlier_first(gpu_ctx):
     # keys alike everywhere; alike in runs; scores of zero, +0 and -0
     _say("blocks alike")
