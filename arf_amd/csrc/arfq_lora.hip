@@ -8,7 +8,7 @@
 // enters the second product as two f16 parts of 22 bits of the row's largest.  Every adapter has accumulators of its own: a NaN
 // in one does not reach another's rows.  Bound by memory and latency: 64 rows of 32 adapters, 5120 x 7168, rank 16, 17.6 MB
 // in 8.6 us (4.1 and 5.2 of it on the device: the row's id, then what it names); 2048 rows of four, 5120 x 17408, rank 64,
-// f16, 318 MB in 98: 21, of which the f16 products are 3, and 78 for base and out at 3.7 TB/s (rank 16: 13 and 66).
+// f16, 318 MB in 86: 18, of which the f16 products are 3, and 68 for base and out at 4.5 TB/s (rank 16: 10 and 55).
 #include "arfq_step.h"
 
 #include <math.h>
@@ -355,31 +355,61 @@ __global__ __launch_bounds__(64 * A_WAVES, 2) void lora_tiles_a(LoraArgs a, int 
 // B_ROWS rows, of KS runs of 32 ranks.  Their h first, into LDS: the parts added, and as two f16 parts of it times a power of
 // two that puts a row's largest into [2^14, 2^15).  Then each wave has 16 NT outputs and goes over the rows' tiles: B_e
 // stays in registers while the adapter does, base is loaded a tile ahead.
+// A lane's results are four outputs of each of NT tiles, its neighbours' those of the next rows; they are exchanged
+// for a piece of as many rows, so that a load of base or a store has 64 NT contiguous bytes of a row (2048 rows of 17408 outputs,
+// rank 16: 59 us for 66 with 64 bytes).
 constexpr int B_WAVES = 4;
+template <int CTRL>
+__device__ __forceinline__ void exchange(f32x4 &a, f32x4 &b, bool upper) {  // b of the lower lane for a of the upper
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const float got = dpp<CTRL>(upper ? a[i] : b[i]);
+        if (upper) a[i] = got;
+        else b[i] = got;
+    }
+}
+// Of NT neighbouring lanes: v[j] of lane p becomes v[p] of lane j.
+template <int NT>
+__device__ __forceinline__ void turn_lanes(f32x4 (&v)[NT]) {
+    const int p = threadIdx.x;
+#pragma unroll
+    for (int i = 0; i < NT; i += 2) exchange<0xb1>(v[i], v[i + 1], p & 1);  // quad_perm:[1,0,3,2]
+    if constexpr (NT == 4) {
+        exchange<0x4e>(v[0], v[2], p & 2);  // quad_perm:[2,3,0,1]
+        exchange<0x4e>(v[1], v[3], p & 2);
+    }
+}
 template <int KS>
 struct TileB {
     static constexpr int ROWS = KS <= 4 ? 64 : 32, NT = KS <= 4 ? 4 : 2, RANK = 32 * KS, LD = RANK + 8, OUT = B_WAVES * NT * 16;
 };
-template <int KS, bool VEC>
-__global__ __launch_bounds__(64 * B_WAVES) void lora_tiles_b(LoraArgs a, int splits, int parts) {
+// VEC: four outputs at a time; PAST: base and out go past the caches.  (Three waves a SIMD at two runs, whose registers
+// would be two's: 2048 rows of 17408 outputs 70 us for 80.)
+template <int KS, bool VEC, bool PAST>
+__global__ __launch_bounds__(64 * B_WAVES, KS == 2 ? 3 : 1) void lora_tiles_b(LoraArgs a, int splits, int parts) {
     using T = TileB<KS>;
     constexpr int NT = T::NT, ROWS = T::ROWS;
     __shared__ __align__(16) _Float16 sh[2][ROWS][T::LD];
-    __shared__ float unit[ROWS];
-    __shared__ int ids[ROWS];
+    __shared__ __align__(16) float unit[ROWS];
+    __shared__ __align__(16) int ids[ROWS];
     const int block = block_of(), part = block % parts, t0 = block / parts * ROWS;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
     if (t0 >= a.rows) return;
     const int rank = (int)a.l.rank;
     const int64_t n = a.l.n, n0 = (int64_t)part * T::OUT + wave * (NT * 16);
+    // behind the exchange: rows c0 .. of a tile, outputs `own` ..
+    const int c0 = c & ~(NT - 1);
+    const int64_t own = n0 + 16 * (c & (NT - 1)) + 4 * g;
     f32x4 next[NT];  // base of the tile to come
     auto load_base = [&](int s) {
 #pragma unroll
-        for (int i = 0; i < NT; i++) {
-            const int64_t at = n0 + 16 * i + 4 * g;
-            next[i] = f32x4{0, 0, 0, 0};
-            if (VEC && a.base && at < n && t0 + 16 * s + c < a.rows)
-                next[i] = *(const f32x4 *)(a.base + (int64_t)(t0 + 16 * s + c) * a.base_stride + at);
+        for (int j = 0; j < NT; j++) {
+            const int t = t0 + 16 * s + c0 + j;
+            next[j] = f32x4{0, 0, 0, 0};
+            if (VEC && a.base && own < n && t < a.rows) {
+                const f32x4 *from = (const f32x4 *)(a.base + (int64_t)t * a.base_stride + own);
+                next[j] = PAST ? __builtin_nontemporal_load(from) : *from;
+            }
         }
     };
     f16x8 w[NT][KS];
@@ -451,11 +481,7 @@ __global__ __launch_bounds__(64 * B_WAVES) void lora_tiles_b(LoraArgs a, int spl
 #pragma unroll
         for (int i = 0; i < NT; i++) base[i] = next[i];
         if (s + 1 < ROWS / 16) load_base(s + 1);
-        const int t = t0 + 16 * s + c;
         const int mine = ids[16 * s + c];
-        const float f = unit[16 * s + c];
-        float *out = a.out + (int64_t)t * a.out_stride;
-        const float *from = a.base ? a.base + (int64_t)t * a.base_stride : nullptr;
         uint64_t done = 0;
         for (int e; (e = next_id(mine, done)) != -2;) {
             f32x4 acc[NT];
@@ -473,13 +499,27 @@ __global__ __launch_bounds__(64 * B_WAVES) void lora_tiles_b(LoraArgs a, int spl
                         for (int i = 0; i < NT; i++) acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[i][q], h, acc[i], 0, 0, 0);
                     }
             }
-            if (mine != e || t >= a.rows || (e < 0 && from == out)) continue;
+            if constexpr (VEC) {
+                if (e >= 0) turn_lanes<NT>(acc);
 #pragma unroll
-            for (int i = 0; i < NT; i++) {
-                const int64_t at = n0 + 16 * i + 4 * g;
-                if constexpr (VEC) {
-                    if (at < n) *(f32x4 *)(out + at) = e < 0 ? base[i] : base[i] + acc[i] * f;
-                } else {
+                for (int j = 0; j < NT; j++) {
+                    const int at = 16 * s + c0 + j;
+                    if (ids[at] != e || t0 + at >= a.rows || own >= n) continue;
+                    float *o = a.out + (int64_t)(t0 + at) * a.out_stride;
+                    if (e < 0 && a.base && a.base + (int64_t)(t0 + at) * a.base_stride == o) continue;
+                    const f32x4 v = e < 0 ? base[j] : base[j] + acc[j] * unit[at];
+                    if (PAST) __builtin_nontemporal_store(v, (f32x4 *)(o + own));
+                    else *(f32x4 *)(o + own) = v;
+                }
+            } else {
+                const int t = t0 + 16 * s + c;
+                float *out = a.out + (int64_t)t * a.out_stride;
+                const float *from = a.base ? a.base + (int64_t)t * a.base_stride : nullptr;
+                if (mine != e || t >= a.rows || (e < 0 && from == out)) continue;
+                const float f = unit[16 * s + c];
+#pragma unroll
+                for (int i = 0; i < NT; i++) {
+                    const int64_t at = n0 + 16 * i + 4 * g;
 #pragma unroll
                     for (int j = 0; j < 4; j++)
                         if (at + j < n) {
@@ -526,14 +566,20 @@ hipError_t tiles_a(const LoraArgs &a, const LoraPlan &p, hipStream_t s) {
     return hipGetLastError();
 }
 
+// Bytes of base and out from which on they go past the caches.  us past them / through: rank 64, k = 5120, 2048 rows of 17408
+// outputs (285 MB) 86 / 92, 1024 rows (143) 56.5 / 59; 2048 rows of 5120 (84) 43 / 39, 512 rows of 17408 (71) 37 / 34.
+constexpr int64_t PAST_BYTES = (int64_t)112 << 20;
+
 template <int KS>
 hipError_t tiles_b(const LoraArgs &a, const LoraPlan &p, hipStream_t s) {
     const int parts = (int)((a.l.n + TileB<KS>::OUT - 1) / TileB<KS>::OUT);
     const dim3 grid = grid_of((int64_t)((a.rows + TileB<KS>::ROWS - 1) / TileB<KS>::ROWS) * parts);
     const bool vec = a.l.n % 4 == 0 && a.out_stride % 4 == 0 && (uintptr_t)a.out % 16 == 0 &&
                      (!a.base || (a.base_stride % 4 == 0 && (uintptr_t)a.base % 16 == 0));
-    if (vec) lora_tiles_b<KS, true><<<grid, 64 * B_WAVES, 0, s>>>(a, p.splits, parts);
-    else lora_tiles_b<KS, false><<<grid, 64 * B_WAVES, 0, s>>>(a, p.splits, parts);
+    const bool past = a.rows * a.l.n * (int64_t)sizeof(float) * (a.base ? 2 : 1) >= PAST_BYTES;
+    if (!vec) lora_tiles_b<KS, false, false><<<grid, 64 * B_WAVES, 0, s>>>(a, p.splits, parts);
+    else if (past) lora_tiles_b<KS, true, true><<<grid, 64 * B_WAVES, 0, s>>>(a, p.splits, parts);
+    else lora_tiles_b<KS, true, false><<<grid, 64 * B_WAVES, 0, s>>>(a, p.splits, parts);
     return hipGetLastError();
 }
 
