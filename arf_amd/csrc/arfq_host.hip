@@ -855,7 +855,7 @@ int arfq_lora_add(arfq_ctx *ctx, const arfq_lora *lora, const int32_t *ids, int6
     const arfq::LoraPlan plan = arfq::lora_plan(ctx->cus, *lora, rows);
     if (int rc = take_workspace(ctx, "lora_add", plan.ws_bytes, workspace_bytes, &workspace)) return rc;
     const arfq::LoraArgs a = {*lora, ids, (int)rows, x, x_dtype == ARFQ_F16, base, out, base_stride, out_stride, (float *)workspace};
-    const hipError_t e = arfq::launch_lora(a, plan, ctx->stream);
+    const hipError_t e = arfq::launch_lora(a, plan, ctx->cus, ctx->stream);
     return e == hipSuccess ? ARFQ_OK : hip_fail(ctx, e, "lora_add launch");
 }
 

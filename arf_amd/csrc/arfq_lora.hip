@@ -383,32 +383,39 @@ template <int KS>
 struct TileB {
     static constexpr int ROWS = KS <= 4 ? 64 : 32, NT = KS <= 4 ? 4 : 2, RANK = 32 * KS, LD = RANK + 8, OUT = B_WAVES * NT * 16;
 };
-// VEC: four outputs at a time; PAST: base and out go past the caches.  (Three waves a SIMD at two runs, whose registers
-// would be two's: 2048 rows of 17408 outputs 70 us for 80.)
-template <int KS, bool VEC, bool PAST>
-__global__ __launch_bounds__(64 * B_WAVES, KS == 2 ? 3 : 1) void lora_tiles_b(LoraArgs a, int splits, int parts) {
+// Base and out four at a time, at any address of a float.  PAST: past the caches.  `span`: rows of a workgroup, up to ROWS.
+// (Three waves a SIMD at two runs, whose registers would be two's: 2048 rows of 17408 outputs 70 us for 80.)
+typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
+template <int KS, bool PAST>
+__global__ __launch_bounds__(64 * B_WAVES, KS == 2 ? 3 : 1) void lora_tiles_b(LoraArgs a, int splits, int parts, int span) {
     using T = TileB<KS>;
     constexpr int NT = T::NT, ROWS = T::ROWS;
     __shared__ __align__(16) _Float16 sh[2][ROWS][T::LD];
     __shared__ __align__(16) float unit[ROWS];
     __shared__ __align__(16) int ids[ROWS];
-    const int block = block_of(), part = block % parts, t0 = block / parts * ROWS;
+    const int block = block_of(), part = block % parts, t0 = block / parts * span;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
     if (t0 >= a.rows) return;
-    const int rank = (int)a.l.rank;
+    const int rank = (int)a.l.rank, rows = min(span, a.rows - t0);
     const int64_t n = a.l.n, n0 = (int64_t)part * T::OUT + wave * (NT * 16);
     // behind the exchange: rows c0 .. of a tile, outputs `own` ..
     const int c0 = c & ~(NT - 1);
     const int64_t own = n0 + 16 * (c & (NT - 1)) + 4 * g;
+    const int left = (int)max((int64_t)0, min(n - own, (int64_t)4));  // of its four outputs
     f32x4 next[NT];  // base of the tile to come
     auto load_base = [&](int s) {
 #pragma unroll
         for (int j = 0; j < NT; j++) {
-            const int t = t0 + 16 * s + c0 + j;
+            const int at = 16 * s + c0 + j;
             next[j] = f32x4{0, 0, 0, 0};
-            if (VEC && a.base && own < n && t < a.rows) {
-                const f32x4 *from = (const f32x4 *)(a.base + (int64_t)t * a.base_stride + own);
-                next[j] = PAST ? __builtin_nontemporal_load(from) : *from;
+            if (!a.base || at >= rows) continue;
+            const float *from = a.base + (int64_t)(t0 + at) * a.base_stride + own;
+            if (left == 4) {
+                next[j] = PAST ? __builtin_nontemporal_load((const f32x4_any *)from) : *(const f32x4_any *)from;
+            } else {
+#pragma unroll
+                for (int i = 0; i < 3; i++)
+                    if (i < left) next[j][i] = from[i];
             }
         }
     };
@@ -429,7 +436,7 @@ __global__ __launch_bounds__(64 * B_WAVES, KS == 2 ? 3 : 1) void lora_tiles_b(Lo
     constexpr int APART = 64 * B_WAVES / LANES;
 #pragma unroll
     for (int it = 0; it < ITEMS; it++) {
-        of[it] = t0 + row0 + it * APART < a.rows ? id_of(a, t0 + row0 + it * APART) : -1;
+        of[it] = row0 + it * APART < rows ? id_of(a, t0 + row0 + it * APART) : -1;
 #pragma unroll
         for (int j = 0; j < 8; j++) h[it][j] = 0.0f;
     }
@@ -438,6 +445,7 @@ __global__ __launch_bounds__(64 * B_WAVES, KS == 2 ? 3 : 1) void lora_tiles_b(Lo
     for (int p = 0; p < splits; p++)
 #pragma unroll
         for (int it = 0; it < ITEMS; it++) {
+            if (it * APART >= rows) continue;
             float v[8];
             load8<false>(a.h, ((int64_t)p * a.rows + min(t0 + row0 + it * APART, a.rows - 1)) * rank + min(8 * u, rank - 8), v);
 #pragma unroll
@@ -476,11 +484,11 @@ __global__ __launch_bounds__(64 * B_WAVES, KS == 2 ? 3 : 1) void lora_tiles_b(Lo
     lds_barrier();
     if (n0 >= n) return;
 #pragma unroll 1
-    for (int s = 0; s < ROWS / 16 && t0 + 16 * s < a.rows; s++) {
+    for (int s = 0; 16 * s < rows; s++) {
         f32x4 base[NT];
 #pragma unroll
         for (int i = 0; i < NT; i++) base[i] = next[i];
-        if (s + 1 < ROWS / 16) load_base(s + 1);
+        if (16 * (s + 1) < rows) load_base(s + 1);
         const int mine = ids[16 * s + c];
         uint64_t done = 0;
         for (int e; (e = next_id(mine, done)) != -2;) {
@@ -499,44 +507,33 @@ __global__ __launch_bounds__(64 * B_WAVES, KS == 2 ? 3 : 1) void lora_tiles_b(Lo
                         for (int i = 0; i < NT; i++) acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[i][q], h, acc[i], 0, 0, 0);
                     }
             }
-            if constexpr (VEC) {
-                if (e >= 0) turn_lanes<NT>(acc);
+            if (e >= 0) turn_lanes<NT>(acc);
 #pragma unroll
-                for (int j = 0; j < NT; j++) {
-                    const int at = 16 * s + c0 + j;
-                    if (ids[at] != e || t0 + at >= a.rows || own >= n) continue;
-                    float *o = a.out + (int64_t)(t0 + at) * a.out_stride;
-                    if (e < 0 && a.base && a.base + (int64_t)(t0 + at) * a.base_stride == o) continue;
-                    const f32x4 v = e < 0 ? base[j] : base[j] + acc[j] * unit[at];
-                    if (PAST) __builtin_nontemporal_store(v, (f32x4 *)(o + own));
-                    else *(f32x4 *)(o + own) = v;
-                }
-            } else {
-                const int t = t0 + 16 * s + c;
-                float *out = a.out + (int64_t)t * a.out_stride;
-                const float *from = a.base ? a.base + (int64_t)t * a.base_stride : nullptr;
-                if (mine != e || t >= a.rows || (e < 0 && from == out)) continue;
-                const float f = unit[16 * s + c];
+            for (int j = 0; j < NT; j++) {
+                const int at = 16 * s + c0 + j;
+                if (at >= rows || ids[at] != e) continue;
+                float *o = a.out + (int64_t)(t0 + at) * a.out_stride;
+                if (e < 0 && a.base && a.base + (int64_t)(t0 + at) * a.base_stride == o) continue;
+                const f32x4 v = e < 0 ? base[j] : base[j] + acc[j] * unit[at];
+                if (left == 4) {
+                    if (PAST) __builtin_nontemporal_store(v, (f32x4_any *)(o + own));
+                    else *(f32x4_any *)(o + own) = v;
+                } else {
 #pragma unroll
-                for (int i = 0; i < NT; i++) {
-                    const int64_t at = n0 + 16 * i + 4 * g;
-#pragma unroll
-                    for (int j = 0; j < 4; j++)
-                        if (at + j < n) {
-                            const float v = from ? from[at + j] : 0.0f;
-                            out[at + j] = e < 0 ? v : v + acc[i][j] * f;
-                        }
+                    for (int i = 0; i < 3; i++)
+                        if (i < left) o[own + i] = v[i];
                 }
             }
         }
     }
 }
 
-// rows * (k + n) from which on tiles are taken.  us one by one and in tiles, rows of two adapters in two runs / rows of 32 in any
-// order: rank 16, k + n = 12288, 256 rows 16.8 and 17.4 / 19 and 65, 512 rows 28 and 19 / 30 and 82; k + n = 22528, 128 rows
-// 17.7 and 17.7 / 19.6 and 55; rank 64, k + n = 12288, 256 rows 29 and 28 / 44 and 124; k + n = 1024, 1024 rows 11.6 and 21.
-// (The ids are on the device: the border leans to the side that loses less.)
-constexpr int64_t TILE_VALUES = 4 << 20;
+// rows * (k + n) * rank (64 at least) from which on tiles are taken.  us one by one and in tiles, rows of two adapters in two runs /
+// rows of 32 in any order: rank 16, k + n = 12288, 256 rows 17.2 and 14.2 / 19 and 37, 512 rows 29 and 17.8 / 30 and 62;
+// rank 64, 256 rows 28 and 18.7 / 43 and 65, 512 rows 47 and 23.5 / 75 and 111; rank 128, 128 rows 28 and 20 / 46 and
+// 71, 256 rows 49 and 26 / 91 and 115; k + n = 4096, rank 64, 1024 rows 34 and 17.7 / 34 and 77; k + n = 1024, 1024 rows 11.7 and
+// 13.4 / 12.9 and 37.  (The ids are on the device: the border leans to the side that loses less.)
+constexpr int64_t TILE_VALUES = (int64_t)1 << 28;
 
 // Values of A_e, and of it over all workgroups, up to which both products of rows one by one are one launch.  us in one and
 // in two: k = n = 512, rank 16, any rows up to 256 4.3 and 6.8; k = n = 2048, rank 64 (2^17 of A), one row 7.1 and 8.2;
@@ -571,15 +568,15 @@ hipError_t tiles_a(const LoraArgs &a, const LoraPlan &p, hipStream_t s) {
 constexpr int64_t PAST_BYTES = (int64_t)112 << 20;
 
 template <int KS>
-hipError_t tiles_b(const LoraArgs &a, const LoraPlan &p, hipStream_t s) {
+hipError_t tiles_b(const LoraArgs &a, const LoraPlan &p, int cus, hipStream_t s) {
     const int parts = (int)((a.l.n + TileB<KS>::OUT - 1) / TileB<KS>::OUT);
-    const dim3 grid = grid_of((int64_t)((a.rows + TileB<KS>::ROWS - 1) / TileB<KS>::ROWS) * parts);
-    const bool vec = a.l.n % 4 == 0 && a.out_stride % 4 == 0 && (uintptr_t)a.out % 16 == 0 &&
-                     (!a.base || (a.base_stride % 4 == 0 && (uintptr_t)a.base % 16 == 0));
+    // fewer rows a workgroup where these would not fill the chip (701 rows of 138 outputs, rank 40: 9.3 us for 27)
+    int span = TileB<KS>::ROWS;
+    while (span > 16 && (int64_t)((a.rows + span - 1) / span) * parts <= cus) span /= 2;
+    const dim3 grid = grid_of((int64_t)((a.rows + span - 1) / span) * parts);
     const bool past = a.rows * a.l.n * (int64_t)sizeof(float) * (a.base ? 2 : 1) >= PAST_BYTES;
-    if (!vec) lora_tiles_b<KS, false, false><<<grid, 64 * B_WAVES, 0, s>>>(a, p.splits, parts);
-    else if (past) lora_tiles_b<KS, true, true><<<grid, 64 * B_WAVES, 0, s>>>(a, p.splits, parts);
-    else lora_tiles_b<KS, true, false><<<grid, 64 * B_WAVES, 0, s>>>(a, p.splits, parts);
+    if (past) lora_tiles_b<KS, true><<<grid, 64 * B_WAVES, 0, s>>>(a, p.splits, parts, span);
+    else lora_tiles_b<KS, false><<<grid, 64 * B_WAVES, 0, s>>>(a, p.splits, parts, span);
     return hipGetLastError();
 }
 
@@ -587,7 +584,7 @@ hipError_t tiles_b(const LoraArgs &a, const LoraPlan &p, hipStream_t s) {
 
 LoraPlan lora_plan(int cus, const arfq_lora &l, int64_t rows) {
     LoraPlan p;
-    p.tiles = rows * (l.k + l.n) > TILE_VALUES;
+    p.tiles = rows * (l.k + l.n) > TILE_VALUES / std::max<int64_t>(l.rank, 64);
     if (p.tiles) {
         // a workgroup a compute unit, and not fewer than four steps a wave
         const int64_t tiles = (rows + A_TILES * TR - 1) / (A_TILES * TR);
@@ -603,12 +600,12 @@ LoraPlan lora_plan(int cus, const arfq_lora &l, int64_t rows) {
     return p;
 }
 
-hipError_t launch_lora(const LoraArgs &a, const LoraPlan &p, hipStream_t s) {
+hipError_t launch_lora(const LoraArgs &a, const LoraPlan &p, int cus, hipStream_t s) {
     if (p.tiles) {
         hipError_t e = a.l.rank <= 16 ? tiles_a<1>(a, p, s) : a.l.rank <= 32 ? tiles_a<2>(a, p, s) : tiles_a<4>(a, p, s);
         if (e != hipSuccess) return e;
         const int64_t runs = (a.l.rank + 31) / 32;
-        return runs <= 1 ? tiles_b<1>(a, p, s) : runs <= 2 ? tiles_b<2>(a, p, s) : runs <= 4 ? tiles_b<4>(a, p, s) : tiles_b<8>(a, p, s);
+        return runs <= 1 ? tiles_b<1>(a, p, cus, s) : runs <= 2 ? tiles_b<2>(a, p, cus, s) : runs <= 4 ? tiles_b<4>(a, p, cus, s) : tiles_b<8>(a, p, cus, s);
     }
     if (!p.one) {
         const dim3 grid = grid_of((int64_t)a.rows * p.splits);

@@ -50,7 +50,7 @@ struct LoraArgs {
     int64_t base_stride, out_stride;
     float *h;  // the workspace
 };
-hipError_t launch_lora(const LoraArgs &a, const LoraPlan &p, hipStream_t stream);
+hipError_t launch_lora(const LoraArgs &a, const LoraPlan &p, int cus, hipStream_t stream);
 
 // ---- arfq_blocks.hip ----
 hipError_t launch_kv_bounds(const KvArgs &a, int dim, _Float16 *bounds, int cus, hipStream_t stream);

@@ -275,11 +275,12 @@ def test_lora_many_rows(gpu_ctx, xt, rank, k, n):
 
 
 # (base and out of more bytes than the caches are used for)
-@pytest.mark.parametrize("rank,based,strides", [(8, True, (0, 0)), (40, True, (4, 12)), (72, False, (0, 4)), (136, True, (0, 0))])
+@pytest.mark.parametrize("rank,based,strides", [(8, True, (0, 0)), (40, True, (4, 12)), (72, False, (0, 4)), (136, True, (0, 0)),
+                                                 (24, True, (1, 2))])
 def test_lora_large_outputs(gpu_ctx, rank, based, strides):
     _say("lora large", rank, based, strides)
     rng = np.random.default_rng(rank)
-    rows, k, n = 2051, 64, 8196 if based else 16388
+    rows, k, n = 2051, 64, (8196 if based else 16388) + strides[0] % 2
     _lora_case(gpu_ctx, rng, rows, k, n, rank, 4, _runs(rng, rows, 4), np.float16, True, based, strides)
 
 
