@@ -8,7 +8,7 @@
 // enters the second product as two f16 parts of 22 bits of the row's largest.  Every adapter has accumulators of its own: a NaN
 // in one does not reach another's rows.  Bound by memory and latency: 64 rows of 32 adapters, 5120 x 7168, rank 16, 17.6 MB
 // in 8.6 us (4.1 and 5.2 of it on the device: the row's id, then what it names); 2048 rows of four, 5120 x 17408, rank 64,
-// f16, 318 MB in 86: 18, of which the f16 products are 3, and 68 for base and out at 4.5 TB/s (rank 16: 10 and 55).
+// f16, 318 MB in 84: 18, of which the f16 products are 3, and 68 for base and out at 4.5 TB/s (rank 16: 10 and 55).
 #include "arfq_step.h"
 
 #include <math.h>
@@ -605,7 +605,8 @@ hipError_t launch_lora(const LoraArgs &a, const LoraPlan &p, int cus, hipStream_
         hipError_t e = a.l.rank <= 16 ? tiles_a<1>(a, p, s) : a.l.rank <= 32 ? tiles_a<2>(a, p, s) : tiles_a<4>(a, p, s);
         if (e != hipSuccess) return e;
         const int64_t runs = (a.l.rank + 31) / 32;
-        return runs <= 1 ? tiles_b<1>(a, p, cus, s) : runs <= 2 ? tiles_b<2>(a, p, cus, s) : runs <= 4 ? tiles_b<4>(a, p, cus, s) : tiles_b<8>(a, p, cus, s);
+        return runs <= 1 ? tiles_b<1>(a, p, cus, s) : runs <= 2 ? tiles_b<2>(a, p, cus, s) :
+               runs <= 4 ? tiles_b<4>(a, p, cus, s) : tiles_b<8>(a, p, cus, s);
     }
     if (!p.one) {
         const dim3 grid = grid_of((int64_t)a.rows * p.splits);
