@@ -147,3 +147,12 @@ def attend_blocks(q, k, v, page, scale, count, first, last, softcap=0.0, absent=
             for all_, one in zip(res, got):
                 all_[t, mine] = one[0]
     return (*res, min(length, count * page), chosen)
+
+
+def lora_norm_tolerance(out, base, k, rank):
+    """On the norm of all errors, where x, A and B have random signs and one size.  A sum of n terms is rounded n times, by at most
+    2^-24 of a partial sum each; these errors have signs of their own and partial sums are no larger than the sum in root
+    mean square, so their norm is at most sqrt(n) 2^-24 of the sums'.  n is k, then rank; h in two f16 parts is off by 2^-22
+    of its row's largest, at most four times its root mean square; scale and product round h twice more, the sum with base once."""
+    own = out if base is None else out - base
+    return np.linalg.norm(own) * ((np.sqrt(k) + np.sqrt(rank) + 4) * 2.0 ** -24 + 2.0 ** -20) + np.linalg.norm(out) * 2.0 ** -24

@@ -1,0 +1,66 @@
+"""Where a serving step's operators could be off without the other tests' notice: adapters' bits by the norm of the errors, in every
+form of the tiles and one by one."""
+import numpy as np
+import pytest
+
+import arf_amd
+import stepref
+from test_gpu_kv import _say
+from test_step_edges_cpu import RANKS, SHAPES
+
+pytestmark = pytest.mark.gpu
+
+
+def _sample(rng, rows):
+    """Rows that are looked at: the first, the last, others in between."""
+    return np.unique(np.concatenate([np.arange(min(rows, 40)), np.arange(max(rows - 40, 0), rows), rng.integers(0, rows, 150)]))
+
+
+def _adapters(ctx, rng, rows, k, n, rank, ids, xt, based=True, skip=0):
+    """out = base + adapters' products, `skip` elements of x into an allocation; against the oracle by value and by norm."""
+    adapters = 4
+    a = (rng.standard_normal((adapters, rank, k)) / np.sqrt(k)).astype(np.float16)
+    b = rng.standard_normal((adapters, n, rank)).astype(np.float16)
+    x = rng.standard_normal((rows, k), dtype=np.float32).astype(xt)
+    scale = (rng.random(adapters) + 0.5).astype(np.float32)
+    base = rng.standard_normal((rows, n), dtype=np.float32) if based else None
+    dx = ctx.to_device(np.concatenate([np.zeros(skip, xt), x.reshape(-1)]))
+    lora = arf_amd.Lora(ctx.to_device(a), ctx.to_device(b), ctx.to_device(scale))
+    out = ctx.empty((rows, n), np.float32)
+    ctx.lora_add(lora, ctx.to_device(np.asarray(ids, np.int32)), dx.columns(skip) if skip else dx, rows, out,
+                 base=ctx.to_device(base) if based else None)
+    s = _sample(rng, rows)
+    own = base[s] if based else None
+    want, mags = stepref.lora(x[s], np.asarray(ids)[s], a, b, scale, own)
+    off = out.numpy()[s] - want
+    assert (np.abs(off) <= stepref.lora_tolerance(want, mags, own, k, rank)).all()
+    most = stepref.lora_norm_tolerance(want, own, k, rank)
+    print("share of the norm's tolerance", float(np.linalg.norm(off) / most), flush=True)
+    assert np.linalg.norm(off) <= most
+
+
+def _runs(rng, rows):
+    return np.repeat(rng.integers(0, 4, rows), rng.choice([1, 2, 15, 16, 33, 200], rows))[:rows]
+
+
+# rows * (k + n) * (rank + 8) from which on every shape and type is taken in tiles
+IN_TILES = 1.3e9
+
+
+@pytest.mark.parametrize("xt", [np.float32, np.float16])
+@pytest.mark.parametrize("rank", RANKS)
+@pytest.mark.parametrize("k,n", SHAPES)
+def test_adapters_in_tiles_keep_their_bits(gpu_ctx, xt, rank, k, n):
+    rows = int(IN_TILES / ((k + n) * (rank + 8))) + 19
+    _say("adapters' bits", np.dtype(xt).name, rank, rows, k, n)
+    rng = np.random.default_rng(rank + k)
+    _adapters(gpu_ctx, rng, rows, k, n, rank, _runs(rng, rows), xt, based=rank % 16 == 8 or rank == 64)
+
+
+@pytest.mark.parametrize("xt", [np.float32, np.float16])
+@pytest.mark.parametrize("rank", [8, 64, 136])
+@pytest.mark.parametrize("rows,k,n", [(1, 5120, 700), (33, 2056, 2050), (70, 264, 1172)])
+def test_adapters_one_by_one_keep_their_bits(gpu_ctx, xt, rank, rows, k, n):
+    _say("adapters' bits, few rows", np.dtype(xt).name, rank, rows, k, n)
+    rng = np.random.default_rng(rank + k)
+    _adapters(gpu_ctx, rng, rows, k, n, rank, rng.integers(0, 4, rows), xt)
