@@ -48,6 +48,13 @@ __device__ __forceinline__ void load8(const void *x, int64_t i, float (&o)[8]) {
     }
 }
 
+// The same as a vector.  (x is 16-byte aligned, an f32x8 would have to be 32.)
+__device__ __forceinline__ f16x8 eight(const _Float16 *x) { return *(const f16x8 *)x; }
+__device__ __forceinline__ f32x8 eight(const float *x) {
+    const f32x4 v = *(const f32x4 *)x, w = *(const f32x4 *)(x + 4);
+    return __builtin_shufflevector(v, w, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
 // ---- few rows ----
 
 template <int CTRL>
@@ -300,7 +307,7 @@ __global__ __launch_bounds__(64 * A_WAVES, 2) void lora_tiles_a(LoraArgs a, int 
 #pragma unroll
             for (int i = 0; i < RT; i++) o.w[i] = on ? *(const f16x8 *)(wp[i] + at) : zero8();
 #pragma unroll
-            for (int s = 0; s < A_TILES; s++) o.x[s] = on ? *(const X *)(xp[s] + at) : X{};
+            for (int s = 0; s < A_TILES; s++) o.x[s] = on ? eight(xp[s] + at) : X{};
         };
         auto add = [&](const Operands<RT, X> &o) {
 #pragma unroll

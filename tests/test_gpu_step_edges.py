@@ -64,3 +64,14 @@ def test_adapters_one_by_one_keep_their_bits(gpu_ctx, xt, rank, rows, k, n):
     _say("adapters' bits, few rows", np.dtype(xt).name, rank, rows, k, n)
     rng = np.random.default_rng(rank + k)
     _adapters(gpu_ctx, rng, rows, k, n, rank, rng.integers(0, 4, rows), xt)
+
+
+@pytest.mark.parametrize("xt", [np.float32, np.float16])
+@pytest.mark.parametrize("rank", [8, 32, 64])
+@pytest.mark.parametrize("rows", [0, 3, 70])  # 0: in tiles
+def test_adapters_of_x_at_any_16_bytes(gpu_ctx, xt, rank, rows):
+    _say("adapters, x 16 bytes on", np.dtype(xt).name, rank, rows)
+    rng = np.random.default_rng(rank + rows)
+    k, n = 520, 648
+    rows = rows or int(IN_TILES / ((k + n) * (rank + 8))) + 19
+    _adapters(gpu_ctx, rng, rows, k, n, rank, _runs(rng, rows), xt, skip=16 // np.dtype(xt).itemsize)
