@@ -50,6 +50,11 @@ int fail(arfq_ctx *ctx, int code, const std::string &msg) {
     return code;
 }
 
+// A call (`what`) refused; its text is built here, where a call that goes through has no need of it.
+static int refuse(arfq_ctx *ctx, int code, const char *what, const std::string &why) {
+    return fail(ctx, code, std::string(what) + ": " + why);
+}
+
 int hip_fail(arfq_ctx *ctx, hipError_t e, const char *what) {
     std::string m = std::string(what) + ": " + hipGetErrorString(e);
     return fail(ctx, ARFQ_E_DEVICE, m);
@@ -509,16 +514,15 @@ int arfq_kv_info(const arfq_kv *kv, int *heads, int *head_dim, int *page_size, i
 
 // The cache and batch of a call: checks, and the kernels' form of them.
 static int kv_args(arfq_ctx *ctx, const arfq_kv *kv, const arfq_kv_seqs *s, const char *what, arfq::KvArgs *a) {
-    const std::string w = std::string(what) + ": ";
-    if (!kv || !s) return fail(ctx, ARFQ_E_INVALID, w + "null argument");
-    if (kv->device != ctx->device) return fail(ctx, ARFQ_E_INVALID, w + "the cache is on another device than the context");
-    if (s->batch < 0 || s->tokens < 0 || s->max_pages < 0) return fail(ctx, ARFQ_E_SHAPE, w + "negative size");
+    if (!kv || !s) return refuse(ctx, ARFQ_E_INVALID, what, "null argument");
+    if (kv->device != ctx->device) return refuse(ctx, ARFQ_E_INVALID, what, "the cache is on another device than the context");
+    if (s->batch < 0 || s->tokens < 0 || s->max_pages < 0) return refuse(ctx, ARFQ_E_SHAPE, what, "negative size");
     if (s->batch > arfq::KV_BATCH_MAX || s->max_pages > arfq::KV_KEYS_MAX / kv->page)
-        return fail(ctx, ARFQ_E_SHAPE, w + "batch above 16384, or max_pages * page_size above 2^29");
-    if (s->tokens > arfq::KV_ROWS_MAX / kv->heads) return fail(ctx, ARFQ_E_SHAPE, w + "tokens * heads above 2^30");
-    if (!s->start && s->tokens > s->batch) return fail(ctx, ARFQ_E_SHAPE, w + "more rows than sequences, and no start");
+        return refuse(ctx, ARFQ_E_SHAPE, what, "batch above 16384, or max_pages * page_size above 2^29");
+    if (s->tokens > arfq::KV_ROWS_MAX / kv->heads) return refuse(ctx, ARFQ_E_SHAPE, what, "tokens * heads above 2^30");
+    if (!s->start && s->tokens > s->batch) return refuse(ctx, ARFQ_E_SHAPE, what, "more rows than sequences, and no start");
     if (s->tokens > 0 && s->batch > 0 && (!s->len || (s->max_pages > 0 && !s->pages)))
-        return fail(ctx, ARFQ_E_INVALID, w + "null len or pages");
+        return refuse(ctx, ARFQ_E_INVALID, what, "null len or pages");
     const arfq::KvLayout l = arfq::kv_layout(kv->page, kv->dim);
     a->data = kv->data;
     a->region = l.region;
@@ -543,14 +547,13 @@ static int kv_args(arfq_ctx *ctx, const arfq_kv *kv, const arfq_kv_seqs *s, cons
 
 // A [tokens, heads, dim] array of a call.
 static int kv_rows(arfq_ctx *ctx, const char *what, const void *p, int64_t stride, int64_t heads, int dim, int dtype) {
-    auto refuse = [&](int rc, const std::string &why) { return fail(ctx, rc, std::string(what) + ": " + why); };
-    if (dtype != ARFQ_F32 && dtype != ARFQ_F16) return refuse(ARFQ_E_INVALID, "unknown dtype");
-    if (!p) return refuse(ARFQ_E_INVALID, "null argument");
+    if (dtype != ARFQ_F32 && dtype != ARFQ_F16) return refuse(ctx, ARFQ_E_INVALID, what, "unknown dtype");
+    if (!p) return refuse(ctx, ARFQ_E_INVALID, what, "null argument");
     if (stride < heads * dim || stride > (int64_t)1 << 40)
-        return refuse(ARFQ_E_SHAPE, "token stride " + std::to_string(stride) + " below heads * head_dim = " +
-                                        std::to_string(heads * dim) + ", or above 2^40");
+        return refuse(ctx, ARFQ_E_SHAPE, what, "token stride " + std::to_string(stride) + " below heads * head_dim = " +
+                                                     std::to_string(heads * dim) + ", or above 2^40");
     if ((uintptr_t)p % 16 || stride % (dtype == ARFQ_F16 ? 8 : 4))
-        return refuse(ARFQ_E_INVALID, "pointers and token strides must be multiples of 16 bytes");
+        return refuse(ctx, ARFQ_E_INVALID, what, "pointers and token strides must be multiples of 16 bytes");
     return ARFQ_OK;
 }
 
@@ -582,27 +585,25 @@ int arfq_kv_read(arfq_ctx *ctx, const arfq_kv *kv, const arfq_kv_seqs *seqs, voi
 
 static int kv_q_heads(arfq_ctx *ctx, const arfq_kv *kv, int64_t batch, int64_t tokens, int q_heads,
                       const char *what = "kv_attention") {
-    const std::string w = std::string(what) + ": ";
-    if (!kv) return fail(ctx, ARFQ_E_INVALID, w + "null argument");
+    if (!kv) return refuse(ctx, ARFQ_E_INVALID, what, "null argument");
     if (q_heads < 1 || q_heads % kv->heads)
-        return fail(ctx, ARFQ_E_SHAPE, w + "q_heads must be a multiple of the cache's heads");
+        return refuse(ctx, ARFQ_E_SHAPE, what, "q_heads must be a multiple of the cache's heads");
     if (batch < 0 || batch > arfq::KV_BATCH_MAX || tokens < 0 || tokens > arfq::KV_ROWS_MAX / q_heads)
-        return fail(ctx, ARFQ_E_SHAPE, w + "batch above 16384, or tokens * q_heads above 2^30");
+        return refuse(ctx, ARFQ_E_SHAPE, what, "batch above 16384, or tokens * q_heads above 2^30");
     return ARFQ_OK;
 }
 
 // A call's workspace of `want` bytes: the caller's, or the context's scratch, which a captured graph cannot have.
 static int take_workspace(arfq_ctx *ctx, const char *what, size_t want, size_t bytes, void **workspace) {
-    const std::string w = std::string(what) + ": ";
     if (*workspace) {
         if (bytes < want || (uintptr_t)*workspace % 16)
-            return fail(ctx, ARFQ_E_SHAPE, w + "workspace of " + std::to_string(bytes) + " bytes, " + std::to_string(want) +
-                                               " (16-byte aligned) are wanted");
+            return refuse(ctx, ARFQ_E_SHAPE, what, "workspace of " + std::to_string(bytes) + " bytes, " + std::to_string(want) +
+                                                         " (16-byte aligned) are wanted");
     } else if (want) {
         hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
         HIP_TRY(ctx, hipStreamIsCapturing(ctx->stream, &cap));
         if (cap != hipStreamCaptureStatusNone)
-            return fail(ctx, ARFQ_E_INVALID, w + "a call under stream capture needs a workspace");
+            return refuse(ctx, ARFQ_E_INVALID, what, "a call under stream capture needs a workspace");
         if (int rc = ensure_scratch(ctx, want)) return rc;
         *workspace = ctx->scratch;
     }
@@ -815,16 +816,15 @@ int arfq_kv_attention_blocks(arfq_ctx *ctx, const arfq_kv *kv, const arfq_kv_seq
 }
 
 static int lora_check(arfq_ctx *ctx, const arfq_lora *l, int64_t rows, const char *what) {
-    const std::string w = std::string(what) + ": ";
-    if (!l) return fail(ctx, ARFQ_E_INVALID, w + "null argument");
+    if (!l) return refuse(ctx, ARFQ_E_INVALID, what, "null argument");
     constexpr int64_t MOST = (int64_t)1 << 30;
-    if (rows < 0 || rows > arfq::LORA_ROWS_MAX) return fail(ctx, ARFQ_E_SHAPE, w + "rows must be in [0, 2^24]");
+    if (rows < 0 || rows > arfq::LORA_ROWS_MAX) return refuse(ctx, ARFQ_E_SHAPE, what, "rows must be in [0, 2^24]");
     if (l->adapters < 1 || l->n < 1 || l->k < 1 || l->adapters > INT32_MAX || l->n > MOST || l->k > MOST)
-        return fail(ctx, ARFQ_E_SHAPE, w + "adapters, n and k must be positive, n and k at most 2^30");
-    if (l->k % 8) return fail(ctx, ARFQ_E_UNSUPPORTED, w + "k must be a multiple of 8");
-    if (l->rank < 1) return fail(ctx, ARFQ_E_SHAPE, w + "rank must be positive");
+        return refuse(ctx, ARFQ_E_SHAPE, what, "adapters, n and k must be positive, n and k at most 2^30");
+    if (l->k % 8) return refuse(ctx, ARFQ_E_UNSUPPORTED, what, "k must be a multiple of 8");
+    if (l->rank < 1) return refuse(ctx, ARFQ_E_SHAPE, what, "rank must be positive");
     if (l->rank % 8 || l->rank > arfq::LORA_RANK_MAX)
-        return fail(ctx, ARFQ_E_UNSUPPORTED, w + "rank must be a multiple of 8 up to 256 (smaller ones: zeros behind them)");
+        return refuse(ctx, ARFQ_E_UNSUPPORTED, what, "rank must be a multiple of 8 up to 256 (smaller ones: zeros behind them)");
     return ARFQ_OK;
 }
 

@@ -75,3 +75,25 @@ def test_adapters_of_x_at_any_16_bytes(gpu_ctx, xt, rank, rows):
     k, n = 520, 648
     rows = rows or int(IN_TILES / ((k + n) * (rank + 8))) + 19
     _adapters(gpu_ctx, rng, rows, k, n, rank, _runs(rng, rows), xt, skip=16 // np.dtype(xt).itemsize)
+
+
+def test_refusals_name_their_call(gpu_ctx):
+    _say("refusals' names")
+    up = lambda shape, t=np.float32: gpu_ctx.to_device(np.zeros(shape, t))
+    kv, seqs = gpu_ctx.kv_cache(2, 64, 16, 8), arf_amd.KVSeqs(up((1, 4), np.int32), up(1, np.int32))
+    bounds, q = up((8, 2, 2, 64), np.float16), up((1, 4, 64))
+    wide = arf_amd.Lora(up((1, 12, 16), np.float16), up((1, 5, 12), np.float16))
+    few = arf_amd.KVSeqs(up((1, 4), np.int32), up(1, np.int32), None, 2)
+    for call, name, why in (
+            (lambda: gpu_ctx.kv_attention_blocks(kv, seqs, bounds, q, q, 3, 0.1, 2), "kv_attention_blocks", "multiple of the cache's heads"),
+            (lambda: gpu_ctx.kv_attention_blocks_workspace(kv, seqs, 3, 2), "kv_attention_blocks_workspace", "multiple of the cache's heads"),
+            (lambda: gpu_ctx.kv_attention_blocks(kv, seqs, bounds, q, q, 4, 0.1, 2, workspace=up(16, np.uint8)), "kv_attention_blocks",
+             "workspace of 16 bytes, [0-9]+ \\(16-byte aligned\\) are wanted"),
+            (lambda: gpu_ctx.kv_attention(kv, seqs, q, q, 3, 0.1), "kv_attention", "multiple of the cache's heads"),
+            (lambda: gpu_ctx.kv_bounds(kv, few, bounds), "kv_bounds", "more rows than sequences, and no start"),
+            (lambda: gpu_ctx.rope(arf_amd.Rope.sections([16]), up(1, np.int32), q, q, 1, 2, 64, x_stride=130), "rope: x", "multiples of 16 bytes"),
+            (lambda: gpu_ctx.lora_add(wide, up(1, np.int32), up((1, 16)), 1, up((1, 5))), "lora_add", "rank must be a multiple of 8 up to 256"),
+            (lambda: gpu_ctx.lora_workspace(wide, 1), "lora_workspace", "rank must be a multiple of 8 up to 256")):
+        with pytest.raises((ValueError, arf_amd.ArfqError), match=f"{name}: .*{why}"):
+            call()
+    kv.free()
