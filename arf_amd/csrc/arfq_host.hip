@@ -832,7 +832,9 @@ int arfq_lora_workspace(arfq_ctx *ctx, const arfq_lora *lora, int64_t rows, size
     if (!ctx) return ARFQ_E_INVALID;
     if (!bytes) return fail(ctx, ARFQ_E_INVALID, "lora_workspace: null argument");
     if (int rc = lora_check(ctx, lora, rows, "lora_workspace")) return rc;
-    *bytes = rows ? arfq::lora_plan(ctx->cus, *lora, rows).ws_bytes : 0;
+    *bytes = 0;
+    for (const bool f16 : {false, true})  // (enough for either type of x)
+        if (rows) *bytes = std::max(*bytes, arfq::lora_plan(ctx->cus, *lora, rows, f16).ws_bytes);
     return ARFQ_OK;
 }
 
@@ -852,7 +854,7 @@ int arfq_lora_add(arfq_ctx *ctx, const arfq_lora *lora, const int32_t *ids, int6
     if (base == out && base_stride != out_stride)
         return fail(ctx, ARFQ_E_INVALID, "lora_add: in place the strides of base and out are the same");
     if (int rc = use_device(ctx)) return rc;
-    const arfq::LoraPlan plan = arfq::lora_plan(ctx->cus, *lora, rows);
+    const arfq::LoraPlan plan = arfq::lora_plan(ctx->cus, *lora, rows, x_dtype == ARFQ_F16);
     if (int rc = take_workspace(ctx, "lora_add", plan.ws_bytes, workspace_bytes, &workspace)) return rc;
     const arfq::LoraArgs a = {*lora, ids, (int)rows, x, x_dtype == ARFQ_F16, base, out, base_stride, out_stride, (float *)workspace};
     const hipError_t e = arfq::launch_lora(a, plan, ctx->cus, ctx->stream);

@@ -359,7 +359,7 @@ __global__ __launch_bounds__(64 * A_WAVES, 2) void lora_tiles_a(LoraArgs a, int 
     }
 }
 
-// B_ROWS rows, of KS runs of 32 ranks.  Their h first, into LDS: the parts added, and as two f16 parts of it times a power of
+// TileB::ROWS rows at most, of KS runs of 32 ranks.  Their h first, into LDS: the parts added, and as two f16 parts of it times a power of
 // two that puts a row's largest into [2^14, 2^15).  Then each wave has 16 NT outputs and goes over the rows' tiles: B_e
 // stays in registers while the adapter does, base is loaded a tile ahead.
 // A lane's results are four outputs of each of NT tiles, its neighbours' those of the next rows; they are exchanged
@@ -535,12 +535,20 @@ __global__ __launch_bounds__(64 * B_WAVES, KS == 2 ? 3 : 1) void lora_tiles_b(Lo
     }
 }
 
-// rows * (k + n) * rank (64 at least) from which on tiles are taken.  us one by one and in tiles, rows of two adapters in two runs /
-// rows of 32 in any order: rank 16, k + n = 12288, 256 rows 17.2 and 14.2 / 19 and 37, 512 rows 29 and 17.8 / 30 and 62;
-// rank 64, 256 rows 28 and 18.7 / 43 and 65, 512 rows 47 and 23.5 / 75 and 111; rank 128, 128 rows 28 and 20 / 46 and
-// 71, 256 rows 49 and 26 / 91 and 115; k + n = 4096, rank 64, 1024 rows 34 and 17.7 / 34 and 77; k + n = 1024, 1024 rows 11.7 and
-// 13.4 / 12.9 and 37.  (The ids are on the device: the border leans to the side that loses less.)
-constexpr int64_t TILE_VALUES = (int64_t)1 << 28;
+// rows * (k + n) * (rank + 8) above which rows are taken in tiles; twice that for an f32 x, whose products there are eight for an f16
+// x's one, and twice that again where k passes 3 / 2 n, as a tile forms A_e x anew for each adapter that it names.  The ids are on
+// the device: the border stands where rows in runs lose about as large a factor one by one as mixed rows lose in tiles.  us one by one and in
+// tiles, rows of two adapters in two runs / rows of 32 in any order; 5120 x 7168, f16 x: rank 16, 512 rows (1.5e8) 29 and 18 / 30
+// and 61, 1024 rows (3.02e8) 51 and 23 / 52 and 111; rank 64, 256 rows (2.3e8) 29 and 18.6 / 44 and 65, 512 rows (4.5e8) 48 and
+// 23.5 / 74 and 111; rank 128, 128 rows (2.1e8) 29 and 20 / 46 and 70, 256 rows (4.3e8) 50 and 25.5 / 91 and 114; f32 x, rank 16, 1024 rows
+// 51 and 25 / 52 and 148, 2048 rows (6.04e8) 113 and 47 / 115 and 273.  4096 x 1024, rank 64, f16, 1024 rows (3.8e8) 36 and 19 /
+// 38 and 104, 2048 rows (7.5e8) 64 and 26 / 67 and 193.  Over 377 sizes the factors are at most 1.5 apart on the side that is taken for an f16 x; for an
+// f32 x with k far above n mixed rows lose more there (2048 rows of 8192 x 512, rank 64, 100 and 51 / 107 and 549).
+constexpr int64_t TILE_WORK = 300 * 1000 * 1000;
+bool in_tiles(const arfq_lora &l, int64_t rows, bool x_f16) {
+    const int64_t most = TILE_WORK * (x_f16 ? 1 : 2) * (2 * l.k > 3 * l.n ? 2 : 1);
+    return rows * (l.k + l.n) > most / (l.rank + 8);
+}
 
 // Values of A_e, and of it over all workgroups, up to which both products of rows one by one are one launch.  us in one and
 // in two: k = n = 512, rank 16, any rows up to 256 4.3 and 6.8; k = n = 2048, rank 64 (2^17 of A), one row 7.1 and 8.2;
@@ -589,9 +597,9 @@ hipError_t tiles_b(const LoraArgs &a, const LoraPlan &p, int cus, hipStream_t s)
 
 }  // namespace
 
-LoraPlan lora_plan(int cus, const arfq_lora &l, int64_t rows) {
+LoraPlan lora_plan(int cus, const arfq_lora &l, int64_t rows, bool x_f16) {
     LoraPlan p;
-    p.tiles = rows * (l.k + l.n) > TILE_VALUES / std::max<int64_t>(l.rank, 64);
+    p.tiles = in_tiles(l, rows, x_f16);
     if (p.tiles) {
         // a workgroup a compute unit, and not fewer than four steps a wave
         const int64_t tiles = (rows + A_TILES * TR - 1) / (A_TILES * TR);

@@ -38,7 +38,7 @@ struct LoraPlan {
     int k_part = 0;      // values of a part
     size_t ws_bytes = 0; // [splits][rows][rank] f32
 };
-LoraPlan lora_plan(int cus, const arfq_lora &l, int64_t rows);
+LoraPlan lora_plan(int cus, const arfq_lora &l, int64_t rows, bool x_f16);
 struct LoraArgs {
     arfq_lora l;
     const int32_t *ids;

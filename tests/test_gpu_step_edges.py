@@ -6,6 +6,7 @@ import pytest
 import arf_amd
 import stepref
 from test_gpu_kv import _say
+from test_gpu_step import _lora_case
 from test_step_edges_cpu import RANKS, SHAPES
 
 pytestmark = pytest.mark.gpu
@@ -97,3 +98,69 @@ def test_refusals_name_their_call(gpu_ctx):
         with pytest.raises((ValueError, arf_amd.ArfqError), match=f"{name}: .*{why}"):
             call()
     kv.free()
+
+
+def test_adapters_mixed_rows_stay_one_by_one(gpu_ctx):
+    # 512 rows of rank 16 whose adapters may change from row to row: the parts of k are those of rows one by one (11 of 512)
+    _say("adapters' border")
+    rng = np.random.default_rng(1)
+    k, n, rank = 5128, 7160, 16
+    lora = arf_amd.Lora(gpu_ctx.empty((4, rank, k), np.float16), gpu_ctx.empty((4, n, rank), np.float16))
+    assert gpu_ctx.lora_workspace(lora, 512) == 11 * 512 * rank * 4
+    # a workspace of the bytes that are asked for does for both types, on either side of either's border
+    k, n, rank = 1032, 1040, 64
+    a, b = ((rng.standard_normal(s) / 8).astype(np.float16) for s in ((4, rank, k), (4, n, rank)))
+    lora = arf_amd.Lora(gpu_ctx.to_device(a), gpu_ctx.to_device(b))
+    for rows in (2000, 2100, 4000, 4100):
+        ids, x = rng.integers(0, 4, rows), rng.standard_normal((rows, k), dtype=np.float32)
+        need = gpu_ctx.lora_workspace(lora, rows)
+        ws, d_ids, out = gpu_ctx.to_device(np.zeros(need, np.uint8)), gpu_ctx.to_device(ids.astype(np.int32)), gpu_ctx.empty((rows, n), np.float32)
+        for xt in (np.float32, np.float16):
+            gpu_ctx.lora_add(lora, d_ids, gpu_ctx.to_device(x.astype(xt)), rows, out, workspace=ws)
+            s = _sample(rng, rows)
+            want, mags = stepref.lora(x.astype(xt)[s], ids[s], a, b, None, None)
+            assert (np.abs(out.numpy()[s] - want) <= stepref.lora_tolerance(want, mags, None, k, rank)).all()
+
+
+def _rows_in_tiles(k, n, rank, xt):
+    return int((6.1e8 if xt == np.float32 else 3.1e8) / ((k + n) * (rank + 8))) + 19
+
+
+@pytest.mark.parametrize("xt", [np.float32, np.float16])
+@pytest.mark.parametrize("rank,scaled,based,strides", [(16, False, True, (0, 0)), (16, True, False, (0, 3)), (40, False, False, (0, 4)),
+                                                       (16, True, True, (8, 3)), (136, True, True, (4, 8)), (72, True, True, (1, 0))])
+def test_adapters_in_tiles_without_scale_or_base_and_with_strides(gpu_ctx, xt, rank, scaled, based, strides):
+    _say("adapters in tiles, forms", np.dtype(xt).name, rank, scaled, based, strides)
+    rng = np.random.default_rng(rank)
+    rows = _rows_in_tiles(1032, 1024, rank, xt)
+    _lora_case(gpu_ctx, rng, rows, 1032, 1024, rank, 40, rng.integers(-2, 42, rows), xt, scaled, based, strides)
+
+
+def test_adapters_in_tiles_of_the_smallest_rank_past_the_caches(gpu_ctx):
+    _say("adapters in tiles, large")
+    rng = np.random.default_rng(8)
+    rows = _rows_in_tiles(64, 8196, 8, np.float16)
+    _lora_case(gpu_ctx, rng, rows, 64, 8196, 8, 4, _runs(rng, rows), np.float16)
+
+
+@pytest.mark.parametrize("xt", [np.float32, np.float16])
+@pytest.mark.parametrize("rank", [16, 72])
+def test_adapters_in_tiles_what_is_not_finite_stays_with_its_rows(gpu_ctx, xt, rank):
+    # and rows of every size: h's parts go by the row's largest
+    _say("adapters in tiles, not finite", np.dtype(xt).name, rank)
+    rng = np.random.default_rng(rank)
+    k, n, adapters = 520, 640, 3
+    rows = _rows_in_tiles(k, n, rank, xt)
+    a = rng.standard_normal((adapters, rank, k)).astype(np.float16)
+    b = rng.standard_normal((adapters, n, rank)).astype(np.float16)
+    x = (rng.standard_normal((rows, k)) * 10.0 ** rng.integers(-4, 4, (rows, 1))).astype(xt)
+    ids = np.arange(rows) // 5 % adapters
+    out, d_ids = gpu_ctx.empty((rows, n), np.float32), gpu_ctx.to_device(ids.astype(np.int32))
+    gpu_ctx.lora_add(arf_amd.Lora(gpu_ctx.to_device(a), gpu_ctx.to_device(b)), d_ids, gpu_ctx.to_device(x), rows, out)
+    want, mags = stepref.lora(x, ids, a, b, None, None)
+    assert (np.abs(out.numpy() - want) <= stepref.lora_tolerance(want, mags, None, k, rank)).all()
+    a[1, 3, 5], b[2, 7, 1], x[3, 9] = np.nan, np.inf, np.inf  # (row 3 has adapter 0)
+    gpu_ctx.lora_add(arf_amd.Lora(gpu_ctx.to_device(a), gpu_ctx.to_device(b)), d_ids, gpu_ctx.to_device(x), rows, out)
+    got, rest = out.numpy(), np.arange(n) != 7
+    assert np.isfinite(got[(ids == 0) & (np.arange(rows) != 3)]).all() and np.isnan(got[ids == 1]).all() and not np.isfinite(got[3]).any()
+    assert np.isfinite(got[ids == 2][:, rest]).all() and not np.isfinite(got[ids == 2][:, 7]).any()
