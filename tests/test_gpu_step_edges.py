@@ -1,12 +1,12 @@
 """Where a serving step's operators could be off without the other tests' notice: adapters' bits by the norm of the errors, in every
-form of the tiles and one by one."""
+form of the tiles and one by one, and on both sides of the borders between kernels."""
 import numpy as np
 import pytest
 
 import arf_amd
 import stepref
-from test_gpu_kv import _say
-from test_gpu_step import _lora_case
+from test_gpu_kv import Batch, _filled, _rows, _say
+from test_gpu_step import _attend, _bounds, _check, _lora_case
 from test_step_edges_cpu import RANKS, SHAPES
 
 pytestmark = pytest.mark.gpu
@@ -164,3 +164,24 @@ def test_adapters_in_tiles_what_is_not_finite_stays_with_its_rows(gpu_ctx, xt, r
     got, rest = out.numpy(), np.arange(n) != 7
     assert np.isfinite(got[(ids == 0) & (np.arange(rows) != 3)]).all() and np.isnan(got[ids == 1]).all() and not np.isfinite(got[3]).any()
     assert np.isfinite(got[ids == 2][:, rest]).all() and not np.isfinite(got[ids == 2][:, 7]).any()
+
+
+# ---- attention over chosen blocks ----
+
+@pytest.mark.parametrize("dtype", [np.float32, np.float16])
+@pytest.mark.parametrize("width", [2047, 2048, 2049, 2300])
+def test_choices_where_a_launch_of_their_own_begins(gpu_ctx, dtype, width):
+    _say("blocks' border", np.dtype(dtype).name, width)
+    rng = np.random.default_rng(width)
+    page, heads, dim, group = 16, 2, 64, 2
+    batch = Batch(gpu_ctx, [width * page - 3, 1000], [1, 2], page, rng)
+    kv = gpu_ctx.kv_cache(heads, dim, page, batch.n_pages)
+    hk, hv = _filled(gpu_ctx, kv, batch, rng)
+    q, d_bounds = _rows(rng, batch.tokens, heads * group, dim, dtype, False), _bounds(gpu_ctx, kv, batch)
+    for kw in (dict(count=64, first=1, last=2), dict(count=1500), dict(count=width - 1, last=3)):
+        got, chosen = _attend(gpu_ctx, kv, batch, d_bounds, q, dtype, 0.125, **kw)
+        _check(batch, got, chosen, q, hk, hv, 0.125, **kw)
+    # 4096 rows: scores, and a place for the choices of wider tables only
+    many = arf_amd.KVSeqs(gpu_ctx.to_device(np.zeros((1, width), np.int32)), gpu_ctx.to_device(np.zeros(1, np.int32)),
+                          gpu_ctx.to_device(np.zeros(2, np.int32)), 4096)
+    assert gpu_ctx.kv_attention_blocks_workspace(kv, many, heads * group, 64) == 4096 * heads * (width * 8 + (64 * 4 if width > 2048 else 0))
