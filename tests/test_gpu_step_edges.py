@@ -4,6 +4,7 @@ import numpy as np
 import pytest
 
 import arf_amd
+import kvref
 import stepref
 from test_gpu_kv import Batch, _filled, _rows, _say
 from test_gpu_step import _attend, _bounds, _check, _lora_case
@@ -185,3 +186,30 @@ def test_choices_where_a_launch_of_their_own_begins(gpu_ctx, dtype, width):
     many = arf_amd.KVSeqs(gpu_ctx.to_device(np.zeros((1, width), np.int32)), gpu_ctx.to_device(np.zeros(1, np.int32)),
                           gpu_ctx.to_device(np.zeros(2, np.int32)), 4096)
     assert gpu_ctx.kv_attention_blocks_workspace(kv, many, heads * group, 64) == 4096 * heads * (width * 8 + (64 * 4 if width > 2048 else 0))
+
+
+@pytest.mark.parametrize("dtype", [np.float32, np.float16])
+@pytest.mark.parametrize("dim,heads,group", [(64, 1, 4), (128, 2, 4), (256, 2, 20)])
+def test_all_blocks_are_attentions_own_result(gpu_ctx, dtype, dim, heads, group):
+    # count from the table's width on: kv_attention itself, within what either's roundings allow
+    _say("all blocks", np.dtype(dtype).name, dim, heads, group)
+    rng = np.random.default_rng(dim)
+    batch = Batch(gpu_ctx, [500, 31, 0, 1000, 130], [4, 1, 1, 1, 130], 32, rng)
+    kv = gpu_ctx.kv_cache(heads, dim, 32, batch.n_pages)
+    hk, hv = _filled(gpu_ctx, kv, batch, rng)
+    q = _rows(rng, batch.tokens, heads * group, dim, dtype, False)
+    out = gpu_ctx.empty(q.shape, dtype)
+    for count, softcap in ((32, 0.0), (100, 20.0)):
+        got, chosen = _attend(gpu_ctx, kv, batch, _bounds(gpu_ctx, kv, batch), q, dtype, 0.1, count, softcap=softcap)
+        gpu_ctx.kv_attention(kv, batch.seqs, gpu_ctx.to_device(q), out, heads * group, 0.1, softcap=softcap)
+        full = out.numpy().astype(np.float64)
+        for b, (ln, n) in enumerate(zip(batch.lens, batch.news)):
+            r, c = batch.start[b], batch.cached(b)
+            if ln == 0:
+                assert (got[r:r + n] == 0).all() and (full[r:r + n] == 0).all() and (chosen[r:r + n] == -1).all()
+                continue
+            want, mag, eps, floor = kvref.attention(q[r:r + n], hk[c], hv[c], 0.1, softcap=softcap)
+            tol = kvref.tolerance(want, mag, eps, floor, ln, dtype == np.float16)
+            assert (np.abs(got[r:r + n] - full[r:r + n]) <= 2 * tol).all(), b
+            seen = (ln - n + np.arange(n)) // 32 + 1
+            assert np.array_equal(chosen[r:r + n], np.where(np.arange(count) < seen[:, None], np.arange(count), -1)[:, None].repeat(heads, 1))
