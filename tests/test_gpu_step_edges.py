@@ -213,3 +213,45 @@ def test_all_blocks_are_attentions_own_result(gpu_ctx, dtype, dim, heads, group)
             assert (np.abs(got[r:r + n] - full[r:r + n]) <= 2 * tol).all(), b
             seen = (ln - n + np.arange(n)) // 32 + 1
             assert np.array_equal(chosen[r:r + n], np.where(np.arange(count) < seen[:, None], np.arange(count), -1)[:, None].repeat(heads, 1))
+
+
+@pytest.mark.parametrize("dtype", [np.float32, np.float16])
+def test_scores_that_are_nan_or_infinite_beside_pages_that_are_not_the_caches(gpu_ctx, dtype):
+    _say("blocks' scores not finite", np.dtype(dtype).name)
+    rng = np.random.default_rng(4)
+    page, heads, dim, group, count = 16, 2, 128, 4, 6
+    batch = Batch(gpu_ctx, [page * 30 + 4, page * 10], [1, 1], page, rng)
+    kv = gpu_ctx.kv_cache(heads, dim, page, batch.n_pages)
+    rows = int(batch.whole_start[-1])
+    k, v = (_rows(rng, rows, heads, dim, np.float32) for _ in "kv")
+    k[7 * page + 3, 1, 9] = np.nan  # block 7 of the first sequence's head 1
+    gpu_ctx.kv_write(kv, batch.whole, gpu_ctx.to_device(k), gpu_ctx.to_device(v))
+    hk, hv = kvref.held_pair(k, v)
+    d_bounds = _bounds(gpu_ctx, kv, batch)
+    table, absent = batch.table.copy(), [np.zeros(31, bool), np.zeros(10, bool)]
+    table[0, [0, 12, 20]] = [-1, batch.n_pages, 2 ** 31 - 1]
+    table[1, 2] = -5
+    absent[0][[0, 12, 20]] = absent[1][2] = True
+    batch.d_table.upload(table)
+    q = _rows(rng, 2, heads * group, dim, dtype, False)
+    q[0, 1, 5], q[1, 6, 6] = np.nan, np.inf  # of head 0 in the first row, of head 1 in the second
+    got, chosen = _attend(gpu_ctx, kv, batch, d_bounds, q, dtype, dim ** -0.5, count=count)
+    # NaN scores before all others, the earliest of them; what is not the cache's after them; then the row's own
+    assert np.array_equal(chosen[0, 0], [1, 2, 3, 4, 5, 30])
+    with np.errstate(invalid="ignore"):
+        for t in (0, 1):
+            bnd = stepref.bounds(hk[batch.cached(t)], page)
+            for h in range(heads):
+                mine = slice(h * group, (h + 1) * group)
+                blocks = stepref.choose(q[t, mine], bnd[:, h], [31, 10][t], count, 0, 1, absent=absent[t])
+                assert np.array_equal(chosen[t, h], blocks), (t, h)
+    assert 7 in chosen[0, 1] and np.isnan(got[0, 4:]).all()  # (a key that is NaN: its block comes first, its rows are NaN)
+    assert np.isnan(got[0, 1]).all() and np.isfinite(got[0, [0, 2, 3]]).all() and np.isfinite(got[1, :4]).all()
+    # the rows without such values, against the oracle
+    for t, heads_of in ((0, [0, 2, 3]), (1, [0, 1, 2, 3])):
+        c = batch.cached(t)
+        keys = (chosen[t, 0][:, None] * page + np.arange(page)).ravel()
+        keys = keys[keys < batch.lens[t]]
+        want, mag, eps, floor = kvref.attention(q[t:t + 1, heads_of], hk[c][keys, :1], hv[c][keys, :1], dim ** -0.5, absent=absent[t][keys // page])
+        tol = kvref.tolerance(want, mag, eps, floor, keys.size, dtype == np.float16)
+        assert (np.abs(got[t:t + 1, heads_of] - want) <= tol).all()
