@@ -18,13 +18,13 @@ namespace {
 
 constexpr int SEL = 256, SEL_WAVES = SEL / WAVE;  // threads that choose for a row
 constexpr int KEPT = 8;                           // keys of a thread in registers
-// Blocks to choose from up to which the attention's workgroups choose by themselves, each its row's pages, into its LDS: a launch and a
-// table's way through memory less, but every piece of a row's keys chooses for itself.  In LDS while the threads' registers have all keys;
-// beyond, each piece reads them again and again.  us by a launch of its own and in LDS, pages of 16, 8 K/V heads of 128, f32, one
-// token: 64 of 1024 blocks 27.5 and 26.8, 64 of 2048 28.5 and 27.6, 1024 of 2048 32.9 and 31.8, 64 of 4096 41.2 and 39.7, 2048 of 4096 54
-// and 60, 2048 of 16384 131 and 196; 16 sequences, 4 heads of 64, f16: 256 of 2048 42.5 and 44, 256 of 4096 66 and 91, 256 of 8192 106
-// and 194; 256 rows of a prompt, 8 heads of 64, f16: 32 of 512 65.6 and 63.2, 512 of 2048 318 and 311.
-constexpr int BLOCKS_LDS = SEL * KEPT;
+// The attention's workgroups choose for themselves, each its row's pages, into its LDS (a launch and a table's way through memory
+// less) where a row is one workgroup's, or where the threads' registers have all keys: otherwise every piece of a row's keys reads them
+// again and again.  us by a launch of its own and in LDS, pages of 16.  All keys in registers: 8 K/V heads of 128, f32, one token, 64 of
+// 1024 blocks 27.5 and 26.8, 1024 of 2048 32.9 and 31.8; 16 sequences, 4 of 64, f16, 256 of 2048 42.5 and 44.  More: those 256 of 4096 66
+// and 91, of 8192 106 and 194; one token, 64 of 4096 41.2 and 39.7, 2048 of 16384 131 and 196.  A row one workgroup's: prompts, 8 of
+// 64, f16, 256 rows, 32 of 512 65.6 and 63.2, 32 of 4096 423 and 335, 256 of 8192 1235 and 1042 (64 rows, two pieces each, 124 and 138 at 256 of 4096).
+constexpr int WIDTH_LDS = 2048, BLOCKS_KEPT = SEL * KEPT;  // (chosen pages that LDS has room for)
 
 // ---- rows ------------------------------------------------------------------------------------
 
@@ -465,7 +465,7 @@ __device__ __forceinline__ uint32_t run_max(uint32_t v) { return wave_run(v, [](
 // range of the keys' upper halves that the last chosen one lies in is cut into 256 parts and counted, until a
 // part's keys are all chosen or all alike; then, where they are alike, that of their lower halves.  (n > count, the
 // workgroup's threads all come here.)  take(rank, block, page).
-// most: places of keys and pages.  ALL: no more than the threads keep.
+// most: places of keys and pages.
 struct Kept {
     uint64_t key[KEPT];
     // (before n is known: the loads do not wait for it)
@@ -476,7 +476,7 @@ struct Kept {
         for (int i = 0; i < KEPT; i++) key[i] = keys[min(j0 + i, most - 1)];
     }
 };
-template <bool ALL, class Take>
+template <class Take>
 __device__ __forceinline__ void choose(const uint64_t *keys, const Kept &kept, const int32_t *pages, int most, int n, int count,
                                        int first, int last, SelLds &sh, Take take) {
     const int tid = threadIdx.x, wave = tid >> 6;
@@ -489,8 +489,7 @@ __device__ __forceinline__ void choose(const uint64_t *keys, const Kept &kept, c
 #pragma unroll
         for (int i = 0; i < KEPT; i++)
             if (j0 + i < j1) f(j0 + i, kept.key[i]);
-        if constexpr (!ALL)
-            for (int j = j0 + KEPT; j < j1; j++) f(j, keys[j]);
+        for (int j = j0 + KEPT; j < j1; j++) f(j, keys[j]);
     };
     sh.bins[tid] = 0;
     // The `need` largest of the candidates' words: all from `at` on (true), or those above `at` and `need` more of those that
@@ -594,8 +593,7 @@ __device__ __forceinline__ void choose(const uint64_t *keys, const Kept &kept, c
 #pragma unroll
     for (int i = 0; i < KEPT; i++)
         if (j0 + i < j1) step(j0 + i, kept.key[i], [&] { return page[i]; });
-    if constexpr (!ALL)
-        for (int j = j0 + KEPT; j < j1; j++) step(j, keys[j], [&] { return pages[j]; });
+    for (int j = j0 + KEPT; j < j1; j++) step(j, keys[j], [&] { return pages[j]; });
 }
 
 // What a row chooses.  A row's pages of a K/V head are put into `table` (LDS or memory); `write`: its blocks into chosen, too.
@@ -609,7 +607,6 @@ struct ChooseArgs {
 __device__ __forceinline__ const uint64_t *keys_of(const ChooseArgs &a, int row, int head) {
     return a.keys + ((int64_t)row * a.c.heads + head) * a.c.max_pages;
 }
-template <bool ALL>
 __device__ __forceinline__ void choose_row(const ChooseArgs &a, const Row &r, const Kept &kept, int row, int head, int32_t *table,
                                            bool write, SelLds &sh) {
     const int32_t *pages = a.c.table + (int64_t)r.b * a.c.max_pages;
@@ -621,7 +618,7 @@ __device__ __forceinline__ void choose_row(const ChooseArgs &a, const Row &r, co
     if (r.seen <= a.count) {
         for (int j = threadIdx.x; j < r.seen; j += SEL) take(j, j, pages[j]);
     } else {
-        choose<ALL>(keys_of(a, row, head), kept, pages, a.c.max_pages, r.seen, a.count, a.first, a.last, sh, take);
+        choose(keys_of(a, row, head), kept, pages, a.c.max_pages, r.seen, a.count, a.first, a.last, sh, take);
     }
     if (chosen)
         for (int i = min(r.seen, a.count) + (int)threadIdx.x; i < a.count; i += SEL) chosen[i] = -1;
@@ -634,7 +631,7 @@ __global__ __launch_bounds__(SEL) void blocks_select(ChooseArgs a) {
     const Kept kept(keys_of(a, row, head), a.c.max_pages > a.count ? a.c.max_pages : 0);
     const Row r = row_of(a.c, a.row0 + row);
     if (r.b < 0) return;
-    choose_row<false>(a, r, kept, row, head, a.table + ((int64_t)row * a.c.heads + head) * a.width, true, sh);
+    choose_row(a, r, kept, row, head, a.table + ((int64_t)row * a.c.heads + head) * a.width, true, sh);
 }
 
 // ---- attention -------------------------------------------------------------------------------
@@ -675,7 +672,7 @@ __global__ __launch_bounds__(256, attend_waves(NG, PARTS)) void blocks_attend(Ro
     const int32_t *table;
     if constexpr (CHOOSE) {
         int32_t *own = (int32_t *)((uint8_t *)lds + rows16_k::lds_bytes(NG));
-        choose_row<true>(r.ch, x.r, kept, x.row, head, own, x.tile == 0 && x.piece == 0, sh);
+        choose_row(r.ch, x.r, kept, x.row, head, own, x.tile == 0 && x.piece == 0, sh);
         __syncthreads();
         table = own;
     } else {
@@ -706,7 +703,7 @@ hipError_t attend_launch(const RowsArgs &r, hipStream_t s) {
     static std::atomic<uint64_t> done{0};
     constexpr size_t lds = rows16_k::lds_bytes(NG);
     const size_t all = lds + (CHOOSE ? (size_t)r.ch.width * sizeof(int32_t) : 0);
-    const hipError_t e = set_max_lds_once((const void *)blocks_attend<NG, PARTS, CHOOSE>, lds + (CHOOSE ? BLOCKS_LDS * sizeof(int32_t) : 0), done);
+    const hipError_t e = set_max_lds_once((const void *)blocks_attend<NG, PARTS, CHOOSE>, lds + (CHOOSE ? WIDTH_LDS * sizeof(int32_t) : 0), done);
     if (e != hipSuccess) return e;
     blocks_attend<NG, PARTS, CHOOSE><<<grid_of((int64_t)r.ch.rows * r.tiles * r.pieces * r.a.c.heads), 256, all, s>>>(r);
     return hipGetLastError();
@@ -774,12 +771,21 @@ BlocksPlan blocks_plan(int cus, int heads, int dim, int page, int64_t tokens, in
     const int64_t group = q_heads / heads;
     p.tiles = (int)((group + 15) / 16);
     p.width = (int)std::max<int64_t>(1, std::min(count, max_pages));
-    p.in_lds = max_pages <= BLOCKS_LDS;
-    const int64_t keys = max_pages > count ? heads * max_pages * 8 : 0, table = p.in_lds ? 0 : (int64_t)heads * p.width * 4;
-    p.rows = (int)std::min<int64_t>(keys + table ? std::max<int64_t>(CHUNK_BYTES / (keys + table), 1) : INT32_MAX, std::max<int64_t>(tokens, 1));
-    const int64_t items = (int64_t)p.rows * heads * p.tiles, target = (int64_t)rows16_waves(dim / KV_GROUP) * cus;
+    const int64_t keys = max_pages > count ? heads * max_pages * 8 : 0, pages = (int64_t)heads * p.width * 4;
+    const int64_t target = (int64_t)rows16_waves(dim / KV_GROUP) * cus;
     const int64_t most = std::min((p.width * (int64_t)page + MIN_PIECE - 1) / MIN_PIECE, (int64_t)0x7fff);
-    p.pieces = (int)std::min(std::max<int64_t>(target / items, 1), most);
+    int64_t table = 0, items = 0;
+    auto split = [&] {  // rows of a chunk, and pieces
+        p.rows = (int)std::min<int64_t>(keys + table ? std::max<int64_t>(CHUNK_BYTES / (keys + table), 1) : INT32_MAX, std::max<int64_t>(tokens, 1));
+        items = (int64_t)p.rows * heads * p.tiles;
+        p.pieces = (int)std::min(std::max<int64_t>(target / items, 1), most);
+    };
+    split();
+    p.in_lds = p.width <= WIDTH_LDS && (max_pages <= BLOCKS_KEPT || p.pieces * p.tiles == 1);
+    if (!p.in_lds) {
+        table = pages;
+        split();
+    }
     auto align = [](int64_t n) { return (n + 255) / 256 * 256; };
     p.off_table = (size_t)align(p.rows * keys);
     p.off_part = p.off_table + (size_t)align(p.rows * table);

@@ -182,10 +182,13 @@ def test_choices_where_a_launch_of_their_own_begins(gpu_ctx, dtype, width):
     for kw in (dict(count=64, first=1, last=2), dict(count=1500), dict(count=width - 1, last=3)):
         got, chosen = _attend(gpu_ctx, kv, batch, d_bounds, q, dtype, 0.125, **kw)
         _check(batch, got, chosen, q, hk, hv, 0.125, **kw)
-    # 4096 rows: scores, and a place for the choices of wider tables only
-    many = arf_amd.KVSeqs(gpu_ctx.to_device(np.zeros((1, width), np.int32)), gpu_ctx.to_device(np.zeros(1, np.int32)),
-                          gpu_ctx.to_device(np.zeros(2, np.int32)), 4096)
-    assert gpu_ctx.kv_attention_blocks_workspace(kv, many, heads * group, 64) == 4096 * heads * (width * 8 + (64 * 4 if width > 2048 else 0))
+    # the workspace: scores, a place for the choices where wide tables' rows are cut into pieces, and the pieces' parts
+    def need(tokens):
+        seqs = arf_amd.KVSeqs(gpu_ctx.to_device(np.zeros((1, width), np.int32)), gpu_ctx.to_device(np.zeros(1, np.int32)),
+                              gpu_ctx.to_device(np.zeros(2, np.int32)), tokens)
+        return gpu_ctx.kv_attention_blocks_workspace(kv, seqs, heads * group, 64)
+    assert need(4096) == 4096 * heads * width * 8
+    assert need(16) == 16 * heads * (width * 8 + (64 * 4 if width > 2048 else 0) + 4 * 16 * (dim + 4) * 4)
 
 
 @pytest.mark.parametrize("dtype", [np.float32, np.float16])
