@@ -258,3 +258,33 @@ def test_scores_that_are_nan_or_infinite_beside_pages_that_are_not_the_caches(gp
         want, mag, eps, floor = kvref.attention(q[t:t + 1, heads_of], hk[c][keys, :1], hv[c][keys, :1], dim ** -0.5, absent=absent[t][keys // page])
         tol = kvref.tolerance(want, mag, eps, floor, keys.size, dtype == np.float16)
         assert (np.abs(got[t:t + 1, heads_of] - want) <= tol).all()
+
+
+@pytest.mark.parametrize("dtype", [np.float32, np.float16])
+@pytest.mark.parametrize("lens,news,width", [([30000], [1], 0), ([700, 2500], [60, 1], 0), ([193], [1], 0), ([9000], [2], 3000)])
+def test_the_same_call_gives_the_same_bits(gpu_ctx, dtype, lens, news, width):
+    # whatever the workspace and the outputs held before: keys in pieces, rows of prompts, choices of either kind
+    _say("blocks again", np.dtype(dtype).name, lens, news, width)
+    rng = np.random.default_rng(lens[0])
+    page, heads, dim, group = 16, 2, 128, 4
+    batch = Batch(gpu_ctx, lens, news, page, rng)
+    if width:
+        wide = np.full((len(lens), width), -1, np.int32)
+        wide[:, :batch.table.shape[1]] = batch.table
+        batch.d_table = gpu_ctx.to_device(wide)
+        batch.seqs = arf_amd.KVSeqs(batch.d_table, batch.d_len, batch.d_start, batch.tokens)
+        batch.whole = arf_amd.KVSeqs(batch.d_table, batch.d_len, batch.d_whole, int(batch.whole_start[-1]))
+    kv = gpu_ctx.kv_cache(heads, dim, page, batch.n_pages)
+    _filled(gpu_ctx, kv, batch, rng)
+    d_bounds = _bounds(gpu_ctx, kv, batch)
+    q = _rows(rng, batch.tokens, heads * group, dim, dtype, False)
+    need = gpu_ctx.kv_attention_blocks_workspace(kv, batch.seqs, heads * group, 40)
+    dq, shape = gpu_ctx.to_device(q), (batch.tokens, heads, 40)
+    first = None
+    for fill in (0, 255, 127, 1, 60):
+        ws = gpu_ctx.to_device(np.full(need + 16, fill, np.uint8))
+        out, chosen = gpu_ctx.to_device(np.full(q.shape, fill, dtype)), gpu_ctx.to_device(np.full(shape, fill, np.int32))
+        gpu_ctx.kv_attention_blocks(kv, batch.seqs, d_bounds, dq, out, heads * group, 0.1, 40, first=1, last=2, chosen=chosen, workspace=ws)
+        got = out.numpy(), chosen.numpy()
+        first = first or got
+        assert np.array_equal(got[0], first[0]) and np.array_equal(got[1], first[1])
