@@ -425,7 +425,7 @@ int arfq_kv_plan(arfq_ctx *ctx, const arfq_kv_step *step);
 #define ARFQ_ROPE_HALVES 0
 #define ARFQ_ROPE_NEIGHBOURS 1
 typedef struct {
-    int rot_dim;           /* a multiple of 8 up to 256 */
+    int rot_dim;           /* a multiple of 8 up to 256 and head_dim (others: ARFQ_E_SHAPE) */
     int pairs;             /* ARFQ_ROPE_* */
     int axes;              /* 1..4 */
     const uint8_t *axis;   /* host, [rot_dim / 2], each below axes; NULL: 0 */
@@ -456,7 +456,8 @@ int arfq_kv_bounds(arfq_ctx *ctx, const arfq_kv *kv, const arfq_kv_seqs *seqs, v
  * chosen: NULL, or int32 [tokens, heads, count] on the device: the blocks' numbers within the sequence, ascending, then
  * -1; all -1 for a row that attends to nothing; rows of no sequence are left as they were.
  * q, out, rows that attend to nothing, arithmetic and workspace (arfq_kv_attention_blocks_workspace bytes) as in
- * arfq_kv_attention. */
+ * arfq_kv_attention, whose whole attention is faster on short sequences (one of up to some 65000 tokens, 32 of up to 7000,
+ * prompts up to 18000) and wherever all blocks are chosen. */
 int arfq_kv_attention_blocks(arfq_ctx *ctx, const arfq_kv *kv, const arfq_kv_seqs *seqs, const void *bounds, int q_heads,
                              const void *q, int64_t q_stride, int q_dtype, void *out, int64_t out_stride, int out_dtype,
                              float scale, float softcap, int64_t count, int64_t first, int64_t last, int32_t *chosen,
@@ -479,7 +480,7 @@ typedef struct {
 /* ids: device, int32 [rows].  x: [rows, k], f32 or f16, packed, 16-byte aligned.  base and out: f32 with the elements
  * from one row to the next; base may be out (where the strides are the same too), or NULL for zeros.  Rows of one
  * adapter need not lie together; in long batches they are fastest where they do.  At most 2^24 rows.  workspace
- * (16-byte aligned, arfq_lora_workspace bytes): as in arfq_kv_attention. */
+ * (16-byte aligned, arfq_lora_workspace bytes, for either type of x): as in arfq_kv_attention. */
 int arfq_lora_add(arfq_ctx *ctx, const arfq_lora *lora, const int32_t *ids, int64_t rows, const void *x, int x_dtype,
                   const float *base, int64_t base_stride, float *out, int64_t out_stride, void *workspace,
                   size_t workspace_bytes);
