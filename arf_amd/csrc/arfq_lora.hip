@@ -554,6 +554,8 @@ bool in_tiles(const arfq_lora &l, int64_t rows, bool x_f16) {
 // in two: k = n = 512, rank 16, any rows up to 256 4.3 and 6.8; k = n = 2048, rank 64 (2^17 of A), one row 7.1 and 8.2;
 // k = 5120, n = 17408, rank 16, 8 rows (11 M) 5.4 and 6.6; k = n = 2048, rank 64, 64 rows (17 M) 9.1 and 8.8; k = 1024,
 // n = 4096, rank 16, 256 rows (17 M) 12.3 and 9.6; k = 17408, rank 16 (2^18), one row 8.7 and 6.7.
+// And not in more workgroups than two a compute unit, one above rank 32 (a unit's registers hold one at a time): 512 of them at k = n =
+// 512, rank 16 6.5 and 7.6, 1024 11.3 and 7.7; k = n = 64, rank 8, 2048 17 and 7.6; rank 64, k = n = 256, 256 5.7 and 7.7, 512 9.7 and 7.9.
 constexpr int64_t ONE_A = 1 << 17, ONE_READ = 12 << 20;
 
 template <int LP>
@@ -609,7 +611,8 @@ LoraPlan lora_plan(int cus, const arfq_lora &l, int64_t rows, bool x_f16) {
     } else {
         p.k_part = K_PART;
         p.splits = (int)((l.k + K_PART - 1) / K_PART);
-        p.one = l.k * l.rank <= ONE_A && rows * ((l.n + ONE_OUT - 1) / ONE_OUT) * l.k * l.rank <= ONE_READ;
+        const int64_t groups = rows * ((l.n + ONE_OUT - 1) / ONE_OUT), a_e = l.k * l.rank;
+        p.one = a_e <= ONE_A && groups <= cus * (l.rank <= 32 ? 2 : 1) && groups * a_e <= ONE_READ;
     }
     p.ws_bytes = p.one ? 0 : (size_t)p.splits * rows * l.rank * sizeof(float);
     return p;

@@ -123,6 +123,19 @@ def test_adapters_mixed_rows_stay_one_by_one(gpu_ctx):
             assert (np.abs(out.numpy()[s] - want) <= stepref.lora_tolerance(want, mags, None, k, rank)).all()
 
 
+@pytest.mark.parametrize("xt", [np.float32, np.float16])
+@pytest.mark.parametrize("rank,k,n", [(8, 64, 64), (16, 256, 2049), (64, 264, 700)])
+def test_adapters_of_many_small_rows_take_two_launches(gpu_ctx, xt, rank, k, n):
+    # one launch while two workgroups (of 1024 outputs) a compute unit do, one above rank 32
+    most = (256 if rank > 32 else 512) // -(-n // 1024)
+    for rows in (most, most + 1, 3 * most):
+        _say("adapters, small rows", np.dtype(xt).name, rank, rows, k, n)
+        rng = np.random.default_rng(rank + rows)
+        _adapters(gpu_ctx, rng, rows, k, n, rank, rng.integers(0, 4, rows), xt)
+        lora = arf_amd.Lora(gpu_ctx.empty((4, rank, k), np.float16), gpu_ctx.empty((4, n, rank), np.float16))
+        assert (gpu_ctx.lora_workspace(lora, rows) == 0) == (rows == most)
+
+
 def _rows_in_tiles(k, n, rank, xt):
     return int((6.1e8 if xt == np.float32 else 3.1e8) / ((k + n) * (rank + 8))) + 19
 
